@@ -215,6 +215,127 @@ int kgh_device_free(void* ptr);
 int kgh_memcpy_htod(void* dst, const void* src, size_t bytes);
 int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
 
+/* ------------------------------------------------------------------------ */
+/* Operators on the caller's device tensors: the parts of a transformer block
+ * that attends to an encoder's states, for programs that build such blocks
+ * around the nets of this library (no counterpart in the reference, whose
+ * blocks exist only inside a model). Beside the blocks of a layer program
+ * they take bf16, the caller's strides, positions and lengths.
+ *
+ * Conventions of the three calls:
+ *  - Every pointer is a device pointer on `device`; strides count elements and
+ *    the last axis is contiguous. Elements need their own type's alignment
+ *    only; 16-byte aligned rows are read fastest.
+ *  - They run on hip_stream (a hipStream_t, NULL for the null stream) and are
+ *    asynchronous; the calling thread's current device is left as it was. They
+ *    allocate nothing and may be captured into a HIP graph.
+ *  - Sums and statistics are kept in fp32, and a result is rounded to the
+ *    tensors' type once. Results do not depend on what ran before, and the
+ *    same call gives the same bits.
+ *  - An axis of length zero (rows, tokens, batch, queries) makes the call a
+ *    no-op. Unless stated otherwise the output overlaps no input.
+ *  - A workspace may be NULL. Calls that may overlap need workspaces of their
+ *    own; so do captured graphs that may replay at the same time. Its contents
+ *    need no initialisation and mean nothing after the call. */
+#define KGH_DTYPE_FP32 0
+#define KGH_DTYPE_FP16 1
+#define KGH_DTYPE_BF16 2
+
+/* Activations of kgh_linear: the codes of activations.h, and GELU. */
+#define KGH_ACTIVATION_IDENTITY 0
+#define KGH_ACTIVATION_RELU 1
+#define KGH_ACTIVATION_MISH 2
+#define KGH_ACTIVATION_SILU 3
+#define KGH_ACTIVATION_GELU 20 /* x Phi(x), by the error function */
+
+/* out[m][n] = act(sum_k x[m][k] weights[n][k] + bias[n]) + residual[m][n].
+ * residual may be out itself (with its stride). in_channels and out_channels
+ * are at least 1. */
+typedef struct kgh_linear_params {
+  int32_t dtype;      /* KGH_DTYPE_* of x, weights, residual and out */
+  int32_t activation; /* KGH_ACTIVATION_* */
+  int64_t rows;
+  int32_t in_channels, out_channels;
+  const void* x; /* [rows][in_channels] */
+  int64_t x_stride;
+  const void* weights; /* [out_channels][in_channels] */
+  int64_t weights_stride;
+  const float* bias;    /* [out_channels] fp32, or NULL */
+  const void* residual; /* [rows][out_channels], or NULL */
+  int64_t residual_stride;
+  void* out; /* [rows][out_channels] */
+  int64_t out_stride;
+  void* workspace; /* 16-byte aligned, or NULL: no split of K over workgroups */
+  uint64_t workspace_bytes;
+} kgh_linear_params;
+
+/* The workspace that kgh_linear makes use of for these sizes (0: none; it reads
+ * no pointer of params). */
+int kgh_linear_workspace(int32_t device, const kgh_linear_params* params, uint64_t* bytes);
+int kgh_linear(int32_t device, const kgh_linear_params* params, void* hip_stream);
+
+/* Rotary positions with several axes: pair p of head h of token t turns by
+ *   angle = sum_a positions[t][a] * freqs[h / (heads / tables)][p][a],
+ * (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos), the angle in 64 bits. The
+ * pairs are channels (2p, 2p + 1) or (p, p + pairs) of a head; channels from
+ * 2 * pairs on are copied. `inverse` turns back (the transpose). An axis that
+ * leaves a pair alone has frequency 0 there. tables divides heads. out may be x
+ * itself (with its strides). */
+#define KGH_ROPE_INTERLEAVED 0
+#define KGH_ROPE_HALVES 1
+#define KGH_ROPE_MAX_AXES 4
+typedef struct kgh_rope_params {
+  int32_t dtype; /* KGH_DTYPE_* of x and out */
+  int32_t layout;
+  int32_t inverse;
+  int32_t axes; /* 1 to KGH_ROPE_MAX_AXES */
+  int64_t tokens;
+  int32_t heads, head_dim, pairs, tables;
+  const void* x; /* [tokens][heads][head_dim] */
+  int64_t x_token_stride, x_head_stride;
+  const int32_t* positions; /* [tokens][axes] */
+  int64_t positions_stride;
+  const float* freqs; /* [tables][pairs][axes], contiguous */
+  void* out;          /* [tokens][heads][head_dim] */
+  int64_t out_token_stride, out_head_stride;
+} kgh_rope_params;
+
+int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_stream);
+
+/* Attention of q to the states of an encoder, which have a length of their own:
+ *   out[b][i][h] = sum_j softmax_j(scale * q[b][i][h] . k[b][j][g]) v[b][j][g],
+ * g = h / (heads / kv_heads), over the keys j < key_lengths[b] with
+ * key_mask[b][j] != 0 (either may be NULL; lengths are taken into
+ * 0..k_len). What k and v hold at other keys is not used, whatever it is. A row
+ * without a key, or whose every score is minus infinity, is zeros. Head dims are
+ * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and
+ * finite. */
+#define KGH_ATTENTION_MAX_HEAD_DIM 128
+typedef struct kgh_attention_params {
+  int32_t dtype; /* KGH_DTYPE_* of q, k, v and out */
+  int32_t batch, q_len, k_len;
+  int32_t heads, kv_heads, q_head_dim, v_head_dim;
+  float scale;
+  const void* q; /* [batch][q_len][heads][q_head_dim] */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  const void* k; /* [batch][k_len][kv_heads][q_head_dim] */
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  const void* v; /* [batch][k_len][kv_heads][v_head_dim] */
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  void* out; /* [batch][q_len][heads][v_head_dim] */
+  int64_t out_batch_stride, out_token_stride, out_head_stride;
+  const int32_t* key_lengths; /* [batch], or NULL */
+  const uint8_t* key_mask;    /* [batch][k_len], or NULL */
+  int64_t key_mask_stride;
+  void* workspace; /* 16-byte aligned, or NULL: no split of the keys over workgroups */
+  uint64_t workspace_bytes;
+} kgh_attention_params;
+
+/* The workspace that kgh_cross_attention makes use of for these sizes (0: none;
+ * it reads no pointer of params). */
+int kgh_cross_attention_workspace(int32_t device, const kgh_attention_params* params, uint64_t* bytes);
+int kgh_cross_attention(int32_t device, const kgh_attention_params* params, void* hip_stream);
+
 /* Layer-level evaluation used by NeuralNet::testEvaluate* (nninterface.h:134-180):
  * the program is a single CONV, a BN+ACT pair, or one residual block
  * (ORDINARY / GPOOL / NBT). Input, mask and output are NHWC / NHW float32

@@ -10,6 +10,7 @@
 // activation + mask of the updated stream. Each stream level therefore keeps
 // two tensors: the raw residual stream R and its activated copy A.
 #include "kgh_kernels.h"
+#include "kgh_ops.h"
 
 #include <algorithm>
 #include <atomic>
@@ -2305,6 +2306,67 @@ int kgh_selftest_mfma(int32_t device) {
     KGH_HIP_CHECK(hipSetDevice(device));
     int bad = kgh::runMfmaSelfTest();
     if(bad != 0) throw KghError(KGH_ERR_INTERNAL, "matrix-core layout self-test: " + std::to_string(bad) + " mismatching elements");
+  });
+}
+
+// Operators on the caller's tensors (kgh_op_*.hip).
+namespace kgh {
+DeviceScope::DeviceScope(int device) {
+  int count = 0;
+  KGH_HIP_CHECK(hipGetDevice(&before));
+  if(device == before) return;
+  KGH_HIP_CHECK(hipGetDeviceCount(&count));
+  if(device < 0 || device >= count) throw KghError(KGH_ERR_INVALID_ARGUMENT, "no device " + std::to_string(device));
+  KGH_HIP_CHECK(hipSetDevice(device));
+  changed = true;
+}
+DeviceScope::~DeviceScope() {
+  if(changed) (void)hipSetDevice(before);
+}
+}  // namespace kgh
+
+int kgh_linear_workspace(int32_t device, const kgh_linear_params* params, uint64_t* bytes) {
+  return guarded([&] {
+    if(params == nullptr || bytes == nullptr) invalid("null argument");
+    kgh::checkLinear(*params, false);
+    (void)device;
+    *bytes = kgh::linearWorkspace(*params);
+  });
+}
+
+int kgh_linear(int32_t device, const kgh_linear_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkLinear(*params, true);
+    kgh::DeviceScope scope(device);
+    kgh::launchLinear(*params, (hipStream_t)hip_stream);
+  });
+}
+
+int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkRope(*params);
+    kgh::DeviceScope scope(device);
+    kgh::launchRope(*params, (hipStream_t)hip_stream);
+  });
+}
+
+int kgh_cross_attention_workspace(int32_t device, const kgh_attention_params* params, uint64_t* bytes) {
+  return guarded([&] {
+    if(params == nullptr || bytes == nullptr) invalid("null argument");
+    kgh::checkAttention(*params, false);
+    (void)device;
+    *bytes = kgh::attentionWorkspace(*params);
+  });
+}
+
+int kgh_cross_attention(int32_t device, const kgh_attention_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkAttention(*params, true);
+    kgh::DeviceScope scope(device);
+    kgh::launchAttention(*params, (hipStream_t)hip_stream);
   });
 }
 

@@ -1,0 +1,185 @@
+// Rotary positions with several axes (kgh_rope_axes).
+#include "kgh_ops_device.h"
+
+#include <algorithm>
+
+namespace {
+
+struct RopeArgs {
+  const void* x;
+  void* out;
+  const int32_t* positions;
+  const float* freqs;
+  int64_t xToken, xHead, outToken, outHead, ldPos;
+  int64_t items;  // tokens x head runs x groups
+  int heads, dim, pairs, axes, tables, headRun, headRuns, groups, pairGroups;
+  float sign;
+};
+
+// Sine and cosine of an angle given in turns, |turns| <= 1/2. The hardware's own
+// functions take turns; their error of about 1e-6 is below 16 bits' rounding.
+template<typename T>
+__device__ __forceinline__ void sinCosTurns(float turns, float& s, float& c) {
+  if constexpr(sizeof(T) == 4) sincospif(2.0f * turns, &s, &c);
+  else {
+    s = __builtin_amdgcn_sinf(turns);
+    c = __builtin_amdgcn_cosf(turns);
+  }
+}
+
+// n <= VEC elements of a 16-byte group to p, which is aligned to an element.
+template<typename T>
+__device__ __forceinline__ void storeGroup(T* p, const T (&v)[16 / sizeof(T)], int n) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  if(n >= VEC) __builtin_memcpy(p, v, 16);
+  else {
+#pragma unroll
+    for(int j = 0; j < VEC - 1; j++)
+      if(j < n) p[j] = v[j];
+  }
+}
+
+// A thread takes VEC pairs (two 16-byte groups) of a token, or as many of the
+// channels behind the pairs, and a run of heads that share a table: the angles
+// are computed once for the run.
+template<typename T, bool HALVES>
+__global__ __launch_bounds__(256) void ropeAxesKernel(RopeArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if(id >= a.items) return;
+  const int64_t rest = id / a.groups;
+  const int group = (int)(id - rest * a.groups);
+  const int64_t token = rest / a.headRuns;
+  const int h0 = (int)(rest - token * a.headRuns) * a.headRun;
+  const bool turns = group < a.pairGroups;
+  // The two groups' first channels, and their lengths.
+  int c0, c1, n0, n1;
+  float cs[VEC], sn[VEC];
+  if(turns) {
+    const int p0 = group * VEC;
+    const int np = min(VEC, a.pairs - p0);
+    if(HALVES) {
+      c0 = p0;
+      c1 = a.pairs + p0;
+      n0 = n1 = np;
+    }
+    else {
+      c0 = 2 * p0;
+      c1 = c0 + VEC;
+      n0 = min(VEC, 2 * np);
+      n1 = 2 * np - n0;
+    }
+    const int table = h0 / (a.heads / a.tables);
+    const float* f = a.freqs + ((int64_t)table * a.pairs + p0) * a.axes;
+    const int32_t* pos = a.positions + token * a.ldPos;
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      if(j >= np) {
+        cs[j] = sn[j] = 0.0f;
+        continue;
+      }
+      double angle = 0.0;
+      for(int x = 0; x < a.axes; x++) angle = fma((double)pos[x], (double)f[j * a.axes + x], angle);
+      // Far positions turn many times: whole turns are taken off in 64 bits.
+      const double t = angle * 0.15915494309189533577;
+      sinCosTurns<T>((float)(t - rint(t)), sn[j], cs[j]);
+      sn[j] *= a.sign;
+    }
+  }
+  else {
+    c0 = 2 * a.pairs + (group - a.pairGroups) * 2 * VEC;
+    c1 = c0 + VEC;
+    n0 = min(VEC, a.dim - c0);
+    n1 = min(VEC, max(0, a.dim - c1));
+  }
+  const int h1 = min(h0 + a.headRun, a.heads);
+  for(int h = h0; h < h1; h++) {
+    const T* src = (const T*)a.x + token * a.xToken + h * a.xHead;
+    T* dst = (T*)a.out + token * a.outToken + h * a.outHead;
+    union {
+      uint4 v;
+      T e[VEC];
+    } u0, u1;
+    u0.v = loadGroup(src + c0, n0);
+    u1.v = loadGroup(src + c1, n1);
+    if(turns) {
+#pragma unroll
+      for(int j = 0; j < VEC; j++) {
+        T& e0 = HALVES ? u0.e[j] : (2 * j < VEC ? u0.e[(2 * j) % VEC] : u1.e[(2 * j) % VEC]);
+        T& e1 = HALVES ? u1.e[j] : (2 * j < VEC ? u0.e[(2 * j + 1) % VEC] : u1.e[(2 * j + 1) % VEC]);
+        float y0, y1;
+        kgh_rope_pair((float)e0, (float)e1, cs[j], sn[j], y0, y1);
+        e0 = (T)y0;
+        e1 = (T)y1;
+      }
+    }
+    storeGroup(dst + c0, u0.e, n0);
+    storeGroup(dst + c1, u1.e, n1);
+  }
+}
+
+}  // namespace
+
+namespace kgh {
+
+void checkRope(const kgh_rope_params& p) {
+  const char* op = "kgh_rope_axes";
+  opCheckDtype(op, p.dtype);
+  if(p.layout != KGH_ROPE_INTERLEAVED && p.layout != KGH_ROPE_HALVES) opInvalid(op, "layout " + std::to_string(p.layout) + " is none of KGH_ROPE_*");
+  if(p.axes < 1 || p.axes > KGH_ROPE_MAX_AXES) opInvalid(op, "axes " + std::to_string(p.axes) + " outside 1.." + std::to_string(KGH_ROPE_MAX_AXES));
+  if(p.tokens < 0) opInvalid(op, "negative number of tokens");
+  if(p.heads < 1 || p.head_dim < 1 || p.pairs < 1 || p.head_dim > (1 << 20)) opInvalid(op, "heads, head_dim and pairs must be positive (head_dim at most 2^20)");
+  if(2 * (int64_t)p.pairs > p.head_dim) opInvalid(op, "a head of " + std::to_string(p.head_dim) + " channels has no " + std::to_string(p.pairs) + " pairs");
+  if(p.tables < 1 || p.heads % p.tables != 0) opInvalid(op, "tables must divide heads");
+  if(p.x_token_stride < 0 || p.x_head_stride < 0 || p.positions_stride < 0) opInvalid(op, "negative stride");
+  if(p.tokens == 0) return;
+  // Rows of the output lie apart: heads inside a token or tokens inside a head.
+  const int64_t ht = p.out_head_stride, tt = p.out_token_stride;
+  const bool headsInside = (p.heads == 1 || ht >= p.head_dim) && (p.tokens == 1 || tt >= (p.heads - 1) * ht + p.head_dim);
+  const bool tokensInside = (p.tokens == 1 || tt >= p.head_dim) && (p.heads == 1 || ht >= (p.tokens - 1) * tt + p.head_dim);
+  if(ht < 0 || tt < 0 || (!headsInside && !tokensInside)) opInvalid(op, "the output's strides make its rows overlap");
+  const size_t e = opElemBytes(p.dtype);
+  opCheckPointer(op, "x", p.x, e);
+  opCheckPointer(op, "out", p.out, e);
+  opCheckPointer(op, "positions", p.positions, 4);
+  opCheckPointer(op, "freqs", p.freqs, 4);
+  if(p.x == p.out && p.tokens > 1 && p.x_token_stride != tt) opInvalid(op, "in place, the strides must be the same");
+  if(p.x == p.out && p.heads > 1 && p.x_head_stride != ht) opInvalid(op, "in place, the strides must be the same");
+}
+
+void launchRope(const kgh_rope_params& p, hipStream_t stream) {
+  if(p.tokens == 0) return;
+  const int vec = 16 / (int)opElemBytes(p.dtype);
+  RopeArgs a{};
+  a.x = p.x;
+  a.out = p.out;
+  a.positions = p.positions;
+  a.freqs = p.freqs;
+  a.xToken = p.x_token_stride;
+  a.xHead = p.x_head_stride;
+  a.outToken = p.out_token_stride;
+  a.outHead = p.out_head_stride;
+  a.ldPos = p.positions_stride;
+  a.heads = p.heads;
+  a.dim = p.head_dim;
+  a.pairs = p.pairs;
+  a.axes = p.axes;
+  a.tables = p.tables;
+  a.sign = p.inverse ? -1.0f : 1.0f;
+  a.pairGroups = (p.pairs + vec - 1) / vec;
+  a.groups = a.pairGroups + (p.head_dim - 2 * p.pairs + 2 * vec - 1) / (2 * vec);
+  a.headRun = 1;
+  a.headRuns = p.heads / a.headRun;
+  a.items = p.tokens * a.headRuns * a.groups;
+  const int64_t blocks = (a.items + 255) / 256;
+  // The launch counts threads in 32 bits.
+  if(blocks >= (1 << 24)) opInvalid("kgh_rope_axes", "too many tokens for one call");
+  withDtype(p.dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if(p.layout == KGH_ROPE_HALVES) ropeAxesKernel<T, true><<<dim3((unsigned)blocks), 256, 0, stream>>>(a);
+    else ropeAxesKernel<T, false><<<dim3((unsigned)blocks), 256, 0, stream>>>(a);
+  });
+  KGH_CHECK_LAUNCH();
+}
+
+}  // namespace kgh

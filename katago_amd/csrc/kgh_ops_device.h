@@ -1,0 +1,57 @@
+// Device code shared by the operators on the caller's tensors.
+#ifndef KGH_OPS_DEVICE_H
+#define KGH_OPS_DEVICE_H
+
+#include "kgh_ops.h"
+
+namespace {
+
+// A 16-byte group of T, as loaded and as the matrix cores take it.
+template<typename T> struct Vec16;
+template<> struct Vec16<half_t> { typedef half8_t V; };
+template<> struct Vec16<bf16_t> { typedef bf16x8_t V; };
+template<> struct Vec16<float> { typedef floatx4 V; };
+
+// Elements [0, n) of the 16-byte group at p, zeros behind them; p need not be
+// aligned to more than an element (the memory takes any alignment).
+template<typename T>
+__device__ __forceinline__ uint4 loadGroup(const T* __restrict__ p, int n) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  union {
+    uint4 v;
+    T e[VEC];
+  } u;
+  if(n >= VEC) __builtin_memcpy(&u.v, p, 16);
+  else {
+    u.v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for(int j = 0; j < VEC - 1; j++)
+      if(j < n) u.e[j] = p[j];
+  }
+  return u.v;
+}
+
+// One 16-byte group of k per lane half times the other operand's: 32 x 32
+// results, lane l, register r at row (r/4)*8 + (l/32)*4 + r%4, column l % 32.
+// In 16 bits a half's group is 8 consecutive k of v_mfma_f32_32x32x16; in fp32
+// its four k go to four v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).
+__device__ __forceinline__ floatx16 mma32(half8_t a, half8_t b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mma32(bf16x8_t a, bf16x8_t b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mma32(floatx4 a, floatx4 b, floatx16 c) {
+#pragma unroll
+  for(int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+// The same for 16 x 16 results and four lane groups: lane l, register r at row
+// (l/16)*4 + r, column l % 16.
+__device__ __forceinline__ floatx4 mma16(half8_t a, half8_t b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx4 mma16(bf16x8_t a, bf16x8_t b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx4 mma16(floatx4 a, floatx4 b, floatx4 c) {
+#pragma unroll
+  for(int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+}  // namespace
+
+#endif

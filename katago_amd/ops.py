@@ -1,0 +1,307 @@
+"""Operators of the device library on the caller's tensors (include/katago_hip.h):
+a matrix product with bias, activation and residual (``linear``), rotary
+positions with several axes (``rope_axes``) and attention to an encoder's states
+(``cross_attention``).
+
+Tensors are torch tensors, or ``DeviceTensor`` views of device memory: anything
+with ``data_ptr()``, ``stride()``, ``shape``, ``dtype`` and ``device``. Calls are
+asynchronous on ``stream`` (a hipStream_t as an int, None for the null stream;
+``torch.cuda.current_stream().cuda_stream``); the caller keeps the tensors alive
+until they have run. Every call returns its output tensor. Arguments that do not
+fit raise ``StringError``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from .nn import StringError, hip_check, hip_library
+
+FP32, FP16, BF16 = 0, 1, 2
+ACTIVATIONS = {"identity": 0, "relu": 1, "mish": 2, "silu": 3, "gelu": 20}
+ROPE_LAYOUTS = {"interleaved": 0, "halves": 1}
+_INVALID = 1  # KGH_ERR_INVALID_ARGUMENT
+_MOST = 1 << 30  # of an axis; the library counts some in 32 bits
+
+_i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+
+
+class _LinearParams(ctypes.Structure):
+    """kgh_linear_params."""
+    _fields_ = [("dtype", _i32), ("activation", _i32), ("rows", _i64), ("in_channels", _i32), ("out_channels", _i32),
+                ("x", _ptr), ("x_stride", _i64), ("weights", _ptr), ("weights_stride", _i64), ("bias", _ptr),
+                ("residual", _ptr), ("residual_stride", _i64), ("out", _ptr), ("out_stride", _i64),
+                ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class _RopeParams(ctypes.Structure):
+    """kgh_rope_params."""
+    _fields_ = [("dtype", _i32), ("layout", _i32), ("inverse", _i32), ("axes", _i32), ("tokens", _i64), ("heads", _i32),
+                ("head_dim", _i32), ("pairs", _i32), ("tables", _i32), ("x", _ptr), ("x_token_stride", _i64),
+                ("x_head_stride", _i64), ("positions", _ptr), ("positions_stride", _i64), ("freqs", _ptr), ("out", _ptr),
+                ("out_token_stride", _i64), ("out_head_stride", _i64)]
+
+
+class _AttentionParams(ctypes.Structure):
+    """kgh_attention_params."""
+    _fields_ = [("dtype", _i32), ("batch", _i32), ("q_len", _i32), ("k_len", _i32), ("heads", _i32), ("kv_heads", _i32),
+                ("q_head_dim", _i32), ("v_head_dim", _i32), ("scale", ctypes.c_float),
+                ("q", _ptr), ("q_strides", _i64 * 3), ("k", _ptr), ("k_strides", _i64 * 3), ("v", _ptr), ("v_strides", _i64 * 3),
+                ("out", _ptr), ("out_strides", _i64 * 3), ("key_lengths", _ptr), ("key_mask", _ptr), ("key_mask_stride", _i64),
+                ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
+
+
+_lib = None
+
+
+def _library() -> ctypes.CDLL:
+    global _lib
+    if _lib is None:
+        lib = hip_library()
+        for name, params in (("kgh_linear", _LinearParams), ("kgh_rope_axes", _RopeParams), ("kgh_cross_attention", _AttentionParams)):
+            getattr(lib, name).argtypes = [_i32, ctypes.POINTER(params), _ptr]
+        for name, params in (("kgh_linear_workspace", _LinearParams), ("kgh_cross_attention_workspace", _AttentionParams)):
+            getattr(lib, name).argtypes = [_i32, ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
+        _lib = lib
+    return _lib
+
+
+class Device:
+    """What ``DeviceTensor.device`` holds."""
+
+    def __init__(self, index: int):
+        self.type, self.index = "cuda", index
+
+
+class DeviceTensor:
+    """A view of device memory for callers without torch: a pointer (an int or
+    ctypes.c_void_p, for instance ``DeviceBuffer.ptr``), a shape, the name of a
+    type ("float32", "float16", "bfloat16", "int32", "uint8", "bool") and
+    strides in elements (None: contiguous)."""
+
+    def __init__(self, ptr, shape, dtype: str, strides=None, device: int = 0):
+        self._ptr = ptr.value or 0 if isinstance(ptr, _ptr) else int(ptr)
+        self.shape = tuple(shape)
+        if strides is None:
+            strides, n = [], 1
+            for s in reversed(self.shape):
+                strides.insert(0, n)
+                n *= max(s, 1)
+        self._strides = tuple(strides)
+        self.dtype = dtype
+        self.device = Device(device)
+
+    def data_ptr(self) -> int:
+        return self._ptr
+
+    def stride(self):
+        return self._strides
+
+
+def _invalid(message: str):
+    raise StringError(message, _INVALID)
+
+
+_CODES = {"float32": FP32, "float16": FP16, "bfloat16": BF16, "int32": "int32", "uint8": "uint8", "bool": "bool"}
+_codes = {}  # the same by the tensors' own type objects
+
+
+def _code(op, name, t):
+    """A tensor's type: FP32, FP16, BF16 or the name of another one."""
+    try:
+        return _codes[t.dtype]
+    except KeyError:
+        pass
+    code = _CODES.get(str(t.dtype).rsplit(".", 1)[-1])
+    if code is None:
+        _invalid(f"{op}: {name} is of type {t.dtype}")
+    _codes[t.dtype] = code
+    return code
+
+
+def _look(op, name, t, ndim, code, device):
+    """Checks a tensor's axes, type and device; returns its strides."""
+    strides = t.stride()
+    if len(strides) != ndim:
+        _invalid(f"{op}: {name} has {len(strides)} axes, not {ndim}")
+    if max(t.shape) > _MOST:
+        _invalid(f"{op}: an axis of {name} is longer than {_MOST}")
+    if strides[-1] != 1 and t.shape[-1] > 1:
+        _invalid(f"{op}: the last axis of {name} is not contiguous")
+    if _code(op, name, t) != code:
+        _invalid(f"{op}: {name} is of type {t.dtype}")
+    d = t.device
+    if d.index != device or d.type != "cuda":
+        _invalid(f"{op}: {name} is not on the same device as the first tensor")
+    return strides
+
+
+def _first(op, name, t):
+    """The type and device index that the call goes by."""
+    d = t.device
+    if d.type != "cuda":
+        _invalid(f"{op}: {name} is not on a GPU")
+    code = _code(op, name, t)
+    if code not in (FP32, FP16, BF16):
+        _invalid(f"{op}: {name} is of type {t.dtype}")
+    return code, d.index
+
+
+def _shape(op, name, t, *want):
+    if tuple(t.shape) != want:
+        _invalid(f"{op}: {name} has shape {tuple(t.shape)}, not {want}")
+
+
+def _workspace(op, workspace, device):
+    """Pointer and bytes of a workspace: a contiguous tensor of any type."""
+    if workspace is None:
+        return None, 0
+    if workspace.device.type != "cuda" or workspace.device.index != device:
+        _invalid(f"{op}: the workspace is not on the same device as the first tensor")
+    n = 1
+    for size, stride in zip(reversed(tuple(workspace.shape)), reversed(tuple(workspace.stride()))):
+        if stride != n and size > 1:
+            _invalid(f"{op}: the workspace is not contiguous")
+        n *= size
+    code = _code(op, "the workspace", workspace)
+    return workspace.data_ptr(), n * {FP32: 4, FP16: 2, BF16: 2, "int32": 4}.get(code, 1)
+
+
+def _linear_params(x, weights, out, bias, activation, residual, workspace):
+    code, device = _first("linear", "x", x)
+    xs = _look("linear", "x", x, 2, code, device)
+    ws = _look("linear", "weights", weights, 2, code, device)
+    rows, in_c = x.shape
+    out_c = weights.shape[0]
+    if weights.shape[1] != in_c:
+        _invalid(f"linear: weights have {weights.shape[1]} input channels, x has {in_c}")
+    act = ACTIVATIONS.get(activation or "identity")
+    if act is None:
+        _invalid(f"linear: unknown activation {activation!r}")
+    p = _LinearParams(code, act, rows, in_c, out_c, x.data_ptr(), xs[0], weights.data_ptr(), ws[0])
+    if out is not None:
+        os = _look("linear", "out", out, 2, code, device)
+        _shape("linear", "out", out, rows, out_c)
+        p.out, p.out_stride = out.data_ptr(), os[0]
+    if bias is not None:
+        _look("linear", "bias", bias, 1, FP32, device)
+        _shape("linear", "bias", bias, out_c)
+        p.bias = bias.data_ptr()
+    if residual is not None:
+        rs = _look("linear", "residual", residual, 2, code, device)
+        _shape("linear", "residual", residual, rows, out_c)
+        p.residual, p.residual_stride = residual.data_ptr(), rs[0]
+    if workspace is not None:
+        p.workspace, p.workspace_bytes = _workspace("linear", workspace, device)
+    return p, device
+
+
+def linear_workspace(x, weights) -> int:
+    """kgh_linear_workspace: bytes of workspace that ``linear`` makes use of for
+    tensors of these shapes and types (0: none). A larger one serves too."""
+    p, device = _linear_params(x, weights, None, None, None, None, None)
+    p.out_stride = p.out_channels
+    n = ctypes.c_uint64()
+    hip_check(_library().kgh_linear_workspace(device, p, n))
+    return n.value
+
+
+def linear(x, weights, out, bias=None, activation=None, residual=None, workspace=None, stream=None):
+    """kgh_linear: out = activation(x @ weights.T + bias) + residual.
+
+    x [rows, in], weights [out, in], out and residual [rows, out] of one type
+    (float32, float16, bfloat16) with any row strides; bias [out] float32;
+    activation one of ``ACTIVATIONS``. residual may be out itself. workspace: at
+    least ``linear_workspace`` bytes of its own for calls that may overlap."""
+    p, device = _linear_params(x, weights, out, bias, activation, residual, workspace)
+    hip_check((_lib or _library()).kgh_linear(device, p, stream))
+    return out
+
+
+def rope_axes(x, positions, freqs, out, layout="interleaved", inverse=False, stream=None):
+    """kgh_rope_axes: pair p of head h of token t turns by the angle
+    sum_a positions[t, a] * freqs[h // (heads // tables), p, a].
+
+    x and out [tokens, heads, dim] of one type with any token and head strides;
+    positions [tokens, axes] int32, 1 to 4 axes; freqs [tables, pairs, axes]
+    float32, contiguous; layout "interleaved" (channels 2p and 2p + 1) or
+    "halves" (p and p + pairs). Channels from 2 * pairs on are copied; inverse
+    turns back. out may be x itself."""
+    code, device = _first("rope_axes", "x", x)
+    xs = _look("rope_axes", "x", x, 3, code, device)
+    os = _look("rope_axes", "out", out, 3, code, device)
+    ps = _look("rope_axes", "positions", positions, 2, "int32", device)
+    fs = _look("rope_axes", "freqs", freqs, 3, FP32, device)
+    tokens, heads, dim = x.shape
+    tables, pairs, axes = freqs.shape
+    if tuple(out.shape) != (tokens, heads, dim):
+        _shape("rope_axes", "out", out, tokens, heads, dim)
+    if tuple(positions.shape) != (tokens, axes):
+        _shape("rope_axes", "positions", positions, tokens, axes)
+    if (fs[0] != pairs * axes and tables > 1) or (fs[1] != axes and pairs > 1):
+        _invalid("rope_axes: freqs is not contiguous")
+    kind = ROPE_LAYOUTS.get(layout)
+    if kind is None:
+        _invalid(f"rope_axes: unknown layout {layout!r}")
+    p = _RopeParams(code, kind, 1 if inverse else 0, axes, tokens, heads, dim, pairs, tables, x.data_ptr(), xs[0], xs[1],
+                    positions.data_ptr(), ps[0], freqs.data_ptr(), out.data_ptr(), os[0], os[1])
+    hip_check((_lib or _library()).kgh_rope_axes(device, p, stream))
+    return out
+
+
+def _attention_params(q, k, v, scale):
+    code, device = _first("cross_attention", "q", q)
+    qs = _look("cross_attention", "q", q, 4, code, device)
+    ks = _look("cross_attention", "k", k, 4, code, device)
+    vs = _look("cross_attention", "v", v, 4, code, device)
+    batch, lq, heads, dq = q.shape
+    _, lk, kv_heads, _ = k.shape
+    dv = v.shape[3]
+    if tuple(k.shape) != (batch, lk, kv_heads, dq):
+        _shape("cross_attention", "k", k, batch, lk, kv_heads, dq)
+    if tuple(v.shape) != (batch, lk, kv_heads, dv):
+        _shape("cross_attention", "v", v, batch, lk, kv_heads, dv)
+    p = _AttentionParams(code, batch, lq, lk, heads, kv_heads, dq, dv, max(dq, 1) ** -0.5 if scale is None else scale,
+                         q.data_ptr(), qs[:3], k.data_ptr(), ks[:3], v.data_ptr(), vs[:3])
+    return p, code, device
+
+
+def cross_attention_workspace(q, k, v) -> int:
+    """kgh_cross_attention_workspace: bytes of workspace that ``cross_attention``
+    makes use of for tensors of these shapes and types (0: none). A larger one
+    serves too."""
+    p, _, device = _attention_params(q, k, v, None)
+    n = ctypes.c_uint64()
+    hip_check(_library().kgh_cross_attention_workspace(device, p, n))
+    return n.value
+
+
+def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, workspace=None, stream=None):
+    """kgh_cross_attention: softmax(scale * q k^T) v over the keys that take part.
+
+    q [batch, queries, heads, dq], k [batch, keys, kv_heads, dq], v [batch, keys,
+    kv_heads, dv], out [batch, queries, heads, dv] of one type, any strides but
+    that of the last axis; heads // kv_heads query heads share a kv head. scale
+    defaults to dq ** -0.5. key_lengths [batch] int32: keys from there on take no
+    part; key_mask [batch, keys] uint8 or bool: nor do those with 0. What k and v
+    hold there is not used. A row without a key is zeros. workspace: at least
+    ``cross_attention_workspace`` bytes of its own for calls that may overlap;
+    without one, long keys are not split over workgroups."""
+    p, code, device = _attention_params(q, k, v, scale)
+    os = _look("cross_attention", "out", out, 4, code, device)
+    batch = q.shape[0]
+    if tuple(out.shape) != (batch, p.q_len, p.heads, p.v_head_dim):
+        _shape("cross_attention", "out", out, batch, p.q_len, p.heads, p.v_head_dim)
+    p.out, p.out_strides = out.data_ptr(), os[:3]
+    if key_lengths is not None:
+        ls = _look("cross_attention", "key_lengths", key_lengths, 1, "int32", device)
+        _shape("cross_attention", "key_lengths", key_lengths, batch)
+        p.key_lengths = key_lengths.data_ptr()
+    if key_mask is not None:
+        kind = _code("cross_attention", "key_mask", key_mask)
+        ms = _look("cross_attention", "key_mask", key_mask, 2, kind if kind in ("uint8", "bool") else "uint8", device)
+        _shape("cross_attention", "key_mask", key_mask, batch, p.k_len)
+        p.key_mask, p.key_mask_stride = key_mask.data_ptr(), ms[0]
+    if workspace is not None:
+        p.workspace, p.workspace_bytes = _workspace("cross_attention", workspace, device)
+    hip_check((_lib or _library()).kgh_cross_attention(device, p, stream))
+    return out

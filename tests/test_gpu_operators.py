@@ -1,0 +1,484 @@
+"""The operators on the caller's tensors against their formulas in 64 bits, at
+the sizes, strides and masks where their tiles, tails and softmax can go wrong,
+and as a program runs them: together, on its own stream, captured and replayed,
+in place, without torch. Bounds: operator_reference.py."""
+import threading
+
+import pytest
+import torch
+
+import operator_reference as ref
+from katago_amd import nn, ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+ids = lambda v: str(v).replace("torch.", "").replace(" ", "")
+
+
+def _rand(*shape, dtype=torch.float16, seed=0, scale=1.0, pad=0, shift=0):
+    """Normal values whose rows lie pad apart and start shift elements past a
+    16-byte border."""
+    g = torch.Generator().manual_seed(hash((shape, seed)) % (1 << 31))
+    row = shape[-1] + pad
+    flat = torch.empty(shift + (torch.Size(shape[:-1]).numel()) * row, dtype=dtype, device="cuda").fill_(float("nan"))
+    t = flat[shift:].view(*shape[:-1], row)[..., :shape[-1]]
+    t.copy_((torch.randn(*shape, generator=g) * scale).to(dtype))
+    return t
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _guarded(*shape, dtype, pad=3, shift=5):
+    """An output whose surroundings must stay as they are: (tensor, check)."""
+    row = shape[-1] + pad
+    n = torch.Size(shape[:-1]).numel()
+    flat = torch.full((shift + n * row + 64,), 7.0, dtype=dtype, device="cuda")
+    t = flat[shift:shift + n * row].view(*shape[:-1], row)[..., :shape[-1]]
+
+    def untouched():
+        rest = flat.clone()
+        rest[shift:shift + n * row].view(*shape[:-1], row)[..., :shape[-1]] = 7.0
+        assert bool((rest == 7.0).all()), "written outside the output"
+    return t, untouched
+
+
+def _linear(x, w, out, **kw):
+    need = ops.linear_workspace(x, w)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+    return ops.linear(x, w, out, workspace=ws, stream=_stream(), **kw)
+
+
+def _attention(q, k, v, out, **kw):
+    need = ops.cross_attention_workspace(q, k, v)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+    return ops.cross_attention(q, k, v, out, workspace=ws, stream=_stream(), **kw)
+
+
+# -- linear -------------------------------------------------------------------
+
+LINEAR_SIZES = [(1, 1, 1), (1, 384, 1024), (3, 40, 8), (1, 4104, 24), (7, 1000, 72), (16, 256, 64), (17, 264, 40), (31, 8, 33),
+                (33, 520, 129), (64, 64, 64), (65, 96, 257), (100, 33, 31), (129, 72, 63), (200, 1032, 136), (300, 17, 520)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("m,k,n", LINEAR_SIZES, ids=ids)
+def test_linear_sizes(dtype, m, k, n):
+    x, w = _rand(m, k, dtype=dtype), _rand(n, k, dtype=dtype, seed=1, scale=k ** -0.5)
+    bias, res = _rand(n, dtype=torch.float32, seed=2), _rand(m, n, dtype=dtype, seed=3, pad=1)
+    out, untouched = _guarded(m, n, dtype=dtype)
+    ref.check(_linear(x, w, out, bias=bias, activation="gelu", residual=res), ref.linear(x, w, bias, "gelu", res))
+    untouched()
+    plain = torch.empty(m, n, dtype=dtype, device="cuda")
+    ref.check(_linear(x, w, plain), ref.linear(x, w))
+    assert torch.equal(plain, _linear(x, w, torch.empty_like(plain))), "not the same bits again"
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("pad,shift", [(8, 0), (1, 0), (0, 1), (3, 5), (7, 8)])
+@pytest.mark.parametrize("m,k,n", [(5, 72, 40), (70, 200, 96)], ids=ids)
+def test_linear_strides(dtype, pad, shift, m, k, n):
+    x, w = _rand(m, k, dtype=dtype, pad=pad, shift=shift), _rand(n, k, dtype=dtype, seed=1, scale=k ** -0.5, pad=pad, shift=shift)
+    out, untouched = _guarded(m, n, dtype=dtype, pad=pad, shift=shift)
+    ref.check(_linear(x, w, out), ref.linear(x, w))
+    untouched()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("act", ops.ACTIVATIONS)
+@pytest.mark.parametrize("m", [2, 80])
+def test_linear_activations(dtype, act, m):
+    """Values from the far left tail to the far right one."""
+    x, w = _rand(m, 64, dtype=dtype, scale=2.0), _rand(96, 64, dtype=dtype, seed=1)
+    bias = torch.linspace(-90, 90, 96, device="cuda")
+    out = torch.empty(m, 96, dtype=dtype, device="cuda")
+    ref.check(_linear(x, w, out, bias=bias, activation=act), ref.linear(x, w, bias, act), act)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("m", [1, 90])
+def test_linear_in_place_residual(dtype, m):
+    x, w, res = _rand(m, 136, dtype=dtype), _rand(72, 136, dtype=dtype, seed=1, scale=0.1), _rand(m, 72, dtype=dtype, seed=2)
+    want = ref.linear(x, w, None, "silu", res)
+    ref.check(_linear(x, w, res, activation="silu", residual=res), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("m", [3, 90])
+def test_linear_infinities_stay_in_their_rows(dtype, m):
+    """An infinite or NaN input reaches its own row only, and columns of exact
+    zeros in fp32's own arithmetic."""
+    x, w = _rand(m, 80, dtype=dtype), _rand(48, 80, dtype=dtype, seed=1)
+    x[1, 7], x[2, 9] = float("inf"), float("nan")
+    out = torch.empty(m, 48, dtype=dtype, device="cuda")
+    _linear(x, w, out)
+    want = x.double() @ w.double().t()
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isinf(out), torch.isinf(want))
+    assert torch.equal(out[1], want[1].to(dtype))
+    keep = [i for i in range(m) if i not in (1, 2)]
+    y, bound = ref.linear(x[keep], w)
+    ref.check(out[keep], (y, bound))
+
+
+def test_linear_shared_rows_and_far_offsets():
+    """One row for all (stride 0), and rows more than 2^31 elements apart."""
+    x, w = _rand(1, 64).expand(5, 64), _rand(32, 64, seed=1)
+    out = torch.empty(5, 32, dtype=torch.float16, device="cuda")
+    ref.check(_linear(x, w, out), ref.linear(x, w))
+    far = torch.empty((1 << 31) + 4096, dtype=torch.float16, device="cuda")
+    stride = (1 << 30) + 1024
+    x = far.as_strided((3, 64), (stride, 1))
+    x.copy_(_rand(3, 64, seed=4))
+    ref.check(_linear(x, w, out[:3]), ref.linear(x, w))
+    ref.check(_linear(w, x, torch.empty(32, 3, dtype=torch.float16, device="cuda")), ref.linear(w, x))
+    y = far.as_strided((3, 32), (stride, 1), 256)
+    ref.check(_linear(x, w, y), ref.linear(x, w))
+
+
+def test_linear_no_rows():
+    out = torch.full((0, 8), 3.0, dtype=torch.float16, device="cuda")
+    assert ops.linear(torch.empty(0, 16, dtype=torch.float16, device="cuda"), _rand(8, 16), out, stream=_stream()) is out
+
+
+# -- rope ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("layout", ops.ROPE_LAYOUTS)
+@pytest.mark.parametrize("tokens,heads,dim,pairs,axes,tables", [
+    (1, 1, 2, 1, 1, 1), (1, 6, 64, 32, 2, 6), (5, 4, 33, 16, 3, 2), (3, 6, 62, 27, 4, 1), (100, 3, 96, 48, 3, 3), (7, 32, 128, 64, 2, 1),
+    (2, 5, 80, 8, 1, 5), (11, 8, 17, 5, 2, 4), (361, 12, 64, 32, 2, 6)], ids=ids)
+def test_rope(dtype, layout, tokens, heads, dim, pairs, axes, tables):
+    x = _rand(tokens, heads, dim, dtype=dtype, pad=dim % 3)
+    g = torch.Generator().manual_seed(pairs)
+    pos = torch.randint(-30, 4000, (tokens, axes), generator=g, dtype=torch.int32).cuda()
+    freqs = torch.randn(tables, pairs, axes, generator=g).cuda()
+    for inverse in (False, True):
+        out, untouched = _guarded(tokens, heads, dim, dtype=dtype)
+        ops.rope_axes(x, pos, freqs, out, layout=layout, inverse=inverse, stream=_stream())
+        ref.check(out, ref.rope(x, pos, freqs, layout, inverse))
+        untouched()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_rope_far_positions(dtype):
+    """Angles of up to 2^31 radians, and positions at the ends of their type."""
+    x = _rand(4, 2, 32, dtype=dtype)
+    pos = torch.tensor([[2 ** 31 - 1, 0], [-2 ** 31, 5], [2 ** 31 - 1, -2 ** 31], [0, 0]], dtype=torch.int32, device="cuda")
+    freqs = torch.rand(1, 16, 2, generator=torch.Generator().manual_seed(2)).cuda()
+    out = torch.empty_like(x)
+    ops.rope_axes(x, pos, freqs, out, stream=_stream())
+    ref.check(out, ref.rope(x, pos, freqs))
+    assert torch.equal(out[3], x[3])
+
+
+@pytest.mark.parametrize("layout", ops.ROPE_LAYOUTS)
+def test_rope_in_place_in_a_fused_projection(layout):
+    """Query and key heads of [Q|K|V] rows, the values beside them untouched."""
+    qkv = _rand(50, 9 * 32, dtype=torch.bfloat16)
+    before = qkv.clone()
+    qk = qkv[:, :6 * 32].unflatten(1, (6, 32))
+    pos = torch.randint(0, 19, (50, 2), dtype=torch.int32, device="cuda")
+    freqs = torch.rand(3, 16, 2, device="cuda")
+    want = ref.rope(qk, pos, freqs, layout)
+    ops.rope_axes(qk, pos, freqs, qk, layout=layout, stream=_stream())
+    ref.check(qk, want)
+    assert torch.equal(qkv[:, 6 * 32:], before[:, 6 * 32:])
+
+
+def test_rope_far_offsets_and_head_major():
+    far = torch.empty((1 << 31) + 4096, dtype=torch.float16, device="cuda")
+    x = far.as_strided((3, 2, 32), ((1 << 30) + 512, 40, 1))
+    x.copy_(_rand(3, 2, 32))
+    pos, freqs = torch.arange(6, dtype=torch.int32, device="cuda").view(3, 2), torch.rand(1, 16, 2, device="cuda")
+    out = torch.empty(2, 3, 32, dtype=torch.float16, device="cuda").transpose(0, 1)  # tokens inside heads
+    want = ref.rope(x, pos, freqs)
+    ops.rope_axes(x, pos, freqs, out, stream=_stream())
+    ref.check(out, want)
+    ops.rope_axes(x, pos, freqs, x, stream=_stream())
+    ref.check(x, want)
+    ops.rope_axes(x[:0], pos[:0], freqs, out[:0], stream=_stream())
+
+
+def test_rope_is_the_boards_rotary_embedding():
+    """The trunk's fixed rotary embedding (first half of the pairs by one axis,
+    second half by the other, theta 100) at a board's positions."""
+    pairs, side = 16, 9
+    f = 100.0 ** (-torch.arange(pairs // 2) / (pairs // 2))
+    freqs = torch.zeros(1, pairs, 2)
+    freqs[0, :pairs // 2, 0], freqs[0, pairs // 2:, 1] = f, f
+    at = torch.arange(side * side)
+    pos = torch.stack((at % side, at // side), 1)
+    x = _rand(side * side, 2, 2 * pairs, dtype=torch.float32)
+    out = torch.empty_like(x)
+    ops.rope_axes(x, pos.int().cuda(), freqs.cuda(), out, stream=_stream())
+    ref.check(out, ref.rope(x, pos, freqs))
+
+
+# -- attention ----------------------------------------------------------------
+
+ATTENTION_SIZES = [  # batch, queries, keys, heads, kv heads, dq, dv
+    (1, 1, 1, 1, 1, 1, 1), (1, 1, 361, 6, 6, 64, 64), (2, 3, 31, 4, 4, 32, 32), (1, 5, 32, 8, 2, 64, 64), (2, 7, 33, 4, 1, 48, 80),
+    (1, 1, 63, 32, 8, 128, 128), (3, 2, 64, 4, 4, 80, 80), (1, 130, 65, 2, 2, 64, 64), (1, 33, 200, 6, 3, 32, 16), (2, 129, 129, 2, 1, 128, 128),
+    (1, 40, 127, 3, 3, 13, 37), (2, 1, 1000, 8, 8, 96, 64), (1, 260, 300, 4, 2, 64, 128), (4, 1, 5000, 4, 1, 128, 128), (1, 9, 0, 2, 2, 64, 64),
+    (1, 17, 3000, 2, 2, 64, 64)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("size", ATTENTION_SIZES, ids=ids)
+def test_attention_sizes(dtype, size):
+    b, lq, lk, h, kv, dq, dv = size
+    q, k, v = _rand(b, lq, h, dq, dtype=dtype, scale=1.5), _rand(b, lk, kv, dq, dtype=dtype, seed=1, scale=1.5), _rand(b, lk, kv, dv, dtype=dtype, seed=2)
+    out, untouched = _guarded(b, lq, h, dv, dtype=dtype)
+    ref.check(_attention(q, k, v, out), ref.attention(q, k, v))
+    untouched()
+    alone = ops.cross_attention(q, k, v, torch.empty_like(out), stream=_stream())  # no workspace: no split
+    ref.check(alone, ref.attention(q, k, v))
+    assert torch.equal(out, _attention(q, k, v, torch.empty_like(out))), "not the same bits again"
+
+
+def _masks(kind, b, lk, g):
+    lengths = mask = None
+    if kind in ("lengths", "both"):
+        lengths = torch.tensor([[0, lk, 1, lk // 2, lk + 9, -3][i % 6] for i in range(b)], dtype=torch.int32, device="cuda")
+    if kind in ("mask", "both", "bool"):
+        mask = (torch.rand(b, lk + 3, generator=g) < 0.4).to(torch.bool if kind == "bool" else torch.uint8).cuda()[:, :lk]
+        mask[1, :] = False  # a row without a key
+        mask[0, :lk - 1] = False  # only the last key
+        if kind != "bool":
+            mask[2] *= 255  # anything but 0 takes part
+    return lengths, mask
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("kind", ["lengths", "mask", "both", "bool"])
+@pytest.mark.parametrize("lq,lk,h,kv,d", [(1, 200, 4, 2, 64), (1, 4100, 8, 1, 128), (70, 130, 2, 2, 32), (150, 260, 4, 1, 128), (3, 70, 2, 1, 37)], ids=ids)
+def test_attention_masks(dtype, kind, lq, lk, h, kv, d):
+    """Masks that leave rows empty or one key; what masked keys hold (NaN,
+    infinities, the type's lowest value) does not matter."""
+    g = torch.Generator().manual_seed(lk)
+    b = 6
+    q, k, v = _rand(b, lq, h, d, dtype=dtype), _rand(b, lk, kv, d, dtype=dtype, seed=1), _rand(b, lk, kv, d, dtype=dtype, seed=2)
+    lengths, mask = _masks(kind, b, lk, g)
+    on = torch.ones(b, lk, dtype=torch.bool, device="cuda")
+    if lengths is not None:
+        on &= torch.arange(lk, device="cuda") < lengths[:, None]
+    if mask is not None:
+        on &= mask != 0
+    want = ref.attention(q, k, v, lengths=lengths, mask=mask)
+    for fill_k, fill_v in ((float("nan"), float("inf")), (torch.finfo(dtype).min, float("nan")), (float("inf"), float("-inf"))):
+        k.masked_fill_(~on[:, :, None, None], fill_k)
+        v.masked_fill_(~on[:, :, None, None], fill_v)
+        out, untouched = _guarded(b, lq, h, d, dtype=dtype)
+        ref.check(_attention(q, k, v, out, key_lengths=lengths, key_mask=mask), want, kind)
+        untouched()
+        assert not out[~on.any(1)].any()
+        ref.check(ops.cross_attention(q, k, v, torch.empty_like(out), key_lengths=lengths, key_mask=mask, stream=_stream()), want, kind)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("pad,shift", [(8, 0), (1, 0), (0, 1), (3, 5), (64, 8)])
+@pytest.mark.parametrize("lq,d", [(1, 64), (1, 128), (40, 64), (150, 128)])
+def test_attention_strides(dtype, pad, shift, lq, d):
+    """Heads inside tokens with gaps and shifts, and heads outside tokens."""
+    q, k, v = (_rand(2, n, 4, d, dtype=dtype, seed=i, pad=pad, shift=shift) for i, n in enumerate((lq, 90, 90)))
+    out, untouched = _guarded(2, lq, 4, d, dtype=dtype, pad=pad, shift=shift)
+    want = ref.attention(q, k, v, scale=0.3)
+    ref.check(_attention(q, k, v, out, scale=0.3), want)
+    untouched()
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    out = torch.empty(2, 4, lq, d, dtype=dtype, device="cuda").transpose(1, 2)
+    ref.check(_attention(*turned, out, scale=0.3), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lq,lk", [(1, 700), (64, 200)])
+def test_attention_scores_that_grow(dtype, lq, lk):
+    """Scores of up to hundreds, growing and falling along the keys: the softmax's
+    reference point moves, and the last or first key decides."""
+    for ramp in (torch.linspace(-1, 1, lk), torch.linspace(1, -1, lk)):
+        q = torch.full((1, lq, 2, 32), 4.0, dtype=dtype, device="cuda")
+        k = (ramp[None, :, None, None] * 5).expand(1, lk, 2, 32).to(dtype).cuda()
+        v = _rand(1, lk, 2, 32, dtype=dtype)
+        ref.check(_attention(q, k, v, torch.empty_like(q), scale=1.0), ref.attention(q, k, v, scale=1.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lq", [1, 50])
+def test_attention_non_finite_keys_that_take_part(dtype, lq):
+    """A NaN key or an infinite score makes its item's rows NaN and no other's;
+    a row of scores of minus infinity is zeros."""
+    q, k, v = (_rand(4, n, 2, 64, dtype=dtype, seed=i) for i, n in enumerate((lq, 75, 75)))
+    q[1:3].abs_()
+    k[0, 40, 1, 3] = float("nan")
+    k[1, 70, 0] = float("inf")
+    k[2] = float("-inf")
+    want = ref.attention(q[3:], k[3:], v[3:])
+    out = _attention(q, k, v, torch.empty_like(q))
+    assert out[0, :, 1].isnan().all() and not out[0, :, 0].isnan().any()
+    assert out[1, :, 0].isnan().all() and not out[1, :, 1].isnan().any()
+    assert not out[2].any()
+    ref.check(out[3:], want)
+
+
+def test_attention_far_offsets():
+    """Keys and values more than 2^31 elements from their base."""
+    far = torch.empty((1 << 31) + (1 << 16), dtype=torch.float16, device="cuda")
+    q = _rand(2, 3, 2, 64)
+    k = far.as_strided((2, 70, 1, 64), ((1 << 31) - 4096, 128, 64, 1))
+    v = far.as_strided((2, 70, 1, 64), ((1 << 31) - 4096, 128, 64, 1), 64)
+    k.copy_(_rand(2, 70, 1, 64, seed=1))
+    v.copy_(_rand(2, 70, 1, 64, seed=2))
+    ref.check(_attention(q, k, v, torch.empty_like(q)), ref.attention(q, k, v))
+    tokens = far.as_strided((1, 3, 1, 64), (0, (1 << 30) + 64, 64, 1))
+    tokens.copy_(_rand(1, 3, 1, 64, seed=3))
+    ref.check(_attention(q[:1], tokens, tokens, torch.empty_like(q[:1])), ref.attention(q[:1], tokens, tokens))
+
+
+def test_attention_no_queries():
+    e = lambda *s: torch.empty(*s, dtype=torch.float16, device="cuda")
+    ops.cross_attention(e(2, 0, 4, 64), e(2, 9, 4, 64), e(2, 9, 4, 64), e(2, 0, 4, 64), stream=_stream())
+    ops.cross_attention(e(0, 3, 4, 64), e(0, 9, 4, 64), e(0, 9, 4, 64), e(0, 3, 4, 64), stream=_stream())
+
+
+# -- together, and as a program calls them ------------------------------------
+
+class Block:
+    """A cross-attending block with a feed-forward layer: boards' positions
+    attend to an encoder's states."""
+
+    def __init__(self, dtype, boards=3, side=9, states=50, width=64, heads=4, kv=2, d=16):
+        t = dict(dtype=dtype)
+        self.b, self.l, self.s, self.h, self.kv, self.d = boards, side * side, states, heads, kv, d
+        self.x, self.enc = _rand(boards * self.l, width, **t), _rand(boards * states, width, seed=1, **t)
+        self.w = {n: _rand(o, i, seed=j, scale=i ** -0.5, **t) for j, (n, o, i) in enumerate(
+            (("q", heads * d, width), ("kv", 2 * kv * d, width), ("o", width, heads * d), ("up", 2 * width, width), ("down", width, 2 * width)))}
+        self.bias = _rand(2 * width, dtype=torch.float32, seed=9)
+        at = torch.arange(self.l)
+        self.pos = torch.stack((at % side, at // side), 1).repeat(boards, 1).int().cuda()
+        self.enc_pos = torch.arange(states).repeat(boards)[:, None].expand(-1, 2).int().contiguous().cuda()
+        self.freqs = _rand(kv, d // 2, 2, dtype=torch.float32, seed=5, scale=0.3)
+        self.lengths = torch.tensor([states, 0, 17], dtype=torch.int32, device="cuda")[:boards]
+        e = lambda *s: torch.empty(*s, dtype=dtype, device="cuda")
+        self.q, self.kvs, self.a = e(boards * self.l, heads * d), e(boards * states, 2 * kv * d), e(boards * self.l, heads * d)
+        self.y, self.up, self.out = torch.empty_like(self.x), e(boards * self.l, 2 * width), torch.empty_like(self.x)
+        q, k = self.q.view(boards, self.l, heads, d), self.kvs[:, :kv * d].view(boards, states, kv, d)
+        n = max(ops.cross_attention_workspace(q, k, k), ops.linear_workspace(self.x, self.w["up"]), ops.linear_workspace(self.up, self.w["down"]), 16)
+        self.ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+
+    def run(self, stream):
+        k = self.kvs[:, :self.kv * self.d].unflatten(1, (self.kv, self.d))
+        v = self.kvs[:, self.kv * self.d:].unflatten(1, (self.kv, self.d))
+        q = self.q.view(-1, self.h, self.d)
+        run = dict(workspace=self.ws, stream=stream)
+        ops.linear(self.x, self.w["q"], self.q, **run)
+        ops.linear(self.enc, self.w["kv"], self.kvs, **run)
+        ops.rope_axes(q, self.pos, self.freqs, q, stream=stream)
+        ops.rope_axes(k, self.enc_pos, self.freqs, k, stream=stream)
+        ops.cross_attention(q.view(self.b, self.l, self.h, self.d), k.unflatten(0, (self.b, self.s)), v.unflatten(0, (self.b, self.s)),
+                            self.a.view(self.b, self.l, self.h, self.d), key_lengths=self.lengths, **run)
+        ops.linear(self.a, self.w["o"], self.y, residual=self.x, **run)
+        ops.linear(self.y, self.w["up"], self.up, bias=self.bias, activation="gelu", **run)
+        return ops.linear(self.up, self.w["down"], self.out, residual=self.y, **run)
+
+    def want(self):
+        w = {n: t.double().cpu() for n, t in self.w.items()}
+        x, enc = self.x.double().cpu(), self.enc.double().cpu()
+        q, _ = ref.rope((x @ w["q"].t()).view(-1, self.h, self.d), self.pos, self.freqs)
+        k, v = (enc @ w["kv"].t()).view(-1, 2, self.kv, self.d).unbind(1)
+        k, _ = ref.rope(k, self.enc_pos, self.freqs)
+        a, _ = ref.attention(q.view(self.b, self.l, self.h, self.d), *(t.reshape(self.b, self.s, self.kv, self.d) for t in (k, v)), lengths=self.lengths)
+        y = a.view(x.shape[0], -1) @ w["o"].t() + x
+        return ref.activate(y @ w["up"].t() + self.bias.double().cpu(), "gelu") @ w["down"].t() + y
+
+
+# Off by half a step each: the projections, q and k turned, p and the attention,
+# the output projection, the two layers: eight roundings, no one of which the
+# later steps make more than twice as large against the residual stream.
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_block(dtype):
+    block = Block(dtype)
+    got, want = block.run(_stream()).double().cpu(), block.want()
+    assert (got - want).norm() <= 16 * ref.HALF_STEP[dtype] * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=ids)
+def test_captured_and_replayed(dtype):
+    """A captured block replays to the eager bits, with other work between the
+    replays, and follows inputs and lengths that change in place."""
+    block = Block(dtype)
+    stream = torch.cuda.Stream()
+    block.run(_stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        block.run(_stream())
+    for i in range(4):
+        block.x.copy_(_rand(*block.x.shape, dtype=dtype, seed=20 + i))
+        block.lengths.copy_(torch.tensor([(5 * i) % 50, 50, i], dtype=torch.int32))
+        block.out.fill_(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = block.out.clone()
+        assert torch.equal(block.run(_stream()), replayed), i
+        torch.cuda.synchronize()
+
+
+def test_other_stream_and_null_stream():
+    block = Block(torch.float16)
+    want = block.run(None).clone()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    block.out.zero_()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = block.run(s.cuda_stream).clone()
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_two_threads_at_once():
+    """Calls from two threads on streams and workspaces of their own."""
+    blocks = [Block(torch.bfloat16, boards=1 + i) for i in range(2)]
+    want = [b.run(None).clone() for b in blocks]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        for _ in range(20):
+            blocks[i].out.zero_()
+            torch.cuda.current_stream().synchronize()
+            blocks[i].run(s.cuda_stream)
+            s.synchronize()
+            if not torch.equal(blocks[i].out, want[i]):
+                bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_without_torch_tensors():
+    """DeviceTensor views of the library's own buffers."""
+    import numpy as np
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal((5, 24)).astype(np.float32), rng.standard_normal((7, 24)).astype(np.float32)
+    bx, bw, bo = nn.DeviceBuffer.from_array(x), nn.DeviceBuffer.from_array(w), nn.DeviceBuffer(5 * 7 * 4)
+    ops.linear(ops.DeviceTensor(bx.ptr, x.shape, "float32"), ops.DeviceTensor(bw.ptr, w.shape, "float32"),
+               ops.DeviceTensor(bo.ptr, (5, 7), "float32"))
+    torch.cuda.synchronize()
+    ref.check(torch.from_numpy(bo.to_array(np.float32, (5, 7))), ref.linear(torch.from_numpy(x), torch.from_numpy(w)))
+
+
+def test_refusals_leave_no_error_behind():
+    x, w, out = _rand(4, 16), _rand(8, 16), torch.empty(4, 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(nn.StringError, match="same device"):
+        ops.linear(x, w.cpu(), out)
+    with pytest.raises(nn.StringError, match="not on a GPU"):
+        ops.linear(x.cpu(), w, out)
+    p, _ = ops._linear_params(x, w, out, None, None, None, None)
+    assert ops._library().kgh_linear(99, p, None) == 1 and b"no device 99" in nn.hip_library().kgh_last_error()
+    assert nn.peek_last_error() == 0
+    ref.check(_linear(x, w, out), ref.linear(x, w))
