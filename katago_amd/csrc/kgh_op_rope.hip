@@ -27,18 +27,6 @@ __device__ __forceinline__ void sinCosTurns(float turns, float& s, float& c) {
   }
 }
 
-// n <= VEC elements of a 16-byte group to p, which is aligned to an element.
-template<typename T>
-__device__ __forceinline__ void storeGroup(T* p, const T (&v)[16 / sizeof(T)], int n) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  if(n >= VEC) __builtin_memcpy(p, v, 16);
-  else {
-#pragma unroll
-    for(int j = 0; j < VEC - 1; j++)
-      if(j < n) p[j] = v[j];
-  }
-}
-
 // A thread takes VEC pairs (two 16-byte groups) of a token, or as many of the
 // channels behind the pairs, and a run of heads that share a table: the angles
 // are computed once for the run.
@@ -113,8 +101,8 @@ __global__ __launch_bounds__(256) void ropeAxesKernel(RopeArgs a) {
         e1 = (T)y1;
       }
     }
-    storeGroup(dst + c0, u0.e, n0);
-    storeGroup(dst + c1, u1.e, n1);
+    storeGroup(dst + c0, u0.v, n0);
+    storeGroup(dst + c1, u1.v, n1);
   }
 }
 

@@ -6,6 +6,9 @@
 
 namespace {
 
+// 16 bytes as a vector value (HIP's uint4 is a struct, whose copies can end in memory).
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+
 // A 16-byte group of T, as loaded and as the matrix cores take it.
 template<typename T> struct Vec16;
 template<> struct Vec16<half_t> { typedef half8_t V; };
@@ -29,6 +32,48 @@ __device__ __forceinline__ uint4 loadGroup(const T* __restrict__ p, int n) {
       if(j < n) u.e[j] = p[j];
   }
   return u.v;
+}
+
+// A group's elements one place down or up, for the loops over part of a group
+// (a few instructions, where the cases written out would be the bulk of a kernel).
+template<typename T>
+__device__ __forceinline__ uint4 shiftDown(uint4 v) {
+  if constexpr(sizeof(T) == 4) return make_uint4(v.y, v.z, v.w, 0);
+  else return make_uint4(__builtin_amdgcn_alignbit(v.y, v.x, 16), __builtin_amdgcn_alignbit(v.z, v.y, 16), __builtin_amdgcn_alignbit(v.w, v.z, 16), v.w >> 16);
+}
+
+// The first n elements of a 16-byte group to p, which is aligned to an element.
+template<typename T>
+__device__ __forceinline__ void storeGroup(T* p, uint4 v, int n) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  if(n >= VEC) __builtin_memcpy(p, &v, 16);
+  else {
+#pragma unroll 1
+    for(int j = 0; j < n; j++) {
+      T e;
+      __builtin_memcpy(&e, &v.x, sizeof(T));
+      p[j] = e;
+      v = shiftDown<T>(v);
+    }
+  }
+}
+
+// loadGroup in few instructions, for the tails of epilogues.
+template<typename T>
+__device__ __forceinline__ uint4 loadGroupSmall(const T* __restrict__ p, int n) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if(n >= VEC) __builtin_memcpy(&v, p, 16);
+  else {
+#pragma unroll 1
+    for(int j = 0; j < VEC; j++) {  // element j enters at the top and moves down to its place
+      unsigned e = 0;
+      if(j < n) __builtin_memcpy(&e, p + j, sizeof(T));
+      v = shiftDown<T>(v);
+      v.w |= sizeof(T) == 4 ? e : e << 16;
+    }
+  }
+  return v;
 }
 
 // One 16-byte group of k per lane half times the other operand's: 32 x 32

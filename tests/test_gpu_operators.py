@@ -60,7 +60,9 @@ def _attention(q, k, v, out, **kw):
 # -- linear -------------------------------------------------------------------
 
 LINEAR_SIZES = [(1, 1, 1), (1, 384, 1024), (3, 40, 8), (1, 4104, 24), (7, 1000, 72), (16, 256, 64), (17, 264, 40), (31, 8, 33),
-                (33, 520, 129), (64, 64, 64), (65, 96, 257), (100, 33, 31), (129, 72, 63), (200, 1032, 136), (300, 17, 520)]
+                (33, 520, 129), (64, 64, 64), (65, 96, 257), (100, 33, 31), (129, 72, 63), (200, 1032, 136), (300, 17, 520),
+                # K split over workgroups, 128- and 256-row tiles, each with ends inside a tile and a step
+                (5, 12296, 40), (40, 8192, 24), (70, 4100, 72), (66, 2056, 65), (1900, 136, 1990), (1905, 1032, 6408)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
@@ -78,7 +80,7 @@ def test_linear_sizes(dtype, m, k, n):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("pad,shift", [(8, 0), (1, 0), (0, 1), (3, 5), (7, 8)])
-@pytest.mark.parametrize("m,k,n", [(5, 72, 40), (70, 200, 96)], ids=ids)
+@pytest.mark.parametrize("m,k,n", [(5, 72, 40), (70, 200, 96), (1800, 150, 1900)], ids=ids)
 def test_linear_strides(dtype, pad, shift, m, k, n):
     x, w = _rand(m, k, dtype=dtype, pad=pad, shift=shift), _rand(n, k, dtype=dtype, seed=1, scale=k ** -0.5, pad=pad, shift=shift)
     out, untouched = _guarded(m, n, dtype=dtype, pad=pad, shift=shift)

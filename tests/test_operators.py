@@ -54,6 +54,7 @@ def _linear(**change):
     (dict(weights=Meta(0, 16), out=Meta(4, 0)), "out_channels"), (dict(bias=Meta(8, dtype="float32", at=AT + 2)), "aligned"),
     (dict(x=Meta(1 << 31, 16, strides=(0, 1)), out=Meta(1 << 31, 8)), "longer"),
     (dict(x=Meta(1 << 30, 16, strides=(0, 1)), weights=Meta(1 << 20, 16), out=Meta(1 << 30, 1 << 20)), "too large"),
+    (dict(weights=Meta((1 << 26) + 1, 16), out=Meta(4, (1 << 26) + 1)), "out_channels"),
     (dict(workspace=Meta(64, dtype="uint8", device=1)), "workspace"), (dict(workspace=Meta(64, dtype="uint8", at=AT + 8)), "aligned"),
 ])
 def test_linear_refuses(change, word):
