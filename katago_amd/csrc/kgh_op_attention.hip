@@ -1,4 +1,5 @@
 // Attention to an encoder's states (kgh_cross_attention).
+#include "kgh_conv_device.h"
 #include "kgh_ops_device.h"
 
 #include <algorithm>
@@ -22,15 +23,67 @@ struct AttnArgs {
   float scaleLog2;  // scale * log2(e): exponents are taken to base 2
 };
 
-// Keys 64 tile .. + 63 that take part, lane l's key in bit l; wave-uniform.
-__device__ __forceinline__ unsigned long long validKeys(const AttnArgs& a, int b, int len, int k0) {
-  const int j = k0 + (int)(threadIdx.x & 63);
-  const bool on = j < len && (a.mask == nullptr || a.mask[b * a.maskB + j] != 0);
-  return __ballot(on);
-}
+// Where a split's sums go: [split][row][v dim] in fp32, then [split][row] pairs of
+// reference point and sum. Rows are counted over batch, kv head and (query, head
+// of the group).
+struct AttnSplit {
+  int splits;
+  float* out;   // null without a split
+  float* state;
+};
 
 __device__ __forceinline__ int validLength(const AttnArgs& a, int b) {
   return a.lengths == nullptr ? a.lk : min(max(a.lengths[b], 0), a.lk);
+}
+
+// ---------------------------------------------------------------------------
+// LDS layouts of key rows of D elements. K rows are read 16 bytes a lane, 16
+// consecutive rows a phase, the same group: the groups are permuted so that they
+// fall in distinct banks. V rows in 16 bits are read transposed, 8 bytes a lane,
+// four consecutive rows of 64 bytes a phase: 64-byte granules are permuted. V
+// rows in fp32 are read a float a lane, from rows 4 apart in the two lane halves.
+template<typename T, int D>
+__device__ __forceinline__ int kAt(int key, int group) {  // bytes
+  constexpr int GROUPS = D * (int)sizeof(T) / 16;
+  const int term = GROUPS >= 16 ? key : GROUPS == 8 ? key >> 1 : key >> 2;
+  return (key * GROUPS + (group ^ (term & (GROUPS - 1) & 15))) * 16;
+}
+template<typename T, int D>
+__device__ __forceinline__ int vAt(int key, int group) {
+  constexpr int GROUPS = D * (int)sizeof(T) / 16;
+  int term;
+  if constexpr(sizeof(T) == 4) term = D >= 64 ? ((key >> 2) & 1) * 8 : 0;
+  else term = GROUPS >= 16 ? (key & 3) * 4 : GROUPS == 8 ? ((key >> 1) & 1) * 4 : 0;
+  return (key * GROUPS + (group ^ term)) * 16;
+}
+
+// The V^T operand of keys base .. base + VEC / 4 * 8 - 1 (the accumulator's row
+// order: a lane half has keys half * 4 + {0..3}, + 8, ...) and dims d0 + laneRow.
+template<typename T, int D>
+__device__ __forceinline__ typename Vec16<T>::V readV(const unsigned char* vs, int base, int d0) {
+  const int lane = threadIdx.x & 63;
+  typename Vec16<T>::V v;
+  if constexpr(sizeof(T) == 4) {
+    const int key = base + (lane >> 5) * 4, d = d0 + (lane & 31);
+#pragma unroll
+    for(int j = 0; j < 4; j++) v[j] = *(const float*)(vs + vAt<T, D>(key + j, d >> 2) + (d & 3) * 4);
+  }
+  else {
+    // Sixteen lanes read four rows of 16 dims and get a column each.
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4v* Ptr;
+    const int key = base + (lane >> 5) * 4 + ((lane & 15) >> 2);
+    const int d = d0 + (lane & 16) + (lane & 3) * 4;
+    union {
+      short4v h[2];
+      typename Vec16<T>::V v;
+    } u;
+#pragma unroll
+    for(int h = 0; h < 2; h++)
+      u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(vs + vAt<T, D>(key + h * 8, d >> 3) + (d & 7) * 2));
+    v = u.v;
+  }
+  return v;
 }
 
 // One row's running softmax: p = 2^(s c - ref), with a reference point that only
@@ -40,40 +93,88 @@ struct RowState {
   float ref = -INFINITY, sum = 0.0f;
 };
 
+// The scores of BLOCKS * 32 keys become p; returns what the accumulators before
+// them are to be multiplied by. valid: bit per key.
+template<int BLOCKS>
+__device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], unsigned long long valid, float scaleLog2, RowState& row) {
+  const int half = (threadIdx.x & 63) >> 5;
+  if(valid != (BLOCKS == 2 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+    for(int kb = 0; kb < BLOCKS; kb++) {
+      const unsigned bits = (unsigned)(valid >> (kb * 32)) >> (half * 4);
+#pragma unroll
+      for(int i = 0; i < 16; i++)
+        if(!((bits >> ((i >> 2) * 8 + (i & 3))) & 1)) s[kb][i] = -INFINITY;
+    }
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for(int kb = 0; kb < BLOCKS; kb++)
+#pragma unroll
+    for(int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, s[kb][i]), s[kb][i + 1]);
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+  top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scaleLog2;
+  float corr = 1.0f;
+  if(top > row.ref + 8.0f) {
+    corr = __builtin_amdgcn_exp2f(row.ref - top);
+    row.ref = top;
+  }
+  // While a row has met no score above -inf its offset is 0: every p is 0.
+  const float off = row.ref == -INFINITY ? 0.0f : -row.ref;
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for(int kb = 0; kb < BLOCKS; kb++)
+#pragma unroll
+    for(int i = 0; i < 16; i++) {
+      s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scaleLog2, off));
+      part[i & 3] += s[kb][i];
+    }
+  const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+  row.sum = row.sum * corr + sum;  // of this lane half's keys; joined at the end
+  return corr;
+}
+
+// The two lane halves' sums.
+__device__ __forceinline__ float joinHalves(float v) { return v + __shfl_xor(v, 32); }
+
 // ---------------------------------------------------------------------------
-// Any sizes, strides and alignment. The rows of a kv head are (query, head of
-// the group) pairs, so that grouped heads share the keys that are staged. A wave
-// owns 32 rows and computes S^T = K Q^T (lane = row, 16 of 32 keys per lane), so
-// a row's softmax is in one lane and its partner lane ^ 32, and P^T is the
-// second product's operand as it stands: the key order inside that product's k
-// is the accumulator's row order, and V^T is read in the same order.
+// At most 32 rows a kv head: (query, head of the group) pairs, so that grouped
+// heads share the keys that are read. Bound by the keys' and values' bytes: each
+// of four waves goes through 32-key tiles of its own, the next tile's loads under
+// way while it computes, and nothing but the end makes waves wait for each other;
+// the keys are split over workgroups too where there are few. S^T = K Q^T (lane =
+// row, 16 of 32 keys), so that P^T is the second product's operand as it stands.
+// Here the matrix cores have time: P goes through them in two pieces, so that the
+// result is not off by P's rounding.
 template<typename T, int D>
-__global__ __launch_bounds__(256) void attentionTileKernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;
-  constexpr int VEC = 16 / (int)sizeof(T);
-  constexpr int KLD = D + VEC;                    // elements of a K row (16-byte gap)
-  constexpr int VLD = 64 + 8 / (int)sizeof(T);    // of a V^T row (8-byte gap)
-  constexpr int GROUPS = D / VEC;                 // 16-byte groups of a row
-  constexpr int LOADS = 64 * GROUPS / 256;
-  __shared__ __attribute__((aligned(16))) T Ks[64 * KLD];
-  __shared__ __attribute__((aligned(16))) T Vt[D * VLD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, LOADS = 32 * GROUPS / 64;
+  constexpr int ROWS_BYTES = 32 * D * (int)sizeof(T);
+  constexpr int OLD = 33;  // floats between dims of a wave's sums [dim][row]
+  constexpr int WAVE_BYTES = 2 * ROWS_BYTES > D * OLD * 4 ? 2 * ROWS_BYTES : D * OLD * 4;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4][WAVE_BYTES];
+  __shared__ float refs[4][32], totals[4][32];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int laneRow = lane & 31, half = lane >> 5;
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int group = a.heads / a.kvHeads;
   const int rows = a.lq * group;
-  const int r = ((int)blockIdx.x * 4 + wave) * 32 + laneRow;
-  const int rc = min(r, rows - 1);
-  const int qi = rc / group, h = kvh * group + (rc - qi * group);
-  const T* qRow = (const T*)a.q + b * a.qB + qi * a.qT + h * a.qH;
+  const int rc = min(laneRow, rows - 1);
+  const T* qRow = (const T*)a.q + b * a.qB + (int64_t)(rc / group) * a.qT + (int64_t)(kvh * group + rc % group) * a.qH;
   const T* kBase = (const T*)a.k + b * a.kB + kvh * a.kH;
   const T* vBase = (const T*)a.v + b * a.vB + kvh * a.vH;
+  const int len = validLength(a, b);
+  const int tiles = (len + 31) / 32;
+  const int first = (int)((int64_t)tiles * blockIdx.x / split.splits) + wave;
+  const int end = (int)((int64_t)tiles * (blockIdx.x + 1) / split.splits);
 
   V qf[D / VEC / 2];
 #pragma unroll
   for(int i = 0; i < D / VEC / 2; i++) {
     const int c = (2 * i + half) * VEC;
-    const uint4 u = loadGroup(qRow + c, a.dq - c);
+    const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
     qf[i] = *(const V*)&u;
   }
   floatx16 o[D / 32];
@@ -83,75 +184,215 @@ __global__ __launch_bounds__(256) void attentionTileKernel(AttnArgs a) {
     for(int i = 0; i < 16; i++) o[db][i] = 0.0f;
   RowState row;
 
-  const int len = validLength(a, b);
-  for(int k0 = 0; k0 < len; k0 += 64) {
-    const unsigned long long valid = validKeys(a, b, len, k0);
-    if(valid == 0) continue;  // the same for every wave
-    uint4 kr[LOADS], vr[LOADS];
+  // A tile's rows in registers: lane's group lane % GROUPS of keys lane / GROUPS + ...
+  const int lg = lane % GROUPS, lk = lane / GROUPS;
+  const RowGroup<T> kGroup(lg, a.dq), vGroup(lg, a.dv);
+  struct Rows {
+    u32x4_t k[LOADS], v[LOADS];
+    unsigned long long mask;
+  };
+  auto load = [&](int tile, Rows& r) {
+    const int k0 = min(tile, end - 1) * 32;
+    const int key = k0 + laneRow;
+    r.mask = a.mask != nullptr && key < len ? a.mask[b * a.maskB + key] : 1;
 #pragma unroll
     for(int i = 0; i < LOADS; i++) {
-      const int key = (tid + i * 256) / GROUPS, c = (tid + i * 256) % GROUPS * VEC;
-      const bool on = (valid >> key) & 1;
-      kr[i] = loadGroup(kBase + (k0 + key) * a.kT + c, on ? a.dq - c : 0);
-      vr[i] = loadGroup(vBase + (k0 + key) * a.vT + c, on ? a.dv - c : 0);
+      const int64_t at = min(k0 + lk + i * (64 / GROUPS), len - 1);
+      r.k[i] = kGroup.load(kBase + at * a.kT);
+      r.v[i] = vGroup.load(vBase + at * a.vT);
     }
-    __syncthreads();
+  };
+  unsigned char* ks = lds[wave];
+  unsigned char* vs = lds[wave] + ROWS_BYTES;
+  Rows r;
+  if(first < end) load(first, r);
+  for(int t = first; t < end; t += 4) {
+    const unsigned valid = (unsigned)__ballot(r.mask != 0 && t * 32 + laneRow < len);
+    asm volatile("" ::: "memory");  // a wave's LDS accesses run in order
 #pragma unroll
     for(int i = 0; i < LOADS; i++) {
-      const int key = (tid + i * 256) / GROUPS, c = (tid + i * 256) % GROUPS * VEC;
-      *(uint4*)&Ks[key * KLD + c] = kr[i];
-      const T* e = (const T*)&vr[i];
-#pragma unroll
-      for(int j = 0; j < VEC; j++) Vt[(c + j) * VLD + key] = e[j];
+      const int key = lk + i * (64 / GROUPS);
+      const u32x4_t zero = {0, 0, 0, 0};
+      *(u32x4_t*)(ks + kAt<T, D>(key, lg)) = kGroup.place(r.k[i], a.dq == D);
+      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (valid >> key) & 1 ? vGroup.place(r.v[i], a.dv == D) : zero;
     }
-    __syncthreads();
-
-    floatx16 s[2];
+    asm volatile("" ::: "memory");
+    load(t + 4, r);
+    floatx16 s[1];
 #pragma unroll
-    for(int kb = 0; kb < 2; kb++) {
+    for(int i = 0; i < 16; i++) s[0][i] = 0.0f;
 #pragma unroll
-      for(int i = 0; i < 16; i++) s[kb][i] = 0.0f;
-#pragma unroll
-      for(int i = 0; i < D / VEC / 2; i++) {
-        const V kf = *(const V*)&Ks[(kb * 32 + laneRow) * KLD + (2 * i + half) * VEC];
-        s[kb] = mma32(kf, qf[i], s[kb]);
-      }
-      if(valid != ~0ull) {
-#pragma unroll
-        for(int i = 0; i < 16; i++)
-          if(!((valid >> (kb * 32 + (i >> 2) * 8 + half * 4 + (i & 3))) & 1)) s[kb][i] = -INFINITY;
-      }
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for(int kb = 0; kb < 2; kb++)
-#pragma unroll
-      for(int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
-    top = fmaxf(top, __shfl_xor(top, 32)) * a.scaleLog2;
-    float corr = 1.0f;
-    if(top > row.ref + 8.0f) {
-      corr = __builtin_amdgcn_exp2f(row.ref - top);
-      row.ref = top;
-    }
-    // While a row has met no score above -inf its offset is 0: every p is 0.
-    const float off = row.ref == -INFINITY ? 0.0f : -row.ref;
-    float sum = 0.0f;
-#pragma unroll
-    for(int kb = 0; kb < 2; kb++)
-#pragma unroll
-      for(int i = 0; i < 16; i++) {
-        s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], a.scaleLog2, off));
-        sum += s[kb][i];
-      }
-    sum += __shfl_xor(sum, 32);
-    row.sum = row.sum * corr + sum;
+    for(int i = 0; i < D / VEC / 2; i++) s[0] = mma32(*(const V*)(ks + kAt<T, D>(laneRow, 2 * i + half)), qf[i], s[0]);
+    const float corr = softmaxTile<1>(s, valid, a.scaleLog2, row);
     if(__any(corr != 1.0f)) {
 #pragma unroll
       for(int db = 0; db < D / 32; db++)
 #pragma unroll
         for(int i = 0; i < 16; i++) o[db][i] *= corr;
     }
-    // VEC accumulator rows per 16-byte group of keys.
+#pragma unroll
+    for(int g = 0; g < 16 / VEC; g++) {
+      V hi, lo;
+#pragma unroll
+      for(int i = 0; i < VEC; i++) {
+        hi[i] = (T)s[0][g * VEC + i];
+        lo[i] = (T)(s[0][g * VEC + i] - (float)hi[i]);
+      }
+#pragma unroll
+      for(int db = 0; db < D / 32; db++) {
+        const V vf = readV<T, D>(vs, g * VEC / 4 * 8, db * 32);
+        o[db] = mma32(vf, hi, o[db]);
+        if constexpr(sizeof(T) == 2) o[db] = mma32(vf, lo, o[db]);
+      }
+    }
+  }
+
+  // The waves' sums, on one reference point.
+  row.sum = joinHalves(row.sum);
+  if(half == 0) {
+    refs[wave][laneRow] = row.ref;
+    totals[wave][laneRow] = row.sum;
+  }
+  __syncthreads();
+  float ref = -INFINITY;
+#pragma unroll
+  for(int w = 0; w < 4; w++) ref = fmaxf(ref, refs[w][laneRow]);
+  const float mine = row.ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(row.ref - ref);
+  float* sums = (float*)lds[wave];
+#pragma unroll
+  for(int db = 0; db < D / 32; db++)
+#pragma unroll
+    for(int i = 0; i < 16; i++) sums[(db * 32 + (i >> 2) * 8 + half * 4 + (i & 3)) * OLD + laneRow] = o[db][i] * mine;
+  __syncthreads();
+  for(int e = tid; e < rows * a.dv; e += 256) {
+    const int m = e / a.dv, d = e - m * a.dv;
+    float top = -INFINITY, total = 0.0f, v = 0.0f;
+#pragma unroll
+    for(int w = 0; w < 4; w++) top = fmaxf(top, refs[w][m]);
+#pragma unroll
+    for(int w = 0; w < 4; w++) {
+      total += refs[w][m] == -INFINITY ? totals[w][m] : totals[w][m] * __builtin_amdgcn_exp2f(refs[w][m] - top);
+      v += ((const float*)lds[w])[d * OLD + m];
+    }
+    if(split.out != nullptr) {
+      const int64_t at = ((int64_t)blockIdx.x * gridDim.z + b) * a.kvHeads * rows + (int64_t)kvh * rows + m;
+      split.out[at * a.dv + d] = v;
+      if(d == 0) {
+        split.state[at * 2] = top;
+        split.state[at * 2 + 1] = total;
+      }
+    }
+    else {
+      T* out = (T*)a.out + b * a.oB + (int64_t)(m / group) * a.oT + (int64_t)(kvh * group + m % group) * a.oH;
+      out[d] = (T)(total == 0.0f ? 0.0f : v / total);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of WAVES waves has 32 rows a wave of one kv head, and
+// goes through 64-key tiles that all of them read from LDS. Of tile t + 1 the
+// scores are computed before tile t's softmax, so that the matrix cores have them
+// to do while the vector units work; a tile's rows are loaded into registers two
+// barriers before they are read.
+constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
+
+template<typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, AttnSplit split) {
+  typedef typename Vec16<T>::V V;
+  constexpr int THREADS = 64 * WAVES;
+  constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, LOADS = 64 * GROUPS / THREADS;
+  static_assert(LOADS * THREADS == 64 * GROUPS && THREADS % GROUPS == 0, "whole loads");
+  constexpr int TILE = 64 * D * (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) unsigned char k0s[TILE];
+  __shared__ __attribute__((aligned(16))) unsigned char k1s[TILE];
+  __shared__ __attribute__((aligned(16))) unsigned char v0s[TILE];
+  __shared__ __attribute__((aligned(16))) unsigned char v1s[TILE];
+  // Tiles with a key that takes part, and which keys (bits), in order.
+  __shared__ unsigned long long listBits[ATT_LIST + 1];
+  __shared__ int listTile[ATT_LIST];
+  __shared__ int listCount;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int laneRow = lane & 31, half = lane >> 5;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int group = a.heads / a.kvHeads;
+  const int rows = a.lq * group;
+  const int rowBlock = blockIdx.x / split.splits, part = blockIdx.x - rowBlock * split.splits;
+  const int r = (rowBlock * WAVES + wave) * 32 + laneRow;
+  const int rc = min(r, rows - 1);
+  const int qi = rc / group, h = kvh * group + (rc - qi * group);
+  const T* qRow = (const T*)a.q + b * a.qB + qi * a.qT + h * a.qH;
+  const T* kBase = (const T*)a.k + b * a.kB + kvh * a.kH;
+  const T* vBase = (const T*)a.v + b * a.vB + kvh * a.vH;
+  const int len = validLength(a, b);
+  const int allTiles = (len + 63) / 64;
+  const int begin = (int)((int64_t)allTiles * part / split.splits), end = (int)((int64_t)allTiles * (part + 1) / split.splits);
+
+  V qf[D / VEC / 2];
+#pragma unroll
+  for(int i = 0; i < D / VEC / 2; i++) {
+    const int c = (2 * i + half) * VEC;
+    const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
+    qf[i] = *(const V*)&u;
+  }
+  floatx16 o[D / 32];
+#pragma unroll
+  for(int db = 0; db < D / 32; db++)
+#pragma unroll
+    for(int i = 0; i < 16; i++) o[db][i] = 0.0f;
+  RowState row;
+
+  const int lg = tid % GROUPS, lk = tid / GROUPS;
+  const RowGroup<T> kGroup(lg, a.dq), vGroup(lg, a.dv);
+  struct Rows {
+    u32x4_t v[LOADS];
+  };
+  int count = 0, from = begin;  // tiles of this round, and its first
+  // What item i of the round is: a tile, and which of its keys take part.
+  auto tileOf = [&](int i) { return a.mask == nullptr ? from + i : listTile[i]; };
+  auto bitsOf = [&](int i) -> unsigned long long {
+    if(a.mask != nullptr) {
+      const unsigned long long v = listBits[i];
+      return ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+    }
+    const int n = len - (from + i) * 64;
+    return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
+  };
+  auto load = [&](const T* base, int64_t stride, const RowGroup<T>& g, int i, Rows& x) {
+    const int k0 = tileOf(min(i, count - 1)) * 64;
+#pragma unroll
+    for(int j = 0; j < LOADS; j++) {
+      const int64_t at = min(k0 + lk + j * (THREADS / GROUPS), len - 1);
+      x.v[j] = g.load(base + at * stride);
+    }
+  };
+  auto loadK = [&](int i, Rows& x) { load(kBase, a.kT, kGroup, i, x); };
+  auto loadV = [&](int i, Rows& x) { load(vBase, a.vT, vGroup, i, x); };
+  auto stageK = [&](unsigned char* ks, const Rows& x) {
+#pragma unroll
+    for(int j = 0; j < LOADS; j++) *(u32x4_t*)(ks + kAt<T, D>(lk + j * (THREADS / GROUPS), lg)) = kGroup.place(x.v[j], a.dq == D);
+  };
+  // What V holds at keys that take no part must not meet their p of 0.
+  auto stageV = [&](unsigned char* vs, const Rows& x, unsigned long long bits) {
+#pragma unroll
+    for(int j = 0; j < LOADS; j++) {
+      const int key = lk + j * (THREADS / GROUPS);
+      const u32x4_t zero = {0, 0, 0, 0};
+      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (bits >> key) & 1 ? vGroup.place(x.v[j], a.dv == D) : zero;
+    }
+  };
+  auto scores = [&](const unsigned char* ks, floatx16 (&s)[2]) {
+#pragma unroll
+    for(int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for(int i = 0; i < 16; i++) s[kb][i] = 0.0f;
+#pragma unroll
+    for(int i = 0; i < D / VEC / 2; i++)
+#pragma unroll
+      for(int kb = 0; kb < 2; kb++) s[kb] = mma32(*(const V*)(ks + kAt<T, D>(kb * 32 + laneRow, 2 * i + half)), qf[i], s[kb]);
+  };
+  auto values = [&](const unsigned char* vs, const floatx16 (&s)[2]) {
 #pragma unroll
     for(int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -160,28 +401,145 @@ __global__ __launch_bounds__(256) void attentionTileKernel(AttnArgs a) {
 #pragma unroll
         for(int i = 0; i < VEC; i++) pf[i] = (T)s[kb][g * VEC + i];
 #pragma unroll
-        for(int db = 0; db < D / 32; db++) {
-          V vf;
-          const T* vRow = &Vt[(db * 32 + laneRow) * VLD + kb * 32 + half * 4];
-#pragma unroll
-          for(int q = 0; q < VEC / 4; q++)
-#pragma unroll
-            for(int i = 0; i < 4; i++) vf[q * 4 + i] = vRow[(g * VEC / 4 + q) * 8 + i];
-          o[db] = mma32(vf, pf, o[db]);
-        }
+        for(int db = 0; db < D / 32; db++) o[db] = mma32(readV<T, D>(vs, kb * 32 + g * VEC / 4 * 8, db * 32), pf, o[db]);
       }
+  };
+  Rows kr, vr;
+  // Item i: its scores are in s; K of i + 1 and V of i are in LDS, K of i + 2 and V
+  // of i + 1 in registers.
+  auto step = [&](int i, floatx16 (&s)[2], floatx16 (&sNext)[2], unsigned char* kNow, const unsigned char* kNext, const unsigned char* vNow,
+                  unsigned char* vNext) {
+    const unsigned long long bits = bitsOf(i), bitsNext = bitsOf(min(i + 1, count - 1));
+    scores(kNext, sNext);
+    const float corr = softmaxTile<2>(s, bits, a.scaleLog2, row);
+    if(__any(corr != 1.0f)) {
+#pragma unroll
+      for(int db = 0; db < D / 32; db++)
+#pragma unroll
+        for(int j = 0; j < 16; j++) o[db][j] *= corr;
+    }
+    values(vNow, s);
+    stageK(kNow, kr);
+    stageV(vNext, vr, bitsNext);
+    loadK(i + 3, kr);
+    loadV(i + 2, vr);
+    barrierLds();
+  };
+
+  for(; from < end; from += ATT_LIST) {
+    count = min(ATT_LIST, end - from);
+    if(a.mask != nullptr) {
+      __syncthreads();
+      for(int t = wave; t < count; t += WAVES) {
+        const int j = (from + t) * 64 + lane;
+        const unsigned long long bits = __ballot(j < len && a.mask[b * a.maskB + j] != 0);
+        if(lane == 0) listBits[t] = bits;
+      }
+      __syncthreads();
+      if(wave == 0) {
+        int n = 0;
+        for(int t0 = 0; t0 < count; t0 += 64) {
+          const unsigned long long bits = t0 + lane < count ? listBits[t0 + lane] : 0;
+          const unsigned long long on = __ballot(bits != 0);
+          const int at = n + __popcll(on & ((1ull << lane) - 1));
+          // Entries move down only, and the 64 of a round are read before any is written.
+          if(bits != 0) {
+            listBits[at] = bits;
+            listTile[at] = from + t0 + lane;
+          }
+          n += __popcll(on);
+        }
+        if(lane == 0) listCount = n;
+      }
+      __syncthreads();
+      count = listCount;
+      if(count == 0) continue;
+    }
+    loadK(0, kr);
+    loadV(0, vr);
+    __syncthreads();  // the buffers' readers of the round before
+    stageK(k0s, kr);
+    stageV(v0s, vr, bitsOf(0));
+    loadK(1, kr);
+    __syncthreads();
+    floatx16 sA[2], sB[2];
+    scores(k0s, sA);
+    stageK(k1s, kr);
+    loadK(2, kr);
+    loadV(1, vr);
+    __syncthreads();
+    int i = 0;
+    for(; i + 2 <= count; i += 2) {
+      step(i, sA, sB, k0s, k1s, v0s, v1s);
+      step(i + 1, sB, sA, k1s, k0s, v1s, v0s);
+    }
+    if(i < count) step(i, sA, sB, k0s, k1s, v0s, v1s);
   }
 
+  row.sum = joinHalves(row.sum);
   if(r >= rows) return;
+  if(split.out != nullptr) {
+    const int64_t at = ((int64_t)part * gridDim.z + b) * a.kvHeads * rows + (int64_t)kvh * rows + r;
+    if(half == 0) {
+      split.state[at * 2] = row.ref;
+      split.state[at * 2 + 1] = row.sum;
+    }
+#pragma unroll
+    for(int db = 0; db < D / 32; db++)
+#pragma unroll
+      for(int q = 0; q < 4; q++) {
+        const int d = db * 32 + q * 8 + half * 4;
+        const floatx4 v = {o[db][q * 4], o[db][q * 4 + 1], o[db][q * 4 + 2], o[db][q * 4 + 3]};
+        if(d < a.dv) storeGroup(split.out + at * a.dv + d, *(const uint4*)&v, a.dv - d);
+      }
+    return;
+  }
   const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
   T* oRow = (T*)a.out + b * a.oB + qi * a.oT + h * a.oH;
 #pragma unroll
   for(int db = 0; db < D / 32; db++)
 #pragma unroll
-    for(int i = 0; i < 16; i++) {
-      const int d = db * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
-      if(d < a.dv) oRow[d] = (T)(o[db][i] * inv);
+    for(int q = 0; q < 4; q++) {
+      const int d = db * 32 + q * 8 + half * 4;
+#pragma unroll
+      for(int i = 0; i < 4; i++)
+        if(d + i < a.dv) oRow[d + i] = (T)(o[db][q * 4 + i] * inv);
     }
+}
+
+// The splits' sums on one reference point, a thread four dims of a row.
+template<typename T>
+__global__ __launch_bounds__(256) void attentionJoinKernel(AttnArgs a, AttnSplit split, int64_t rowsAll) {
+  const int quads = (a.dv + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r = id / quads;
+  if(r >= rowsAll) return;
+  const int d = (int)(id - r * quads) * 4, n = min(4, a.dv - d);
+  float top = -INFINITY;
+  for(int s = 0; s < split.splits; s++) top = fmaxf(top, split.state[(s * rowsAll + r) * 2]);
+  float total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for(int s = 0; s < split.splits; s++) {
+    const float* st = split.state + (s * rowsAll + r) * 2;
+    const float f = st[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st[0] - top);
+    const uint4 u = loadGroup(split.out + (s * rowsAll + r) * a.dv + d, n);
+    total = fmaf(st[1], f, total);
+    v[0] = fmaf(__uint_as_float(u.x), f, v[0]);
+    v[1] = fmaf(__uint_as_float(u.y), f, v[1]);
+    v[2] = fmaf(__uint_as_float(u.z), f, v[2]);
+    v[3] = fmaf(__uint_as_float(u.w), f, v[3]);
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  // r counts batch, kv head, query, head of the group.
+  const int group = a.heads / a.kvHeads;
+  const int64_t rows = (int64_t)a.lq * group, outer = r / rows;
+  const int at = (int)(r - outer * rows);
+  const int64_t b = outer / a.kvHeads;
+  const int h = (int)(outer - b * a.kvHeads) * group + at % group;
+  T* out = (T*)a.out + b * a.oB + (int64_t)(at / group) * a.oT + h * a.oH + d;
+#pragma unroll
+  for(int j = 0; j < 4; j++)
+    if(j < n) out[j] = (T)(v[j] * inv);
 }
 
 }  // namespace
@@ -224,7 +582,61 @@ void checkAttention(const kgh_attention_params& p, bool pointers) {
   if(p.workspace != nullptr) opCheckPointer(op, "workspace", p.workspace, 16);
 }
 
-uint64_t attentionWorkspace(const kgh_attention_params&) { return 0; }
+namespace {
+
+struct AttentionPlan {
+  bool few;   // at most 32 rows a kv head
+  int waves;  // of the kernel for more
+  int splits; // of the keys
+  int64_t rows;
+};
+
+// Which kernel runs, and in how many splits of the keys with `bytes` of workspace.
+AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
+  AttentionPlan plan;
+  const int64_t rows = (int64_t)p.q_len * (p.heads / p.kv_heads);
+  plan.rows = rows * p.batch * p.kv_heads;
+  plan.few = rows <= 32;
+  plan.waves = rows <= 128 || p.dtype == KGH_DTYPE_FP32 ? 4 : 8;
+  const int64_t groups = plan.few ? (int64_t)p.batch * p.kv_heads : (rows + plan.waves * 32 - 1) / (plan.waves * 32) * p.batch * p.kv_heads;
+  const int64_t wanted = plan.few ? 1024 : 256;
+  int64_t splits = std::min<int64_t>({wanted / groups, p.k_len / 256, 64});
+  const uint64_t one = (uint64_t)plan.rows * (p.v_head_dim + 2) * 4;
+  splits = std::min<int64_t>(splits, (int64_t)std::min<uint64_t>(bytes / one, 64));
+  plan.splits = (int)std::max<int64_t>(1, splits);
+  return plan;
+}
+
+template<typename T, int D>
+void runAttention(const AttentionPlan& plan, const AttnArgs& a, const AttnSplit& split, int batch, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.lq * (a.heads / a.kvHeads);
+  if(plan.few) attentionFewKernel<T, D><<<dim3((unsigned)plan.splits, (unsigned)a.kvHeads, (unsigned)batch), 256, 0, stream>>>(a, split);
+  else {
+    const int64_t blocks = (rows + plan.waves * 32 - 1) / (plan.waves * 32);
+    const dim3 grid((unsigned)(blocks * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
+    if(sizeof(T) == 2 && D >= 64 && plan.waves == 8) {
+      if constexpr(sizeof(T) == 2 && D >= 64) attentionManyKernel<T, D, 8><<<grid, 512, 0, stream>>>(a, split);
+    }
+    else {
+      const dim3 grid4((unsigned)((rows + 127) / 128 * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
+      attentionManyKernel<T, D, 4><<<grid4, 256, 0, stream>>>(a, split);
+    }
+  }
+  KGH_CHECK_LAUNCH();
+  if(plan.splits > 1) {
+    const int64_t threads = plan.rows * ((a.dv + 3) / 4);
+    attentionJoinKernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, stream>>>(a, split, plan.rows);
+    KGH_CHECK_LAUNCH();
+  }
+}
+
+}  // namespace
+
+uint64_t attentionWorkspace(const kgh_attention_params& p) {
+  if(p.batch == 0 || p.q_len == 0) return 0;
+  const AttentionPlan plan = planAttention(p, UINT64_MAX);
+  return plan.splits > 1 ? (uint64_t)plan.splits * plan.rows * (p.v_head_dim + 2) * 4 : 0;
+}
 
 void launchAttention(const kgh_attention_params& p, hipStream_t stream) {
   if(p.batch == 0 || p.q_len == 0) return;
@@ -247,16 +659,19 @@ void launchAttention(const kgh_attention_params& p, hipStream_t stream) {
   a.dq = p.q_head_dim;
   a.dv = p.v_head_dim;
   a.scaleLog2 = p.scale * 1.44269504088896341f;
-  const int64_t rows = (int64_t)p.q_len * (p.heads / p.kv_heads);
-  const dim3 grid((unsigned)((rows + 127) / 128), (unsigned)p.kv_heads, (unsigned)p.batch);
+  const AttentionPlan plan = planAttention(p, p.workspace != nullptr ? p.workspace_bytes : 0);
+  AttnSplit split{plan.splits, nullptr, nullptr};
+  if(plan.splits > 1) {
+    split.out = (float*)p.workspace;
+    split.state = split.out + (size_t)plan.splits * plan.rows * p.v_head_dim;
+  }
   const int d = std::max(p.q_head_dim, p.v_head_dim);
   withDtype(p.dtype, [&](auto t) {
     typedef decltype(t) T;
-    if(d <= 32) attentionTileKernel<T, 32><<<grid, 256, 0, stream>>>(a);
-    else if(d <= 64) attentionTileKernel<T, 64><<<grid, 256, 0, stream>>>(a);
-    else attentionTileKernel<T, 128><<<grid, 256, 0, stream>>>(a);
+    if(d <= 32) runAttention<T, 32>(plan, a, split, p.batch, stream);
+    else if(d <= 64) runAttention<T, 64>(plan, a, split, p.batch, stream);
+    else runAttention<T, 128>(plan, a, split, p.batch, stream);
   });
-  KGH_CHECK_LAUNCH();
 }
 
 }  // namespace kgh

@@ -59,13 +59,6 @@ __device__ __forceinline__ void blockedTile(int rowTiles, int colTiles, int& row
   rowTile = run * 8 + (at - colTile * height);
 }
 
-// A workgroup barrier for LDS alone: __syncthreads() would wait for the loads that
-// are to arrive during the next step too.
-__device__ __forceinline__ void barrierLds() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  barrierNoFence();
-}
-
 // XOR swizzle of a row's eight 16-byte groups: the rows that a ds_read_b128 phase
 // reads (eight consecutive ones, the same group) fall in distinct banks.
 __device__ __forceinline__ int swizzled128(int row, int group) { return row * 128 + ((group ^ (row & 7)) << 4); }

@@ -2,6 +2,7 @@
 #ifndef KGH_OPS_DEVICE_H
 #define KGH_OPS_DEVICE_H
 
+#include "kgh_conv_device.h"
 #include "kgh_ops.h"
 
 namespace {
@@ -74,6 +75,54 @@ __device__ __forceinline__ uint4 loadGroupSmall(const T* __restrict__ p, int n) 
     }
   }
   return v;
+}
+
+// Groups of rows of `dims` elements, group `g` a lane, in two steps, so that loads
+// stay in flight (a load under a lane's own condition makes the compiler wait
+// where its register is cleared first): load() reads 16 bytes that lie in the row
+// wherever the group ends, place() puts the group's elements in their places and
+// zeros behind the row's end.
+template<typename T>
+struct RowGroup {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  int at;      // first element read
+  int excess;  // elements to drop: VEC where the whole group lies behind the row
+  int dims;
+  __device__ __forceinline__ RowGroup(int g, int d) {
+    dims = d;
+    at = max(0, min(g * VEC, d - VEC));
+    excess = min(VEC, g * VEC - at);
+  }
+  __device__ __forceinline__ u32x4_t load(const T* __restrict__ row) const {
+    u32x4_t v;
+    if(dims >= VEC) __builtin_memcpy(&v, row + at, 16);
+    else {
+      const uint4 u = loadGroupSmall(row, dims);
+      v = u32x4_t{u.x, u.y, u.z, u.w};
+    }
+    return v;
+  }
+  // full: the rows are as long as the groups of all lanes.
+  __device__ __forceinline__ u32x4_t place(u32x4_t v, bool full) const {
+    if(!full) {
+      if(dims % VEC != 0 && excess < VEC) {
+        uint4 u = make_uint4(v.x, v.y, v.z, v.w);
+#pragma unroll 1
+        for(int i = 0; i < excess; i++) u = shiftDown<T>(u);
+        v = u32x4_t{u.x, u.y, u.z, u.w};
+      }
+      const u32x4_t zero = {0, 0, 0, 0};
+      v = excess >= VEC ? zero : v;
+    }
+    return v;
+  }
+};
+
+// A workgroup barrier for LDS alone: __syncthreads() would wait for the loads that
+// are to arrive during the next step too.
+__device__ __forceinline__ void barrierLds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  barrierNoFence();
 }
 
 // One 16-byte group of k per lane half times the other operand's: 32 x 32
