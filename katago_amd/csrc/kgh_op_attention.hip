@@ -57,34 +57,49 @@ __device__ __forceinline__ int vAt(int key, int group) {
   return (key * GROUPS + (group ^ term)) * 16;
 }
 
-// The V^T operand of keys base .. base + VEC / 4 * 8 - 1 (the accumulator's row
-// order: a lane half has keys half * 4 + {0..3}, + 8, ...) and dims d0 + laneRow.
+// Where a lane reads its V^T operands: of keys base .. base + VEC / 4 * 8 - 1 (base
+// a multiple of 8, in the accumulator's row order: a lane half has keys half * 4 +
+// {0..3}, + 8, ...) and dims 32 db + laneRow. One offset for each db; what is added
+// for base is a constant.
 template<typename T, int D>
-__device__ __forceinline__ typename Vec16<T>::V readV(const unsigned char* vs, int base, int d0) {
-  const int lane = threadIdx.x & 63;
-  typename Vec16<T>::V v;
-  if constexpr(sizeof(T) == 4) {
-    const int key = base + (lane >> 5) * 4, d = d0 + (lane & 31);
+struct ValueReads {
+  int at[D / 32];
+  __device__ __forceinline__ ValueReads() {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for(int j = 0; j < 4; j++) v[j] = *(const float*)(vs + vAt<T, D>(key + j, d >> 2) + (d & 3) * 4);
+    for(int db = 0; db < D / 32; db++) {
+      if constexpr(sizeof(T) == 4) {
+        const int d = db * 32 + (lane & 31);
+        at[db] = vAt<T, D>((lane >> 5) * 4, d >> 2) + (d & 3) * 4;
+      }
+      else {
+        // Sixteen lanes read four rows of 16 dims and get a column each.
+        const int d = db * 32 + (lane & 16) + (lane & 3) * 4;
+        at[db] = vAt<T, D>((lane >> 5) * 4 + ((lane & 15) >> 2), d >> 3) + (d & 7) * 2;
+      }
+    }
   }
-  else {
-    // Sixteen lanes read four rows of 16 dims and get a column each.
-    typedef short short4v __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) short4v* Ptr;
-    const int key = base + (lane >> 5) * 4 + ((lane & 15) >> 2);
-    const int d = d0 + (lane & 16) + (lane & 3) * 4;
-    union {
-      short4v h[2];
-      typename Vec16<T>::V v;
-    } u;
+  __device__ __forceinline__ typename Vec16<T>::V read(const unsigned char* vs, int base, int db) const {
+    constexpr int ROW = D * (int)sizeof(T);
+    typename Vec16<T>::V v;
+    if constexpr(sizeof(T) == 4) {
 #pragma unroll
-    for(int h = 0; h < 2; h++)
-      u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(vs + vAt<T, D>(key + h * 8, d >> 3) + (d & 7) * 2));
-    v = u.v;
+      for(int j = 0; j < 4; j++) v[j] = *(const float*)(vs + at[db] + (base + j) * ROW);
+    }
+    else {
+      typedef short short4v __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) short4v* Ptr;
+      union {
+        short4v h[2];
+        typename Vec16<T>::V v;
+      } u;
+#pragma unroll
+      for(int h = 0; h < 2; h++) u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(vs + at[db] + (base + h * 8) * ROW));
+      v = u.v;
+    }
+    return v;
   }
-  return v;
-}
+};
 
 // One row's running softmax: p = 2^(s c - ref), with a reference point that only
 // moves when a tile's maximum passes it by more than 8 (p is at most 256, summed
@@ -93,10 +108,9 @@ struct RowState {
   float ref = -INFINITY, sum = 0.0f;
 };
 
-// The scores of BLOCKS * 32 keys become p; returns what the accumulators before
-// them are to be multiplied by. valid: bit per key.
+// Scores of keys that take no part become minus infinity. valid: bit per key.
 template<int BLOCKS>
-__device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], unsigned long long valid, float scaleLog2, RowState& row) {
+__device__ __forceinline__ void maskTile(floatx16 (&s)[BLOCKS], unsigned long long valid) {
   const int half = (threadIdx.x & 63) >> 5;
   if(valid != (BLOCKS == 2 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
@@ -107,6 +121,12 @@ __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], unsigned lon
         if(!((bits >> ((i >> 2) * 8 + (i & 3))) & 1)) s[kb][i] = -INFINITY;
     }
   }
+}
+
+// The scores of BLOCKS * 32 keys become p; returns what the accumulators before
+// them are to be multiplied by.
+template<int BLOCKS>
+__device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], float scaleLog2, RowState& row) {
   float top = -INFINITY;
 #pragma unroll
   for(int kb = 0; kb < BLOCKS; kb++)
@@ -114,13 +134,11 @@ __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], unsigned lon
     for(int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, s[kb][i]), s[kb][i + 1]);
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
   top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scaleLog2;
-  float corr = 1.0f;
-  if(top > row.ref + 8.0f) {
-    corr = __builtin_amdgcn_exp2f(row.ref - top);
-    row.ref = top;
-  }
+  const float ref = top > row.ref + 8.0f ? top : row.ref;
+  const float corr = ref == row.ref ? 1.0f : __builtin_amdgcn_exp2f(row.ref - ref);
+  row.ref = ref;
   // While a row has met no score above -inf its offset is 0: every p is 0.
-  const float off = row.ref == -INFINITY ? 0.0f : -row.ref;
+  const float off = ref == -INFINITY ? 0.0f : -ref;
   float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for(int kb = 0; kb < BLOCKS; kb++)
@@ -129,8 +147,7 @@ __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], unsigned lon
       s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scaleLog2, off));
       part[i & 3] += s[kb][i];
     }
-  const float sum = (part[0] + part[1]) + (part[2] + part[3]);
-  row.sum = row.sum * corr + sum;  // of this lane half's keys; joined at the end
+  row.sum = row.sum * corr + ((part[0] + part[1]) + (part[2] + part[3]));  // of this lane half's keys; joined at the end
   return corr;
 }
 
@@ -146,8 +163,8 @@ __device__ __forceinline__ float joinHalves(float v) { return v + __shfl_xor(v, 
 // row, 16 of 32 keys), so that P^T is the second product's operand as it stands.
 // Here the matrix cores have time: P goes through them in two pieces, so that the
 // result is not off by P's rounding.
-template<typename T, int D>
-__global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit split) {
+template<typename T, int D, bool FULL>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;
   constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, LOADS = 32 * GROUPS / 64;
   constexpr int ROWS_BYTES = 32 * D * (int)sizeof(T);
@@ -186,7 +203,7 @@ __global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit 
 
   // A tile's rows in registers: lane's group lane % GROUPS of keys lane / GROUPS + ...
   const int lg = lane % GROUPS, lk = lane / GROUPS;
-  const RowGroup<T> kGroup(lg, a.dq), vGroup(lg, a.dv);
+  const RowGroup<T, FULL> kGroup(lg, a.dq), vGroup(lg, a.dv);
   struct Rows {
     u32x4_t k[LOADS], v[LOADS];
     unsigned long long mask;
@@ -202,6 +219,7 @@ __global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit 
       r.v[i] = vGroup.load(vBase + at * a.vT);
     }
   };
+  const ValueReads<T, D> reads;
   unsigned char* ks = lds[wave];
   unsigned char* vs = lds[wave] + ROWS_BYTES;
   Rows r;
@@ -213,8 +231,8 @@ __global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit 
     for(int i = 0; i < LOADS; i++) {
       const int key = lk + i * (64 / GROUPS);
       const u32x4_t zero = {0, 0, 0, 0};
-      *(u32x4_t*)(ks + kAt<T, D>(key, lg)) = kGroup.place(r.k[i], a.dq == D);
-      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (valid >> key) & 1 ? vGroup.place(r.v[i], a.dv == D) : zero;
+      *(u32x4_t*)(ks + kAt<T, D>(key, lg)) = kGroup.place(r.k[i]);
+      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (valid >> key) & 1 ? vGroup.place(r.v[i]) : zero;
     }
     asm volatile("" ::: "memory");
     load(t + 4, r);
@@ -223,7 +241,8 @@ __global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit 
     for(int i = 0; i < 16; i++) s[0][i] = 0.0f;
 #pragma unroll
     for(int i = 0; i < D / VEC / 2; i++) s[0] = mma32(*(const V*)(ks + kAt<T, D>(laneRow, 2 * i + half)), qf[i], s[0]);
-    const float corr = softmaxTile<1>(s, valid, a.scaleLog2, row);
+    maskTile<1>(s, valid);
+    const float corr = softmaxTile<1>(s, a.scaleLog2, row);
     if(__any(corr != 1.0f)) {
 #pragma unroll
       for(int db = 0; db < D / 32; db++)
@@ -240,7 +259,7 @@ __global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit 
       }
 #pragma unroll
       for(int db = 0; db < D / 32; db++) {
-        const V vf = readV<T, D>(vs, g * VEC / 4 * 8, db * 32);
+        const V vf = reads.read(vs, g * VEC / 4 * 8, db);
         o[db] = mma32(vf, hi, o[db]);
         if constexpr(sizeof(T) == 2) o[db] = mma32(vf, lo, o[db]);
       }
@@ -291,19 +310,25 @@ __global__ __launch_bounds__(256) void attentionFewKernel(AttnArgs a, AttnSplit 
 
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of WAVES waves has 32 rows a wave of one kv head, and
-// goes through 64-key tiles that all of them read from LDS. Of tile t + 1 the
+// goes through tiles of 64 keys (or 32) that all of them read from LDS. Of tile t + 1 the
 // scores are computed before tile t's softmax, so that the matrix cores have them
 // to do while the vector units work; a tile's rows are loaded into registers two
 // barriers before they are read.
 constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
 
-template<typename T, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, AttnSplit split) {
+// 32-key blocks of a tile: one where two would not leave registers for the reads
+// ahead (4096 queries to 5000 keys, heads of 128: 822 us, two 1064).
+template<typename T, int D>
+constexpr int attBlocks() { return sizeof(T) == 2 && D == 128 ? 1 : 2; }
+__device__ __forceinline__ constexpr unsigned long long attWhole(int blocks) { return blocks == 2 ? ~0ull : 0xffffffffull; }
+
+template<typename T, int D, int WAVES, bool FULL>
+__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionManyKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;
   constexpr int THREADS = 64 * WAVES;
-  constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, LOADS = 64 * GROUPS / THREADS;
-  static_assert(LOADS * THREADS == 64 * GROUPS && THREADS % GROUPS == 0, "whole loads");
-  constexpr int TILE = 64 * D * (int)sizeof(T);
+  constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, BLOCKS = attBlocks<T, D>(), KEYS = 32 * BLOCKS, LOADS = KEYS * GROUPS / THREADS;
+  static_assert(LOADS * THREADS == KEYS * GROUPS && THREADS % GROUPS == 0, "whole loads");
+  constexpr int TILE = KEYS * D * (int)sizeof(T);
   __shared__ __attribute__((aligned(16))) unsigned char k0s[TILE];
   __shared__ __attribute__((aligned(16))) unsigned char k1s[TILE];
   __shared__ __attribute__((aligned(16))) unsigned char v0s[TILE];
@@ -326,7 +351,7 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
   const T* kBase = (const T*)a.k + b * a.kB + kvh * a.kH;
   const T* vBase = (const T*)a.v + b * a.vB + kvh * a.vH;
   const int len = validLength(a, b);
-  const int allTiles = (len + 63) / 64;
+  const int allTiles = (len + KEYS - 1) / KEYS;
   const int begin = (int)((int64_t)allTiles * part / split.splits), end = (int)((int64_t)allTiles * (part + 1) / split.splits);
 
   V qf[D / VEC / 2];
@@ -344,7 +369,7 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
   RowState row;
 
   const int lg = tid % GROUPS, lk = tid / GROUPS;
-  const RowGroup<T> kGroup(lg, a.dq), vGroup(lg, a.dv);
+  const RowGroup<T, FULL> kGroup(lg, a.dq), vGroup(lg, a.dv);
   struct Rows {
     u32x4_t v[LOADS];
   };
@@ -356,11 +381,11 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
       const unsigned long long v = listBits[i];
       return ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
     }
-    const int n = len - (from + i) * 64;
-    return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
+    const int n = len - (from + i) * KEYS;
+    return n >= KEYS ? attWhole(BLOCKS) : (1ull << max(n, 0)) - 1;
   };
-  auto load = [&](const T* base, int64_t stride, const RowGroup<T>& g, int i, Rows& x) {
-    const int k0 = tileOf(min(i, count - 1)) * 64;
+  auto load = [&](const T* base, int64_t stride, const RowGroup<T, FULL>& g, int i, Rows& x) {
+    const int k0 = tileOf(min(i, count - 1)) * KEYS;
 #pragma unroll
     for(int j = 0; j < LOADS; j++) {
       const int64_t at = min(k0 + lk + j * (THREADS / GROUPS), len - 1);
@@ -371,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
   auto loadV = [&](int i, Rows& x) { load(vBase, a.vT, vGroup, i, x); };
   auto stageK = [&](unsigned char* ks, const Rows& x) {
 #pragma unroll
-    for(int j = 0; j < LOADS; j++) *(u32x4_t*)(ks + kAt<T, D>(lk + j * (THREADS / GROUPS), lg)) = kGroup.place(x.v[j], a.dq == D);
+    for(int j = 0; j < LOADS; j++) *(u32x4_t*)(ks + kAt<T, D>(lk + j * (THREADS / GROUPS), lg)) = kGroup.place(x.v[j]);
   };
   // What V holds at keys that take no part must not meet their p of 0.
   auto stageV = [&](unsigned char* vs, const Rows& x, unsigned long long bits) {
@@ -379,46 +404,83 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
     for(int j = 0; j < LOADS; j++) {
       const int key = lk + j * (THREADS / GROUPS);
       const u32x4_t zero = {0, 0, 0, 0};
-      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (bits >> key) & 1 ? vGroup.place(x.v[j], a.dv == D) : zero;
+      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (bits >> key) & 1 ? vGroup.place(x.v[j]) : zero;
     }
   };
-  auto scores = [&](const unsigned char* ks, floatx16 (&s)[2]) {
+  auto scores = [&](const unsigned char* ks, floatx16 (&s)[BLOCKS]) {
 #pragma unroll
-    for(int kb = 0; kb < 2; kb++)
+    for(int kb = 0; kb < BLOCKS; kb++)
 #pragma unroll
       for(int i = 0; i < 16; i++) s[kb][i] = 0.0f;
 #pragma unroll
     for(int i = 0; i < D / VEC / 2; i++)
 #pragma unroll
-      for(int kb = 0; kb < 2; kb++) s[kb] = mma32(*(const V*)(ks + kAt<T, D>(kb * 32 + laneRow, 2 * i + half)), qf[i], s[kb]);
+      for(int kb = 0; kb < BLOCKS; kb++) s[kb] = mma32(*(const V*)(ks + kAt<T, D>(kb * 32 + laneRow, 2 * i + half)), qf[i], s[kb]);
   };
-  auto values = [&](const unsigned char* vs, const floatx16 (&s)[2]) {
+  const ValueReads<T, D> reads;
+  constexpr int GROUPS_P = KEYS / 2 / VEC;  // 16-byte groups of a lane's p
+  struct Values {
+    V v[D / 32];
+  };
+  auto readValues = [&](const unsigned char* vs, int g, Values& x) {
 #pragma unroll
-    for(int kb = 0; kb < 2; kb++)
+    for(int db = 0; db < D / 32; db++) x.v[db] = reads.read(vs, g * VEC / 4 * 8, db);
+  };
+  // x: the operands of the first group. The next group's are read behind a group's
+  // first product, whose wait for its own operands then waits for nothing else.
+  auto values = [&](const unsigned char* vs, const V (&p)[GROUPS_P], Values& x) {
+    Values y;
 #pragma unroll
-      for(int g = 0; g < 16 / VEC; g++) {
-        V pf;
+    for(int g = 0; g < GROUPS_P; g++) {
+      const Values& now = g % 2 == 0 ? x : y;
+      o[0] = mma32(now.v[0], p[g], o[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      if(g + 1 < GROUPS_P) readValues(vs, g + 1, g % 2 == 0 ? y : x);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for(int i = 0; i < VEC; i++) pf[i] = (T)s[kb][g * VEC + i];
-#pragma unroll
-        for(int db = 0; db < D / 32; db++) o[db] = mma32(readV<T, D>(vs, kb * 32 + g * VEC / 4 * 8, db * 32), pf, o[db]);
-      }
+      for(int db = 1; db < D / 32; db++) o[db] = mma32(now.v[db], p[g], o[db]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   Rows kr, vr;
   // Item i: its scores are in s; K of i + 1 and V of i are in LDS, K of i + 2 and V
   // of i + 1 in registers.
-  auto step = [&](int i, floatx16 (&s)[2], floatx16 (&sNext)[2], unsigned char* kNow, const unsigned char* kNext, const unsigned char* vNow,
+  auto step = [&](int i, floatx16 (&s)[BLOCKS], floatx16 (&sNext)[BLOCKS], unsigned char* kNow, const unsigned char* kNext, const unsigned char* vNow,
                   unsigned char* vNext) {
     const unsigned long long bits = bitsOf(i), bitsNext = bitsOf(min(i + 1, count - 1));
+    maskTile<BLOCKS>(s, bits);
+    __builtin_amdgcn_sched_barrier(0);
     scores(kNext, sNext);
-    const float corr = softmaxTile<2>(s, bits, a.scaleLog2, row);
+    const float corr = softmaxTile<BLOCKS>(s, a.scaleLog2, row);
+    V p[GROUPS_P];
+#pragma unroll
+    for(int g = 0; g < GROUPS_P; g++) {
+#pragma unroll
+      for(int j = 0; j < VEC; j++) p[g][j] = (T)s[g * VEC / 16][g * VEC % 16 + j];
+      // Here, not where it is used: beside the scores' products.
+      asm volatile("" : "+v"(p[g]));
+    }
+    if constexpr(sizeof(T) == 2) {
+      // A product, then vector work in its shadow.
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for(int j = 0; j < D / 16 * BLOCKS; j++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, D == 128 ? 12 : 22, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    Values x;
+    readValues(vNow, 0, x);
+    __builtin_amdgcn_sched_barrier(0);
     if(__any(corr != 1.0f)) {
 #pragma unroll
       for(int db = 0; db < D / 32; db++)
 #pragma unroll
         for(int j = 0; j < 16; j++) o[db][j] *= corr;
     }
-    values(vNow, s);
+    values(vNow, p, x);
     stageK(kNow, kr);
     stageV(vNext, vr, bitsNext);
     loadK(i + 3, kr);
@@ -431,8 +493,8 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
     if(a.mask != nullptr) {
       __syncthreads();
       for(int t = wave; t < count; t += WAVES) {
-        const int j = (from + t) * 64 + lane;
-        const unsigned long long bits = __ballot(j < len && a.mask[b * a.maskB + j] != 0);
+        const int j = (from + t) * KEYS + lane % KEYS;
+        const unsigned long long bits = __ballot(j < len && a.mask[b * a.maskB + j] != 0) & attWhole(BLOCKS);
         if(lane == 0) listBits[t] = bits;
       }
       __syncthreads();
@@ -462,7 +524,7 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
     stageV(v0s, vr, bitsOf(0));
     loadK(1, kr);
     __syncthreads();
-    floatx16 sA[2], sB[2];
+    floatx16 sA[BLOCKS], sB[BLOCKS];
     scores(k0s, sA);
     stageK(k1s, kr);
     loadK(2, kr);
@@ -507,39 +569,50 @@ __global__ __launch_bounds__(64 * WAVES) void attentionManyKernel(AttnArgs a, At
     }
 }
 
-// The splits' sums on one reference point, a thread four dims of a row.
+// The splits' sums on one reference point: a workgroup takes a row, a thread four
+// dims of every eighth split (their loads are what takes time, one round trip
+// instead of one for each split), added in order in LDS.
 template<typename T>
 __global__ __launch_bounds__(256) void attentionJoinKernel(AttnArgs a, AttnSplit split, int64_t rowsAll) {
-  const int quads = (a.dv + 3) / 4;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = id / quads;
-  if(r >= rowsAll) return;
-  const int d = (int)(id - r * quads) * 4, n = min(4, a.dv - d);
-  float top = -INFINITY;
-  for(int s = 0; s < split.splits; s++) top = fmaxf(top, split.state[(s * rowsAll + r) * 2]);
+  __shared__ float sums[8][128];
+  __shared__ float totals[8];
+  const int64_t r = blockIdx.x;
+  const int quad = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int d = quad * 4, n = min(4, a.dv - d);
+  float ref = -INFINITY;
+  for(int s = quad; s < split.splits; s += 32) ref = fmaxf(ref, split.state[(s * rowsAll + r) * 2]);
+#pragma unroll
+  for(int w = 16; w > 0; w >>= 1) ref = fmaxf(ref, __shfl_xor(ref, w));
   float total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for(int s = 0; s < split.splits; s++) {
+  for(int s = slice; s < split.splits; s += 8) {
     const float* st = split.state + (s * rowsAll + r) * 2;
-    const float f = st[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st[0] - top);
-    const uint4 u = loadGroup(split.out + (s * rowsAll + r) * a.dv + d, n);
+    const uint4 u = n > 0 ? loadGroup(split.out + (s * rowsAll + r) * a.dv + d, n) : make_uint4(0, 0, 0, 0);
+    const float f = st[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st[0] - ref);
     total = fmaf(st[1], f, total);
     v[0] = fmaf(__uint_as_float(u.x), f, v[0]);
     v[1] = fmaf(__uint_as_float(u.y), f, v[1]);
     v[2] = fmaf(__uint_as_float(u.z), f, v[2]);
     v[3] = fmaf(__uint_as_float(u.w), f, v[3]);
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  *(float4*)&sums[slice][d] = make_float4(v[0], v[1], v[2], v[3]);
+  if(quad == 0) totals[slice] = total;
+  __syncthreads();
+  const int e = threadIdx.x;
+  if(e >= a.dv) return;
+  float all = 0.0f, y = 0.0f;
+#pragma unroll
+  for(int i = 0; i < 8; i++) {
+    all += totals[i];
+    y += sums[i][e];
+  }
   // r counts batch, kv head, query, head of the group.
   const int group = a.heads / a.kvHeads;
   const int64_t rows = (int64_t)a.lq * group, outer = r / rows;
   const int at = (int)(r - outer * rows);
   const int64_t b = outer / a.kvHeads;
   const int h = (int)(outer - b * a.kvHeads) * group + at % group;
-  T* out = (T*)a.out + b * a.oB + (int64_t)(at / group) * a.oT + h * a.oH + d;
-#pragma unroll
-  for(int j = 0; j < 4; j++)
-    if(j < n) out[j] = (T)(v[j] * inv);
+  ((T*)a.out)[b * a.oB + (int64_t)(at / group) * a.oT + h * a.oH + e] = (T)(all == 0.0f ? 0.0f : y / all);
 }
 
 }  // namespace
@@ -597,35 +670,31 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   const int64_t rows = (int64_t)p.q_len * (p.heads / p.kv_heads);
   plan.rows = rows * p.batch * p.kv_heads;
   plan.few = rows <= 32;
-  plan.waves = rows <= 128 || p.dtype == KGH_DTYPE_FP32 ? 4 : 8;
+  plan.waves = p.dtype == KGH_DTYPE_FP32 || rows <= 128 || std::max(p.q_head_dim, p.v_head_dim) <= 32 ? 4 : 8;
   const int64_t groups = plan.few ? (int64_t)p.batch * p.kv_heads : (rows + plan.waves * 32 - 1) / (plan.waves * 32) * p.batch * p.kv_heads;
-  const int64_t wanted = plan.few ? 1024 : 256;
-  int64_t splits = std::min<int64_t>({wanted / groups, p.k_len / 256, 64});
+  // Workgroups that the CUs hold at a time: two a CU of the kernel for few rows in
+  // 16 bits, one of the others; and at least 128 keys a split. One query of 8 kv
+  // heads to 16384 keys, us: whole 306, 8 splits 47, 32 21.6, 64 22.1; of 32
+  // streams and 8 kv heads: whole 92, two 76, four 80; 361 queries of 6 heads to
+  // 4096 keys: whole 98, 16 21.6, 32 28.
+  const int64_t wanted = plan.few && p.dtype != KGH_DTYPE_FP32 ? 512 : 256;
+  int64_t splits = std::min<int64_t>({wanted / groups, p.k_len / 128, 64});
   const uint64_t one = (uint64_t)plan.rows * (p.v_head_dim + 2) * 4;
   splits = std::min<int64_t>(splits, (int64_t)std::min<uint64_t>(bytes / one, 64));
   plan.splits = (int)std::max<int64_t>(1, splits);
   return plan;
 }
 
-template<typename T, int D>
+template<typename T, int D, bool FULL>
 void runAttention(const AttentionPlan& plan, const AttnArgs& a, const AttnSplit& split, int batch, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.lq * (a.heads / a.kvHeads);
-  if(plan.few) attentionFewKernel<T, D><<<dim3((unsigned)plan.splits, (unsigned)a.kvHeads, (unsigned)batch), 256, 0, stream>>>(a, split);
-  else {
-    const int64_t blocks = (rows + plan.waves * 32 - 1) / (plan.waves * 32);
-    const dim3 grid((unsigned)(blocks * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
-    if(sizeof(T) == 2 && D >= 64 && plan.waves == 8) {
-      if constexpr(sizeof(T) == 2 && D >= 64) attentionManyKernel<T, D, 8><<<grid, 512, 0, stream>>>(a, split);
-    }
-    else {
-      const dim3 grid4((unsigned)((rows + 127) / 128 * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
-      attentionManyKernel<T, D, 4><<<grid4, 256, 0, stream>>>(a, split);
-    }
-  }
+  const int64_t rows = (int64_t)a.lq * (a.heads / a.kvHeads), block = plan.waves * 32;
+  const dim3 grid((unsigned)((plan.few ? 1 : (rows + block - 1) / block) * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
+  if(plan.few) attentionFewKernel<T, D, FULL><<<grid, 256, 0, stream>>>(a, split);
+  else if(plan.waves == 4) attentionManyKernel<T, D, 4, FULL><<<grid, 256, 0, stream>>>(a, split);
+  else if constexpr(sizeof(T) == 2 && D >= 64) attentionManyKernel<T, D, 8, FULL><<<grid, 512, 0, stream>>>(a, split);
   KGH_CHECK_LAUNCH();
   if(plan.splits > 1) {
-    const int64_t threads = plan.rows * ((a.dv + 3) / 4);
-    attentionJoinKernel<T><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, stream>>>(a, split, plan.rows);
+    attentionJoinKernel<T><<<dim3((unsigned)plan.rows), 256, 0, stream>>>(a, split, plan.rows);
     KGH_CHECK_LAUNCH();
   }
 }
@@ -668,9 +737,14 @@ void launchAttention(const kgh_attention_params& p, hipStream_t stream) {
   const int d = std::max(p.q_head_dim, p.v_head_dim);
   withDtype(p.dtype, [&](auto t) {
     typedef decltype(t) T;
-    if(d <= 32) runAttention<T, 32>(plan, a, split, p.batch, stream);
-    else if(d <= 64) runAttention<T, 64>(plan, a, split, p.batch, stream);
-    else runAttention<T, 128>(plan, a, split, p.batch, stream);
+    const auto run = [&](auto dim) {
+      constexpr int D = decltype(dim)::value;
+      if(p.q_head_dim == D && p.v_head_dim == D) runAttention<T, D, true>(plan, a, split, p.batch, stream);
+      else runAttention<T, D, false>(plan, a, split, p.batch, stream);
+    };
+    if(d <= 32) run(std::integral_constant<int, 32>());
+    else if(d <= 64) run(std::integral_constant<int, 64>());
+    else run(std::integral_constant<int, 128>());
   });
 }
 

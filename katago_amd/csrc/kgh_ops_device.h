@@ -82,7 +82,8 @@ __device__ __forceinline__ uint4 loadGroupSmall(const T* __restrict__ p, int n) 
 // where its register is cleared first): load() reads 16 bytes that lie in the row
 // wherever the group ends, place() puts the group's elements in their places and
 // zeros behind the row's end.
-template<typename T>
+// FULL: the rows are as long as the groups of all lanes.
+template<typename T, bool FULL>
 struct RowGroup {
   static constexpr int VEC = 16 / (int)sizeof(T);
   int at;      // first element read
@@ -95,16 +96,15 @@ struct RowGroup {
   }
   __device__ __forceinline__ u32x4_t load(const T* __restrict__ row) const {
     u32x4_t v;
-    if(dims >= VEC) __builtin_memcpy(&v, row + at, 16);
+    if(FULL || dims >= VEC) __builtin_memcpy(&v, row + at, 16);
     else {
       const uint4 u = loadGroupSmall(row, dims);
       v = u32x4_t{u.x, u.y, u.z, u.w};
     }
     return v;
   }
-  // full: the rows are as long as the groups of all lanes.
-  __device__ __forceinline__ u32x4_t place(u32x4_t v, bool full) const {
-    if(!full) {
+  __device__ __forceinline__ u32x4_t place(u32x4_t v) const {
+    if constexpr(!FULL) {
       if(dims % VEC != 0 && excess < VEC) {
         uint4 u = make_uint4(v.x, v.y, v.z, v.w);
 #pragma unroll 1
