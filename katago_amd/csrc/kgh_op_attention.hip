@@ -679,6 +679,8 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   // 4096 keys: whole 98, 16 21.6, 32 28.
   const int64_t wanted = plan.few && p.dtype != KGH_DTYPE_FP32 ? 512 : 256;
   int64_t splits = std::min<int64_t>({wanted / groups, p.k_len / 128, 64});
+  // Many rows' sums are many bytes: 96 workgroups, 361 keys, whole 20, in two 29.
+  if(!plan.few && groups > 64) splits = 1;
   const uint64_t one = (uint64_t)plan.rows * (p.v_head_dim + 2) * 4;
   splits = std::min<int64_t>(splits, (int64_t)std::min<uint64_t>(bytes / one, 64));
   plan.splits = (int)std::max<int64_t>(1, splits);
