@@ -4,7 +4,7 @@ positions with several axes (``rope_axes``) and attention to an encoder's states
 (``cross_attention``).
 
 Tensors are torch tensors, or ``DeviceTensor`` views of device memory: anything
-with ``data_ptr()``, ``stride()``, ``shape``, ``dtype`` and ``device``. Calls are
+with ``data_ptr()``, ``stride()``, ``shape``, ``dtype`` and ``get_device()``. Calls are
 asynchronous on ``stream`` (a hipStream_t as an int, None for the null stream;
 ``torch.cuda.current_stream().cuda_stream``); the caller keeps the tensors alive
 until they have run. Every call returns its output tensor. Arguments that do not
@@ -65,13 +65,6 @@ def _library() -> ctypes.CDLL:
     return _lib
 
 
-class Device:
-    """What ``DeviceTensor.device`` holds."""
-
-    def __init__(self, index: int):
-        self.type, self.index = "cuda", index
-
-
 class DeviceTensor:
     """A view of device memory for callers without torch: a pointer (an int or
     ctypes.c_void_p, for instance ``DeviceBuffer.ptr``), a shape, the name of a
@@ -88,7 +81,7 @@ class DeviceTensor:
                 n *= max(s, 1)
         self._strides = tuple(strides)
         self.dtype = dtype
-        self.device = Device(device)
+        self._device = device
 
     def data_ptr(self) -> int:
         return self._ptr
@@ -96,13 +89,18 @@ class DeviceTensor:
     def stride(self):
         return self._strides
 
+    def get_device(self) -> int:
+        return self._device
+
 
 def _invalid(message: str):
     raise StringError(message, _INVALID)
 
 
 _CODES = {"float32": FP32, "float16": FP16, "bfloat16": BF16, "int32": "int32", "uint8": "uint8", "bool": "bool"}
-_codes = {}  # the same by the tensors' own type objects
+_BYTES = {FP32: 4, FP16: 2, BF16: 2, "int32": 4, "uint8": 1, "bool": 1}
+_codes = dict(_CODES)  # the same by the tensors' own type objects
+_types = {code: name for name, code in _CODES.items()}  # the type object met last of each
 
 
 def _code(op, name, t):
@@ -115,35 +113,47 @@ def _code(op, name, t):
     if code is None:
         _invalid(f"{op}: {name} is of type {t.dtype}")
     _codes[t.dtype] = code
+    _types[code] = t.dtype
     return code
 
 
-def _look(op, name, t, ndim, code, device):
-    """Checks a tensor's axes, type and device; returns its strides."""
+def _look(op, name, t, ndim, dtype, device):
+    """Checks a tensor's axes, type (by a type object) and device; returns its
+    strides."""
     strides = t.stride()
+    if len(strides) != ndim or t.dtype != dtype or t.get_device() != device or strides[-1] != 1:
+        _look_again(op, name, t, strides, ndim, dtype, device)
+    return strides
+
+
+def _look_again(op, name, t, strides, ndim, dtype, device):
+    """What does not fit, if anything does not."""
     if len(strides) != ndim:
         _invalid(f"{op}: {name} has {len(strides)} axes, not {ndim}")
-    if max(t.shape) > _MOST:
-        _invalid(f"{op}: an axis of {name} is longer than {_MOST}")
     if strides[-1] != 1 and t.shape[-1] > 1:
         _invalid(f"{op}: the last axis of {name} is not contiguous")
-    if _code(op, name, t) != code:
+    if _code(op, name, t) != _codes[dtype]:
         _invalid(f"{op}: {name} is of type {t.dtype}")
-    d = t.device
-    if d.index != device or d.type != "cuda":
+    if t.get_device() != device:
         _invalid(f"{op}: {name} is not on the same device as the first tensor")
-    return strides
 
 
 def _first(op, name, t):
     """The type and device index that the call goes by."""
-    d = t.device
-    if d.type != "cuda":
+    device = t.get_device()
+    if device < 0:
         _invalid(f"{op}: {name} is not on a GPU")
-    code = _code(op, name, t)
+    code = _codes.get(t.dtype)
+    if code is None:
+        code = _code(op, name, t)
     if code not in (FP32, FP16, BF16):
         _invalid(f"{op}: {name} is of type {t.dtype}")
-    return code, d.index
+    return code, device
+
+
+def _sizes(op, *sizes):
+    if max(sizes) > _MOST:
+        _invalid(f"{op}: an axis is longer than {_MOST}")
 
 
 def _shape(op, name, t, *want):
@@ -155,44 +165,45 @@ def _workspace(op, workspace, device):
     """Pointer and bytes of a workspace: a contiguous tensor of any type."""
     if workspace is None:
         return None, 0
-    if workspace.device.type != "cuda" or workspace.device.index != device:
+    if workspace.get_device() != device:
         _invalid(f"{op}: the workspace is not on the same device as the first tensor")
     n = 1
-    for size, stride in zip(reversed(tuple(workspace.shape)), reversed(tuple(workspace.stride()))):
+    for size, stride in zip(reversed(workspace.shape), reversed(workspace.stride())):
         if stride != n and size > 1:
             _invalid(f"{op}: the workspace is not contiguous")
         n *= size
-    code = _code(op, "the workspace", workspace)
-    return workspace.data_ptr(), n * {FP32: 4, FP16: 2, BF16: 2, "int32": 4}.get(code, 1)
+    return workspace.data_ptr(), n * _BYTES[_code(op, "the workspace", workspace)]
 
 
 def _linear_params(x, weights, out, bias, activation, residual, workspace):
     code, device = _first("linear", "x", x)
-    xs = _look("linear", "x", x, 2, code, device)
-    ws = _look("linear", "weights", weights, 2, code, device)
+    dtype = x.dtype
+    xs = _look("linear", "x", x, 2, dtype, device)
+    ws = _look("linear", "weights", weights, 2, dtype, device)
     rows, in_c = x.shape
-    out_c = weights.shape[0]
-    if weights.shape[1] != in_c:
-        _invalid(f"linear: weights have {weights.shape[1]} input channels, x has {in_c}")
+    out_c, w_in = weights.shape
+    if w_in != in_c:
+        _invalid(f"linear: weights have {w_in} input channels, x has {in_c}")
+    _sizes("linear", rows, in_c, out_c)
     act = ACTIVATIONS.get(activation or "identity")
     if act is None:
         _invalid(f"linear: unknown activation {activation!r}")
-    p = _LinearParams(code, act, rows, in_c, out_c, x.data_ptr(), xs[0], weights.data_ptr(), ws[0])
+    op = os = bp = None
+    rs = space = (None, 0)
     if out is not None:
-        os = _look("linear", "out", out, 2, code, device)
+        os = _look("linear", "out", out, 2, dtype, device)[0]
         _shape("linear", "out", out, rows, out_c)
-        p.out, p.out_stride = out.data_ptr(), os[0]
+        op = out.data_ptr()
     if bias is not None:
-        _look("linear", "bias", bias, 1, FP32, device)
+        _look("linear", "bias", bias, 1, _types[FP32], device)
         _shape("linear", "bias", bias, out_c)
-        p.bias = bias.data_ptr()
+        bp = bias.data_ptr()
     if residual is not None:
-        rs = _look("linear", "residual", residual, 2, code, device)
+        rs = (residual.data_ptr(), _look("linear", "residual", residual, 2, dtype, device)[0])
         _shape("linear", "residual", residual, rows, out_c)
-        p.residual, p.residual_stride = residual.data_ptr(), rs[0]
     if workspace is not None:
-        p.workspace, p.workspace_bytes = _workspace("linear", workspace, device)
-    return p, device
+        space = _workspace("linear", workspace, device)
+    return _LinearParams(code, act, rows, in_c, out_c, x.data_ptr(), xs[0], weights.data_ptr(), ws[0], bp, *rs, op, os or 0, *space), device
 
 
 def linear_workspace(x, weights) -> int:
@@ -227,16 +238,15 @@ def rope_axes(x, positions, freqs, out, layout="interleaved", inverse=False, str
     "halves" (p and p + pairs). Channels from 2 * pairs on are copied; inverse
     turns back. out may be x itself."""
     code, device = _first("rope_axes", "x", x)
-    xs = _look("rope_axes", "x", x, 3, code, device)
-    os = _look("rope_axes", "out", out, 3, code, device)
-    ps = _look("rope_axes", "positions", positions, 2, "int32", device)
-    fs = _look("rope_axes", "freqs", freqs, 3, FP32, device)
+    xs = _look("rope_axes", "x", x, 3, x.dtype, device)
+    os = _look("rope_axes", "out", out, 3, x.dtype, device)
+    ps = _look("rope_axes", "positions", positions, 2, _types["int32"], device)
+    fs = _look("rope_axes", "freqs", freqs, 3, _types[FP32], device)
     tokens, heads, dim = x.shape
     tables, pairs, axes = freqs.shape
-    if tuple(out.shape) != (tokens, heads, dim):
-        _shape("rope_axes", "out", out, tokens, heads, dim)
-    if tuple(positions.shape) != (tokens, axes):
-        _shape("rope_axes", "positions", positions, tokens, axes)
+    _shape("rope_axes", "out", out, tokens, heads, dim)
+    _shape("rope_axes", "positions", positions, tokens, axes)
+    _sizes("rope_axes", tokens, heads, dim, tables, pairs, axes)
     if (fs[0] != pairs * axes and tables > 1) or (fs[1] != axes and pairs > 1):
         _invalid("rope_axes: freqs is not contiguous")
     kind = ROPE_LAYOUTS.get(layout)
@@ -250,26 +260,27 @@ def rope_axes(x, positions, freqs, out, layout="interleaved", inverse=False, str
 
 def _attention_params(q, k, v, scale):
     code, device = _first("cross_attention", "q", q)
-    qs = _look("cross_attention", "q", q, 4, code, device)
-    ks = _look("cross_attention", "k", k, 4, code, device)
-    vs = _look("cross_attention", "v", v, 4, code, device)
+    dtype = q.dtype
+    qs = _look("cross_attention", "q", q, 4, dtype, device)
+    ks = _look("cross_attention", "k", k, 4, dtype, device)
+    vs = _look("cross_attention", "v", v, 4, dtype, device)
     batch, lq, heads, dq = q.shape
     _, lk, kv_heads, _ = k.shape
     dv = v.shape[3]
-    if tuple(k.shape) != (batch, lk, kv_heads, dq):
-        _shape("cross_attention", "k", k, batch, lk, kv_heads, dq)
-    if tuple(v.shape) != (batch, lk, kv_heads, dv):
-        _shape("cross_attention", "v", v, batch, lk, kv_heads, dv)
-    p = _AttentionParams(code, batch, lq, lk, heads, kv_heads, dq, dv, max(dq, 1) ** -0.5 if scale is None else scale,
-                         q.data_ptr(), qs[:3], k.data_ptr(), ks[:3], v.data_ptr(), vs[:3])
-    return p, code, device
+    _shape("cross_attention", "k", k, batch, lk, kv_heads, dq)
+    _shape("cross_attention", "v", v, batch, lk, kv_heads, dv)
+    _sizes("cross_attention", batch, lq, heads, dq, lk, kv_heads, dv)
+    if scale is None:
+        scale = max(dq, 1) ** -0.5
+    return _AttentionParams(code, batch, lq, lk, heads, kv_heads, dq, dv, scale, q.data_ptr(), qs[:3], k.data_ptr(), ks[:3],
+                            v.data_ptr(), vs[:3]), device
 
 
 def cross_attention_workspace(q, k, v) -> int:
     """kgh_cross_attention_workspace: bytes of workspace that ``cross_attention``
     makes use of for tensors of these shapes and types (0: none). A larger one
     serves too."""
-    p, _, device = _attention_params(q, k, v, None)
+    p, device = _attention_params(q, k, v, None)
     n = ctypes.c_uint64()
     hip_check(_library().kgh_cross_attention_workspace(device, p, n))
     return n.value
@@ -286,19 +297,18 @@ def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, w
     hold there is not used. A row without a key is zeros. workspace: at least
     ``cross_attention_workspace`` bytes of its own for calls that may overlap;
     without one, long keys are not split over workgroups."""
-    p, code, device = _attention_params(q, k, v, scale)
-    os = _look("cross_attention", "out", out, 4, code, device)
-    batch = q.shape[0]
-    if tuple(out.shape) != (batch, p.q_len, p.heads, p.v_head_dim):
-        _shape("cross_attention", "out", out, batch, p.q_len, p.heads, p.v_head_dim)
+    p, device = _attention_params(q, k, v, scale)
+    os = _look("cross_attention", "out", out, 4, q.dtype, device)
+    batch = p.batch
+    _shape("cross_attention", "out", out, batch, p.q_len, p.heads, p.v_head_dim)
     p.out, p.out_strides = out.data_ptr(), os[:3]
     if key_lengths is not None:
-        ls = _look("cross_attention", "key_lengths", key_lengths, 1, "int32", device)
+        ls = _look("cross_attention", "key_lengths", key_lengths, 1, _types["int32"], device)
         _shape("cross_attention", "key_lengths", key_lengths, batch)
         p.key_lengths = key_lengths.data_ptr()
     if key_mask is not None:
         kind = _code("cross_attention", "key_mask", key_mask)
-        ms = _look("cross_attention", "key_mask", key_mask, 2, kind if kind in ("uint8", "bool") else "uint8", device)
+        ms = _look("cross_attention", "key_mask", key_mask, 2, _types[kind if kind in ("uint8", "bool") else "uint8"], device)
         _shape("cross_attention", "key_mask", key_mask, batch, p.k_len)
         p.key_mask, p.key_mask_stride = key_mask.data_ptr(), ms[0]
     if workspace is not None:
