@@ -191,8 +191,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
 #pragma unroll
   for(int i = 0; i < D / VEC / 2; i++) {
     const int c = (2 * i + half) * VEC;
-    const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
-    qf[i] = *(const V*)&u;
+    if constexpr(FULL) __builtin_memcpy(&qf[i], qRow + c, 16);
+    else {
+      const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
+      qf[i] = *(const V*)&u;
+    }
   }
   floatx16 o[D / 32];
 #pragma unroll
@@ -314,6 +317,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
 // scores are computed before tile t's softmax, so that the matrix cores have them
 // to do while the vector units work; a tile's rows are loaded into registers two
 // barriers before they are read.
+constexpr int64_t ATT_NEAR = 1 << 23;  // token strides below it: 64 of them are less than 2^31 bytes
 constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
 
 // 32-key blocks of a tile: one where two would not leave registers for the reads
@@ -358,8 +362,11 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
 #pragma unroll
   for(int i = 0; i < D / VEC / 2; i++) {
     const int c = (2 * i + half) * VEC;
-    const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
-    qf[i] = *(const V*)&u;
+    if constexpr(FULL) __builtin_memcpy(&qf[i], qRow + c, 16);
+    else {
+      const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
+      qf[i] = *(const V*)&u;
+    }
   }
   floatx16 o[D / 32];
 #pragma unroll
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
   };
   int count = 0, from = begin;  // tiles of this round, and its first
   // What item i of the round is: a tile, and which of its keys take part.
-  auto tileOf = [&](int i) { return a.mask == nullptr ? from + i : listTile[i]; };
+  auto tileOf = [&](int i) { return a.mask == nullptr ? from + i : __builtin_amdgcn_readfirstlane(listTile[i]); };
   auto bitsOf = [&](int i) -> unsigned long long {
     if(a.mask != nullptr) {
       const unsigned long long v = listBits[i];
@@ -384,16 +391,25 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
     const int n = len - (from + i) * KEYS;
     return n >= KEYS ? attWhole(BLOCKS) : (1ull << max(n, 0)) - 1;
   };
-  auto load = [&](const T* base, int64_t stride, const RowGroup<T, FULL>& g, int i, Rows& x) {
+  // A lane's offset in a tile, where it fits 32 bits (ATT_NEAR): a whole tile's
+  // addresses are then a scalar and this.
+  const unsigned kNear = (unsigned)(lk * a.kT + kGroup.at) * (unsigned)sizeof(T), vNear = (unsigned)(lk * a.vT + vGroup.at) * (unsigned)sizeof(T);
+  auto load = [&](const T* base, int64_t stride, unsigned near, const RowGroup<T, FULL>& g, int i, Rows& x) {
     const int k0 = tileOf(min(i, count - 1)) * KEYS;
+    if(FULL && k0 + KEYS <= len && stride < ATT_NEAR) {
 #pragma unroll
-    for(int j = 0; j < LOADS; j++) {
-      const int64_t at = min(k0 + lk + j * (THREADS / GROUPS), len - 1);
-      x.v[j] = g.load(base + at * stride);
+      for(int j = 0; j < LOADS; j++) __builtin_memcpy(&x.v[j], (const char*)(base + (int64_t)(k0 + j * (THREADS / GROUPS)) * stride) + near, 16);
+    }
+    else {
+#pragma unroll
+      for(int j = 0; j < LOADS; j++) {
+        const int64_t at = min(k0 + lk + j * (THREADS / GROUPS), len - 1);
+        x.v[j] = g.load(base + at * stride);
+      }
     }
   };
-  auto loadK = [&](int i, Rows& x) { load(kBase, a.kT, kGroup, i, x); };
-  auto loadV = [&](int i, Rows& x) { load(vBase, a.vT, vGroup, i, x); };
+  auto loadK = [&](int i, Rows& x) { load(kBase, a.kT, kNear, kGroup, i, x); };
+  auto loadV = [&](int i, Rows& x) { load(vBase, a.vT, vNear, vGroup, i, x); };
   auto stageK = [&](unsigned char* ks, const Rows& x) {
 #pragma unroll
     for(int j = 0; j < LOADS; j++) *(u32x4_t*)(ks + kAt<T, D>(lk + j * (THREADS / GROUPS), lg)) = kGroup.place(x.v[j]);
@@ -517,19 +533,23 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
       count = listCount;
       if(count == 0) continue;
     }
-    loadK(0, kr);
-    loadV(0, vr);
-    __syncthreads();  // the buffers' readers of the round before
-    stageK(k0s, kr);
-    stageV(v0s, vr, bitsOf(0));
-    loadK(1, kr);
-    __syncthreads();
-    floatx16 sA[BLOCKS], sB[BLOCKS];
-    scores(k0s, sA);
-    stageK(k1s, kr);
+    {
+      Rows kFirst;
+      loadK(0, kFirst);
+      loadK(1, kr);
+      loadV(0, vr);
+      if(from > begin) __syncthreads();  // the buffers' readers of the round before
+      stageK(k0s, kFirst);
+      stageK(k1s, kr);
+      stageV(v0s, vr, bitsOf(0));
+    }
     loadK(2, kr);
     loadV(1, vr);
-    __syncthreads();
+    barrierLds();
+    floatx16 sA[BLOCKS], sB[BLOCKS];
+    scores(k0s, sA);
+    // A wave that is ahead puts item 2's keys where others still read item 0's.
+    barrierLds();
     int i = 0;
     for(; i + 2 <= count; i += 2) {
       step(i, sA, sB, k0s, k1s, v0s, v1s);
@@ -539,8 +559,9 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
   }
 
   row.sum = joinHalves(row.sum);
-  if(r >= rows) return;
+  const bool on = r < rows;
   if(split.out != nullptr) {
+    if(!on) return;
     const int64_t at = ((int64_t)part * gridDim.z + b) * a.kvHeads * rows + (int64_t)kvh * rows + r;
     if(half == 0) {
       split.state[at * 2] = row.ref;
@@ -559,14 +580,34 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
   const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
   T* oRow = (T*)a.out + b * a.oB + qi * a.oT + h * a.oH;
 #pragma unroll
-  for(int db = 0; db < D / 32; db++)
+  for(int db = 0; db < D / 32; db++) {
+    if constexpr(sizeof(T) == 4) {
 #pragma unroll
-    for(int q = 0; q < 4; q++) {
-      const int d = db * 32 + q * 8 + half * 4;
-#pragma unroll
-      for(int i = 0; i < 4; i++)
-        if(d + i < a.dv) oRow[d + i] = (T)(o[db][q * 4 + i] * inv);
+      for(int q = 0; q < 4; q++) {
+        const int d = db * 32 + q * 8 + half * 4;
+        const floatx4 v = {o[db][q * 4] * inv, o[db][q * 4 + 1] * inv, o[db][q * 4 + 2] * inv, o[db][q * 4 + 3] * inv};
+        if(on && d < a.dv) storeGroup((float*)oRow + d, *(const uint4*)&v, a.dv - d);
+      }
     }
+    else {
+      // A lane has four of eight consecutive dims, its partner lane ^ 32 the others;
+      // two such groups of both swap halves into 16 bytes a lane.
+#pragma unroll
+      for(int p = 0; p < 2; p++) {
+        union Four {
+          uint2 v;
+          T e[4];
+        } f[2];
+#pragma unroll
+        for(int q = 0; q < 2; q++)
+#pragma unroll
+          for(int i = 0; i < 4; i++) f[q].e[i] = (T)(o[db][(2 * p + q) * 4 + i] * inv);
+        const uint2 x = swapHalves(f[0].v.x, f[1].v.x), y = swapHalves(f[0].v.y, f[1].v.y);
+        const int d = db * 32 + (2 * p + half) * 8;
+        if(on && d < a.dv) storeGroup(oRow + d, make_uint4(x.x, y.x, x.y, y.y), a.dv - d);
+      }
+    }
+  }
 }
 
 // The splits' sums on one reference point: a workgroup takes a row, a thread four
@@ -670,7 +711,10 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   const int64_t rows = (int64_t)p.q_len * (p.heads / p.kv_heads);
   plan.rows = rows * p.batch * p.kv_heads;
   plan.few = rows <= 32;
-  plan.waves = p.dtype == KGH_DTYPE_FP32 || rows <= 128 || std::max(p.q_head_dim, p.v_head_dim) <= 32 ? 4 : 8;
+  // 256-row workgroups where they are at most an eighth empty: 512 rows, heads of
+  // 128, 85 us (90 with 128 rows), 16384 rows 795 (962); 361 rows 112 (94).
+  const bool wide = rows >= 512 && rows * 8 >= (rows + 255) / 256 * 256 * 7;
+  plan.waves = p.dtype != KGH_DTYPE_FP32 && wide && std::max(p.q_head_dim, p.v_head_dim) > 32 ? 8 : 4;
   const int64_t groups = plan.few ? (int64_t)p.batch * p.kv_heads : (rows + plan.waves * 32 - 1) / (plan.waves * 32) * p.batch * p.kv_heads;
   // Workgroups that the CUs hold at a time: two a CU of the kernel for few rows in
   // 16 bits, one of the others; and at least 128 keys a split. One query of 8 kv
@@ -679,6 +723,7 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   // 4096 keys: whole 98, 16 21.6, 32 28.
   const int64_t wanted = plan.few && p.dtype != KGH_DTYPE_FP32 ? 512 : 256;
   int64_t splits = std::min<int64_t>({wanted / groups, p.k_len / 128, 64});
+  if(p.k_len < 512) splits = 1;  // 6 heads, 361 keys: whole 7.9, in two 9.3
   // Many rows' sums are many bytes: 96 workgroups, 361 keys, whole 20, in two 29.
   if(!plan.few && groups > 64) splits = 1;
   const uint64_t one = (uint64_t)plan.rows * (p.v_head_dim + 2) * 4;

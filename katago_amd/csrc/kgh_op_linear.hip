@@ -63,12 +63,6 @@ __device__ __forceinline__ void blockedTile(int rowTiles, int colTiles, int& row
 // reads (eight consecutive ones, the same group) fall in distinct banks.
 __device__ __forceinline__ int swizzled128(int row, int group) { return row * 128 + ((group ^ (row & 7)) << 4); }
 
-// x and y with y's lower 32 lanes and x's upper ones exchanged.
-__device__ __forceinline__ uint2 swapHalves(unsigned x, unsigned y) {
-  const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-  return make_uint2(r[0], r[1]);
-}
-
 // The epilogue of a wave's RB x CB blocks at row mBase, column nBase. The weights
 // are the products' row operand, so a lane has four consecutive columns of row
 // laneRow, and its partner lane ^ 32 the four behind them; in 16 bits two such

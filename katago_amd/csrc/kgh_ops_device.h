@@ -118,6 +118,12 @@ struct RowGroup {
   }
 };
 
+// x and y with y's lower 32 lanes and x's upper ones exchanged.
+__device__ __forceinline__ uint2 swapHalves(unsigned x, unsigned y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  return make_uint2(r[0], r[1]);
+}
+
 // A workgroup barrier for LDS alone: __syncthreads() would wait for the loads that
 // are to arrive during the next step too.
 __device__ __forceinline__ void barrierLds() {
