@@ -250,7 +250,9 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
 
 /* out[m][n] = act(sum_k x[m][k] weights[n][k] + bias[n]) + residual[m][n].
  * residual may be out itself (with its stride). in_channels and out_channels
- * are at least 1. */
+ * are at least 1. Infinities and NaN give what fp32 arithmetic gives, but that a
+ * product of two infinities may be NaN in fp32, and a sum within 2^-8 of the
+ * largest float infinite. */
 typedef struct kgh_linear_params {
   int32_t dtype;      /* KGH_DTYPE_* of x, weights, residual and out */
   int32_t activation; /* KGH_ACTIVATION_* */

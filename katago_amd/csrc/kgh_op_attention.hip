@@ -162,7 +162,9 @@ __device__ __forceinline__ float joinHalves(float v) { return v + __shfl_xor(v, 
 // the keys are split over workgroups too where there are few. S^T = K Q^T (lane =
 // row, 16 of 32 keys), so that P^T is the second product's operand as it stands.
 // Here the matrix cores have time: P goes through them in two pieces, so that the
-// result is not off by P's rounding.
+// result is not off by P's rounding. bf16, 32 streams, 32/8 heads of 128, up to 4096
+// keys each: 69 us, 4.9 TB/s of keys and values (a copy reaches 5.2); one stream of
+// 16384 keys 22 us, where a wave's four tiles take a round trip to memory each.
 template<typename T, int D, bool FULL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;
@@ -316,7 +318,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
 // goes through tiles of 64 keys (or 32) that all of them read from LDS. Of tile t + 1 the
 // scores are computed before tile t's softmax, so that the matrix cores have them
 // to do while the vector units work; a tile's rows are loaded into registers two
-// barriers before they are read.
+// barriers before they are read. Bound by what a wave does between barriers: the
+// softmax's vector work (16 cycles for an exponential, about 28 a score in all)
+// and the products take as long as both one after the other, two waves a SIMD.
+// bf16, 4096 queries to 5000 keys, 32/8 heads: of 128 769 us (873 TFLOP/s), of 64
+// 446 (753); 64 boards of 361 queries to boards of three sizes, fp16, heads of 64,
+// 39 us, where two thirds are a workgroup's start and end.
 constexpr int64_t ATT_NEAR = 1 << 23;  // token strides below it: 64 of them are less than 2^31 bytes
 constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
 

@@ -142,14 +142,19 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
 // ---------------------------------------------------------------------------
 // Any sizes, strides and alignment: tiles of 2 x 2 waves of 32 RB x 32 CB, steps of
 // 128 bytes of K, loaded into registers two steps ahead, put into one LDS buffer
-// while the other one's products run. What is left of K behind the whole steps is a
-// step of its own.
+// while the other one's products run (fp32: one step ahead, one buffer, and two
+// workgroups a CU that overlap). What is left of K behind the whole steps is a step
+// of its own. Bound by the loads, which straddle cache lines where rows are not
+// aligned: bf16 8192 x 4096 x 8192 853 us (503 aligned).
 //
 // fp32 runs on the bf16 matrix cores: a number is three bf16 numbers to within
 // 2^-27 of itself, a product the six bf16 products above 2^-27 of it, 6 x 32 cycles
 // for 16 k of a 32 x 32 block where the fp32 instructions take 8 x 64. The pieces
 // are put into LDS as three 64-byte runs and a gap a row (an odd number of 16-byte
-// groups: the rows of a ds_read_b128 phase fall in distinct banks).
+// groups: the rows of a ds_read_b128 phase fall in distinct banks). 4096 cubed 760
+// us (181 TFLOP/s; fp32 instructions 975, the library 895): with 128 x 128 tiles the
+// splitting, 165 vector instructions a step and wave, takes about as long as the
+// products, and with 64 x 64 LDS is 0.9 busy. Small sizes run fp32 instructions.
 // A number that rounds to a bf16 infinity has the largest bf16 number as its first
 // piece, and an infinity has only a third, so that it meets one piece of the other
 // factor: sums are infinite or NaN as in fp32, but NaN where both factors of a
@@ -321,13 +326,19 @@ __global__ __launch_bounds__(256) void linearTileKernel(LinearArgs a, int rowTil
 
 // ---------------------------------------------------------------------------
 // Rows that are 16-byte aligned (K whole groups of 16 bytes): tiles of WM x WN
-// waves of 32 RB rows x 32 CB columns (KW = 2: twice as many, which share each step's K), steps of 128 bytes of K, whose rows L2 serves
-// in one request (with 64-byte rows its request rate was the limit). A step's rows go from memory to LDS without registers, into the buffer
-// that the last step has left; fragments are read one 32-byte part ahead of their
-// products, over the step's border too: the barrier stands before a step's last
-// part, whose fragments every wave then holds. The buffers are arrays of their
-// own, so that the compiler does not make a fragment read wait for a load in
-// flight to another one.
+// waves of 32 RB rows x 32 CB columns (KW = 2: twice as many, which share each
+// step's K), steps of 128 bytes of K, whose rows L2 serves in one request. (Of 64
+// bytes, in steps of half the K: 13 GB in 208 million requests for 8192 cubed, 0.8
+// of what L2 takes, and 53% of the cycles with products; 0.6 times the rate.)
+// A step's rows go from memory to LDS without registers, into the buffer that the
+// last step has left; fragments are read one 32-byte part ahead of their products,
+// over the step's border too: the barrier stands before a step's last part, whose
+// fragments every wave then holds. The buffers are arrays of their own, so that the
+// compiler does not make a fragment read wait for a load in flight to another one.
+// bf16, us: 8192 x 8192 x 8192 847 (1298 TFLOP/s; the library 781), 8192 x 4096 x
+// 8192 458, with bias, GELU and residual 503 (1092): of a 256 x 256 tile's 117,
+// about 20 are its first loads and its stores, 10 more the residual and GELU. The
+// power limit holds the clock at about 2 GHz.
 template<typename T, int WM, int WN, int KW, int RB, int CB, int PER_CU, int ACT>
 __global__ __launch_bounds__(64 * WM * WN * KW, PER_CU * WM * WN * KW / 4) void linearDmaKernel(LinearArgs a, int rowTiles, int colTiles) {
   typedef typename Vec16<T>::V V;
@@ -495,7 +506,8 @@ void launchDma(const LinearArgs& a, int splits, hipStream_t stream) {
 // and what counts is how many of their bytes are under way. A workgroup has 16 NT
 // output channels; its waves take units of 128 bytes of K in turn (every wave's
 // loads of UNROLL units are issued before the first product), and their sums are
-// added in wave order in LDS.
+// added in wave order in LDS. bf16 8 x 4096 x 8192: 14.4 us, 4.7 TB/s; rows that are
+// not aligned 32, each line read twice.
 template<typename T, int MT, int NT, int WAVES, int UNROLL, int ACT>
 __global__ __launch_bounds__(64 * WAVES) void linearSkinnyKernel(LinearArgs a) {
   typedef typename Vec16<T>::V V;

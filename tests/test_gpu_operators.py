@@ -108,12 +108,12 @@ def test_linear_in_place_residual(dtype, m):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
-@pytest.mark.parametrize("m", [3, 90])
-def test_linear_infinities_stay_in_their_rows(dtype, m):
-    """An infinite or NaN input reaches its own row only, and columns of exact
-    zeros in fp32's own arithmetic."""
-    x, w = _rand(m, 80, dtype=dtype), _rand(48, 80, dtype=dtype, seed=1)
-    x[1, 7], x[2, 9] = float("inf"), float("nan")
+@pytest.mark.parametrize("m,k,pad", [(3, 80, 0), (90, 80, 0), (90, 80, 1), (90, 75, 0), (3, 75, 3)])
+def test_linear_infinities_stay_in_their_rows(dtype, m, k, pad):
+    """An infinite or NaN input reaches its own row only, in a whole step of K and
+    in what is left behind it."""
+    x, w = _rand(m, k, dtype=dtype, pad=pad), _rand(48, k, dtype=dtype, seed=1, pad=pad)
+    x[1, 7 if m == 3 else k - 2], x[2, 9] = float("inf"), float("nan")
     out = torch.empty(m, 48, dtype=dtype, device="cuda")
     _linear(x, w, out)
     want = x.double() @ w.double().t()
@@ -122,6 +122,17 @@ def test_linear_infinities_stay_in_their_rows(dtype, m):
     keep = [i for i in range(m) if i not in (1, 2)]
     y, bound = ref.linear(x[keep], w)
     ref.check(out[keep], (y, bound))
+
+
+@pytest.mark.parametrize("m,pad", [(3, 0), (90, 0), (90, 1)])
+def test_linear_fp32_range(m, pad):
+    """Factors at both ends of fp32: what rounds to infinity in 16 bits, what is
+    too small for three pieces of them, each with sums well inside the range."""
+    x, w = _rand(m, 64, dtype=torch.float32, pad=pad), _rand(40, 64, dtype=torch.float32, seed=1, pad=pad)
+    out = torch.empty(m, 40, dtype=torch.float32, device="cuda")
+    x[1], w[:, :] = x[1].sign() * 3.4e38, w * 1e-3
+    x[0] *= 1e-20
+    ref.check(_linear(x, w * 1e-2, out), ref.linear(x, w * 1e-2))
 
 
 def test_linear_shared_rows_and_far_offsets():

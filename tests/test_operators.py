@@ -2,6 +2,8 @@
 Python calls (no GPU: both look at the arguments before any device is touched),
 and the plain forms that the GPU tests compare with."""
 import ctypes
+import json
+import os
 
 import pytest
 import torch
@@ -114,6 +116,19 @@ def test_c_entries_refuse_null_and_unknown_codes():
     for name, params in (("kgh_linear_workspace", ops._LinearParams), ("kgh_cross_attention_workspace", ops._AttentionParams)):
         assert getattr(lib, name)(0, None, None) == INVALID
         assert getattr(lib, name)(0, params(), None) == INVALID
+
+
+def test_kernels_keep_everything_in_registers():
+    """No kernel of the operators leaves registers for scratch memory, by the
+    compiler's report of the build (see test_host.py's, of the nets' kernels)."""
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "katago_amd", "lib", "kernel_resources.json")
+    with open(path) as f:
+        usage = json.load(f)
+    kernels = ("linearSkinnyKernel", "linearDmaKernel", "linearTileKernel", "linearJoinKernel", "ropeAxesKernel", "attentionFewKernel",
+               "attentionManyKernel", "attentionJoinKernel")
+    for kernel in kernels:
+        found = [u for name, u in usage.items() if kernel in name]
+        assert found and all(u["scratch"] == 0 and u["vgpr_spill"] == 0 for u in found), kernel
 
 
 def test_device_tensor_strides():
