@@ -59,9 +59,10 @@ __device__ __forceinline__ void blockedTile(int rowTiles, int colTiles, int& row
   rowTile = run * 8 + (at - colTile * height);
 }
 
-// XOR swizzle of a row's eight 16-byte groups: the rows that a ds_read_b128 phase
-// reads (eight consecutive ones, the same group) fall in distinct banks.
-__device__ __forceinline__ int swizzled128(int row, int group) { return row * 128 + ((group ^ (row & 7)) << 4); }
+// XOR swizzle of a row's eight 16-byte groups: the sixteen consecutive rows of a
+// ds_read_b128 phase, the same group of each, fall in distinct banks (by row & 7 in
+// place of (row >> 1) & 7, two rows would meet in each).
+__device__ __forceinline__ int swizzled128(int row, int group) { return row * 128 + ((group ^ ((row >> 1) & 7)) << 4); }
 
 // The epilogue of a wave's RB x CB blocks at row mBase, column nBase. The weights
 // are the products' row operand, so a lane has four consecutive columns of row
@@ -359,14 +360,16 @@ __global__ __launch_bounds__(64 * WM * WN * KW, PER_CU * WM * WN * KW / 4) void 
   const int m0 = rowTile * BM, n0 = colTile * BN;
 
   // A load's lane l writes slot l & 7 of row l >> 3 of eight, which holds the
-  // row's group dGroup. Byte offsets of this lane's rows from the tile's first,
+  // row's group dGroup; load i of a wave is of the eight rows i * WAVES + wave, so
+  // that the group is the same for all of them. Byte offsets of this lane's rows from the tile's first,
   // and how far the last step's group lies behind K.
-  const int dRow = lane >> 3, dGroup = (lane & 7) ^ dRow;
+  const int dRow = lane >> 3, dGroup = (lane & 7) ^ ((dRow >> 1) | ((wave & 1) << 2));
+  static_assert(WAVES % 2 == 0, "a wave's rows of eight are all even or all odd");
   unsigned aOff[A_PER], bOff[B_PER];
 #pragma unroll
-  for(int i = 0; i < A_PER; i++) aOff[i] = (unsigned)(min(8 * (wave * A_PER + i) + dRow, a.M - 1 - m0) * a.ldx * SIZE) + dGroup * 16;
+  for(int i = 0; i < A_PER; i++) aOff[i] = (unsigned)(min(8 * (i * WAVES + wave) + dRow, a.M - 1 - m0) * a.ldx * SIZE) + dGroup * 16;
 #pragma unroll
-  for(int i = 0; i < B_PER; i++) bOff[i] = (unsigned)(min(8 * (wave * B_PER + i) + dRow, a.N - 1 - n0) * a.ldw * SIZE) + dGroup * 16;
+  for(int i = 0; i < B_PER; i++) bOff[i] = (unsigned)(min(8 * (i * WAVES + wave) + dRow, a.N - 1 - n0) * a.ldw * SIZE) + dGroup * 16;
   const int k0 = blockIdx.y * a.chunk;
   const int kEnd = min(k0 + a.chunk, a.K);
   const int last = (kEnd - k0 - 1) / STEP;
@@ -386,10 +389,10 @@ __global__ __launch_bounds__(64 * WM * WN * KW, PER_CU * WM * WN * KW / 4) void 
     const unsigned back = st >= last ? past : 0;
 #pragma unroll
     for(int i = 0; i < A_PER; i++)
-      __builtin_amdgcn_global_load_lds((const void*)(xTile + at + (aOff[i] - back)), (lds_void_t*)(aBuf(buf.value) + (wave * A_PER + i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const void*)(xTile + at + (aOff[i] - back)), (lds_void_t*)(aBuf(buf.value) + (i * WAVES + wave) * 1024), 16, 0, 0);
 #pragma unroll
     for(int i = 0; i < B_PER; i++)
-      __builtin_amdgcn_global_load_lds((const void*)(wTile + at + (bOff[i] - back)), (lds_void_t*)(bBuf(buf.value) + (wave * B_PER + i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const void*)(wTile + at + (bOff[i] - back)), (lds_void_t*)(bBuf(buf.value) + (i * WAVES + wave) * 1024), 16, 0, 0);
   };
 
   floatx16 acc[RB][CB];
