@@ -64,6 +64,26 @@ __device__ __forceinline__ void blockedTile(int rowTiles, int colTiles, int& row
 // place of (row >> 1) & 7, two rows would meet in each).
 __device__ __forceinline__ int swizzled128(int row, int group) { return row * 128 + ((group ^ ((row >> 1) & 7)) << 4); }
 
+// Two groups of four columns, bias and activation, and the residual's 16 bytes of
+// this lane's columns, to the 16 bytes of the same columns.
+template<typename T, int ACT>
+__device__ __forceinline__ uint4 finishGroup(floatx4 v0, floatx4 v1, floatx4 b0, floatx4 b1, uint4 res) {
+  const uint2 r01 = swapHalves(res.x, res.z), r23 = swapHalves(res.y, res.w);
+  union Four {
+    uint2 v;
+    T e[4];
+  } ra[2], oa[2];
+  ra[0].v = make_uint2(r01.x, r23.x);
+  ra[1].v = make_uint2(r01.y, r23.y);
+#pragma unroll
+  for(int e = 0; e < 4; e++) {
+    oa[0].e[e] = (T)(linActivate<T, ACT>(v0[e] + b0[e]) + (float)ra[0].e[e]);
+    oa[1].e[e] = (T)(linActivate<T, ACT>(v1[e] + b1[e]) + (float)ra[1].e[e]);
+  }
+  const uint2 o01 = swapHalves(oa[0].v.x, oa[1].v.x), o23 = swapHalves(oa[0].v.y, oa[1].v.y);
+  return make_uint4(o01.x, o23.x, o01.y, o23.y);
+}
+
 // The epilogue of a wave's RB x CB blocks at row mBase, column nBase. The weights
 // are the products' row operand, so a lane has four consecutive columns of row
 // laneRow, and its partner lane ^ 32 the four behind them; in 16 bits two such
@@ -73,6 +93,44 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
   const int lane = threadIdx.x & 63, laneRow = lane & 31, half = lane >> 5;
   const T* res = (const T*)a.residual;
   T* out = (T*)a.out;
+  if constexpr(sizeof(T) == 2) {
+    // A block that lies inside the result: all of the residual is under way before
+    // the first of it is used.
+    if(mBase + 32 * RB <= a.M && nBase + 32 * CB <= a.N && a.part == nullptr) {
+      u32x4_t rv[RB][CB][2];
+#pragma unroll
+      for(int i = 0; i < RB; i++)
+#pragma unroll
+        for(int j = 0; j < CB; j++)
+#pragma unroll
+          for(int p = 0; p < 2; p++) {
+            rv[i][j][p] = u32x4_t{0, 0, 0, 0};
+            if(res != nullptr)
+              __builtin_memcpy(&rv[i][j][p], res + (int64_t)(mBase + i * 32 + laneRow) * a.ldr + nBase + j * 32 + (2 * p + half) * 8, 16);
+          }
+#pragma unroll
+      for(int j = 0; j < CB; j++) {
+        const int nj = nBase + j * 32;
+        floatx4 bias[4];
+#pragma unroll
+        for(int q = 0; q < 4; q++) {
+          bias[q] = (floatx4)0.0f;
+          if(a.bias != nullptr) __builtin_memcpy(&bias[q], a.bias + nj + q * 8 + half * 4, 16);
+        }
+#pragma unroll
+        for(int i = 0; i < RB; i++)
+#pragma unroll
+          for(int p = 0; p < 2; p++) {
+            const u32x4_t r = rv[i][j][p];
+            const floatx4 v0 = {acc[i][j][8 * p], acc[i][j][8 * p + 1], acc[i][j][8 * p + 2], acc[i][j][8 * p + 3]};
+            const floatx4 v1 = {acc[i][j][8 * p + 4], acc[i][j][8 * p + 5], acc[i][j][8 * p + 6], acc[i][j][8 * p + 7]};
+            const uint4 o = finishGroup<T, ACT>(v0, v1, bias[2 * p], bias[2 * p + 1], make_uint4(r.x, r.y, r.z, r.w));
+            __builtin_memcpy(out + (int64_t)(mBase + i * 32 + laneRow) * a.ldo + nj + (2 * p + half) * 8, &o, 16);
+          }
+      }
+      return;
+    }
+  }
 #pragma unroll
   for(int j = 0; j < CB; j++) {
     const int nj = nBase + j * 32;
@@ -118,22 +176,11 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
         }
 #pragma unroll
         for(int p = 0; p < 2; p++) {
-          // Groups q = 2 p and 2 p + 1 of four columns each.
-          const uint2 r01 = swapHalves(rv[p].x, rv[p].z), r23 = swapHalves(rv[p].y, rv[p].w);
-          union Four {
-            uint2 v;
-            T e[4];
-          } ra[2], oa[2];
-          ra[0].v = make_uint2(r01.x, r23.x);
-          ra[1].v = make_uint2(r01.y, r23.y);
-#pragma unroll
-          for(int q = 0; q < 2; q++)
-#pragma unroll
-            for(int e = 0; e < 4; e++)
-              oa[q].e[e] = (T)(linActivate<T, ACT>(acc[i][j][(2 * p + q) * 4 + e] + bias[2 * p + q][e]) + (float)ra[q].e[e]);
-          const uint2 o01 = swapHalves(oa[0].v.x, oa[1].v.x), o23 = swapHalves(oa[0].v.y, oa[1].v.y);
+          const floatx4 v0 = {acc[i][j][8 * p], acc[i][j][8 * p + 1], acc[i][j][8 * p + 2], acc[i][j][8 * p + 3]};
+          const floatx4 v1 = {acc[i][j][8 * p + 4], acc[i][j][8 * p + 5], acc[i][j][8 * p + 6], acc[i][j][8 * p + 7]};
+          const uint4 o = finishGroup<T, ACT>(v0, v1, bias[2 * p], bias[2 * p + 1], rv[p]);
           const int n = nj + (2 * p + half) * 8;
-          if(m < a.M && n < a.N) storeGroup(out + (int64_t)m * a.ldo + n, make_uint4(o01.x, o23.x, o01.y, o23.y), a.N - n);
+          if(m < a.M && n < a.N) storeGroup(out + (int64_t)m * a.ldo + n, o, a.N - n);
         }
       }
     }
