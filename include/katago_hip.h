@@ -310,9 +310,11 @@ int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_strea
  * key_mask[b][j] != 0 (either may be NULL; lengths are taken into
  * 0..k_len). What k and v hold at other keys is not used, whatever it is. A row
  * without a key, or whose every score is minus infinity, is zeros. Head dims are
- * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and
- * finite. */
+ * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and at
+ * most KGH_ATTENTION_MAX_SCALE. Scores are taken to base 2 in fp32: one that
+ * passes the largest float divided by log2(e) counts as infinite. */
 #define KGH_ATTENTION_MAX_HEAD_DIM 128
+#define KGH_ATTENTION_MAX_SCALE 1e30f
 typedef struct kgh_attention_params {
   int32_t dtype; /* KGH_DTYPE_* of q, k, v and out */
   int32_t batch, q_len, k_len;

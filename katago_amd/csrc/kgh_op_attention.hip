@@ -104,6 +104,10 @@ struct ValueReads {
 // One row's running softmax: p = 2^(s c - ref), with a reference point that only
 // moves when a tile's maximum passes it by more than 8 (p is at most 256, summed
 // in fp32; the normalisation by the sum of the same p makes the choice cancel).
+// In fp16 p is 2^7 times that: as large as the type allows, so that many keys of
+// little weight each are not lost below its smallest numbers.
+template<typename T>
+constexpr float P_SHIFT = sizeof(T) == 2 && !__is_same(T, bf16_t) ? 7.0f : 0.0f;
 struct RowState {
   float ref = -INFINITY, sum = 0.0f;
 };
@@ -125,7 +129,7 @@ __device__ __forceinline__ void maskTile(floatx16 (&s)[BLOCKS], unsigned long lo
 
 // The scores of BLOCKS * 32 keys become p; returns what the accumulators before
 // them are to be multiplied by.
-template<int BLOCKS>
+template<typename T, int BLOCKS>
 __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], float scaleLog2, RowState& row) {
   float top = -INFINITY;
 #pragma unroll
@@ -138,7 +142,7 @@ __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], float scaleL
   const float corr = ref == row.ref ? 1.0f : __builtin_amdgcn_exp2f(row.ref - ref);
   row.ref = ref;
   // While a row has met no score above -inf its offset is 0: every p is 0.
-  const float off = ref == -INFINITY ? 0.0f : -ref;
+  const float off = ref == -INFINITY ? 0.0f : P_SHIFT<T> - ref;
   float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for(int kb = 0; kb < BLOCKS; kb++)
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
 #pragma unroll
     for(int i = 0; i < D / VEC / 2; i++) s[0] = mma32(*(const V*)(ks + kAt<T, D>(laneRow, 2 * i + half)), qf[i], s[0]);
     maskTile<1>(s, valid);
-    const float corr = softmaxTile<1>(s, a.scaleLog2, row);
+    const float corr = softmaxTile<T, 1>(s, a.scaleLog2, row);
     if(__any(corr != 1.0f)) {
 #pragma unroll
       for(int db = 0; db < D / 32; db++)
@@ -474,7 +478,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionM
     maskTile<BLOCKS>(s, bits);
     __builtin_amdgcn_sched_barrier(0);
     scores(kNext, sNext);
-    const float corr = softmaxTile<BLOCKS>(s, a.scaleLog2, row);
+    const float corr = softmaxTile<T, BLOCKS>(s, a.scaleLog2, row);
     V p[GROUPS_P];
 #pragma unroll
     for(int g = 0; g < GROUPS_P; g++) {
@@ -675,7 +679,7 @@ void checkAttention(const kgh_attention_params& p, bool pointers) {
   if(p.kv_heads < 1 || p.heads < 1 || p.heads % p.kv_heads != 0) opInvalid(op, "kv_heads must divide heads");
   for(int d : {p.q_head_dim, p.v_head_dim})
     if(d < 1 || d > KGH_ATTENTION_MAX_HEAD_DIM) opInvalid(op, "head dim " + std::to_string(d) + " outside 1.." + std::to_string(KGH_ATTENTION_MAX_HEAD_DIM));
-  if(!(p.scale > 0.0f) || !std::isfinite(p.scale)) opInvalid(op, "scale must be positive and finite");
+  if(!(p.scale > 0.0f) || p.scale > KGH_ATTENTION_MAX_SCALE) opInvalid(op, "scale must be positive and at most 1e30");
   for(int64_t s : {p.q_batch_stride, p.q_token_stride, p.q_head_stride, p.k_batch_stride, p.k_token_stride, p.k_head_stride, p.v_batch_stride,
                    p.v_token_stride, p.v_head_stride, p.out_batch_stride, p.out_token_stride, p.out_head_stride, p.key_mask_stride})
     if(s < 0) opInvalid(op, "negative stride");
@@ -701,6 +705,9 @@ void checkAttention(const kgh_attention_params& p, bool pointers) {
   }
   if(p.key_lengths != nullptr) opCheckPointer(op, "key_lengths", p.key_lengths, 4);
   if(p.workspace != nullptr) opCheckPointer(op, "workspace", p.workspace, 16);
+  opCheckApart(op, "q", p.q, p.out);
+  opCheckApart(op, "k", p.k, p.out);
+  opCheckApart(op, "v", p.v, p.out);
 }
 
 namespace {

@@ -714,6 +714,9 @@ void checkLinear(const kgh_linear_params& p, bool pointers) {
   if(p.residual != nullptr) opCheckPointer(op, "residual", p.residual, e);
   if(p.bias != nullptr) opCheckPointer(op, "bias", p.bias, 4);
   if(p.workspace != nullptr) opCheckPointer(op, "workspace", p.workspace, 16);
+  opCheckApart(op, "x", p.x, p.out);
+  opCheckApart(op, "weights", p.weights, p.out);
+  if(p.residual == p.out && p.rows > 1 && p.residual_stride != p.out_stride) opInvalid(op, "in place, residual_stride must be out_stride");
 }
 
 namespace {

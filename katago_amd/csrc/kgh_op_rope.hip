@@ -5,6 +5,8 @@
 
 namespace {
 
+constexpr int64_t ROPE_MAX_TOKENS = (int64_t)1 << 32;
+
 struct RopeArgs {
   const void* x;
   void* out;
@@ -156,9 +158,11 @@ void checkRope(const kgh_rope_params& p) {
   opCheckDtype(op, p.dtype);
   if(p.layout != KGH_ROPE_INTERLEAVED && p.layout != KGH_ROPE_HALVES) opInvalid(op, "layout " + std::to_string(p.layout) + " is none of KGH_ROPE_*");
   if(p.axes < 1 || p.axes > KGH_ROPE_MAX_AXES) opInvalid(op, "axes " + std::to_string(p.axes) + " outside 1.." + std::to_string(KGH_ROPE_MAX_AXES));
-  if(p.tokens < 0) opInvalid(op, "negative number of tokens");
+  if(p.tokens < 0 || p.tokens > ROPE_MAX_TOKENS) opInvalid(op, "tokens " + std::to_string(p.tokens) + " outside 0.." + std::to_string(ROPE_MAX_TOKENS));
   if(p.heads < 1 || p.head_dim < 1 || p.pairs < 1 || p.head_dim > (1 << 20)) opInvalid(op, "heads, head_dim and pairs must be positive (head_dim at most 2^20)");
   if(2 * (int64_t)p.pairs > p.head_dim) opInvalid(op, "a head of " + std::to_string(p.head_dim) + " channels has no " + std::to_string(p.pairs) + " pairs");
+  // A launch takes 2^32 groups of channels; so many are no tensor either.
+  if((double)p.tokens * p.heads * p.head_dim > 1099511627776.0) opInvalid(op, "too many tokens for one call");
   if(p.tables < 1 || p.heads % p.tables != 0) opInvalid(op, "tables must divide heads");
   if(p.x_token_stride < 0 || p.x_head_stride < 0 || p.positions_stride < 0) opInvalid(op, "negative stride");
   if(p.tokens == 0) return;

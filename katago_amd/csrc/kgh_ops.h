@@ -43,6 +43,10 @@ inline void opCheckPointer(const char* op, const char* name, const void* p, size
   if(p == nullptr) opInvalid(op, std::string(name) + " is null");
   if((uintptr_t)p % elem != 0) opInvalid(op, std::string(name) + " is not aligned to its elements");
 }
+// An input that the output must not overlap.
+inline void opCheckApart(const char* op, const char* name, const void* in, const void* out) {
+  if(in == out) opInvalid(op, std::string("out is ") + name + " itself");
+}
 // Calls f(T()) for the element type of dtype.
 template<typename F>
 void withDtype(int dtype, F&& f) {

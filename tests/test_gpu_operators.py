@@ -2,6 +2,7 @@
 the sizes, strides and masks where their tiles, tails and softmax can go wrong,
 and as a program runs them: together, on its own stream, captured and replayed,
 in place, without torch. Bounds: operator_reference.py."""
+import math
 import threading
 
 import pytest
@@ -333,6 +334,27 @@ def test_attention_non_finite_keys_that_take_part(dtype, lq):
     assert out[1, :, 0].isnan().all() and not out[1, :, 1].isnan().any()
     assert not out[2].any()
     ref.check(out[3:], want)
+
+
+@pytest.mark.parametrize("lq", [1, 40, 300])
+def test_attention_many_keys_of_little_weight(lq):
+    """One key with nearly all of the weight and a value of 0, and 1999 with 2^-24.5
+    of its weight each and values of 1: below fp16's smallest numbers, were the
+    largest p 1. It is at least 2^7, so a p is off by half of fp16's smallest number
+    over 2^7, besides its own rounding; the scores are exact but for the float that
+    the product with the scale gives (2^-23 of 24.5)."""
+    q, k, v = torch.zeros(1, lq, 2, 64), torch.zeros(1, 2000, 2, 64), torch.ones(1, 2000, 2, 64)
+    q[..., 0] = 1.0
+    k[:, 700, :, 0] = 16.984375
+    v[:, 700] = 0.0
+    q, k, v = (t.half().cuda() for t in (q, k, v))
+    out = torch.empty_like(q)
+    for workspace in (False, True):
+        space = torch.empty(ops.cross_attention_workspace(q, k, v) * workspace, dtype=torch.uint8, device="cuda")
+        ops.cross_attention(q, k, v, out, scale=1.0, workspace=space if len(space) else None, stream=_stream())
+        want = 1999.0 / (1999.0 + math.exp(16.984375))
+        bound = 2000 * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -17) + 2.0 ** -25
+        assert (out.double() - want).abs().max().item() <= bound
 
 
 def test_attention_far_offsets():

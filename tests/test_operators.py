@@ -118,6 +118,28 @@ def test_c_entries_refuse_null_and_unknown_codes():
         assert getattr(lib, name)(0, params(), None) == INVALID
 
 
+def test_outputs_on_inputs_are_refused():
+    far = dict(at=2 * AT)
+    _refused(_linear(x=Meta(4, 8), weights=Meta(8, 8, **far)), "x itself")
+    _refused(_linear(x=Meta(8, 8, **far), weights=Meta(8, 8), out=Meta(8, 8)), "weights itself")
+    _refused(_linear(x=Meta(4, 16, **far), weights=Meta(8, 16, **far), residual=Meta(4, 8, strides=(16, 1))), "residual_stride")
+    _refused(_attention(k=Meta(2, 9, 2, 32, **far), v=Meta(2, 9, 2, 24, **far)), "q itself")
+    _refused(_attention(q=Meta(2, 3, 4, 32, **far), v=Meta(2, 9, 2, 24, **far)), "k itself")
+    _refused(_attention(q=Meta(2, 3, 4, 32, **far), k=Meta(2, 9, 2, 32, **far)), "v itself")
+
+
+def test_largest_sizes_are_refused_in_64_bits():
+    """Sizes of the C entries whose counts pass 64 bits."""
+    lib = ops._library()
+    p = ops._RopeParams(0, 0, 0, 1, 1 << 62, 4, 64, 32, 1, AT, 64, 64, AT, 1, AT, 2 * AT, 256, 64)
+    for tokens, heads, dim in ((1 << 62, 4, 64), (1 << 32, (1 << 31) - 1, 1 << 20), (1 << 20, 1 << 20, 64)):
+        p.tokens, p.heads, p.head_dim = tokens, heads, dim
+        p.out_head_stride, p.out_token_stride = dim, heads * dim
+        assert lib.kgh_rope_axes(0, p, None) == INVALID
+        assert b"tokens" in lib.kgh_last_error()
+    _refused(_attention(scale=1e31), "scale")
+
+
 def test_kernels_keep_everything_in_registers():
     """No kernel of the operators leaves registers for scratch memory, by the
     compiler's report of the build (see test_host.py's, of the nets' kernels)."""
