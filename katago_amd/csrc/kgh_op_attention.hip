@@ -332,16 +332,17 @@ constexpr int64_t ATT_NEAR = 1 << 23;  // token strides below it: 64 of them are
 constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
 
 // 32-key blocks of a tile: one where two would not leave registers for the reads
-// ahead (4096 queries to 5000 keys, heads of 128: 822 us, two 1064).
+// ahead (16 bits, 4096 queries to 5000 keys, heads of 128: 822 us, two 1064); and
+// in fp32, heads up to 64, where one lets a CU hold two workgroups (`pairs`).
 template<typename T, int D>
-constexpr int attBlocks() { return sizeof(T) == 2 && D == 128 ? 1 : 2; }
+constexpr int attBlocks(bool pairs) { return pairs || (sizeof(T) == 2 && D == 128) ? 1 : 2; }
 __device__ __forceinline__ constexpr unsigned long long attWhole(int blocks) { return blocks == 2 ? ~0ull : 0xffffffffull; }
 
-template<typename T, int D, int WAVES, bool FULL>
-__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 2 : 1) void attentionManyKernel(AttnArgs a, AttnSplit split) {
+template<typename T, int D, int WAVES, bool FULL, bool PAIRS = sizeof(T) == 2>
+__global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;
   constexpr int THREADS = 64 * WAVES;
-  constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, BLOCKS = attBlocks<T, D>(), KEYS = 32 * BLOCKS, LOADS = KEYS * GROUPS / THREADS;
+  constexpr int VEC = 16 / (int)sizeof(T), GROUPS = D / VEC, BLOCKS = attBlocks<T, D>(sizeof(T) == 4 && PAIRS), KEYS = 32 * BLOCKS, LOADS = KEYS * GROUPS / THREADS;
   static_assert(LOADS * THREADS == KEYS * GROUPS && THREADS % GROUPS == 0, "whole loads");
   constexpr int TILE = KEYS * D * (int)sizeof(T);
   __shared__ __attribute__((aligned(16))) unsigned char k0s[TILE];
@@ -715,6 +716,7 @@ namespace {
 struct AttentionPlan {
   bool few;   // at most 32 rows a kv head
   int waves;  // of the kernel for more
+  bool pairs; // fp32: of its variant with two workgroups a CU
   int splits; // of the keys
   int64_t rows;
 };
@@ -730,6 +732,9 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   const bool wide = rows >= 512 && rows * 8 >= (rows + 255) / 256 * 256 * 7;
   plan.waves = p.dtype != KGH_DTYPE_FP32 && wide && std::max(p.q_head_dim, p.v_head_dim) > 32 ? 8 : 4;
   const int64_t groups = plan.few ? (int64_t)p.batch * p.kv_heads : (rows + plan.waves * 32 - 1) / (plan.waves * 32) * p.batch * p.kv_heads;
+  // Where there are more workgroups than CUs: 16 boards of 361 queries and keys, 6
+  // heads of 64, 63 us (73 with one a CU and 64 keys a tile), of 32 36.6 (37.3).
+  plan.pairs = p.dtype == KGH_DTYPE_FP32 && groups > 256 && std::max(p.q_head_dim, p.v_head_dim) <= 64;
   // Workgroups that the CUs hold at a time: two a CU of the kernel for few rows in
   // 16 bits, one of the others; and at least 128 keys a split. One query of 8 kv
   // heads to 16384 keys, us: whole 306, 8 splits 47, 32 21.6, 64 22.1; of 32
@@ -751,6 +756,7 @@ void runAttention(const AttentionPlan& plan, const AttnArgs& a, const AttnSplit&
   const int64_t rows = (int64_t)a.lq * (a.heads / a.kvHeads), block = plan.waves * 32;
   const dim3 grid((unsigned)((plan.few ? 1 : (rows + block - 1) / block) * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
   if(plan.few) attentionFewKernel<T, D, FULL><<<grid, 256, 0, stream>>>(a, split);
+  else if(sizeof(T) == 4 && D <= 64 && plan.pairs) attentionManyKernel<T, D, 4, FULL, sizeof(T) == 2 || D <= 64><<<grid, 256, 0, stream>>>(a, split);
   else if(plan.waves == 4) attentionManyKernel<T, D, 4, FULL><<<grid, 256, 0, stream>>>(a, split);
   else if constexpr(sizeof(T) == 2 && D >= 64) attentionManyKernel<T, D, 8, FULL><<<grid, 512, 0, stream>>>(a, split);
   KGH_CHECK_LAUNCH();

@@ -336,6 +336,22 @@ def test_attention_non_finite_keys_that_take_part(dtype, lq):
     ref.check(out[3:], want)
 
 
+@pytest.mark.parametrize("b,lq,lk,d,kind", [(90, 40, 70, 64, "none"), (90, 40, 700, 33, "mask"), (44, 130, 97, 32, "lengths"), (44, 129, 33, 20, "none"),
+                                            (90, 33, 31, 64, "lengths")])
+def test_attention_fp32_of_more_workgroups_than_cus(b, lq, lk, d, kind):
+    q, k, v = (_rand(b, n, 3, d, dtype=torch.float32, seed=s, scale=1.5) for n, s in ((lq, 1), (lk, 2), (lk, 3)))
+    lengths = mask = None
+    if kind == "lengths":
+        lengths = (torch.arange(b, dtype=torch.int32, device="cuda") * 7) % (lk + 1)
+    if kind == "mask":
+        mask = torch.rand(b, lk, device="cuda", generator=torch.Generator("cuda").manual_seed(4)) < 0.5
+        mask[1] = False
+        mask[2, 64:640] = False
+    out = torch.empty_like(q)
+    _attention(q, k, v, out, key_lengths=lengths, key_mask=mask)
+    ref.check(out, ref.attention(q, k, v, lengths=lengths, mask=mask))
+
+
 @pytest.mark.parametrize("lq", [1, 40, 300])
 def test_attention_many_keys_of_little_weight(lq):
     """One key with nearly all of the weight and a value of 0, and 1999 with 2^-24.5
