@@ -13,8 +13,8 @@ struct RopeArgs {
   const int32_t* positions;
   const float* freqs;
   int64_t xToken, xHead, outToken, outHead, ldPos;
-  int64_t items;  // tokens x head runs x groups
-  int heads, dim, pairs, axes, tables, headRun, headRuns, groups, pairGroups;
+  int64_t tokens, items;  // items: token runs x head runs x groups
+  int heads, dim, pairs, axes, tables, tokenRun, headRun, headRuns, groups, pairGroups;
   float sign;
 };
 
@@ -29,26 +29,79 @@ __device__ __forceinline__ void sinCosTurns(float turns, float& s, float& c) {
   }
 }
 
+// The first n elements of v (n may be none), in as few stores as they have bits.
+template<typename T>
+__device__ __forceinline__ void storeParts(T* p, u32x4_t v, int n) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  if(n >= VEC) {
+    __builtin_memcpy(p, &v, 16);
+    return;
+  }
+  if(n >= VEC / 2) {
+    const uint2 u = make_uint2(v.x, v.y);
+    __builtin_memcpy(p, &u, 8);
+    p += VEC / 2;
+    n -= VEC / 2;
+    v.x = v.z;
+    v.y = v.w;
+  }
+  if(n >= VEC / 4) {
+    const unsigned u = v.x;
+    __builtin_memcpy(p, &u, 4);
+    p += VEC / 4;
+    n -= VEC / 4;
+    v.x = v.y;
+  }
+  if(sizeof(T) == 2 && n > 0) {
+    const unsigned short u = (unsigned short)v.x;
+    __builtin_memcpy(p, &u, 2);
+  }
+}
+
 // A thread takes VEC pairs (two 16-byte groups) of a token, or as many of the
 // channels behind the pairs, and a run of heads that share a table: the angles
 // are computed once for the run, whose rows are loaded ROPE_AHEAD heads at a time.
+// Or (TOKENS) it takes them of a run of up to ROPE_AHEAD tokens of one head, for
+// which the frequencies are loaded once.
 // Bound by the tensor's way in and out of memory where a run has four heads and
 // more, else by the angles (about 130 cycles for 64 pairs).
 constexpr int ROPE_AHEAD = 4;
 
-template<typename T, bool HALVES, int AXES>
+template<typename T, bool HALVES, int AXES, bool TOKENS>
 __global__ __launch_bounds__(256) void ropeAxesKernel(RopeArgs a) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if(id >= a.items) return;
   const int64_t rest = id / a.groups;
   const int group = (int)(id - rest * a.groups);
-  const int64_t token = rest / a.headRuns;
-  const int h0 = (int)(rest - token * a.headRuns) * a.headRun;
+  const int64_t tokens = rest / a.headRuns, token = TOKENS ? tokens * a.tokenRun : tokens;
+  const int h0 = (int)(rest - tokens * a.headRuns) * a.headRun;
   const bool turns = group < a.pairGroups;
   // The two groups' first channels, and their lengths.
   int c0, c1, n0, n1;
-  float cs[VEC], sn[VEC];
+  float f[VEC * AXES], cs[VEC], sn[VEC];
+  struct Position {
+    int at[AXES];
+  };
+  auto position = [&](int64_t t, Position& p) {
+#pragma unroll
+    for(int x = 0; x < AXES; x++) p.at[x] = a.positions[t * a.ldPos + x];
+  };
+  auto angles = [&](const Position& p) {
+    double pos[AXES];
+#pragma unroll
+    for(int x = 0; x < AXES; x++) pos[x] = (double)p.at[x];
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      double angle = 0.0;
+#pragma unroll
+      for(int x = 0; x < AXES; x++) angle = fma(pos[x], (double)f[j * AXES + x], angle);
+      // Far positions turn many times: whole turns are taken off in 64 bits.
+      const double t = angle * 0.15915494309189533577;
+      sinCosTurns<T>((float)(t - rint(t)), sn[j], cs[j]);
+      sn[j] *= a.sign;
+    }
+  };
   if(turns) {
     const int p0 = group * VEC;
     const int np = min(VEC, a.pairs - p0);
@@ -65,24 +118,15 @@ __global__ __launch_bounds__(256) void ropeAxesKernel(RopeArgs a) {
     }
     const int table = h0 / (a.heads / a.tables);
     const float* src = a.freqs + ((int64_t)table * a.pairs + p0) * AXES;
-    float f[VEC * AXES];
     if(np == VEC) __builtin_memcpy(f, src, sizeof(f));
     else {
 #pragma unroll
       for(int j = 0; j < VEC * AXES; j++) f[j] = j < np * AXES ? src[j] : 0.0f;
     }
-    double pos[AXES];
-#pragma unroll
-    for(int x = 0; x < AXES; x++) pos[x] = (double)a.positions[token * a.ldPos + x];
-#pragma unroll
-    for(int j = 0; j < VEC; j++) {
-      double angle = 0.0;
-#pragma unroll
-      for(int x = 0; x < AXES; x++) angle = fma(pos[x], (double)f[j * AXES + x], angle);
-      // Far positions turn many times: whole turns are taken off in 64 bits.
-      const double t = angle * 0.15915494309189533577;
-      sinCosTurns<T>((float)(t - rint(t)), sn[j], cs[j]);
-      sn[j] *= a.sign;
+    if(!TOKENS) {
+      Position p;
+      position(token, p);
+      angles(p);
     }
   }
   else {
@@ -108,45 +152,76 @@ __global__ __launch_bounds__(256) void ropeAxesKernel(RopeArgs a) {
       e1 = (T)y1;
     }
   };
-  const int h1 = min(h0 + a.headRun, a.heads);
-  if(n0 == VEC && n1 == VEC) {
-    for(int h = h0; h < h1; h += ROPE_AHEAD) {
+  // The run's rows: heads h0.. of the token, or tokens of head h0.
+  const int64_t xStep = TOKENS ? a.xToken : a.xHead, outStep = TOKENS ? a.outToken : a.outHead;
+  const int rows = TOKENS ? (int)min((int64_t)a.tokenRun, a.tokens - token) : min(a.headRun, a.heads - h0);
+  src += h0 * a.xHead;
+  dst += h0 * a.outHead;
+  if(a.dim >= VEC) {
+    // 16 bytes that lie in the row wherever a group ends, moved to their places
+    // (what other threads write beside them is not used).
+    const int at0 = min(c0, a.dim - VEC), at1 = min(c1, a.dim - VEC);
+    const int drop0 = c0 - at0, drop1 = n1 > 0 ? c1 - at1 : 0;
+    auto drop = [](Group& g, int n) {
+#pragma unroll 1
+      for(int i = 0; i < n; i++) {
+        const uint4 w = shiftDown<T>(make_uint4(g.v.x, g.v.y, g.v.z, g.v.w));
+        g.v = u32x4_t{w.x, w.y, w.z, w.w};
+      }
+    };
+    for(int r = 0; r < rows; r += ROPE_AHEAD) {
       Group u[ROPE_AHEAD][2];
+      Position p[ROPE_AHEAD];
 #pragma unroll
       for(int i = 0; i < ROPE_AHEAD; i++) {
-        const T* row = src + min(h + i, h1 - 1) * a.xHead;
-        __builtin_memcpy(&u[i][0].v, row + c0, 16);
-        __builtin_memcpy(&u[i][1].v, row + c1, 16);
+        if(TOKENS) position(token + min(r + i, rows - 1), p[i]);
+        const T* row = src + min(r + i, rows - 1) * xStep;
+        __builtin_memcpy(&u[i][0].v, row + at0, 16);
+        __builtin_memcpy(&u[i][1].v, row + at1, 16);
       }
 #pragma unroll
       for(int i = 0; i < ROPE_AHEAD; i++) {
-        if(h + i >= h1) break;
-        T* row = dst + (h + i) * a.outHead;
+        if(r + i >= rows) break;
+        T* row = dst + (r + i) * outStep;
+        if(TOKENS && turns) angles(p[i]);
+        drop(u[i][0], drop0);
+        drop(u[i][1], drop1);
         if(turns) turn(u[i][0], u[i][1]);
-        __builtin_memcpy(row + c0, &u[i][0].v, 16);
-        __builtin_memcpy(row + c1, &u[i][1].v, 16);
+        storeParts(row + c0, u[i][0].v, n0);
+        storeParts(row + c1, u[i][1].v, n1);
       }
     }
     return;
   }
-  for(int h = h0; h < h1; h++) {
+  for(int r = 0; r < rows; r++) {
     Group u0, u1;
-    const uint4 v0 = loadGroupSmall(src + h * a.xHead + c0, n0), v1 = loadGroupSmall(src + h * a.xHead + c1, n1);
+    const uint4 v0 = loadGroupSmall(src + r * xStep + c0, n0), v1 = loadGroupSmall(src + r * xStep + c1, n1);
     u0.v = u32x4_t{v0.x, v0.y, v0.z, v0.w};
     u1.v = u32x4_t{v1.x, v1.y, v1.z, v1.w};
+    if(TOKENS && turns) {
+      Position p;
+      position(token + r, p);
+      angles(p);
+    }
     if(turns) turn(u0, u1);
-    storeGroup(dst + h * a.outHead + c0, make_uint4(u0.v.x, u0.v.y, u0.v.z, u0.v.w), n0);
-    storeGroup(dst + h * a.outHead + c1, make_uint4(u1.v.x, u1.v.y, u1.v.z, u1.v.w), n1);
+    storeGroup(dst + r * outStep + c0, make_uint4(u0.v.x, u0.v.y, u0.v.z, u0.v.w), n0);
+    storeGroup(dst + r * outStep + c1, make_uint4(u1.v.x, u1.v.y, u1.v.z, u1.v.w), n1);
   }
+}
+
+template<typename T, bool HALVES, int AXES>
+void launchRuns(const RopeArgs& a, int64_t blocks, hipStream_t stream) {
+  const dim3 grid((unsigned)blocks);
+  if(a.tokenRun > 1) ropeAxesKernel<T, HALVES, AXES, true><<<grid, 256, 0, stream>>>(a);
+  else ropeAxesKernel<T, HALVES, AXES, false><<<grid, 256, 0, stream>>>(a);
 }
 
 template<typename T, bool HALVES>
 void launchAxes(const RopeArgs& a, int64_t blocks, hipStream_t stream) {
-  const dim3 grid((unsigned)blocks);
-  if(a.axes == 1) ropeAxesKernel<T, HALVES, 1><<<grid, 256, 0, stream>>>(a);
-  else if(a.axes == 2) ropeAxesKernel<T, HALVES, 2><<<grid, 256, 0, stream>>>(a);
-  else if(a.axes == 3) ropeAxesKernel<T, HALVES, 3><<<grid, 256, 0, stream>>>(a);
-  else ropeAxesKernel<T, HALVES, 4><<<grid, 256, 0, stream>>>(a);
+  if(a.axes == 1) launchRuns<T, HALVES, 1>(a, blocks, stream);
+  else if(a.axes == 2) launchRuns<T, HALVES, 2>(a, blocks, stream);
+  else if(a.axes == 3) launchRuns<T, HALVES, 3>(a, blocks, stream);
+  else launchRuns<T, HALVES, 4>(a, blocks, stream);
 }
 
 }  // namespace
@@ -209,7 +284,14 @@ void launchRope(const kgh_rope_params& p, hipStream_t stream) {
   a.headRun = 1;
   while(a.headRun < 4 && shared % (2 * a.headRun) == 0 && p.tokens * (p.heads / (2 * a.headRun)) * a.groups >= (1 << 18)) a.headRun *= 2;
   a.headRuns = p.heads / a.headRun;
-  a.items = p.tokens * a.headRuns * a.groups;
+  // Heads with tables of their own: runs of up to 4 tokens, in the same way. 20011
+  // tokens of 32 x 128 bf16, three axes: 82 us with runs of one, 61 of four; 19377 x
+  // 17 x 120 fp16, four axes, 76 and 37 (there with wide loads for a head's last
+  // pairs too); 46208 x 6 x 64 fp32 28 and 25.
+  a.tokenRun = 1;
+  while(a.headRun == 1 && a.tokenRun < ROPE_AHEAD && (p.tokens + 2 * a.tokenRun - 1) / (2 * a.tokenRun) * p.heads * a.groups >= (1 << 18)) a.tokenRun *= 2;
+  a.tokens = p.tokens;
+  a.items = (p.tokens + a.tokenRun - 1) / a.tokenRun * a.headRuns * a.groups;
   const int64_t blocks = (a.items + 255) / 256;
   // The launch counts threads in 32 bits.
   if(blocks >= (1 << 24)) opInvalid("kgh_rope_axes", "too many tokens for one call");

@@ -201,6 +201,29 @@ def test_rope_in_place_in_a_fused_projection(layout):
     assert torch.equal(qkv[:, 6 * 32:], before[:, 6 * 32:])
 
 
+@pytest.mark.parametrize("dtype,layout,tokens,heads,dim,pairs,axes,in_place", [
+    (torch.float16, "halves", 35001, 5, 55, 27, 4, True), (torch.bfloat16, "interleaved", 21003, 7, 120, 60, 2, False),
+    (torch.float32, "interleaved", 20002, 3, 70, 33, 1, True), (torch.float16, "interleaved", 150001, 1, 64, 29, 3, True),
+    (torch.float32, "halves", 41001, 4, 48, 23, 2, False)])
+def test_rope_runs_of_tokens(dtype, layout, tokens, heads, dim, pairs, axes, in_place):
+    """Every head a table of its own, and tokens enough for runs of them."""
+    x = _rand(tokens, heads, dim, dtype=dtype, pad=1)
+    g = torch.Generator().manual_seed(pairs)
+    pos = torch.randint(-30, 4000, (tokens, axes), generator=g, dtype=torch.int32).cuda()
+    freqs = torch.randn(heads, pairs, axes, generator=g).cuda()
+    want = ref.rope(x, pos, freqs, layout)
+    if in_place:
+        flat = x.as_strided((tokens * heads, dim + 1), (dim + 1, 1), x.storage_offset())[:, dim:]
+        ops.rope_axes(x, pos, freqs, x, layout=layout, stream=_stream())
+        ref.check(x, want)
+        assert bool(torch.isnan(flat).all())
+        return
+    out, untouched = _guarded(tokens, heads, dim, dtype=dtype)
+    ops.rope_axes(x, pos, freqs, out, layout=layout, stream=_stream())
+    ref.check(out, want)
+    untouched()
+
+
 def test_rope_far_offsets_and_head_major():
     far = torch.empty((1 << 31) + 4096, dtype=torch.float16, device="cuda")
     x = far.as_strided((3, 2, 32), ((1 << 30) + 512, 40, 1))
