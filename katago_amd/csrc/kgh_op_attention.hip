@@ -196,12 +196,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
   V qf[D / VEC / 2];
 #pragma unroll
   for(int i = 0; i < D / VEC / 2; i++) {
-    const int c = (2 * i + half) * VEC;
-    if constexpr(FULL) __builtin_memcpy(&qf[i], qRow + c, 16);
-    else {
-      const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
-      qf[i] = *(const V*)&u;
-    }
+    const RowGroup<T, FULL> g(2 * i + half, a.dq);
+    const u32x4_t u = g.place(g.load(qRow));
+    qf[i] = *(const V*)&u;
   }
   floatx16 o[D / 32];
 #pragma unroll
@@ -325,9 +322,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
 // barriers before they are read. Bound by what a wave does between barriers: the
 // softmax's vector work (16 cycles for an exponential, about 28 a score in all)
 // and the products take as long as both one after the other, two waves a SIMD.
-// bf16, 4096 queries to 5000 keys, 32/8 heads: of 128 769 us (873 TFLOP/s), of 64
+// bf16, 4096 queries to 5000 keys, 32/8 heads: of 128 745 us (900 TFLOP/s), of 64
 // 446 (753); 64 boards of 361 queries to boards of three sizes, fp16, heads of 64,
-// 39 us, where two thirds are a workgroup's start and end.
+// 36 us, where two thirds are a workgroup's start and end.
 constexpr int64_t ATT_NEAR = 1 << 23;  // token strides below it: 64 of them are less than 2^31 bytes
 constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
 
@@ -373,12 +370,9 @@ __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel
   V qf[D / VEC / 2];
 #pragma unroll
   for(int i = 0; i < D / VEC / 2; i++) {
-    const int c = (2 * i + half) * VEC;
-    if constexpr(FULL) __builtin_memcpy(&qf[i], qRow + c, 16);
-    else {
-      const uint4 u = loadGroupSmall(qRow + c, a.dq - c);
-      qf[i] = *(const V*)&u;
-    }
+    const RowGroup<T, FULL> g(2 * i + half, a.dq);
+    const u32x4_t u = g.place(g.load(qRow));
+    qf[i] = *(const V*)&u;
   }
   floatx16 o[D / 32];
 #pragma unroll
@@ -742,9 +736,13 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   // 4096 keys: whole 98, 16 21.6, 32 28.
   const int64_t wanted = plan.few && p.dtype != KGH_DTYPE_FP32 ? 512 : 256;
   int64_t splits = std::min<int64_t>({wanted / groups, p.k_len / 128, 64});
-  if(p.k_len < 512) splits = 1;  // 6 heads, 361 keys: whole 7.9, in two 9.3
-  // Many rows' sums are many bytes: 96 workgroups, 361 keys, whole 20, in two 29.
-  if(!plan.few && groups > 64) splits = 1;
+  // Many rows in fp32, whose products take longer: 6 heads of 64, 361 queries and keys,
+  // whole 35, in two 24; 84 workgroups, heads of 74, 484 keys 113 and 62 in three.
+  const bool slow = p.dtype == KGH_DTYPE_FP32 && !plan.few;
+  if(p.k_len < (slow ? 256 : 512)) splits = 1;  // 6 heads of 16 bits, 361 keys: whole 7.9, in two 9.3
+  // Many rows' sums are many bytes: 96 workgroups, 361 keys, whole 20, in two 29;
+  // fp32 300 keys 29 and 32, but 500 keys 45 and 38.
+  if(!plan.few && groups > (slow && p.k_len >= 384 ? 128 : 64)) splits = 1;
   const uint64_t one = (uint64_t)plan.rows * (p.v_head_dim + 2) * 4;
   splits = std::min<int64_t>(splits, (int64_t)std::min<uint64_t>(bytes / one, 64));
   plan.splits = (int)std::max<int64_t>(1, splits);

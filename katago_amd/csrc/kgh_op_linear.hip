@@ -193,7 +193,7 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
 // while the other one's products run (fp32: one step ahead, one buffer, and two
 // workgroups a CU that overlap). What is left of K behind the whole steps is a step
 // of its own. Bound by the loads, which straddle cache lines where rows are not
-// aligned: bf16 8192 x 4096 x 8192 853 us (503 aligned).
+// aligned: bf16 8192 x 4096 x 8192 821 us (503 aligned).
 //
 // fp32 runs on the bf16 matrix cores: a number is three bf16 numbers to within
 // 2^-27 of itself, a product the six bf16 products above 2^-27 of it, 6 x 32 cycles
@@ -752,7 +752,7 @@ LinearPlan planLinear(const kgh_linear_params& p, bool aligned, uint64_t bytes) 
   }
   else if(tiles(128) >= 224 && (p.dtype == KGH_DTYPE_FP32 || !aligned)) {
     // fp32 5776 x 1024 x 1024 93 (106 on 64 x 64 tiles), 2888 x 384 x 1152 (207
-    // tiles) 38 (33); unaligned 8192 x 4096 x 8192 853 (1358).
+    // tiles) 38 (33); unaligned 8192 x 4096 x 8192 821 (1358).
     plan.kernel = LIN_TILE_128;
   }
   else if(tiles(128) >= 224) {

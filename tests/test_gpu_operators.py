@@ -375,6 +375,21 @@ def test_attention_fp32_of_more_workgroups_than_cus(b, lq, lk, d, kind):
     ref.check(out, ref.attention(q, k, v, lengths=lengths, mask=mask))
 
 
+@pytest.mark.parametrize("b,lq,lk,h,d", [(2, 130, 290, 3, 64), (33, 33, 400, 2, 20), (33, 40, 384, 2, 74)])
+def test_attention_fp32_keys_split_over_workgroups(b, lq, lk, h, d):
+    """Some streams end before the second split's keys, one has none."""
+    q, k, v = (_rand(b, n, h, d, dtype=torch.float32, seed=s, scale=1.5, pad=s) for n, s in ((lq, 1), (lk, 2), (lk, 3)))
+    lengths = (torch.arange(b, dtype=torch.int32, device="cuda") * 57 + 200) % (lk + 1)
+    lengths[-1] = 0
+    k[0, int(lengths[0]):] = float("nan")
+    v[0, int(lengths[0]):] = float("inf")
+    out, untouched = _guarded(b, lq, h, d, dtype=torch.float32)
+    assert ops.cross_attention_workspace(q, k, v) > 0
+    _attention(q, k, v, out, key_lengths=lengths)
+    ref.check(out, ref.attention(q, k, v, lengths=lengths))
+    untouched()
+
+
 @pytest.mark.parametrize("lq", [1, 40, 300])
 def test_attention_many_keys_of_little_weight(lq):
     """One key with nearly all of the weight and a value of 0, and 1999 with 2^-24.5
