@@ -526,11 +526,13 @@ __global__ __launch_bounds__(64 * WM * WN * KW, PER_CU * WM * WN * KW / 4) void 
     products(f);
   }
 
+  // The loads past the end arrive before the LDS is used otherwise, here or by the
+  // workgroup that has it next.
+  waitVmcnt<0>();
   if constexpr(KW == 2) {
     // The two halves of K, added in order.
     static_assert(RB == 1 && CB == 1, "a wave's sums fit in its part of a buffer");
     float* sums = (float*)a0s + (wave % (WM * WN)) * 1024 + lane;
-    waitVmcnt<0>();
     __syncthreads();
     if(kw == 1) {
 #pragma unroll
