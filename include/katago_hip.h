@@ -311,8 +311,8 @@ int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_strea
  * 0..k_len). What k and v hold at other keys is not used, whatever it is. A row
  * without a key, or whose every score is minus infinity, is zeros. Head dims are
  * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and at
- * most KGH_ATTENTION_MAX_SCALE. Scores are taken to base 2 in fp32: one that
- * passes the largest float divided by log2(e) counts as infinite. */
+ * most KGH_ATTENTION_MAX_SCALE. q . k and the differences of a row's are fp32 numbers
+ * before the scale: one that passes the largest float is infinite. */
 #define KGH_ATTENTION_MAX_HEAD_DIM 128
 #define KGH_ATTENTION_MAX_SCALE 1e30f
 typedef struct kgh_attention_params {

@@ -20,7 +20,7 @@ struct AttnArgs {
   const uint8_t* mask;
   int64_t maskB;
   int lq, lk, heads, kvHeads, dq, dv;
-  float scaleLog2;  // scale * log2(e): exponents are taken to base 2
+  float scaleLog2;  // scale * log2(e): differences of scores, times this, are exponents to base 2
 };
 
 // Where a split's sums go: [split][row][v dim] in fp32, then [split][row] pairs of
@@ -101,9 +101,12 @@ struct ValueReads {
   }
 };
 
-// One row's running softmax: p = 2^(s c - ref), with a reference point that only
-// moves when a tile's maximum passes it by more than 8 (p is at most 256, summed
+// One row's running softmax: p = 2^((s - ref) c), with a reference point that only
+// moves when a tile's maximum passes it by more than 8 / c (p is at most 256, summed
 // in fp32; the normalisation by the sum of the same p makes the choice cancel).
+// The reference is a score, taken off before the product: s c - ref c would have
+// the rounding of ref c, half a step of a number that may be any size, for the
+// largest key's exponent in place of 0.
 // In fp16 p is 2^7 times that: as large as the type allows, so that many keys of
 // little weight each are not lost below its smallest numbers.
 template<typename T>
@@ -137,18 +140,19 @@ __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], float scaleL
 #pragma unroll
     for(int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, s[kb][i]), s[kb][i + 1]);
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-  top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scaleLog2;
-  const float ref = top > row.ref + 8.0f ? top : row.ref;
-  const float corr = ref == row.ref ? 1.0f : __builtin_amdgcn_exp2f(row.ref - ref);
+  top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+  // (of two infinities alike this is NaN, and the reference stays)
+  const float ref = (top - row.ref) * scaleLog2 > 8.0f ? top : row.ref;
+  const float corr = ref == row.ref ? 1.0f : __builtin_amdgcn_exp2f((row.ref - ref) * scaleLog2);
   row.ref = ref;
-  // While a row has met no score above -inf its offset is 0: every p is 0.
-  const float off = ref == -INFINITY ? 0.0f : P_SHIFT<T> - ref;
+  // While a row has met no score above -inf its base is 0: every p is 0.
+  const float base = ref == -INFINITY ? 0.0f : ref;
   float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for(int kb = 0; kb < BLOCKS; kb++)
 #pragma unroll
     for(int i = 0; i < 16; i++) {
-      s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scaleLog2, off));
+      s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i] - base, scaleLog2, P_SHIFT<T>));
       part[i & 3] += s[kb][i];
     }
   row.sum = row.sum * corr + ((part[0] + part[1]) + (part[2] + part[3]));  // of this lane half's keys; joined at the end
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
   float ref = -INFINITY;
 #pragma unroll
   for(int w = 0; w < 4; w++) ref = fmaxf(ref, refs[w][laneRow]);
-  const float mine = row.ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(row.ref - ref);
+  const float mine = row.ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((row.ref - ref) * a.scaleLog2);
   float* sums = (float*)lds[wave];
 #pragma unroll
   for(int db = 0; db < D / 32; db++)
@@ -296,7 +300,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
     for(int w = 0; w < 4; w++) top = fmaxf(top, refs[w][m]);
 #pragma unroll
     for(int w = 0; w < 4; w++) {
-      total += refs[w][m] == -INFINITY ? totals[w][m] : totals[w][m] * __builtin_amdgcn_exp2f(refs[w][m] - top);
+      total += refs[w][m] == -INFINITY ? totals[w][m] : totals[w][m] * __builtin_amdgcn_exp2f((refs[w][m] - top) * a.scaleLog2);
       v += ((const float*)lds[w])[d * OLD + m];
     }
     if(split.out != nullptr) {
@@ -635,7 +639,7 @@ __global__ __launch_bounds__(256) void attentionJoinKernel(AttnArgs a, AttnSplit
   for(int s = slice; s < split.splits; s += 8) {
     const float* st = split.state + (s * rowsAll + r) * 2;
     const uint4 u = n > 0 ? loadGroup(split.out + (s * rowsAll + r) * a.dv + d, n) : make_uint4(0, 0, 0, 0);
-    const float f = st[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st[0] - ref);
+    const float f = st[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((st[0] - ref) * a.scaleLog2);
     total = fmaf(st[1], f, total);
     v[0] = fmaf(__uint_as_float(u.x), f, v[0]);
     v[1] = fmaf(__uint_as_float(u.y), f, v[1]);

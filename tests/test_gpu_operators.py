@@ -571,3 +571,35 @@ def test_refusals_leave_no_error_behind():
     assert ops._library().kgh_linear(99, p, None) == 1 and b"no device 99" in nn.hip_library().kgh_last_error()
     assert nn.peek_last_error() == 0
     ref.check(_linear(x, w, out), ref.linear(x, w))
+
+
+# -- scores, values and masks at the ends of their ranges ---------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("scale", [1.0, 64.0, 1e22, 1e30], ids=ids)
+@pytest.mark.parametrize("lq,lk,d", [(3, 200, 64), (2, 2100, 128), (40, 300, 64), (40, 1100, 32), (512, 130, 64), (512, 70, 128)], ids=ids)
+def test_attention_large_scores(dtype, scale, lq, lk, d):
+    """Scores of 2^27 to 2^28 in magnitude, times scales of up to the largest one:
+    a row's largest has its whole weight whatever its size. The scores are fp32
+    numbers (a row's factor of seven bits times 2^21, and multiples of 16 beside
+    it), so only exponents have errors: 2^-23 of one, which for 16 (the next score
+    below the largest, at scale 1) is less than 2^-18 of a weight of e^-16."""
+    g = torch.Generator().manual_seed(lk)
+    row = torch.randint(0, 64, (lq,), generator=g).double()
+    low = torch.randint(-2, 1, (lk,), generator=g).double() * 16
+    for sign in (1.0, -1.0):
+        for part in (torch.arange(lk) * 4 // lk, 3 - torch.arange(lk) * 4 // lk):  # quarters of the keys that rise or fall
+            q, k = torch.zeros(2, lq, 2, d, dtype=torch.float64), torch.zeros(2, lk, 2, d, dtype=torch.float64)
+            q[..., 0], q[..., 1] = ((64 + row) * 2.0 ** 6)[:, None], 1.0
+            k[..., 0], k[..., 1] = (sign * 2.0 ** 15 * torch.tensor([0.25, 0.5, 0.75, 1.0], dtype=torch.float64)[part])[:, None], low[:, None]
+            q, k = (t.to(dtype).cuda() for t in (q, k))
+            v = _rand(2, lk, 2, d, dtype=dtype, seed=3)
+            qd, kd, vd = (t.double().cpu().transpose(1, 2) for t in (q, k, v))
+            score = qd @ kd.transpose(2, 3).contiguous()
+            assert torch.equal(score, score.float().double())
+            p = torch.softmax(scale * score, -1)
+            want = (p @ vd).transpose(1, 2)
+            off = (ref.HALF_STEP[dtype] + 2.0 ** -18 + 2 * (lk + 4) * ref.U32) * (p @ vd.abs()).transpose(1, 2)
+            bound = off + ref.HALF_STEP[dtype] * (want.abs() + off) + 2 * ref.SMALLEST[dtype]
+            ref.check(_attention(q, k, v, torch.empty_like(q), scale=scale), (want, bound), (sign, part[0]))
+            ref.check(ops.cross_attention(q, k, v, torch.empty_like(q), scale=scale, stream=_stream()), (want, bound), (sign, part[0]))
