@@ -588,6 +588,13 @@ __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel
     return;
   }
   const float inv = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
+  // Without a key the sums may be NaN, of a p of 0 and an infinite value.
+  if(row.sum == 0.0f) {
+#pragma unroll
+    for(int db = 0; db < D / 32; db++)
+#pragma unroll
+      for(int i = 0; i < 16; i++) o[db][i] = 0.0f;
+  }
   T* oRow = (T*)a.out + b * a.oB + qi * a.oT + h * a.oH;
 #pragma unroll
   for(int db = 0; db < D / 32; db++) {

@@ -603,3 +603,19 @@ def test_attention_large_scores(dtype, scale, lq, lk, d):
             bound = off + ref.HALF_STEP[dtype] * (want.abs() + off) + 2 * ref.SMALLEST[dtype]
             ref.check(_attention(q, k, v, torch.empty_like(q), scale=scale), (want, bound), (sign, part[0]))
             ref.check(ops.cross_attention(q, k, v, torch.empty_like(q), scale=scale, stream=_stream()), (want, bound), (sign, part[0]))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("value", ["inf", "-inf", "nan"])
+@pytest.mark.parametrize("lq,lk,d", [(1, 75, 64), (2, 1030, 32), (50, 75, 64), (40, 1100, 128), (600, 70, 64), (768, 40, 128)], ids=ids)
+def test_attention_scores_of_minus_infinity_are_zeros_whatever_the_values(dtype, value, lq, lk, d):
+    """By every kernel, with a split of the keys and without one."""
+    q, k, v = (_rand(3, n, 2, d, dtype=dtype, seed=i) for i, n in enumerate((lq, lk, lk)))
+    want = ref.attention(q[::2], k[::2], v[::2])
+    q[1].abs_()
+    k[1], v[1] = float("-inf"), float(value)
+    for run in (_attention, lambda *t: ops.cross_attention(*t, stream=_stream())):
+        out = torch.full_like(q, 3.0)
+        run(q, k, v, out)
+        assert not out[1].any()
+        ref.check(out[::2], want)
