@@ -159,6 +159,35 @@ __device__ __forceinline__ float softmaxTile(floatx16 (&s)[BLOCKS], float scaleL
   return corr;
 }
 
+// The largest magnitude of a lane's values in 16 bits, as far as to tell whether
+// one is infinite or NaN: bits without the sign, two numbers a register.
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+template<typename T>
+constexpr unsigned short INFINITE_BITS = __is_same(T, bf16_t) ? 0x7f80 : 0x7c00;
+template<typename T>
+struct Magnitude {
+  u16x2_t most = {0, 0};
+  __device__ __forceinline__ void take(u32x4_t v) {
+    if constexpr(sizeof(T) == 2) {
+#pragma unroll
+      for(int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu));
+    }
+  }
+  __device__ __forceinline__ bool infinite() const { return max(most[0], most[1]) >= INFINITE_BITS<T>; }
+};
+// Zeros in the place of a group's infinities and NaN.
+template<typename T>
+__device__ __forceinline__ typename Vec16<T>::V finiteOnly(typename Vec16<T>::V v) {
+  u16x2_t u[4];
+  __builtin_memcpy(u, &v, 16);
+#pragma unroll
+  for(int i = 0; i < 4; i++)
+#pragma unroll
+    for(int j = 0; j < 2; j++) u[i][j] = (u[i][j] & 0x7fff) >= INFINITE_BITS<T> ? 0 : u[i][j];
+  __builtin_memcpy(&v, u, 16);
+  return v;
+}
+
 // The two lane halves' sums.
 __device__ __forceinline__ float joinHalves(float v) { return v + __shfl_xor(v, 32); }
 
@@ -170,7 +199,8 @@ __device__ __forceinline__ float joinHalves(float v) { return v + __shfl_xor(v, 
 // the keys are split over workgroups too where there are few. S^T = K Q^T (lane =
 // row, 16 of 32 keys), so that P^T is the second product's operand as it stands.
 // Here the matrix cores have time: P goes through them in two pieces, so that the
-// result is not off by P's rounding. bf16, 32 streams, 32/8 heads of 128, up to 4096
+// result is not off by P's rounding (an infinite value meets one of them only: times
+// the second one, of any sign or 0, it would be NaN). bf16, 32 streams, 32/8 heads of 128, up to 4096
 // keys each: 69 us, 4.9 TB/s of keys and values (a copy reaches 5.2); one stream of
 // 16384 keys 22 us, where a wave's four tiles take a round trip to memory each.
 template<typename T, int D, bool FULL>
@@ -237,13 +267,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
   for(int t = first; t < end; t += 4) {
     const unsigned valid = (unsigned)__ballot(r.mask != 0 && t * 32 + laneRow < len);
     asm volatile("" ::: "memory");  // a wave's LDS accesses run in order
+    Magnitude<T> largest;
 #pragma unroll
     for(int i = 0; i < LOADS; i++) {
       const int key = lk + i * (64 / GROUPS);
       const u32x4_t zero = {0, 0, 0, 0};
       *(u32x4_t*)(ks + kAt<T, D>(key, lg)) = kGroup.place(r.k[i]);
-      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = (valid >> key) & 1 ? vGroup.place(r.v[i]) : zero;
+      const u32x4_t v = (valid >> key) & 1 ? vGroup.place(r.v[i]) : zero;
+      largest.take(v);
+      *(u32x4_t*)(vs + vAt<T, D>(key, lg)) = v;
     }
+    const bool infinite = __any(largest.infinite());
     asm volatile("" ::: "memory");
     load(t + 4, r);
     floatx16 s[1];
@@ -271,7 +305,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
       for(int db = 0; db < D / 32; db++) {
         const V vf = reads.read(vs, g * VEC / 4 * 8, db);
         o[db] = mma32(vf, hi, o[db]);
-        if constexpr(sizeof(T) == 2) o[db] = mma32(vf, lo, o[db]);
+        if constexpr(sizeof(T) == 2) o[db] = mma32(infinite ? finiteOnly<T>(vf) : vf, lo, o[db]);
       }
     }
   }

@@ -619,3 +619,25 @@ def test_attention_scores_of_minus_infinity_are_zeros_whatever_the_values(dtype,
         run(q, k, v, out)
         assert not out[1].any()
         ref.check(out[::2], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lq,lk,h,kv,d", [(1, 75, 2, 2, 64), (3, 33, 8, 1, 31), (2, 1030, 2, 1, 128), (1, 700, 4, 4, 32), (50, 75, 2, 2, 64),
+                                          (40, 1100, 2, 2, 128), (600, 70, 2, 2, 64)], ids=ids)
+def test_attention_infinite_values_that_take_part(dtype, lq, lk, h, kv, d):
+    """An infinite value makes its dim of its head's rows infinite, two of other
+    signs or a NaN make it NaN; other dims and heads are what they are."""
+    q, k, v = (_rand(2, n, m, d, dtype=dtype, seed=i) for i, (n, m) in enumerate(((lq, h), (lk, kv), (lk, kv))))
+    clean = ref.attention(q, k, v)
+    v[0, 9, 0, 3], v[0, lk - 2, 0, 7], v[0, 5, 0, 8], v[0, 6, 0, 8], v[0, 30, 0, d - 1] = (float(x) for x in ("inf", "-inf", "inf", "-inf", "nan"))
+    g = h // kv
+    for run in (_attention, lambda *t: ops.cross_attention(*t, stream=_stream())):
+        out = run(q, k, v, torch.empty_like(q))
+        assert bool((out[0, :, :g, 3] == float("inf")).all()) and bool((out[0, :, :g, 7] == float("-inf")).all())
+        assert bool(out[0, :, :g, [8, d - 1]].isnan().all())
+        out, want = out.double().cpu(), clean[0].clone()
+        dims = [3, 7, 8, d - 1]
+        assert bool(out[0, :, g:].isfinite().all()) and bool(out[1].isfinite().all())
+        for t in (out, want):
+            t[0, :, :g, dims] = 0.0
+        ref.check(out, (want, clean[1]))
