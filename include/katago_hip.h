@@ -313,8 +313,9 @@ int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_strea
  * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and at
  * most KGH_ATTENTION_MAX_SCALE. q . k and the differences of a row's are fp32 numbers
  * before the scale: one that passes the largest float is infinite. A weight under
- * 2^-126 of its row's largest (2^-31 for fp16 tensors) may be 0: it makes NaN of an
- * infinite value. */
+ * 2^-118 of its row's largest (2^-31 for fp16 tensors) may be 0: it makes NaN of an
+ * infinite value. Values that times k_len pass the largest float may give
+ * infinities. */
 #define KGH_ATTENTION_MAX_HEAD_DIM 128
 #define KGH_ATTENTION_MAX_SCALE 1e30f
 typedef struct kgh_attention_params {

@@ -101,16 +101,18 @@ struct ValueReads {
   }
 };
 
-// One row's running softmax: p = 2^((s - ref) c), with a reference point that only
-// moves when a tile's maximum passes it by more than 8 / c (p is at most 256, summed
-// in fp32; the normalisation by the sum of the same p makes the choice cancel).
+// One row's running softmax: p = 2^((s - ref) c + shift), with a reference point
+// that only moves when a tile's maximum passes it by more than 8 / c (the
+// normalisation by the fp32 sum of the same p makes the choice cancel).
 // The reference is a score, taken off before the product: s c - ref c would have
 // the rounding of ref c, half a step of a number that may be any size, for the
 // largest key's exponent in place of 0.
-// In fp16 p is 2^7 times that: as large as the type allows, so that many keys of
-// little weight each are not lost below its smallest numbers.
+// The shift makes p at most 1 where its type has fp32's exponents, so that sums of
+// p v are no larger than sums of v; fp16's p is at most 2^15, its largest as large
+// as the type allows, so that many keys of little weight each are not lost below
+// its smallest numbers, and its values are far from fp32's end.
 template<typename T>
-constexpr float P_SHIFT = sizeof(T) == 2 && !__is_same(T, bf16_t) ? 7.0f : 0.0f;
+constexpr float P_SHIFT = sizeof(T) == 2 && !__is_same(T, bf16_t) ? 7.0f : -8.0f;
 struct RowState {
   float ref = -INFINITY, sum = 0.0f;
 };

@@ -641,3 +641,22 @@ def test_attention_infinite_values_that_take_part(dtype, lq, lk, h, kv, d):
         for t in (out, want):
             t[0, :, :g, dims] = 0.0
         ref.check(out, (want, clean[1]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=ids)
+@pytest.mark.parametrize("lq,h,kv,d,workspace", [(1, 2, 2, 64, False), (2, 8, 4, 128, True), (40, 2, 2, 64, False), (512, 4, 2, 128, False), (40, 2, 2, 32, True)],
+                         ids=ids)
+def test_attention_values_near_the_end_of_the_range(dtype, lq, h, kv, d, workspace):
+    """Values of the largest float divided by twice the number of keys, and scores
+    that grow by 5.4 (2^7.8 in weight) half way. Exponents are off by less than
+    2^-18, p by half a step, its sums by lk * 2^-24."""
+    lk = 1024 if workspace else 256
+    q, k, v = torch.zeros(1, lq, h, d), torch.zeros(1, lk, kv, d), torch.full((1, lk, kv, d), 2.0 ** 127 / lk)
+    q[..., 0] = 1.0
+    k[:, lk // 2:, :, 0] = 5.375
+    q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+    out = torch.empty_like(q)
+    (_attention if workspace else lambda *t, **s: ops.cross_attention(*t, stream=_stream(), **s))(q, k, v, out, scale=1.0)
+    off = ref.HALF_STEP[dtype] + 2.0 ** -18 + 2 * (lk + 4) * ref.U32
+    want = torch.full(q.shape, 2.0 ** 127 / lk, dtype=torch.float64)
+    ref.check(out, (want, want * (off + ref.HALF_STEP[dtype] * (1 + off))))
