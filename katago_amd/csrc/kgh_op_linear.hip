@@ -42,7 +42,8 @@ __device__ __forceinline__ float normalCdfFast(float x) {
 // (error of about 1e-6) where the result is rounded to 16 bits.
 template<typename T, int ACT>
 __device__ __forceinline__ float linActivate(float v) {
-  if constexpr(ACT == KGH_ACTIVATION_GELU) return sizeof(T) == 4 ? 0.5f * v * erfcf(v * -0.70710678118654752f) : v * normalCdfFast(v);
+  if constexpr(ACT == KGH_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays NaN
+  else if constexpr(ACT == KGH_ACTIVATION_GELU) return sizeof(T) == 4 ? 0.5f * v * erfcf(v * -0.70710678118654752f) : v * normalCdfFast(v);
   else if constexpr(sizeof(T) == 4) return kgh_activate(v, ACT);
   else return kgh_activate_fast(v, ACT);
 }

@@ -660,3 +660,28 @@ def test_attention_values_near_the_end_of_the_range(dtype, lq, h, kv, d, workspa
     off = ref.HALF_STEP[dtype] + 2.0 ** -18 + 2 * (lk + 4) * ref.U32
     want = torch.full(q.shape, 2.0 ** 127 / lk, dtype=torch.float64)
     ref.check(out, (want, want * (off + ref.HALF_STEP[dtype] * (1 + off))))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("act", ops.ACTIVATIONS)
+@pytest.mark.parametrize("m,k,pad", [(4, 80, 0), (8, 12296, 0), (90, 80, 0), (70, 4104, 0), (90, 80, 1), (1800, 72, 0), (1800, 72, 1)], ids=ids)
+def test_linear_not_finite_through_activations(dtype, act, m, k, pad):
+    """A NaN input makes its row NaN whatever the activation, infinite ones what
+    the activation of an infinity is; 1800 rows by 1800 columns are large tiles,
+    long rows are split over workgroups."""
+    n = 1800 if m == 1800 else 40
+    x, w = _rand(m, k, dtype=dtype, pad=pad), _rand(n, k, dtype=dtype, seed=1, scale=k ** -0.5, pad=pad)
+    x[1, k - 2], x[2, 9], x[3] = float("inf"), float("nan"), float("nan")
+    bias = torch.zeros(n, device="cuda")
+    bias[5] = float("nan")
+    out = torch.empty(m, n, dtype=dtype, device="cuda")
+    _linear(x, w, out, bias=bias, activation=act)
+    z = x[:4].double().cpu() @ w.double().cpu().t() + bias.double().cpu()
+    want = ref.activate(z, act)
+    assert bool(out[2:4].isnan().all()) and bool(out[:, 5].isnan().all())
+    assert torch.equal(out[:2].double().cpu().isnan(), want[:2].isnan())
+    assert torch.equal(out[1].double().cpu().nan_to_num(7.0, 9.0, -9.0), want[1].nan_to_num(7.0, 9.0, -9.0))
+    rest = torch.tensor([0] + list(range(4, min(m, 40))))
+    keep = torch.arange(n) != 5
+    y, bound = ref.linear(x[rest], w, bias, act)
+    ref.check(out[rest][:, keep], (y[:, keep], bound[:, keep]), act)
