@@ -28,24 +28,75 @@ struct LinearArgs {
   int chunk;
 };
 
-// Phi(x) to 1e-7 by the rational approximation of erfc in Abramowitz and Stegun,
-// 7.1.26: 1 - erf(z) = (a1 t + ... + a5 t^5) e^(-z^2), t = 1 / (1 + p z), z >= 0.
-__device__ __forceinline__ float normalCdfFast(float x) {
-  const float z = fabsf(x) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float tail = 0.5f * poly * __expf(-z * z);
-  return x < 0.0f ? tail : 1.0f - tail;
+// The activations: a result is rounded to its type once, so what a value left of 0
+// keeps of itself (e^v or erfc) has to be right relative to itself, down to the type's
+// smallest normal numbers.
+constexpr float LIN_LOG2E = 1.44269504088896341f;
+
+// For results in 16 bits, to within 2^-15 of the result. The exponential's
+// instruction gives 0 below fp32's normal numbers, where v times it is not yet: it is
+// taken 2^64 times as large or small, which the denominator or the polynomial's
+// coefficients undo (a product may be below the normal numbers).
+//   silu(v) = v / (1 + e^-v);
+//   mish(v) = v n / (n + 2), n = e^v (e^v + 2); from 20 on v;
+//   gelu(v) = v (1 - q), or v q left of 0, q = erfc(|v| / sqrt(2)) / 2 =
+//             e^(-v^2 / 2) t P(t), t = 1 / (1 + p |v| / sqrt(2)): P and p fitted to
+//             the smallest largest relative error, 4.2e-6 for all |v| < 14.1 (the
+//             result is below every type's numbers behind).
+// fp16 46208 x 384 x 1024, us: identity 62, SiLU 67, mish 71, GELU 77.
+template<int ACT>
+__device__ __forceinline__ float linActivateFast(float v) {
+  if constexpr(ACT == KGH_ACT_SILU) return v * (__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fmaf(v, -LIN_LOG2E, -64.0f)) + 0x1p-64f) * 0x1p-64f);
+  else if constexpr(ACT == KGH_ACT_MISH) {
+    const float big = __builtin_amdgcn_exp2f(fmaf(fminf(v, 20.0f), LIN_LOG2E, 64.0f));
+    const float n = big * fmaf(big, 0x1p-64f, 2.0f);
+    return v * (n * __builtin_amdgcn_rcpf(n + 0x1p65f));
+  }
+  else {
+    constexpr float S = 0x1p-65f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.435f * 0.70710678118654752f, fabsf(v), 1.0f));
+    float poly = fmaf(t, S * -0.15086693f, S * 0.38131212f);
+    poly = fmaf(t, poly, S * 0.01284851f);
+    poly = fmaf(t, poly, S * 0.27344433f);
+    poly = fmaf(t, poly, S * 0.23733569f);
+    poly = fmaf(t, poly, S * 0.24592536f);
+    const float q = t * poly * __builtin_amdgcn_exp2f(fmaf(v * v, -0.5f * LIN_LOG2E, 64.0f));
+    return v * (v < 0.0f ? q : 1.0f - q);
+  }
 }
 
-// The epilogue's activation: accurate forms for fp32 outputs, the fast ones
-// (error of about 1e-6) where the result is rounded to 16 bits.
+// For results in fp32, to within 2^-18 of the result: the same forms by the accurate functions.
+template<int ACT>
+__device__ __forceinline__ float linActivateFp32(float v) {
+  if constexpr(ACT == KGH_ACTIVATION_GELU) {
+    // erfc falls by 2 z times its argument's error, so what the argument's rounding
+    // leaves is put right.
+    constexpr float C = 0.70710678118654752f, REST = (float)(0.70710678118654752440 - (double)C);
+    const float z = v * -C;
+    const float rest = fmaf(v, -C, -z) - v * REST;
+    float q = erfcf(z);
+    if(z > 1.0f) q = fmaf(q * -2.0f * z, rest, q);
+    return 0.5f * v * q;
+  }
+  else if(v < -20.0f) {
+    // Both are v e^v to within 2^-28, by the exponential's root.
+    const float root = expf(0.5f * v);
+    return v * root * root;
+  }
+  else {
+    const float e = expf(-fabsf(v)), twice = e + e;
+    if constexpr(ACT == KGH_ACT_SILU) return v * ((v < 0.0f ? e : 1.0f) / (1.0f + e));
+    else if(v < 0.0f) return v * (fmaf(e, e, twice) / (fmaf(e, e, twice) + 2.0f));
+    else return v * ((1.0f + twice) / fmaf(twice, e, 1.0f + twice));
+  }
+}
+
 template<typename T, int ACT>
 __device__ __forceinline__ float linActivate(float v) {
-  if constexpr(ACT == KGH_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays NaN
-  else if constexpr(ACT == KGH_ACTIVATION_GELU) return sizeof(T) == 4 ? 0.5f * v * erfcf(v * -0.70710678118654752f) : v * normalCdfFast(v);
-  else if constexpr(sizeof(T) == 4) return kgh_activate(v, ACT);
-  else return kgh_activate_fast(v, ACT);
+  if constexpr(ACT == KGH_ACT_IDENTITY) return v;
+  else if constexpr(ACT == KGH_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays NaN
+  else if constexpr(sizeof(T) == 4) return linActivateFp32<ACT>(v);
+  else return linActivateFast<ACT>(v);
 }
 
 // Tiles of a launch in runs of 8 row tiles by 1 column tile, column after column,

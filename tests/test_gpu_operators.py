@@ -685,3 +685,51 @@ def test_linear_not_finite_through_activations(dtype, act, m, k, pad):
     keep = torch.arange(n) != 5
     y, bound = ref.linear(x[rest], w, bias, act)
     ref.check(out[rest][:, keep], (y[:, keep], bound[:, keep]), act)
+
+
+def _every_value(dtype):
+    """Every finite number of a type in 16 bits; of fp32 the tails finely, and
+    numbers of all sizes."""
+    if dtype == torch.float32:
+        sizes = torch.logspace(-25, 38, 4000, dtype=torch.float64)
+        return torch.cat((torch.linspace(-100, 30, 24000, dtype=torch.float64), sizes, -sizes)).float()
+    every = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    return every[every.isfinite()]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("act", ops.ACTIVATIONS)
+@pytest.mark.parametrize("kernel", ["few rows", "split", "aligned tiles", "any tiles"])
+def test_linear_activations_of_every_value(dtype, act, kernel):
+    """Values as they are (products with 1) through the activation, right relative
+    to the result down to the type's smallest normal numbers: 2^-15 in 16 bits,
+    2^-18 in fp32, and a rounding to the type. Fp32 tiles split a value into pieces
+    that are off by 2^-26 of it at most, which a result in a tail follows by |z|
+    times as much."""
+    z = _every_value(dtype)
+    form = 0.0 if act in ("identity", "relu") else 2.0 ** -18 if dtype == torch.float32 else 2.0 ** -15
+    if kernel in ("few rows", "split"):
+        if kernel == "split":
+            z = z[::32]
+        w = torch.zeros(len(z), 6144 if kernel == "split" else 8, dtype=dtype)
+        w[:, 3] = z
+        x = torch.zeros(2, w.shape[1], dtype=dtype)
+        x[:, 3] = 1.0
+        out = torch.empty(2, len(z), dtype=dtype, device="cuda")
+        got = _linear(x.cuda(), w.cuda(), out, activation=act)
+        assert ops.linear_workspace(x.cuda(), w.cuda()) == 0 or kernel == "split"
+        assert torch.equal(got[0], got[1])
+        got = got[0]
+    else:
+        x = torch.zeros(len(z), 8 if kernel == "aligned tiles" else 1, dtype=dtype)
+        x[:, 0] = z
+        w = torch.zeros(9, x.shape[1], dtype=dtype)
+        w[:, 0] = 1.0
+        got = _linear(x.cuda(), w.cuda(), torch.empty(len(z), 9, dtype=dtype, device="cuda"), activation=act)
+        assert bool((got == got[:, :1]).all())
+        got = got[:, 0]
+        if dtype == torch.float32:
+            form = form + 2.0 ** -26 * (1 + z.double().abs().clamp_max(110))
+    y = ref.activate(z.double(), act)
+    smallest = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    ref.check(got, (y, y.abs() * (form + ref.HALF_STEP[dtype] * (1 + form)) + smallest), act)
