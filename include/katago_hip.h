@@ -252,9 +252,8 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
  * residual may be out itself (with its stride). in_channels and out_channels
  * are at least 1. Before its rounding an activation is within 2^-15 of its value for
  * 16 bits and 2^-18 for fp32 (a value below the type's smallest normal number may be
- * 0). Infinities and NaN give what fp32 arithmetic gives, but that a
- * product of two infinities may be NaN in fp32, and a sum within 2^-8 of the
- * largest float infinite. */
+ * 0). Infinities and NaN give what fp32 arithmetic
+ * gives; fp32 numbers below the normal ones may count as 0. */
 typedef struct kgh_linear_params {
   int32_t dtype;      /* KGH_DTYPE_* of x, weights, residual and out */
   int32_t activation; /* KGH_ACTIVATION_* */

@@ -251,38 +251,52 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
 // 2^-27 of itself, a product the six bf16 products above 2^-27 of it, 6 x 32 cycles
 // for 16 k of a 32 x 32 block where the fp32 instructions take 8 x 64. The pieces
 // are put into LDS as three 64-byte runs and a gap a row (an odd number of 16-byte
-// groups: the rows of a ds_read_b128 phase fall in distinct banks). 4096 cubed 760
-// us (181 TFLOP/s; fp32 instructions 975, the library 895): with 128 x 128 tiles the
-// splitting, 165 vector instructions a step and wave, takes about as long as the
+// groups: the rows of a ds_read_b128 phase fall in distinct banks). 4096 cubed 744
+// us (185 TFLOP/s; fp32 instructions 975, the library 895): with 128 x 128 tiles the
+// splitting, about 200 vector instructions a step and wave, takes about as long as the
 // products, and with 64 x 64 LDS is 0.9 busy. Small sizes run fp32 instructions.
-// A number that rounds to a bf16 infinity has the largest bf16 number as its first
-// piece, and an infinity has only a third, so that it meets one piece of the other
-// factor: sums are infinite or NaN as in fp32, but NaN where both factors of a
-// product are infinite.
-constexpr float LIN_BF16_MAX = 0x1.fep127f, LIN_BF16_INF_FROM = 0x1.ffp127f;
+// Pieces hold no number that rounds to a bf16 infinity, and of one below 2^-96 the
+// third may lie below bf16's normal numbers. A tile that has met a small one, or whose
+// sums are not all finite, is computed once more by the fp32 instructions (2.3 times
+// its time in all). Only the first pieces are looked at, two a register, so numbers
+// whose first piece is 0, below 2^-133, count as 0. (A look at every step that sends
+// it to the fp32 instructions costs every product 8% more: 4096 cubed 805 us.)
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+constexpr unsigned LIN_PIECES_FROM = 0x0f80;  // bits of 2^-96
 
-template<bool SPECIAL>
+// The smallest of the pieces but 0, by their bits twice and less one: 0 is the largest.
+__device__ __forceinline__ u16x2_t smallestPiece(u16x2_t least, bf16x4_t piece) {
+  u16x2_t u[2];
+  __builtin_memcpy(u, &piece, 8);
+#pragma unroll
+  for(int i = 0; i < 2; i++) {
+    u16x2_t twice;
+    asm("v_pk_mad_u16 %0, %1, %2, %3" : "=v"(twice) : "v"(u[i]), "v"(0x00020002), "v"(0xffffffff));
+    least = __builtin_elementwise_min(least, twice);
+  }
+  return least;
+}
 __device__ __forceinline__ void splitGroup(u32x4_t v, bf16x4_t (&piece)[3]) {
   float rest[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
 #pragma unroll
   for(int q = 0; q < 3; q++)
 #pragma unroll
     for(int j = 0; j < 4; j++) {
-      __bf16 b = (__bf16)rest[j];
-      if(SPECIAL && q < 2 && fabsf(rest[j]) >= LIN_BF16_INF_FROM) b = (__bf16)(fabsf(rest[j]) == INFINITY ? 0.0f : copysignf(LIN_BF16_MAX, rest[j]));
+      const __bf16 b = (__bf16)rest[j];
       piece[q][j] = b;
       rest[j] -= (float)b;
     }
 }
 
 template<typename T, int RB, int CB, int ACT>
-__global__ __launch_bounds__(256) void linearTileKernel(LinearArgs a, int rowTiles, int colTiles) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? (RB == 2 ? 2 : 4) : 1) void linearTileKernel(LinearArgs a, int rowTiles, int colTiles) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), STEP = 8 * VEC;
   constexpr int BM = 64 * RB, BN = 64 * CB, LD = SPLIT ? 208 : 128, LOADS = 2 * (RB + CB);
   __shared__ __attribute__((aligned(16))) unsigned char lds0[(BM + BN) * LD];
   __shared__ __attribute__((aligned(16))) unsigned char lds1[SPLIT ? 16 : (BM + BN) * LD];
+  __shared__ int again;  // whether a tile is computed once more
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int laneRow = lane & 31, half = lane >> 5;
   int rowTile, colTile;
@@ -308,33 +322,31 @@ __global__ __launch_bounds__(256) void linearTileKernel(LinearArgs a, int rowTil
 #pragma unroll
     for(int i = 0; i < LOADS; i++) __builtin_memcpy(&r.v[i], src[i] + k, 16);
   };
-  auto stage = [&](unsigned char* lds, const Rows& r, auto special) {
+  u16x2_t least = {0xffff, 0xffff};
+  auto stage = [&](unsigned char* lds, const Rows& r, auto pieces) {
 #pragma unroll
     for(int i = 0; i < LOADS; i++) {
-      if constexpr(SPLIT) {
+      if constexpr(decltype(pieces)::value) {
         bf16x4_t piece[3];
-        splitGroup<decltype(special)::value>(r.v[i], piece);
+        splitGroup(r.v[i], piece);
+        least = smallestPiece(least, piece[0]);
 #pragma unroll
         for(int q = 0; q < 3; q++) *(bf16x4_t*)(lds + (lr + 32 * i) * LD + q * 64 + lg * 8) = piece[q];
       }
+      else if constexpr(SPLIT) *(u32x4_t*)(lds + (lr + 32 * i) * LD + lg * 16) = r.v[i];
       else *(u32x4_t*)(lds + swizzled128(lr + 32 * i, lg)) = r.v[i];
     }
   };
-  auto anySpecial = [&](const Rows& r) {
-    unsigned big = 0;
-#pragma unroll
-    for(int i = 0; i < LOADS; i++)
-      big = max(max(max(big, r.v[i].x & 0x7fffffffu), max(r.v[i].y & 0x7fffffffu, r.v[i].z & 0x7fffffffu)), r.v[i].w & 0x7fffffffu);
-    return __any(big >= __float_as_uint(LIN_BF16_INF_FROM));
-  };
-
   floatx16 acc[RB][CB];
+  auto clear = [&] {
 #pragma unroll
-  for(int i = 0; i < RB; i++)
+    for(int i = 0; i < RB; i++)
 #pragma unroll
-    for(int j = 0; j < CB; j++)
+      for(int j = 0; j < CB; j++)
 #pragma unroll
-      for(int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+        for(int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+  };
+  clear();
   const int wm = (wave >> 1) * 32 * RB, wn = (wave & 1) * 32 * CB;
   auto products = [&](const unsigned char* lds) {
     if constexpr(SPLIT) {
@@ -376,12 +388,32 @@ __global__ __launch_bounds__(256) void linearTileKernel(LinearArgs a, int rowTil
           for(int j = 0; j < CB; j++) acc[i][j] = mma32(bf[s][j], af[s][i], acc[i][j]);
     }
   };
+  // fp32 numbers as they are.
+  auto products32 = [&](const unsigned char* lds) {
+    if constexpr(SPLIT) {
+#pragma unroll
+      for(int s = 0; s < 4; s++)
+#pragma unroll
+        for(int i = 0; i < RB; i++)
+#pragma unroll
+          for(int j = 0; j < CB; j++)
+            acc[i][j] = mma32(*(const floatx4*)(lds + (BM + wn + j * 32 + laneRow) * LD + (2 * s + half) * 16),
+                              *(const floatx4*)(lds + (wm + i * 32 + laneRow) * LD + (2 * s + half) * 16), acc[i][j]);
+    }
+  };
   auto put = [&](const Rows& r) {
-    if(SPLIT && anySpecial(r)) stage(lds0, r, std::true_type());
-    else stage(lds0, r, std::false_type());
+    stage(lds0, r, std::integral_constant<bool, SPLIT>());
     barrierLds();
   };
+  auto rest = [&](Rows& r) {
+#pragma unroll
+    for(int i = 0; i < LOADS; i++) {
+      const uint4 u = loadGroupSmall(src[i] + whole * STEP, kEnd - kBegin - whole * STEP - lg * VEC);
+      r.v[i] = u32x4_t{u.x, u.y, u.z, u.w};
+    }
+  };
   if constexpr(SPLIT) {
+    if(tid == 0) again = 0;
     Rows r;
     if(whole > 0) fetch(0, r);
     for(int at = 0; at < whole; at++) {
@@ -413,13 +445,33 @@ __global__ __launch_bounds__(256) void linearTileKernel(LinearArgs a, int rowTil
   }
   if(kBegin + whole * STEP < kEnd) {
     Rows r;
-#pragma unroll
-    for(int i = 0; i < LOADS; i++) {
-      const uint4 u = loadGroupSmall(src[i] + whole * STEP, kEnd - kBegin - whole * STEP - lg * VEC);
-      r.v[i] = u32x4_t{u.x, u.y, u.z, u.w};
-    }
+    rest(r);
     put(r);
     products(lds0);
+  }
+  if constexpr(SPLIT) {
+    // (0 times a sum that is infinite or NaN is NaN)
+    float sum = 0.0f;
+#pragma unroll
+    for(int i = 0; i < RB; i++)
+#pragma unroll
+      for(int j = 0; j < CB; j++)
+#pragma unroll
+        for(int r = 0; r < 16; r++) sum = fmaf(0.0f, acc[i][j][r], sum);
+    if(min(least[0], least[1]) < 2 * LIN_PIECES_FROM - 1 || sum != 0.0f) again = 1;
+    __syncthreads();
+    if(again != 0) {
+      clear();
+      Rows r;
+      for(int at = 0; at <= whole; at++) {
+        if(at < whole) fetch(at, r);
+        else rest(r);
+        __syncthreads();
+        stage(lds0, r, std::false_type());
+        __syncthreads();
+        products32(lds0);
+      }
+    }
   }
   storeTile<T, RB, CB, ACT>(a, acc, m0 + wm, n0 + wn);
 }

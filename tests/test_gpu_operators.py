@@ -733,3 +733,53 @@ def test_linear_activations_of_every_value(dtype, act, kernel):
     y = ref.activate(z.double(), act)
     smallest = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
     ref.check(got, (y, y.abs() * (form + ref.HALF_STEP[dtype] * (1 + form)) + smallest), act)
+
+
+@pytest.mark.parametrize("m,n,pad", [(3, 40, 0), (90, 40, 0), (90, 40, 1), (1800, 1900, 0), (1800, 1900, 1)])
+@pytest.mark.parametrize("at", [-101, -113, -119, -125])
+def test_linear_fp32_small_numbers(m, n, pad, at):
+    """Small normal numbers against large ones on the other side, in a whole step
+    and in what is left of K, and in one of the two beside ordinary numbers: their
+    sums are as right as any."""
+    k = 44
+    for swap in (False, True):
+        for part in (slice(0, k), slice(0, 20), slice(36, k)):
+            x, w = _rand(m, k, dtype=torch.float32, pad=pad), _rand(n, k, dtype=torch.float32, seed=1, pad=pad)
+            a, b = (w, x) if swap else (x, w)
+            a[:, part] = (a[:, part].sign() + a[:, part].clamp(-0.99, 0.99) / 2) * 2.0 ** at
+            b[:, part] *= 2.0 ** -at
+            a[:, 5], a[:, 40] = 0.0, 0.0
+            ref.check(_linear(x, w, torch.empty(m, n, device="cuda")), ref.linear(x, w))
+
+
+@pytest.mark.parametrize("m,n,pad", [(3, 40, 0), (90, 40, 0), (90, 40, 1), (1800, 1900, 0), (1800, 1900, 1)])
+def test_linear_fp32_infinities_times_anything(m, n, pad):
+    """An infinity times an infinity or a number of any size is an infinity of the
+    product's sign, times 0 NaN."""
+    x, w = _rand(m, 70, dtype=torch.float32, pad=pad).abs_(), _rand(n, 70, dtype=torch.float32, seed=1, pad=pad).abs_()
+    for row, (at, a, b) in enumerate(((3, "inf", "inf"), (40, "inf", "-inf"), (68, "-inf", "1e-38"))):
+        x[row, at] = float(a)
+        w[row, at] = float(b)
+    w[10, 40] = 0.0
+    out = _linear(x, w, torch.empty(m, n, device="cuda")).cpu()
+    want = x.double().cpu() @ w.double().cpu().t()
+    special = ~want.isfinite()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out[special].nan_to_num(7.0), want[special].float().nan_to_num(7.0))
+    assert bool(out[~special].isfinite().all())
+
+
+@pytest.mark.parametrize("m,n,pad", [(3, 40, 0), (90, 40, 0), (90, 40, 1), (1800, 1900, 0), (1800, 1900, 1)])
+def test_linear_fp32_sums_near_the_largest(m, n, pad):
+    """Sums of up to the largest float, whose parts are finite: no infinity before
+    that, and one behind it."""
+    most = torch.finfo(torch.float32).max
+    x, w = torch.zeros(m, 40 + pad, device="cuda")[:, :40], torch.zeros(n, 40 + pad, device="cuda")[:, :40]
+    x[:, 3] = most * torch.linspace(0.98, 1.0, m, dtype=torch.float64, device="cuda").float()
+    x[:, 38] = 2.0 ** 125
+    w[:, 3] = torch.tensor([1.0, -1.0, 0.5, 2.0], device="cuda")[torch.arange(n, device="cuda") % 4]
+    w[:, 38] = torch.tensor([0.0, 0.0, 1.0, 0.0], device="cuda")[torch.arange(n, device="cuda") % 4]
+    out = _linear(x, w, torch.empty(m, n, device="cuda")).cpu()
+    want = x.double().cpu() @ w.double().cpu().t()
+    fits = want.abs() <= most
+    assert bool(out[:, 3::4].isinf().all()) and bool(fits[:, torch.arange(n) % 4 != 3].all())
+    ref.check(out[:, torch.arange(n) % 4 != 3], (want[:, torch.arange(n) % 4 != 3], (want.abs() * 4 * ref.U32)[:, torch.arange(n) % 4 != 3]))
