@@ -5,14 +5,15 @@ positions with several axes (``rope_axes``) and attention to an encoder's states
 
 Tensors are torch tensors, or ``DeviceTensor`` views of device memory: anything
 with ``data_ptr()``, ``stride()``, ``shape``, ``dtype`` and ``get_device()``. Calls are
-asynchronous on ``stream`` (a hipStream_t as an int, None for the null stream;
-``torch.cuda.current_stream().cuda_stream``); the caller keeps the tensors alive
-until they have run. Every call returns its output tensor. Arguments that do not
+asynchronous on ``stream``: a hipStream_t as an int, 0 for the null stream; None for
+the stream that torch is on for torch tensors, and the null stream for others. The
+caller keeps the tensors alive until they have run. Every call returns its output tensor. Arguments that do not
 fit raise ``StringError``.
 """
 from __future__ import annotations
 
 import ctypes
+import sys
 
 from .nn import StringError, hip_check, hip_library
 
@@ -151,6 +152,15 @@ def _first(op, name, t):
     return code, device
 
 
+def _stream(t, device):
+    """The stream of a call that names none: torch's for its tensors, which the null
+    stream does not wait for, nor it for the null stream."""
+    torch = sys.modules.get("torch")
+    if torch is not None and isinstance(t, torch.Tensor):
+        return torch.cuda.current_stream(device).cuda_stream
+    return None
+
+
 def _sizes(op, *sizes):
     if max(sizes) > _MOST:
         _invalid(f"{op}: an axis is longer than {_MOST}")
@@ -224,7 +234,7 @@ def linear(x, weights, out, bias=None, activation=None, residual=None, workspace
     activation one of ``ACTIVATIONS``. residual may be out itself. workspace: at
     least ``linear_workspace`` bytes of its own for calls that may overlap."""
     p, device = _linear_params(x, weights, out, bias, activation, residual, workspace)
-    hip_check((_lib or _library()).kgh_linear(device, p, stream))
+    hip_check((_lib or _library()).kgh_linear(device, p, _stream(x, device) if stream is None else stream))
     return out
 
 
@@ -254,7 +264,7 @@ def rope_axes(x, positions, freqs, out, layout="interleaved", inverse=False, str
         _invalid(f"rope_axes: unknown layout {layout!r}")
     p = _RopeParams(code, kind, 1 if inverse else 0, axes, tokens, heads, dim, pairs, tables, x.data_ptr(), xs[0], xs[1],
                     positions.data_ptr(), ps[0], freqs.data_ptr(), out.data_ptr(), os[0], os[1])
-    hip_check((_lib or _library()).kgh_rope_axes(device, p, stream))
+    hip_check((_lib or _library()).kgh_rope_axes(device, p, _stream(x, device) if stream is None else stream))
     return out
 
 
@@ -313,5 +323,5 @@ def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, w
         p.key_mask, p.key_mask_stride = key_mask.data_ptr(), ms[0]
     if workspace is not None:
         p.workspace, p.workspace_bytes = _workspace("cross_attention", workspace, device)
-    hip_check((_lib or _library()).kgh_cross_attention(device, p, stream))
+    hip_check((_lib or _library()).kgh_cross_attention(device, p, _stream(q, device) if stream is None else stream))
     return out

@@ -783,3 +783,35 @@ def test_linear_fp32_sums_near_the_largest(m, n, pad):
     fits = want.abs() <= most
     assert bool(out[:, 3::4].isinf().all()) and bool(fits[:, torch.arange(n) % 4 != 3].all())
     ref.check(out[:, torch.arange(n) % 4 != 3], (want[:, torch.arange(n) % 4 != 3], (want.abs() * 4 * ref.U32)[:, torch.arange(n) % 4 != 3]))
+
+
+def test_calls_without_a_stream_are_on_torchs():
+    """Behind work that is under way on torch's current stream, and in its captures."""
+    x, w = _rand(6, 64), _rand(32, 64, seed=1)
+    q, k = _rand(1, 3, 2, 32, seed=2), _rand(1, 40, 2, 32, seed=3)
+    pos, freqs = torch.arange(6, dtype=torch.int32, device="cuda")[:, None], torch.ones(1, 16, 1, device="cuda")
+    calls = [lambda: ops.linear(x, w, torch.empty(6, 32, dtype=x.dtype, device="cuda")),
+             lambda: ops.rope_axes(x.view(6, 2, 32), pos, freqs, torch.empty(6, 2, 32, dtype=x.dtype, device="cuda")),
+             lambda: ops.cross_attention(q, k, k, torch.empty_like(q))]
+    inputs = [x, x, q]
+    for call, t in zip(calls, inputs):
+        new = torch.randn_like(t)
+        old = t.clone()
+        t.copy_(new)
+        want = call()
+        t.copy_(old)
+        torch.cuda.synchronize()
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(100_000_000)
+            t.copy_(new)
+            got = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            got = call()
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
