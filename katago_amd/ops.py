@@ -7,8 +7,9 @@ Tensors are torch tensors, or ``DeviceTensor`` views of device memory: anything
 with ``data_ptr()``, ``stride()``, ``shape``, ``dtype`` and ``get_device()``. Calls are
 asynchronous on ``stream``: a hipStream_t as an int, 0 for the null stream; None for
 the stream that torch is on for torch tensors, and the null stream for others. The
-caller keeps the tensors alive until they have run. Every call returns its output tensor. Arguments that do not
-fit raise ``StringError``.
+caller keeps the tensors alive until they have run. Nothing here has gradients:
+tensors that require them are taken under ``torch.no_grad()`` only. Every call
+returns its output tensor. Arguments that do not fit raise ``StringError``.
 """
 from __future__ import annotations
 
@@ -161,6 +162,13 @@ def _stream(t, device):
     return None
 
 
+def _no_gradients(op, *tensors):
+    """Refuses tensors that a result's gradients would be wanted of."""
+    for t in tensors:
+        if getattr(t, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
+            _invalid(f"{op}: a tensor requires gradients, and the result would have none (torch.no_grad() takes it)")
+
+
 def _sizes(op, *sizes):
     if max(sizes) > _MOST:
         _invalid(f"{op}: an axis is longer than {_MOST}")
@@ -234,6 +242,7 @@ def linear(x, weights, out, bias=None, activation=None, residual=None, workspace
     activation one of ``ACTIVATIONS``. residual may be out itself. workspace: at
     least ``linear_workspace`` bytes of its own for calls that may overlap."""
     p, device = _linear_params(x, weights, out, bias, activation, residual, workspace)
+    _no_gradients("linear", x, weights, out, bias, residual)
     hip_check((_lib or _library()).kgh_linear(device, p, _stream(x, device) if stream is None else stream))
     return out
 
@@ -259,6 +268,7 @@ def rope_axes(x, positions, freqs, out, layout="interleaved", inverse=False, str
     _sizes("rope_axes", tokens, heads, dim, tables, pairs, axes)
     if (fs[0] != pairs * axes and tables > 1) or (fs[1] != axes and pairs > 1):
         _invalid("rope_axes: freqs is not contiguous")
+    _no_gradients("rope_axes", x, freqs, out)
     kind = ROPE_LAYOUTS.get(layout)
     if kind is None:
         _invalid(f"rope_axes: unknown layout {layout!r}")
@@ -321,6 +331,7 @@ def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, w
         ms = _look("cross_attention", "key_mask", key_mask, 2, _types[kind if kind in ("uint8", "bool") else "uint8"], device)
         _shape("cross_attention", "key_mask", key_mask, batch, p.k_len)
         p.key_mask, p.key_mask_stride = key_mask.data_ptr(), ms[0]
+    _no_gradients("cross_attention", q, k, v, out)
     if workspace is not None:
         p.workspace, p.workspace_bytes = _workspace("cross_attention", workspace, device)
     hip_check((_lib or _library()).kgh_cross_attention(device, p, _stream(q, device) if stream is None else stream))

@@ -179,3 +179,25 @@ def test_plain_forms():
         torch.testing.assert_close(back, z.double())
     with pytest.raises(AssertionError):  # a mistake of one step of bf16 is seen
         ref.check(y * (1 + 2.0 ** -7), (y, y.abs() * 2.0 ** -8))
+
+
+class Trained(Meta):
+    requires_grad = True
+
+
+@pytest.mark.parametrize("call", [
+    _linear(x=Trained(4, 16)), _linear(weights=Trained(8, 16)), _linear(bias=Trained(8, dtype="float32")), _linear(residual=Trained(4, 8)),
+    _linear(out=Trained(4, 8)), _rope(x=Trained(5, 4, 32)), _rope(freqs=Trained(2, 16, 2, dtype="float32")), _attention(q=Trained(2, 3, 4, 32)),
+    _attention(k=Trained(2, 9, 2, 32)), _attention(v=Trained(2, 9, 2, 24))])
+def test_tensors_that_require_gradients_are_refused(call):
+    """Their results would have no history."""
+    _refused(call, "gradients")
+
+
+def test_tensors_that_require_gradients_are_taken_under_no_grad():
+    with torch.no_grad():
+        _refused(_linear(x=Trained(4, 16), weights=Trained(8, 16, at=0)), "null")
+        _refused(_rope(x=Trained(5, 4, 32), freqs=Trained(2, 16, 2, dtype="float32", at=0)), "null")
+        _refused(_attention(q=Trained(2, 3, 4, 32), k=Trained(2, 9, 2, 32, at=0)), "null")
+    assert ops.linear_workspace(Trained(4, 16), Trained(8, 16)) == 0  # sizes only
+    assert ops.cross_attention_workspace(Trained(2, 3, 4, 32), Trained(2, 9, 2, 32), Trained(2, 9, 2, 24)) == 0
