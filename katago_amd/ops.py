@@ -100,8 +100,10 @@ def _invalid(message: str):
 
 
 _CODES = {"float32": FP32, "float16": FP16, "bfloat16": BF16, "int32": "int32", "uint8": "uint8", "bool": "bool"}
-_BYTES = {FP32: 4, FP16: 2, BF16: 2, "int32": 4, "uint8": 1, "bool": 1}
+_BYTES = {"bool": 1, "uint8": 1, "int8": 1, "float16": 2, "bfloat16": 2, "int16": 2, "uint16": 2, "int32": 4, "uint32": 4, "float32": 4,
+          "int64": 8, "uint64": 8, "float64": 8}  # of a workspace's elements
 _codes = dict(_CODES)  # the same by the tensors' own type objects
+_bytes = {}
 _types = {code: name for name, code in _CODES.items()}  # the type object met last of each
 
 
@@ -180,7 +182,7 @@ def _shape(op, name, t, *want):
 
 
 def _workspace(op, workspace, device):
-    """Pointer and bytes of a workspace: a contiguous tensor of any type."""
+    """Pointer and bytes of a workspace: a contiguous tensor of integers or numbers."""
     if workspace is None:
         return None, 0
     if workspace.get_device() != device:
@@ -190,7 +192,12 @@ def _workspace(op, workspace, device):
         if stride != n and size > 1:
             _invalid(f"{op}: the workspace is not contiguous")
         n *= size
-    return workspace.data_ptr(), n * _BYTES[_code(op, "the workspace", workspace)]
+    size = _bytes.get(workspace.dtype)
+    if size is None:
+        size = _bytes[workspace.dtype] = _BYTES.get(str(workspace.dtype).rsplit(".", 1)[-1], 0)
+    if size == 0:
+        _invalid(f"{op}: the workspace is of type {workspace.dtype}")
+    return workspace.data_ptr(), n * size
 
 
 def _linear_params(x, weights, out, bias, activation, residual, workspace):

@@ -201,3 +201,18 @@ def test_tensors_that_require_gradients_are_taken_under_no_grad():
         _refused(_attention(q=Trained(2, 3, 4, 32), k=Trained(2, 9, 2, 32, at=0)), "null")
     assert ops.linear_workspace(Trained(4, 16), Trained(8, 16)) == 0  # sizes only
     assert ops.cross_attention_workspace(Trained(2, 3, 4, 32), Trained(2, 9, 2, 32), Trained(2, 9, 2, 24)) == 0
+
+
+@pytest.mark.parametrize("dtype,size", [("uint8", 1), ("int8", 1), ("bool", 1), ("bfloat16", 2), ("int16", 2), ("float32", 4), ("int32", 4),
+                                        ("int64", 8), ("float64", 8)])
+def test_workspaces_of_any_type(dtype, size):
+    t = torch.empty(5, 3, dtype=getattr(torch, dtype))
+    assert size == t.element_size()
+    assert ops._workspace("linear", t, -1) == (t.data_ptr(), 15 * size)
+    _refused(_linear(workspace=Meta(8, dtype=dtype, at=AT + 8)), "aligned")
+    _refused(_attention(workspace=Meta(8, dtype=dtype, device=1)), "workspace")
+    _refused(_linear(workspace=Meta(8, 3, dtype=dtype, strides=(4, 1))), "contiguous")
+
+
+def test_workspaces_of_other_types_are_refused():
+    _refused(_linear(workspace=Meta(8, dtype="complex64")), "type")
