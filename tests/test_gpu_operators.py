@@ -815,3 +815,147 @@ def test_calls_without_a_stream_are_on_torchs():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+# -- what only large or unusual calls reach -----------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lq,h,kv,d,lk,kind", [
+    (512, 2, 2, 64, 33, "none"), (1000, 1, 1, 80, 200, "none"), (256, 4, 2, 128, 300, "lengths"), (1000, 2, 2, 128, 97, "mask"),
+    (1000, 1, 1, 64, 260, "mask"), (500, 2, 1, 40, 64, "lengths"), (999, 1, 1, 127, 129, "none")], ids=ids)
+def test_attention_of_eight_waves(dtype, lq, h, kv, d, lk, kind):
+    """16 bits, 512 rows a kv head and more of which at most an eighth is empty:
+    workgroups of 256 rows."""
+    b = 3
+    rows = lq * h // kv
+    assert rows >= 512 and rows * 8 >= (rows + 255) // 256 * 256 * 7
+    q, k, v = (_rand(b, n, m, d, dtype=dtype, seed=i, scale=1.2) for i, (n, m) in enumerate(((lq, h), (lk, kv), (lk, kv))))
+    lengths = torch.tensor([lk, 0, lk // 2], dtype=torch.int32, device="cuda") if kind == "lengths" else None
+    mask = None
+    if kind == "mask":
+        mask = torch.rand(b, lk, generator=torch.Generator().manual_seed(lk)).cuda() < 0.5
+        mask[1] = False
+        mask[2, :lk - 3] = False
+    out, untouched = _guarded(b, lq, h, d, dtype=dtype)
+    ref.check(_attention(q, k, v, out, key_lengths=lengths, key_mask=mask), ref.attention(q, k, v, lengths=lengths, mask=mask))
+    untouched()
+
+
+@pytest.mark.parametrize("dtype,d,lq,b", [(torch.float16, 64, 40, 1), (torch.bfloat16, 128, 40, 1), (torch.float16, 128, 520, 1), (torch.bfloat16, 72, 1024, 1),
+                                          (torch.float32, 32, 40, 1), (torch.float32, 16, 40, 260), (torch.bfloat16, 32, 40, 1)], ids=ids)
+@pytest.mark.parametrize("kind", ["none", "all", "empty rounds", "last key", "lengths"])
+def test_attention_of_many_keys_in_rounds(dtype, d, lq, b, kind):
+    """Many rows, more keys than a round of 256 tiles: three rounds, of which masks
+    empty the first, the second, or all but the last key's. The items share keys."""
+    lk = 2 * 256 * (32 if (dtype != torch.float32 and d > 64) or b > 256 else 64) + 100
+    q = _rand(b, lq, 1, d, dtype=dtype, scale=1.2)
+    k, v = _rand(1, lk, 1, d, dtype=dtype, seed=1, scale=1.2), _rand(1, lk, 1, d, dtype=dtype, seed=2)
+    mask = lengths = None
+    if kind == "lengths":
+        lengths = torch.full((b,), lk - 90, dtype=torch.int32, device="cuda")
+    elif kind != "none":
+        mask = torch.rand(1, lk, generator=torch.Generator().manual_seed(d)) < 0.7
+        if kind == "empty rounds":
+            mask[0, :lk // 3 - 64] = False
+            mask[0, lk * 4 // 9:lk - 70] = False
+        if kind == "last key":
+            mask[0, :lk - 1] = False
+            mask[0, lk - 1] = True
+        mask = mask.cuda().expand(b, lk)
+    out = torch.empty_like(q)
+    ops.cross_attention(q, k.expand(b, lk, 1, d), v.expand(b, lk, 1, d), out, key_lengths=lengths, key_mask=mask, stream=_stream())
+    for i in {0, b // 2, b - 1}:
+        ref.check(out[i:i + 1], ref.attention(q[i:i + 1], k, v, lengths=lengths, mask=mask), i)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lq,d", [(40, 64), (40, 50), (600, 128), (3, 64)])
+def test_attention_of_tokens_far_apart(dtype, lq, d):
+    """Token strides of 2^23 elements, where a tile's offsets pass 32 bits, and keys
+    that end 2^31 elements behind the first."""
+    lk, stride = 258, 1 << 23
+    far = torch.empty((lk - 1) * stride + 4096, dtype=dtype, device="cuda")
+    q = _rand(1, lq, 1, d, dtype=dtype)
+    k, v = (far.as_strided((1, lk, 1, d), (0, stride, 0, 1), at) for at in (0, 2048))
+    k.copy_(_rand(1, lk, 1, d, dtype=dtype, seed=1))
+    v.copy_(_rand(1, lk, 1, d, dtype=dtype, seed=2))
+    ref.check(_attention(q, k, v, torch.empty_like(q)), ref.attention(q, k, v))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("m,k,n,pad", [(17, 72, 8192, 0), (20, 72, 8200, 0), (32, 264, 8201, 1), (33, 40, 8192, 0), (50, 72, 8195, 0), (64, 200, 8300, 3)], ids=ids)
+def test_linear_of_few_rows_and_many_columns(dtype, m, k, n, pad):
+    """17 to 64 rows, 8192 columns and more: workgroups of 32 columns."""
+    x, w = _rand(m, k, dtype=dtype, pad=pad), _rand(n, k, dtype=dtype, seed=1, scale=k ** -0.5, pad=pad)
+    bias, res = _rand(n, dtype=torch.float32, seed=2), _rand(m, n, dtype=dtype, seed=3, pad=pad)
+    out, untouched = _guarded(m, n, dtype=dtype)
+    ref.check(_linear(x, w, out, bias=bias, activation="silu", residual=res), ref.linear(x, w, bias, "silu", res))
+    untouched()
+
+
+def _split_block(dtype, **kw):
+    """A block whose attention and last layer split their keys and their K."""
+    block = Block(dtype, states=600, width=1032, **kw)
+    q, k = block.q.view(block.b, block.l, block.h, block.d), block.kvs[:, :block.kv * block.d].view(block.b, block.s, block.kv, block.d)
+    need = (ops.cross_attention_workspace(q, k, k), ops.linear_workspace(block.up, block.w["down"]))
+    assert min(need) > 16 and block.ws.numel() >= max(need)
+    return block
+
+
+# Roundings as in test_block, and four fp32 sums of up to 2064 terms of random signs.
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_split_block(dtype):
+    block = _split_block(dtype)
+    got, want = block.run(_stream()).double().cpu(), block.want()
+    assert (got - want).norm() <= (16 * ref.HALF_STEP[dtype] + 4 * math.sqrt(2064) * ref.U32) * want.norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_split_block_captured_and_replayed(dtype):
+    """Two graphs with workspaces of their own, replayed at the same time on two
+    streams, with the program's own work between; each time the eager bits."""
+    blocks = [_split_block(dtype, boards=2 + i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in blocks]
+    graphs = [torch.cuda.CUDAGraph() for _ in blocks]
+    for block, stream, graph in zip(blocks, streams, graphs):
+        block.run(_stream())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            block.run(stream.cuda_stream)
+    for i in range(4):
+        for block in blocks:
+            block.x.copy_(_rand(*block.x.shape, dtype=dtype, seed=20 + i))
+            block.lengths.copy_(torch.tensor([(150 * i) % 600, 600, i], dtype=torch.int32)[:block.b])
+            block.out.fill_(0)
+            block.ws.fill_(255)
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for block in blocks:
+            replayed = block.out.clone()
+            assert torch.equal(block.run(_stream()), replayed), i
+        torch.cuda.synchronize()
+
+
+def test_split_blocks_of_two_threads():
+    """On streams and workspaces of their own."""
+    blocks = [_split_block(torch.bfloat16, boards=2 + i) for i in range(2)]
+    want = [b.run(0).clone() for b in blocks]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        for _ in range(20):
+            blocks[i].out.zero_()
+            torch.cuda.current_stream().synchronize()
+            blocks[i].run(s.cuda_stream)
+            s.synchronize()
+            if not torch.equal(blocks[i].out, want[i]):
+                bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
