@@ -313,7 +313,10 @@ int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_strea
  * without a key, or whose every score is minus infinity, is zeros. Head dims are
  * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and at
  * most KGH_ATTENTION_MAX_SCALE. q . k and the differences of a row's are fp32 numbers
- * before the scale: one that passes the largest float is infinite. A weight under
+ * before the scale: one that passes the largest float is infinite. In 16 bits a
+ * weight is rounded to its tensors' type for its product with v, which adds about a
+ * third to the result's own error, unless a kv head has at most 32 rows (query, head
+ * of the group) or precise is 1: then it keeps twice as many bits. A weight under
  * 2^-118 of its row's largest (2^-31 for fp16 tensors) may be 0: it makes NaN of an
  * infinite value. Values that times k_len pass the largest float may give
  * infinities. */
@@ -324,7 +327,8 @@ typedef struct kgh_attention_params {
   int32_t batch, q_len, k_len;
   int32_t heads, kv_heads, q_head_dim, v_head_dim;
   float scale;
-  const void* q; /* [batch][q_len][heads][q_head_dim] */
+  int32_t precise; /* 0 or 1, see above */
+  const void* q;   /* [batch][q_len][heads][q_head_dim] */
   int64_t q_batch_stride, q_token_stride, q_head_stride;
   const void* k; /* [batch][k_len][kv_heads][q_head_dim] */
   int64_t k_batch_stride, k_token_stride, k_head_stride;

@@ -360,11 +360,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKerne
 // scores are computed before tile t's softmax, so that the matrix cores have them
 // to do while the vector units work; a tile's rows are loaded into registers two
 // barriers before they are read. Bound by what a wave does between barriers: the
-// softmax's vector work (16 cycles for an exponential, about 28 a score in all)
+// softmax's vector work (16 cycles for an exponential, about 32 a score in all)
 // and the products take as long as both one after the other, two waves a SIMD.
-// bf16, 4096 queries to 5000 keys, 32/8 heads: of 128 745 us (900 TFLOP/s), of 64
-// 446 (753); 64 boards of 361 queries to boards of three sizes, fp16, heads of 64,
-// 36 us, where two thirds are a workgroup's start and end.
+// bf16, 4096 queries to 5000 keys, 32/8 heads: of 128 762 us (881 TFLOP/s), of 64
+// 480 (699); 64 boards of 361 queries to boards of three sizes, fp16, heads of 64,
+// 37 us, where two thirds are a workgroup's start and end.
+// In 16 bits p is rounded to the tensors' type for its product with v (its sum is
+// not): the result is off by a third more than its own rounding (bf16, 5000 keys:
+// 0.0022 of its norm, 0.0017 with p exact). PRECISE, the caller's choice, has p in two
+// pieces: 0.0017, and 1012 us for 762, 655 for 480, 43 for 37.
 constexpr int64_t ATT_NEAR = 1 << 23;  // token strides below it: 64 of them are less than 2^31 bytes
 constexpr int ATT_LIST = 256;  // key tiles whose masks are looked at at a time
 
@@ -375,7 +379,7 @@ template<typename T, int D>
 constexpr int attBlocks(bool pairs) { return pairs || (sizeof(T) == 2 && D == 128) ? 1 : 2; }
 __device__ __forceinline__ constexpr unsigned long long attWhole(int blocks) { return blocks == 2 ? ~0ull : 0xffffffffull; }
 
-template<typename T, int D, int WAVES, bool FULL, bool PAIRS = sizeof(T) == 2>
+template<typename T, int D, int WAVES, bool FULL, bool PAIRS = sizeof(T) == 2, bool PRECISE = false>
 __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;
   constexpr int THREADS = 64 * WAVES;
@@ -490,7 +494,8 @@ __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel
   };
   // x: the operands of the first group. The next group's are read behind a group's
   // first product, whose wait for its own operands then waits for nothing else.
-  auto values = [&](const unsigned char* vs, const V (&p)[GROUPS_P], Values& x) {
+  // PRECISE: p's second piece pl follows (finite values only, see attentionFewKernel).
+  auto values = [&](const unsigned char* vs, const V (&p)[GROUPS_P], const V (&pl)[GROUPS_P], Values& x) {
     Values y;
 #pragma unroll
     for(int g = 0; g < GROUPS_P; g++) {
@@ -501,6 +506,14 @@ __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for(int db = 1; db < D / 32; db++) o[db] = mma32(now.v[db], p[g], o[db]);
+      if constexpr(PRECISE) {
+        Magnitude<T> largest;
+#pragma unroll
+        for(int db = 0; db < D / 32; db++) largest.take(__builtin_bit_cast(u32x4_t, now.v[db]));
+        const bool infinite = __any(largest.infinite());
+#pragma unroll
+        for(int db = 0; db < D / 32; db++) o[db] = mma32(infinite ? finiteOnly<T>(now.v[db]) : now.v[db], pl[g], o[db]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -514,13 +527,18 @@ __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel
     __builtin_amdgcn_sched_barrier(0);
     scores(kNext, sNext);
     const float corr = softmaxTile<T, BLOCKS>(s, a.scaleLog2, row);
-    V p[GROUPS_P];
+    V p[GROUPS_P], pl[GROUPS_P];
 #pragma unroll
     for(int g = 0; g < GROUPS_P; g++) {
 #pragma unroll
       for(int j = 0; j < VEC; j++) p[g][j] = (T)s[g * VEC / 16][g * VEC % 16 + j];
       // Here, not where it is used: beside the scores' products.
       asm volatile("" : "+v"(p[g]));
+      if constexpr(PRECISE) {
+#pragma unroll
+        for(int j = 0; j < VEC; j++) pl[g][j] = (T)(s[g * VEC / 16][g * VEC % 16 + j] - (float)p[g][j]);
+        asm volatile("" : "+v"(pl[g]));
+      }
     }
     if constexpr(sizeof(T) == 2) {
       // A product, then vector work in its shadow.
@@ -542,7 +560,7 @@ __global__ __launch_bounds__(64 * WAVES, PAIRS ? 2 : 1) void attentionManyKernel
 #pragma unroll
         for(int j = 0; j < 16; j++) o[db][j] *= corr;
     }
-    values(vNow, p, x);
+    values(vNow, p, pl, x);
     stageK(kNow, kr);
     stageV(vNext, vr, bitsNext);
     loadK(i + 3, kr);
@@ -721,6 +739,7 @@ void checkAttention(const kgh_attention_params& p, bool pointers) {
   if(p.kv_heads < 1 || p.heads < 1 || p.heads % p.kv_heads != 0) opInvalid(op, "kv_heads must divide heads");
   for(int d : {p.q_head_dim, p.v_head_dim})
     if(d < 1 || d > KGH_ATTENTION_MAX_HEAD_DIM) opInvalid(op, "head dim " + std::to_string(d) + " outside 1.." + std::to_string(KGH_ATTENTION_MAX_HEAD_DIM));
+  if(p.precise != 0 && p.precise != 1) opInvalid(op, "precise must be 0 or 1");
   if(!(p.scale > 0.0f) || p.scale > KGH_ATTENTION_MAX_SCALE) opInvalid(op, "scale must be positive and at most 1e30");
   for(int64_t s : {p.q_batch_stride, p.q_token_stride, p.q_head_stride, p.k_batch_stride, p.k_token_stride, p.k_head_stride, p.v_batch_stride,
                    p.v_token_stride, p.v_head_stride, p.out_batch_stride, p.out_token_stride, p.out_head_stride, p.key_mask_stride})
@@ -758,6 +777,7 @@ struct AttentionPlan {
   bool few;   // at most 32 rows a kv head
   int waves;  // of the kernel for more
   bool pairs; // fp32: of its variant with two workgroups a CU
+  bool precise;  // 16 bits: of its variant with p in two pieces
   int splits; // of the keys
   int64_t rows;
 };
@@ -771,11 +791,14 @@ AttentionPlan planAttention(const kgh_attention_params& p, uint64_t bytes) {
   // 256-row workgroups where they are at most an eighth empty: 512 rows, heads of
   // 128, 85 us (90 with 128 rows), 16384 rows 795 (962); 361 rows 112 (94).
   const bool wide = rows >= 512 && rows * 8 >= (rows + 255) / 256 * 256 * 7;
-  plan.waves = p.dtype != KGH_DTYPE_FP32 && wide && std::max(p.q_head_dim, p.v_head_dim) > 32 ? 8 : 4;
+  // (p in two pieces leaves heads above 64 no registers with four waves)
+  const int dim = std::max(p.q_head_dim, p.v_head_dim);
+  plan.precise = p.precise != 0 && p.dtype != KGH_DTYPE_FP32 && !plan.few;
+  plan.waves = p.dtype != KGH_DTYPE_FP32 && ((wide && dim > 32) || (plan.precise && dim > 64)) ? 8 : 4;
   const int64_t groups = plan.few ? (int64_t)p.batch * p.kv_heads : (rows + plan.waves * 32 - 1) / (plan.waves * 32) * p.batch * p.kv_heads;
   // Where there are more workgroups than CUs: 16 boards of 361 queries and keys, 6
   // heads of 64, 63 us (73 with one a CU and 64 keys a tile), of 32 36.6 (37.3).
-  plan.pairs = p.dtype == KGH_DTYPE_FP32 && groups > 256 && std::max(p.q_head_dim, p.v_head_dim) <= 64;
+  plan.pairs = p.dtype == KGH_DTYPE_FP32 && groups > 256 && dim <= 64;
   // Workgroups that the CUs hold at a time: two a CU of the kernel for few rows in
   // 16 bits, one of the others; and at least 128 keys a split. One query of 8 kv
   // heads to 16384 keys, us: whole 306, 8 splits 47, 32 21.6, 64 22.1; of 32
@@ -802,6 +825,14 @@ void runAttention(const AttentionPlan& plan, const AttnArgs& a, const AttnSplit&
   const dim3 grid((unsigned)((plan.few ? 1 : (rows + block - 1) / block) * plan.splits), (unsigned)a.kvHeads, (unsigned)batch);
   if(plan.few) attentionFewKernel<T, D, FULL><<<grid, 256, 0, stream>>>(a, split);
   else if(sizeof(T) == 4 && D <= 64 && plan.pairs) attentionManyKernel<T, D, 4, FULL, sizeof(T) == 2 || D <= 64><<<grid, 256, 0, stream>>>(a, split);
+  else if(plan.precise) {
+    if constexpr(sizeof(T) == 2) {
+      if(plan.waves == 4) {
+        if constexpr(D <= 64) attentionManyKernel<T, D, 4, FULL, true, true><<<grid, 256, 0, stream>>>(a, split);
+      }
+      else if constexpr(D >= 64) attentionManyKernel<T, D, 8, FULL, true, true><<<grid, 512, 0, stream>>>(a, split);
+    }
+  }
   else if(plan.waves == 4) attentionManyKernel<T, D, 4, FULL><<<grid, 256, 0, stream>>>(a, split);
   else if constexpr(sizeof(T) == 2 && D >= 64) attentionManyKernel<T, D, 8, FULL><<<grid, 512, 0, stream>>>(a, split);
   KGH_CHECK_LAUNCH();

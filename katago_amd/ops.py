@@ -46,7 +46,7 @@ class _RopeParams(ctypes.Structure):
 class _AttentionParams(ctypes.Structure):
     """kgh_attention_params."""
     _fields_ = [("dtype", _i32), ("batch", _i32), ("q_len", _i32), ("k_len", _i32), ("heads", _i32), ("kv_heads", _i32),
-                ("q_head_dim", _i32), ("v_head_dim", _i32), ("scale", ctypes.c_float),
+                ("q_head_dim", _i32), ("v_head_dim", _i32), ("scale", ctypes.c_float), ("precise", _i32),
                 ("q", _ptr), ("q_strides", _i64 * 3), ("k", _ptr), ("k_strides", _i64 * 3), ("v", _ptr), ("v_strides", _i64 * 3),
                 ("out", _ptr), ("out_strides", _i64 * 3), ("key_lengths", _ptr), ("key_mask", _ptr), ("key_mask_stride", _i64),
                 ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
@@ -285,7 +285,7 @@ def rope_axes(x, positions, freqs, out, layout="interleaved", inverse=False, str
     return out
 
 
-def _attention_params(q, k, v, scale):
+def _attention_params(q, k, v, scale, precise):
     code, device = _first("cross_attention", "q", q)
     dtype = q.dtype
     qs = _look("cross_attention", "q", q, 4, dtype, device)
@@ -299,21 +299,21 @@ def _attention_params(q, k, v, scale):
     _sizes("cross_attention", batch, lq, heads, dq, lk, kv_heads, dv)
     if scale is None:
         scale = max(dq, 1) ** -0.5
-    return _AttentionParams(code, batch, lq, lk, heads, kv_heads, dq, dv, scale, q.data_ptr(), qs[:3], k.data_ptr(), ks[:3],
+    return _AttentionParams(code, batch, lq, lk, heads, kv_heads, dq, dv, scale, 1 if precise else 0, q.data_ptr(), qs[:3], k.data_ptr(), ks[:3],
                             v.data_ptr(), vs[:3]), device
 
 
-def cross_attention_workspace(q, k, v) -> int:
+def cross_attention_workspace(q, k, v, precise=False) -> int:
     """kgh_cross_attention_workspace: bytes of workspace that ``cross_attention``
     makes use of for tensors of these shapes and types (0: none). A larger one
     serves too."""
-    p, device = _attention_params(q, k, v, None)
+    p, device = _attention_params(q, k, v, None, precise)
     n = ctypes.c_uint64()
     hip_check(_library().kgh_cross_attention_workspace(device, p, n))
     return n.value
 
 
-def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, workspace=None, stream=None):
+def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, workspace=None, stream=None, precise=False):
     """kgh_cross_attention: softmax(scale * q k^T) v over the keys that take part.
 
     q [batch, queries, heads, dq], k [batch, keys, kv_heads, dq], v [batch, keys,
@@ -323,8 +323,11 @@ def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, w
     part; key_mask [batch, keys] uint8 or bool: nor do those with 0. What k and v
     hold there is not used. A row without a key is zeros. workspace: at least
     ``cross_attention_workspace`` bytes of its own for calls that may overlap;
-    without one, long keys are not split over workgroups."""
-    p, device = _attention_params(q, k, v, scale)
+    without one, long keys are not split over workgroups. precise: in 16 bits the
+    softmax's weights keep twice their type's bits for the product with v, which
+    those of more than 32 rows (query, head of the group) a kv head do not
+    otherwise."""
+    p, device = _attention_params(q, k, v, scale, precise)
     os = _look("cross_attention", "out", out, 4, q.dtype, device)
     batch = p.batch
     _shape("cross_attention", "out", out, batch, p.q_len, p.heads, p.v_head_dim)

@@ -959,3 +959,65 @@ def test_split_blocks_of_two_threads():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lq,lk,h,kv,d,dv", [(3, 90, 4, 2, 64, 64), (40, 90, 2, 2, 64, 64), (520, 130, 2, 1, 64, 64), (40, 200, 2, 2, 128, 128), (300, 70, 4, 2, 128, 128),
+                                             (33, 64, 3, 3, 20, 32), (130, 1100, 2, 1, 80, 50), (40, 1200, 2, 2, 32, 32)], ids=ids)
+@pytest.mark.parametrize("kind", ["none", "both"])
+def test_attention_precise(dtype, lq, lk, h, kv, d, dv, kind):
+    """Weights of twice the type's bits: the result is off by its own rounding, and
+    by what fp32 scores, exponentials and sums and the weights' second piece leave
+    (half a step of it, and half of fp16's smallest number against a weight of at
+    least 2^7)."""
+    b = 6
+    g = torch.Generator().manual_seed(lk)
+    q, k, v = _rand(b, lq, h, d, dtype=dtype), _rand(b, lk, kv, d, dtype=dtype, seed=1), _rand(b, lk, kv, dv, dtype=dtype, seed=2)
+    lengths, mask = _masks(kind, b, lk, g)
+    want, bound = ref.attention(q, k, v, lengths=lengths, mask=mask)
+    out, untouched = _guarded(b, lq, h, dv, dtype=dtype)
+    need = ops.cross_attention_workspace(q, k, v, precise=True)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+    ops.cross_attention(q, k, v, out, key_lengths=lengths, key_mask=mask, workspace=ws, stream=_stream(), precise=True)
+    ref.check(out, (want, bound))
+    untouched()
+    ref.check(ops.cross_attention(q, k, v, torch.empty_like(out), key_lengths=lengths, key_mask=mask, precise=True), (want, bound))
+    size, _ = ref.attention(q, k, v.abs(), lengths=lengths, mask=mask)  # of the weighted values
+    terms = d ** -0.5 * torch.einsum("bqhd,bkhd->bhqk", q.double().cpu().abs(), k.double().cpu().abs().repeat_interleave(h // kv, 2)).amax(-1).transpose(1, 2)
+    off = (ref.HALF_STEP[dtype] ** 2 + 2 * (d + 4) * ref.U32 * terms[..., None] + 2.0 ** -20 + 2 * (lk + 4) * ref.U32) * size + ref.SMALLEST[dtype] * lk * 2.0 ** -5
+    assert (out.double().cpu() - want).norm() <= (want.to(dtype).double() - want).norm() + off.norm() + ref.HALF_STEP[dtype] * off.norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=ids)
+@pytest.mark.parametrize("lq,lk,d", [(50, 75, 64), (40, 1100, 128), (600, 70, 32)])
+def test_attention_precise_infinite_values(dtype, lq, lk, d):
+    q, k, v = (_rand(1, n, 2, d, dtype=dtype, seed=i) for i, n in enumerate((lq, lk, lk)))
+    clean = ref.attention(q, k, v)
+    v[0, 9, 0, 3], v[0, lk - 2, 0, 7], v[0, 30, 0, d - 1] = (float(x) for x in ("inf", "-inf", "nan"))
+    out = ops.cross_attention(q, k, v, torch.empty_like(q), precise=True).double().cpu()
+    assert bool((out[0, :, 0, 3] == float("inf")).all()) and bool((out[0, :, 0, 7] == float("-inf")).all()) and bool(out[0, :, 0, d - 1].isnan().all())
+    dims = [3, 7, d - 1]
+    out[0, :, 0, dims] = clean[0][0, :, 0, dims]
+    ref.check(out, clean)
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=ids)
+@pytest.mark.parametrize("lq,d", [(40, 64), (520, 64), (40, 128), (33, 32)])
+def test_attention_precise_weights_are_not_rounded(dtype, lq, d):
+    """Scores that are exact (multiples of 2^-6 below 8), so that what is left besides
+    the result's own rounding is the weights' second piece, exponents of up to 12
+    that are off by 2^-23 of themselves, and sums. Weights rounded once are seen."""
+    lk, g = 64, torch.Generator().manual_seed(lq)
+    q, k = torch.zeros(1, lq, 2, d), torch.zeros(1, lk, 2, d)
+    q[..., 0] = torch.randint(1, 5, (1, lq, 2), generator=g) / 4
+    k[..., 0] = torch.randint(-32, 33, (1, lk, 2), generator=g) / 16
+    q, k, v = q.to(dtype).cuda(), k.to(dtype).cuda(), _rand(1, lk, 2, d, dtype=dtype)
+    out = ops.cross_attention(q, k, v, torch.empty_like(q), scale=1.0, precise=True).double().cpu()
+    want, _ = ref.attention(q, k, v, scale=1.0)
+    size, _ = ref.attention(q, k, v.abs(), scale=1.0)
+    off = (ref.HALF_STEP[dtype] ** 2 + 2.0 ** -19 + 2 * (lk + 4) * ref.U32) * size + ref.SMALLEST[dtype] * lk * 2.0 ** -5
+    limit = (want.to(dtype).double() - want).norm() + off.norm() * (1 + ref.HALF_STEP[dtype])
+    assert (out - want).norm() <= limit
+    p = torch.exp((q[..., 0].double().cpu().transpose(1, 2)[..., None] * k[..., 0].double().cpu().transpose(1, 2)[:, :, None]))
+    once = (p.to(dtype).double() @ v.double().cpu().transpose(1, 2) / p.sum(-1, keepdim=True)).transpose(1, 2)
+    assert (once.to(dtype).double() - want).norm() > 1.02 * limit

@@ -216,3 +216,12 @@ def test_workspaces_of_any_type(dtype, size):
 
 def test_workspaces_of_other_types_are_refused():
     _refused(_linear(workspace=Meta(8, dtype="complex64")), "type")
+
+
+def test_precise_is_a_truth_value():
+    t = Meta(2, 3, 4, 32), Meta(2, 9, 2, 32), Meta(2, 9, 2, 24)
+    p, _ = ops._attention_params(*t, None, True)
+    assert p.precise == 1
+    p.precise = 2
+    assert ops._library().kgh_cross_attention(0, p, None) == INVALID
+    assert b"precise" in ops._library().kgh_last_error()
