@@ -217,8 +217,8 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
 
 /* ------------------------------------------------------------------------ */
 /* Operators on the caller's device tensors: the parts of a transformer block
- * that attends to an encoder's states, for programs that build such blocks
- * around the nets of this library (no counterpart in the reference, whose
+ * that attends to an encoder's states, for programs that run such blocks of
+ * their own beside the nets of this library (no counterpart in the reference, whose
  * blocks exist only inside a model). Beside the blocks of a layer program
  * they take bf16, the caller's strides, positions and lengths.
  *
@@ -230,7 +230,7 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
  *    asynchronous; the calling thread's current device is left as it was. They
  *    allocate nothing and may be captured into a HIP graph.
  *  - Sums and statistics are kept in fp32, and a result is rounded to the
- *    tensors' type once. Results do not depend on what ran before, and the
+ *    tensors' type once (kgh_cross_attention says what it rounds before). Results do not depend on what ran before, and the
  *    same call gives the same bits.
  *  - An axis of length zero (rows, tokens, batch, queries) makes the call a
  *    no-op. Unless stated otherwise the output overlaps no input.
@@ -311,15 +311,15 @@ int kgh_rope_axes(int32_t device, const kgh_rope_params* params, void* hip_strea
  * key_mask[b][j] != 0 (either may be NULL; lengths are taken into
  * 0..k_len). What k and v hold at other keys is not used, whatever it is. A row
  * without a key, or whose every score is minus infinity, is zeros. Head dims are
- * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; scale is positive and at
- * most KGH_ATTENTION_MAX_SCALE. q . k and the differences of a row's are fp32 numbers
- * before the scale: one that passes the largest float is infinite. In 16 bits a
- * weight is rounded to its tensors' type for its product with v, which adds about a
- * third to the result's own error, unless a kv head has at most 32 rows (query, head
- * of the group) or precise is 1: then it keeps twice as many bits. A weight under
- * 2^-118 of its row's largest (2^-31 for fp16 tensors) may be 0: it makes NaN of an
- * infinite value. Values that times k_len pass the largest float may give
- * infinities. */
+ * 1 to KGH_ATTENTION_MAX_HEAD_DIM; kv_heads divides heads; batch and kv_heads are at
+ * most 65535; scale is positive and at most KGH_ATTENTION_MAX_SCALE.
+ * q . k and the differences of a row's are fp32 numbers before the scale: one that
+ * passes the largest float is infinite. In 16 bits a weight is rounded to its tensors'
+ * type for its product with v, which adds about a third to the result's own error,
+ * unless a kv head has at most 32 rows (query, head of the group) or precise is 1:
+ * then it keeps twice as many bits. A weight under 2^-118 of its row's largest (2^-31
+ * for fp16 tensors) may be 0: it makes NaN of an infinite value. Values that times
+ * k_len pass the largest float may give infinities. */
 #define KGH_ATTENTION_MAX_HEAD_DIM 128
 #define KGH_ATTENTION_MAX_SCALE 1e30f
 typedef struct kgh_attention_params {

@@ -204,7 +204,7 @@ __device__ __forceinline__ float joinHalves(float v) { return v + __shfl_xor(v, 
 // result is not off by P's rounding (an infinite value meets one of them only: times
 // the second one, of any sign or 0, it would be NaN). bf16, 32 streams, 32/8 heads of 128, up to 4096
 // keys each: 69 us, 4.9 TB/s of keys and values (a copy reaches 5.2); one stream of
-// 16384 keys 22 us, where a wave's four tiles take a round trip to memory each.
+// 16384 keys 20 us, where a wave's four tiles take a round trip to memory each.
 template<typename T, int D, bool FULL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attentionFewKernel(AttnArgs a, AttnSplit split) {
   typedef typename Vec16<T>::V V;

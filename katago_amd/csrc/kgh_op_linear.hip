@@ -245,7 +245,7 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
 // while the other one's products run (fp32: one step ahead, one buffer, and two
 // workgroups a CU that overlap). What is left of K behind the whole steps is a step
 // of its own. Bound by the loads, which straddle cache lines where rows are not
-// aligned: bf16 8192 x 4096 x 8192 821 us (503 aligned).
+// aligned: bf16 8192 x 4096 x 8192 830 to 858 us by the card (499 to 514 aligned).
 //
 // fp32 runs on the bf16 matrix cores: a number is three bf16 numbers to within
 // 2^-27 of itself, a product the six bf16 products above 2^-27 of it, 6 x 32 cycles
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (RB == 2 ? 2 : 4) : 1) void l
 // fragments every wave then holds. The buffers are arrays of their own, so that the
 // compiler does not make a fragment read wait for a load in flight to another one.
 // bf16, us: 8192 x 8192 x 8192 847 (1298 TFLOP/s; the library 781), 8192 x 4096 x
-// 8192 458, with bias, GELU and residual 503 (1092): of a 256 x 256 tile's 117,
+// 8192 458, with bias, GELU and residual 505 (1089): of a 256 x 256 tile's 117,
 // about 20 are its first loads and its stores, 10 more the residual and GELU. The
 // power limit holds the clock at about 2 GHz.
 template<typename T, int WM, int WN, int KW, int RB, int CB, int PER_CU, int ACT>
@@ -662,7 +662,7 @@ void launchDma(const LinearArgs& a, int splits, hipStream_t stream) {
 // and what counts is how many of their bytes are under way. A workgroup has 16 NT
 // output channels; its waves take units of 128 bytes of K in turn (every wave's
 // loads of UNROLL units are issued before the first product), and their sums are
-// added in wave order in LDS. bf16 8 x 4096 x 8192: 14.4 us, 4.7 TB/s; rows that are
+// added in wave order in LDS. bf16 8 x 4096 x 8192: 14.6 us, 4.6 TB/s; rows that are
 // not aligned 32, each line read twice.
 template<typename T, int MT, int NT, int WAVES, int UNROLL, int ACT>
 __global__ __launch_bounds__(64 * WAVES) void linearSkinnyKernel(LinearArgs a) {
@@ -835,7 +835,8 @@ struct LinearPlan {
 };
 
 // Which kernel runs, and in how many splits of K with `bytes` of workspace.
-// Times are us a call on bf16 unless said otherwise, replayed from graphs.
+// Times are us a call on bf16 unless said otherwise, replayed from graphs, both
+// sides of a rule measured together (later steps may have made both shorter).
 LinearPlan planLinear(const kgh_linear_params& p, bool aligned, uint64_t bytes) {
   const auto tiles = [&](int64_t side) { return (p.rows + side - 1) / side * ((p.out_channels + side - 1) / side); };
   const int64_t size = (int64_t)opElemBytes(p.dtype), kBytes = p.in_channels * size;
@@ -843,7 +844,7 @@ LinearPlan planLinear(const kgh_linear_params& p, bool aligned, uint64_t bytes) 
   LinearPlan plan;
   int64_t most = 1;  // splits worth their sums' way through memory and a second launch (about 3 us)
   if(p.rows <= 64) {
-    // Against 64-row tiles: 8 x 4096 x 8192 15.3 (35.8), 64 x 4096 x 8192 30
+    // Against 64-row tiles: 8 x 4096 x 8192 14.6 (35.8), 64 x 4096 x 8192 30
     // (37.5), 48 x 8192 x 1024 33 (49). Split where few workgroups would each
     // have long rows: 16 x 8192 x 1024 in four 9.8 (16.7 whole), but 16 x 2048 x
     // 512 in two 7.9 (6.2).
@@ -852,13 +853,13 @@ LinearPlan planLinear(const kgh_linear_params& p, bool aligned, uint64_t bytes) 
   }
   else if(p.dtype != KGH_DTYPE_FP32 && aligned && p.in_channels >= 1024 && big * 10 >= (big + 255) / 256 * 256 * 7) {
     // A tile a CU, where they fill at least 0.7 of their rounds and K is long
-    // enough for a tile's start and end: 8192 x 4096 x 8192 511 (595 on 128 x
+    // enough for a tile's start and end: 8192 x 4096 x 8192 505 (595 on 128 x
     // 128 tiles), 2888 x 4096 x 4096 102 (112); 46208 x 384 x 1152 83 (74).
     plan.kernel = LIN_DMA_256;
   }
   else if(tiles(128) >= 224 && (p.dtype == KGH_DTYPE_FP32 || !aligned)) {
     // fp32 5776 x 1024 x 1024 93 (106 on 64 x 64 tiles), 2888 x 384 x 1152 (207
-    // tiles) 38 (33); unaligned 8192 x 4096 x 8192 821 (1358).
+    // tiles) 38 (33); unaligned 8192 x 4096 x 8192 830 (1358).
     plan.kernel = LIN_TILE_128;
   }
   else if(tiles(128) >= 224) {
@@ -894,7 +895,7 @@ void runLinear(const LinearPlan& plan, const LinearArgs& a, hipStream_t stream) 
   else if(plan.kernel == LIN_TILE_128) launchTile<T, 2, 2, ACT>(a, s, stream);
   else if(plan.kernel == LIN_TILE_64) launchTile<T, 1, 1, ACT>(a, s, stream);
   // fp32's products take long, so that what counts is an even share of them: 64 x
-  // 32 tiles with K over two waves, 2888 x 1024 x 384 33.6 us (39.5 on 64 x 64).
+  // 32 tiles with K over two waves, 2888 x 1024 x 384 33.6 us (39.5 on 64 x 64; now 29.5).
   else if constexpr(sizeof(T) == 4) launchDma<T, 2, 1, 2, 1, 1, 4, ACT>(a, s, stream);
   else if(plan.kernel == LIN_DMA_256) launchDma<T, 2, 4, 1, 4, 2, 1, ACT>(a, s, stream);
   else if(plan.kernel == LIN_DMA_128) launchDma<T, 2, 2, 1, 2, 2, 2, ACT>(a, s, stream);
