@@ -222,7 +222,7 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
  * blocks exist only inside a model). Beside the blocks of a layer program
  * they take bf16, the caller's strides, positions and lengths.
  *
- * Conventions of the three calls:
+ * Conventions of these calls:
  *  - Every pointer is a device pointer on `device`; strides count elements and
  *    the last axis is contiguous. Elements need their own type's alignment
  *    only; 16-byte aligned rows are read fastest.
@@ -234,14 +234,14 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
  *    same call gives the same bits.
  *  - An axis of length zero (rows, tokens, batch, queries) makes the call a
  *    no-op. Unless stated otherwise the output overlaps no input.
- *  - A workspace may be NULL. Calls that may overlap need workspaces of their
+ *  - A workspace may be NULL where nothing else is said. Calls that may overlap need workspaces of their
  *    own; so do captured graphs that may replay at the same time. Its contents
  *    need no initialisation and mean nothing after the call. */
 #define KGH_DTYPE_FP32 0
 #define KGH_DTYPE_FP16 1
 #define KGH_DTYPE_BF16 2
 
-/* Activations of kgh_linear: the codes of activations.h, and GELU. */
+/* Activations of the operators: the codes of activations.h, and GELU. */
 #define KGH_ACTIVATION_IDENTITY 0
 #define KGH_ACTIVATION_RELU 1
 #define KGH_ACTIVATION_MISH 2
@@ -347,6 +347,133 @@ typedef struct kgh_attention_params {
  * it reads no pointer of params). */
 int kgh_cross_attention_workspace(int32_t device, const kgh_attention_params* params, uint64_t* bytes);
 int kgh_cross_attention(int32_t device, const kgh_attention_params* params, void* hip_stream);
+
+/* Rows in 8 bits with a scale each, for kgh_linear_int8 (and its weights, whose rows
+ * are output channels):
+ *   top = max_c |x[r][c]|, scales[r] = top / 127,
+ *   out[r][c] = x[r][c] * (127 / top) to the nearest whole number (ties to even),
+ * in fp32, each operation rounded once: out is in -127..127 and stands for
+ * out * scales[r]. Where top is below 2^-120 the row is zeros with scale 0; a row that
+ * holds an infinity or NaN is zeros with scale NaN, so that what is computed from it is
+ * NaN. */
+typedef struct kgh_quantize_params {
+  int32_t dtype; /* KGH_DTYPE_* of x */
+  int32_t channels;
+  int64_t rows;
+  const void* x; /* [rows][channels] */
+  int64_t x_stride;
+  int8_t* out; /* [rows][channels] */
+  int64_t out_stride;
+  float* scales; /* [rows] */
+} kgh_quantize_params;
+
+int kgh_quantize_rows(int32_t device, const kgh_quantize_params* params, void* hip_stream);
+
+/* Matrix product of 8-bit integers with a scale for each row of x and each output
+ * channel:
+ *   out[m][n] = act(S * x_scales[m] * weight_scales[n] + bias[n]) + residual[m][n],
+ *   S = sum_k x[m][k] weights[n][k].
+ * S is exact; from there on the arithmetic is fp32's, and the result is rounded to its
+ * type once. residual may be out itself (with its stride). in_channels is at most
+ * KGH_LINEAR_INT8_MAX_IN (S then fits 32 bits whatever the bytes are). Activations are
+ * those of kgh_linear. Rows of x and weights that are 16-byte aligned, in_channels and
+ * strides among them, are read fastest. */
+#define KGH_LINEAR_INT8_MAX_IN 131071
+typedef struct kgh_linear_int8_params {
+  int32_t dtype;      /* KGH_DTYPE_* of residual and out */
+  int32_t activation; /* KGH_ACTIVATION_* */
+  int64_t rows;
+  int32_t in_channels, out_channels;
+  const int8_t* x; /* [rows][in_channels] */
+  int64_t x_stride;
+  const float* x_scales; /* [rows] */
+  const int8_t* weights; /* [out_channels][in_channels] */
+  int64_t weights_stride;
+  const float* weight_scales; /* [out_channels] */
+  const float* bias;          /* [out_channels] fp32, or NULL */
+  const void* residual;       /* [rows][out_channels], or NULL */
+  int64_t residual_stride;
+  void* out; /* [rows][out_channels] */
+  int64_t out_stride;
+  void* workspace; /* 16-byte aligned, or NULL: no split of K over workgroups */
+  uint64_t workspace_bytes;
+} kgh_linear_int8_params;
+
+/* The workspace that kgh_linear_int8 makes use of for these sizes (0: none; it reads
+ * no pointer of params). */
+int kgh_linear_int8_workspace(int32_t device, const kgh_linear_int8_params* params, uint64_t* bytes);
+int kgh_linear_int8(int32_t device, const kgh_linear_int8_params* params, void* hip_stream);
+
+/* Group norm with an activation, channels last: channels in `groups` runs of equal
+ * length, and for each item b and group the mean and (biased) variance of x over the
+ * group's channels at the positions that take part,
+ *   out[b][p][c] = act((x[b][p][c] - mean) / sqrt(variance + eps) * weight[c] + bias[c]).
+ * Positions p < lengths[b] with mask[b][p] != 0 take part (either may be NULL; lengths
+ * are taken into 0..positions). What x holds elsewhere is not used, whatever it is, and
+ * out is zero there. One group over one position is a token's layer norm. An infinity or
+ * NaN that takes part makes its item's group NaN. The differences x - mean are fp32
+ * numbers: one that passes the largest float is infinite; the variance may pass it.
+ * out is of x's type, and may be x itself (with its strides). With out_scales it is
+ * int8: rows (b, p) over all channels as kgh_quantize_rows makes them of the results
+ * before they are rounded, and their scales.
+ * statistics, where not NULL, takes mean and 1 / sqrt(variance + eps) of each item's
+ * groups for kgh_group_norm_backward (0 and 0 of an item without a position). */
+typedef struct kgh_group_norm_params {
+  int32_t dtype;      /* KGH_DTYPE_* of x, and of out without out_scales */
+  int32_t activation; /* KGH_ACTIVATION_* */
+  int32_t batch, positions, channels, groups;
+  float eps; /* at least 2^-126 */
+  const void* x; /* [batch][positions][channels] */
+  int64_t x_batch_stride, x_position_stride;
+  const float* weight;    /* [channels] fp32, or NULL: 1 */
+  const float* bias;      /* [channels] fp32, or NULL: 0 */
+  const int32_t* lengths; /* [batch], or NULL */
+  const uint8_t* mask;    /* [batch][positions], or NULL */
+  int64_t mask_stride;
+  void* out; /* [batch][positions][channels] */
+  int64_t out_batch_stride, out_position_stride;
+  float* out_scales; /* [batch][positions], or NULL */
+  float* statistics; /* [batch][groups][2], or NULL */
+  void* workspace;   /* 16-byte aligned; needed where kgh_group_norm_workspace is not 0 */
+  uint64_t workspace_bytes;
+} kgh_group_norm_params;
+
+/* The workspace that kgh_group_norm needs for these sizes (0: none; of the pointers it
+ * looks at whether out_scales is NULL, and reads none). */
+int kgh_group_norm_workspace(int32_t device, const kgh_group_norm_params* params, uint64_t* bytes);
+int kgh_group_norm(int32_t device, const kgh_group_norm_params* params, void* hip_stream);
+
+/* The gradient of kgh_group_norm: with h = (x - mean) rstd of the forward pass's
+ * statistics, u = grad_out act'(h weight + bias) at the positions that take part,
+ *   grad_bias[c] = sum_{b,p} u,   grad_weight[c] = sum_{b,p} u h,
+ *   grad_x = rstd (u weight - mean_g(u weight) - h mean_g(u weight h)),
+ * mean_g over an item's group. grad_x is zero at positions that take no part; relu's
+ * slope at 0 is 0. x and grad_out are not used there, whatever they hold. grad_weight
+ * and grad_bias are of this call alone (not added to what they hold). */
+typedef struct kgh_group_norm_backward_params {
+  int32_t dtype;      /* KGH_DTYPE_* of x, grad_out and grad_x */
+  int32_t activation; /* KGH_ACTIVATION_* */
+  int32_t batch, positions, channels, groups;
+  const void* x; /* [batch][positions][channels] */
+  int64_t x_batch_stride, x_position_stride;
+  const void* grad_out; /* [batch][positions][channels] */
+  int64_t grad_out_batch_stride, grad_out_position_stride;
+  const float* statistics; /* [batch][groups][2] */
+  const float* weight;     /* [channels] fp32, or NULL: 1 */
+  const float* bias;       /* [channels] fp32, or NULL: 0 */
+  const int32_t* lengths;  /* [batch], or NULL */
+  const uint8_t* mask;     /* [batch][positions], or NULL */
+  int64_t mask_stride;
+  void* grad_x; /* [batch][positions][channels] */
+  int64_t grad_x_batch_stride, grad_x_position_stride;
+  float* grad_weight; /* [channels], or NULL */
+  float* grad_bias;   /* [channels], or NULL */
+  void* workspace;    /* 16-byte aligned; needed where kgh_group_norm_backward_workspace is not 0 */
+  uint64_t workspace_bytes;
+} kgh_group_norm_backward_params;
+
+int kgh_group_norm_backward_workspace(int32_t device, const kgh_group_norm_backward_params* params, uint64_t* bytes);
+int kgh_group_norm_backward(int32_t device, const kgh_group_norm_backward_params* params, void* hip_stream);
 
 /* Layer-level evaluation used by NeuralNet::testEvaluate* (nninterface.h:134-180):
  * the program is a single CONV, a BN+ACT pair, or one residual block

@@ -2370,6 +2370,69 @@ int kgh_cross_attention(int32_t device, const kgh_attention_params* params, void
   });
 }
 
+int kgh_quantize_rows(int32_t device, const kgh_quantize_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkQuantize(*params);
+    kgh::DeviceScope scope(device);
+    kgh::launchQuantize(*params, (hipStream_t)hip_stream);
+  });
+}
+
+int kgh_linear_int8_workspace(int32_t device, const kgh_linear_int8_params* params, uint64_t* bytes) {
+  return guarded([&] {
+    if(params == nullptr || bytes == nullptr) invalid("null argument");
+    kgh::checkLinearInt8(*params, false);
+    (void)device;
+    *bytes = kgh::linearInt8Workspace(*params);
+  });
+}
+
+int kgh_linear_int8(int32_t device, const kgh_linear_int8_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkLinearInt8(*params, true);
+    kgh::DeviceScope scope(device);
+    kgh::launchLinearInt8(*params, (hipStream_t)hip_stream);
+  });
+}
+
+int kgh_group_norm_workspace(int32_t device, const kgh_group_norm_params* params, uint64_t* bytes) {
+  return guarded([&] {
+    if(params == nullptr || bytes == nullptr) invalid("null argument");
+    kgh::checkGroupNorm(*params, false);
+    (void)device;
+    *bytes = kgh::groupNormWorkspace(*params);
+  });
+}
+
+int kgh_group_norm(int32_t device, const kgh_group_norm_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkGroupNorm(*params, true);
+    kgh::DeviceScope scope(device);
+    kgh::launchGroupNorm(*params, (hipStream_t)hip_stream);
+  });
+}
+
+int kgh_group_norm_backward_workspace(int32_t device, const kgh_group_norm_backward_params* params, uint64_t* bytes) {
+  return guarded([&] {
+    if(params == nullptr || bytes == nullptr) invalid("null argument");
+    kgh::checkGroupNormBackward(*params, false);
+    (void)device;
+    *bytes = kgh::groupNormBackwardWorkspace(*params);
+  });
+}
+
+int kgh_group_norm_backward(int32_t device, const kgh_group_norm_backward_params* params, void* hip_stream) {
+  return guarded([&] {
+    if(params == nullptr) invalid("null argument");
+    kgh::checkGroupNormBackward(*params, true);
+    kgh::DeviceScope scope(device);
+    kgh::launchGroupNormBackward(*params, (hipStream_t)hip_stream);
+  });
+}
+
 int kgh_evaluate_layers(int32_t device, const kgh_layer* layers, int32_t num_layers, const float* weights, int64_t num_weights,
                         int32_t use_fp16, int32_t batch, int32_t nn_x, int32_t nn_y, const float* input, const float* mask,
                         float* output) {

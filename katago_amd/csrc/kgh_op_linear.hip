@@ -12,7 +12,6 @@ namespace {
 constexpr int64_t LINEAR_MAX = 1 << 30, LINEAR_MAX_OUT = 1 << 26;
 // Row strides from which a tile's offsets would pass 32 bits.
 constexpr int64_t LIN_DMA_STRIDE = 1 << 22;
-constexpr int LIN_ACTS[] = {KGH_ACT_IDENTITY, KGH_ACT_RELU, KGH_ACT_MISH, KGH_ACT_SILU, KGH_ACTIVATION_GELU};
 
 struct LinearArgs {
   const void* x;
@@ -28,94 +27,6 @@ struct LinearArgs {
   int chunk;
 };
 
-// The activations: a result is rounded to its type once, so what a value left of 0
-// keeps of itself (e^v or erfc) has to be right relative to itself, down to the type's
-// smallest normal numbers.
-constexpr float LIN_LOG2E = 1.44269504088896341f;
-
-// For results in 16 bits, to within 2^-15 of the result. The exponential's
-// instruction gives 0 below fp32's normal numbers, where v times it is not yet: it is
-// taken 2^64 times as large or small, which the denominator or the polynomial's
-// coefficients undo (a product may be below the normal numbers).
-//   silu(v) = v / (1 + e^-v);
-//   mish(v) = v n / (n + 2), n = e^v (e^v + 2); from 20 on v;
-//   gelu(v) = v (1 - q), or v q left of 0, q = erfc(|v| / sqrt(2)) / 2 =
-//             e^(-v^2 / 2) t P(t), t = 1 / (1 + p |v| / sqrt(2)): P and p fitted to
-//             the smallest largest relative error, 4.2e-6 for all |v| < 14.1 (the
-//             result is below every type's numbers behind).
-// fp16 46208 x 384 x 1024, us: identity 62, SiLU 67, mish 71, GELU 77.
-template<int ACT>
-__device__ __forceinline__ float linActivateFast(float v) {
-  if constexpr(ACT == KGH_ACT_SILU) return v * (__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fmaf(v, -LIN_LOG2E, -64.0f)) + 0x1p-64f) * 0x1p-64f);
-  else if constexpr(ACT == KGH_ACT_MISH) {
-    const float big = __builtin_amdgcn_exp2f(fmaf(fminf(v, 20.0f), LIN_LOG2E, 64.0f));
-    const float n = big * fmaf(big, 0x1p-64f, 2.0f);
-    return v * (n * __builtin_amdgcn_rcpf(n + 0x1p65f));
-  }
-  else {
-    constexpr float S = 0x1p-65f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.435f * 0.70710678118654752f, fabsf(v), 1.0f));
-    float poly = fmaf(t, S * -0.15086693f, S * 0.38131212f);
-    poly = fmaf(t, poly, S * 0.01284851f);
-    poly = fmaf(t, poly, S * 0.27344433f);
-    poly = fmaf(t, poly, S * 0.23733569f);
-    poly = fmaf(t, poly, S * 0.24592536f);
-    const float q = t * poly * __builtin_amdgcn_exp2f(fmaf(v * v, -0.5f * LIN_LOG2E, 64.0f));
-    return v * (v < 0.0f ? q : 1.0f - q);
-  }
-}
-
-// For results in fp32, to within 2^-18 of the result: the same forms by the accurate functions.
-template<int ACT>
-__device__ __forceinline__ float linActivateFp32(float v) {
-  if constexpr(ACT == KGH_ACTIVATION_GELU) {
-    // erfc falls by 2 z times its argument's error, so what the argument's rounding
-    // leaves is put right.
-    constexpr float C = 0.70710678118654752f, REST = (float)(0.70710678118654752440 - (double)C);
-    const float z = v * -C;
-    const float rest = fmaf(v, -C, -z) - v * REST;
-    float q = erfcf(z);
-    if(z > 1.0f) q = fmaf(q * -2.0f * z, rest, q);
-    return 0.5f * v * q;
-  }
-  else if(v < -20.0f) {
-    // Both are v e^v to within 2^-28, by the exponential's root.
-    const float root = expf(0.5f * v);
-    return v * root * root;
-  }
-  else {
-    const float e = expf(-fabsf(v)), twice = e + e;
-    if constexpr(ACT == KGH_ACT_SILU) return v * ((v < 0.0f ? e : 1.0f) / (1.0f + e));
-    else if(v < 0.0f) return v * (fmaf(e, e, twice) / (fmaf(e, e, twice) + 2.0f));
-    else return v * ((1.0f + twice) / fmaf(twice, e, 1.0f + twice));
-  }
-}
-
-template<typename T, int ACT>
-__device__ __forceinline__ float linActivate(float v) {
-  if constexpr(ACT == KGH_ACT_IDENTITY) return v;
-  else if constexpr(ACT == KGH_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays NaN
-  else if constexpr(sizeof(T) == 4) return linActivateFp32<ACT>(v);
-  else return linActivateFast<ACT>(v);
-}
-
-// Tiles of a launch in runs of 8 row tiles by 1 column tile, column after column,
-// a contiguous part of them to each XCD: what the XCD's CUs work on at a time is
-// about square, so its L2 serves each row of x and of the weights to several tiles.
-__device__ __forceinline__ void blockedTile(int rowTiles, int colTiles, int& rowTile, int& colTile) {
-  const int id = xcdContiguousTile();
-  const int per = 8 * colTiles;
-  const int run = id / per, at = id - run * per;
-  const int height = min(8, rowTiles - run * 8);
-  colTile = at / height;
-  rowTile = run * 8 + (at - colTile * height);
-}
-
-// XOR swizzle of a row's eight 16-byte groups: the sixteen consecutive rows of a
-// ds_read_b128 phase, the same group of each, fall in distinct banks (by row & 7 in
-// place of (row >> 1) & 7, two rows would meet in each).
-__device__ __forceinline__ int swizzled128(int row, int group) { return row * 128 + ((group ^ ((row >> 1) & 7)) << 4); }
-
 // Two groups of four columns, bias and activation, and the residual's 16 bytes of
 // this lane's columns, to the 16 bytes of the same columns.
 template<typename T, int ACT>
@@ -129,8 +40,8 @@ __device__ __forceinline__ uint4 finishGroup(floatx4 v0, floatx4 v1, floatx4 b0,
   ra[1].v = make_uint2(r01.y, r23.y);
 #pragma unroll
   for(int e = 0; e < 4; e++) {
-    oa[0].e[e] = (T)(linActivate<T, ACT>(v0[e] + b0[e]) + (float)ra[0].e[e]);
-    oa[1].e[e] = (T)(linActivate<T, ACT>(v1[e] + b1[e]) + (float)ra[1].e[e]);
+    oa[0].e[e] = (T)(activate<T, ACT>(v0[e] + b0[e]) + (float)ra[0].e[e]);
+    oa[1].e[e] = (T)(activate<T, ACT>(v1[e] + b1[e]) + (float)ra[1].e[e]);
   }
   const uint2 o01 = swapHalves(oa[0].v.x, oa[1].v.x), o23 = swapHalves(oa[0].v.y, oa[1].v.y);
   return make_uint4(o01.x, o23.x, o01.y, o23.y);
@@ -210,7 +121,7 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
             continue;
           }
 #pragma unroll
-          for(int e = 0; e < 4; e++) v[e] = linActivate<T, ACT>(v[e] + bias[q][e]);
+          for(int e = 0; e < 4; e++) v[e] = activate<T, ACT>(v[e] + bias[q][e]);
           if(res != nullptr) {
             const uint4 r = loadGroupSmall((const float*)a.residual + (int64_t)m * a.ldr + n, a.N - n);
             v += *(const floatx4*)&r;
@@ -739,7 +650,7 @@ __global__ __launch_bounds__(64 * WAVES) void linearSkinnyKernel(LinearArgs a) {
       a.part[((int64_t)blockIdx.y * a.M + m) * a.N + n] = v;
       continue;
     }
-    v = linActivate<T, ACT>(v + (a.bias != nullptr ? a.bias[n] : 0.0f));
+    v = activate<T, ACT>(v + (a.bias != nullptr ? a.bias[n] : 0.0f));
     if(res != nullptr) v += (float)res[(int64_t)m * a.ldr + n];
     ((T*)a.out)[(int64_t)m * a.ldo + n] = (T)v;
   }
@@ -773,7 +684,7 @@ __global__ __launch_bounds__(256) void linearJoinKernel(LinearArgs a, int splits
 #pragma unroll
   for(int j = 0; j < 4; j++) {
     if(j >= count) break;
-    float y = linActivate<T, ACT>(v[j] + (a.bias != nullptr ? a.bias[n + j] : 0.0f));
+    float y = activate<T, ACT>(v[j] + (a.bias != nullptr ? a.bias[n + j] : 0.0f));
     if(a.residual != nullptr) y += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n + j];
     ((T*)a.out)[(int64_t)m * a.ldo + n + j] = (T)y;
   }
@@ -785,17 +696,6 @@ void launchSkinny(const LinearArgs& a, int splits, hipStream_t stream) {
   linearSkinnyKernel<T, MT, NT, WAVES, UNROLL, ACT><<<grid, 64 * WAVES, 0, stream>>>(a);
 }
 
-template<typename F>
-void withLinearAct(int act, F&& f) {
-  switch(act) {
-    case KGH_ACTIVATION_RELU: f(std::integral_constant<int, KGH_ACT_RELU>()); break;
-    case KGH_ACTIVATION_MISH: f(std::integral_constant<int, KGH_ACT_MISH>()); break;
-    case KGH_ACTIVATION_SILU: f(std::integral_constant<int, KGH_ACT_SILU>()); break;
-    case KGH_ACTIVATION_GELU: f(std::integral_constant<int, KGH_ACTIVATION_GELU>()); break;
-    default: f(std::integral_constant<int, KGH_ACT_IDENTITY>()); break;
-  }
-}
-
 }  // namespace
 
 namespace kgh {
@@ -803,8 +703,7 @@ namespace kgh {
 void checkLinear(const kgh_linear_params& p, bool pointers) {
   const char* op = "kgh_linear";
   opCheckDtype(op, p.dtype);
-  if(std::find(std::begin(LIN_ACTS), std::end(LIN_ACTS), p.activation) == std::end(LIN_ACTS))
-    opInvalid(op, "activation " + std::to_string(p.activation) + " is none of KGH_ACTIVATION_*");
+  opCheckActivation(op, p.activation);
   if(p.rows < 0 || p.rows > LINEAR_MAX) opInvalid(op, "rows " + std::to_string(p.rows) + " outside 0.." + std::to_string(LINEAR_MAX));
   if(p.in_channels < 1 || p.in_channels > LINEAR_MAX) opInvalid(op, "in_channels must be in 1.." + std::to_string(LINEAR_MAX));
   if(p.out_channels < 1 || p.out_channels > LINEAR_MAX_OUT) opInvalid(op, "out_channels must be in 1.." + std::to_string(LINEAR_MAX_OUT));
@@ -928,7 +827,7 @@ void launchLinear(const kgh_linear_params& p, hipStream_t stream) {
   const LinearPlan plan = planLinear(p, linearAligned(p), p.workspace != nullptr ? p.workspace_bytes : 0);
   const LinearArgs a{p.x, p.weights, p.bias, p.residual, p.out, p.x_stride, p.weights_stride, p.residual_stride, p.out_stride,
                      (int)p.rows, p.out_channels, p.in_channels, plan.splits > 1 ? (float*)p.workspace : nullptr, plan.chunk};
-  withDtype(p.dtype, [&](auto t) { withLinearAct(p.activation, [&](auto act) { runLinear<decltype(t), decltype(act)::value>(plan, a, stream); }); });
+  withDtype(p.dtype, [&](auto t) { withActivation(p.activation, [&](auto act) { runLinear<decltype(t), decltype(act)::value>(plan, a, stream); }); });
 }
 
 }  // namespace kgh

@@ -1,14 +1,17 @@
 """Operators of the device library on the caller's tensors (include/katago_hip.h):
 a matrix product with bias, activation and residual (``linear``), rotary
-positions with several axes (``rope_axes``) and attention to an encoder's states
-(``cross_attention``).
+positions with several axes (``rope_axes``), attention to an encoder's states
+(``cross_attention``), rows in 8 bits (``quantize_rows``) and the matrix product of
+such rows (``linear_int8``), group norm with an activation, channels last
+(``group_norm``), and its gradient (``group_norm_backward``).
 
 Tensors are torch tensors, or ``DeviceTensor`` views of device memory: anything
 with ``data_ptr()``, ``stride()``, ``shape``, ``dtype`` and ``get_device()``. Calls are
 asynchronous on ``stream``: a hipStream_t as an int, 0 for the null stream; None for
 the stream that torch is on for torch tensors, and the null stream for others. The
-caller keeps the tensors alive until they have run. Nothing here has gradients:
-tensors that require them are taken under ``torch.no_grad()`` only. Every call
+caller keeps the tensors alive until they have run. Nothing here records gradients:
+tensors that require them are taken under ``torch.no_grad()`` only, as in the methods
+of a torch.autograd.Function that calls ``group_norm`` and ``group_norm_backward``. Every call
 returns its output tensor. Arguments that do not fit raise ``StringError``.
 """
 from __future__ import annotations
@@ -52,6 +55,38 @@ class _AttentionParams(ctypes.Structure):
                 ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
 
 
+class _QuantizeParams(ctypes.Structure):
+    """kgh_quantize_params."""
+    _fields_ = [("dtype", _i32), ("channels", _i32), ("rows", _i64), ("x", _ptr), ("x_stride", _i64), ("out", _ptr), ("out_stride", _i64),
+                ("scales", _ptr)]
+
+
+class _LinearInt8Params(ctypes.Structure):
+    """kgh_linear_int8_params."""
+    _fields_ = [("dtype", _i32), ("activation", _i32), ("rows", _i64), ("in_channels", _i32), ("out_channels", _i32),
+                ("x", _ptr), ("x_stride", _i64), ("x_scales", _ptr), ("weights", _ptr), ("weights_stride", _i64), ("weight_scales", _ptr),
+                ("bias", _ptr), ("residual", _ptr), ("residual_stride", _i64), ("out", _ptr), ("out_stride", _i64),
+                ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class _GroupNormParams(ctypes.Structure):
+    """kgh_group_norm_params."""
+    _fields_ = [("dtype", _i32), ("activation", _i32), ("batch", _i32), ("positions", _i32), ("channels", _i32), ("groups", _i32),
+                ("eps", ctypes.c_float), ("x", _ptr), ("x_strides", _i64 * 2), ("weight", _ptr), ("bias", _ptr), ("lengths", _ptr), ("mask", _ptr),
+                ("mask_stride", _i64), ("out", _ptr), ("out_strides", _i64 * 2), ("out_scales", _ptr), ("statistics", _ptr),
+                ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class _GroupNormBackwardParams(ctypes.Structure):
+    """kgh_group_norm_backward_params."""
+    _fields_ = [("dtype", _i32), ("activation", _i32), ("batch", _i32), ("positions", _i32), ("channels", _i32), ("groups", _i32),
+                ("x", _ptr), ("x_strides", _i64 * 2), ("grad_out", _ptr), ("grad_out_strides", _i64 * 2), ("statistics", _ptr),
+                ("weight", _ptr), ("bias", _ptr), ("lengths", _ptr), ("mask", _ptr), ("mask_stride", _i64), ("grad_x", _ptr),
+                ("grad_x_strides", _i64 * 2), ("grad_weight", _ptr), ("grad_bias", _ptr), ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
+
+
+_CALLS = {"kgh_linear": _LinearParams, "kgh_rope_axes": _RopeParams, "kgh_cross_attention": _AttentionParams, "kgh_quantize_rows": _QuantizeParams,
+          "kgh_linear_int8": _LinearInt8Params, "kgh_group_norm": _GroupNormParams, "kgh_group_norm_backward": _GroupNormBackwardParams}
 _lib = None
 
 
@@ -59,10 +94,10 @@ def _library() -> ctypes.CDLL:
     global _lib
     if _lib is None:
         lib = hip_library()
-        for name, params in (("kgh_linear", _LinearParams), ("kgh_rope_axes", _RopeParams), ("kgh_cross_attention", _AttentionParams)):
+        for name, params in _CALLS.items():
             getattr(lib, name).argtypes = [_i32, ctypes.POINTER(params), _ptr]
-        for name, params in (("kgh_linear_workspace", _LinearParams), ("kgh_cross_attention_workspace", _AttentionParams)):
-            getattr(lib, name).argtypes = [_i32, ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
+            if hasattr(lib, name + "_workspace"):
+                getattr(lib, name + "_workspace").argtypes = [_i32, ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
         _lib = lib
     return _lib
 
@@ -70,7 +105,7 @@ def _library() -> ctypes.CDLL:
 class DeviceTensor:
     """A view of device memory for callers without torch: a pointer (an int or
     ctypes.c_void_p, for instance ``DeviceBuffer.ptr``), a shape, the name of a
-    type ("float32", "float16", "bfloat16", "int32", "uint8", "bool") and
+    type ("float32", "float16", "bfloat16", "int32", "int8", "uint8", "bool") and
     strides in elements (None: contiguous)."""
 
     def __init__(self, ptr, shape, dtype: str, strides=None, device: int = 0):
@@ -99,7 +134,7 @@ def _invalid(message: str):
     raise StringError(message, _INVALID)
 
 
-_CODES = {"float32": FP32, "float16": FP16, "bfloat16": BF16, "int32": "int32", "uint8": "uint8", "bool": "bool"}
+_CODES = {"float32": FP32, "float16": FP16, "bfloat16": BF16, "int32": "int32", "int8": "int8", "uint8": "uint8", "bool": "bool"}
 _BYTES = {"bool": 1, "uint8": 1, "int8": 1, "float16": 2, "bfloat16": 2, "int16": 2, "uint16": 2, "int32": 4, "uint32": 4, "float32": 4,
           "int64": 8, "uint64": 8, "float64": 8}  # of a workspace's elements
 _codes = dict(_CODES)  # the same by the tensors' own type objects
@@ -346,3 +381,216 @@ def cross_attention(q, k, v, out, scale=None, key_lengths=None, key_mask=None, w
         p.workspace, p.workspace_bytes = _workspace("cross_attention", workspace, device)
     hip_check((_lib or _library()).kgh_cross_attention(device, p, _stream(q, device) if stream is None else stream))
     return out
+
+
+def quantize_rows(x, out, scales, stream=None):
+    """kgh_quantize_rows: x in 8 bits, a scale for each row: out stands for out *
+    scales[:, None].
+
+    x [rows, channels] (float32, float16, bfloat16), out [rows, channels] int8, any row
+    strides; scales [rows] float32. Returns out. A row's largest magnitude becomes 127;
+    rows of zeros have scale 0, rows with an infinity or NaN zeros and scale NaN."""
+    code, device = _first("quantize_rows", "x", x)
+    xs = _look("quantize_rows", "x", x, 2, x.dtype, device)
+    os = _look("quantize_rows", "out", out, 2, _types["int8"], device)
+    _look("quantize_rows", "scales", scales, 1, _types[FP32], device)
+    rows, channels = x.shape
+    _shape("quantize_rows", "out", out, rows, channels)
+    _shape("quantize_rows", "scales", scales, rows)
+    _sizes("quantize_rows", rows, channels)
+    _no_gradients("quantize_rows", x, scales)
+    p = _QuantizeParams(code, channels, rows, x.data_ptr(), xs[0], out.data_ptr(), os[0], scales.data_ptr())
+    hip_check((_lib or _library()).kgh_quantize_rows(device, p, _stream(x, device) if stream is None else stream))
+    return out
+
+
+def linear_int8_workspace(x, weights) -> int:
+    """kgh_linear_int8_workspace: bytes of workspace that ``linear_int8`` makes use of
+    for tensors of these shapes (0: none). A larger one serves too."""
+    rows, in_c = x.shape
+    _sizes("linear_int8", rows, in_c, weights.shape[0])
+    p = _LinearInt8Params(FP32, 0, rows, in_c, weights.shape[0])
+    p.out_stride = p.out_channels
+    n = ctypes.c_uint64()
+    hip_check((_lib or _library()).kgh_linear_int8_workspace(x.get_device(), p, n))
+    return n.value
+
+
+def linear_int8(x, x_scales, weights, weight_scales, out, bias=None, activation=None, residual=None, workspace=None, stream=None):
+    """kgh_linear_int8: out = activation((x @ weights.T) * x_scales[:, None] *
+    weight_scales + bias) + residual, the products of 8-bit integers and their sums
+    exact.
+
+    x [rows, in] and weights [out, in] int8, x_scales [rows] and weight_scales [out]
+    float32, as ``quantize_rows`` makes them; out and residual [rows, out] of one type
+    (float32, float16, bfloat16); any row strides; bias [out] float32; activation one of
+    ``ACTIVATIONS``. residual may be out itself. workspace: at least
+    ``linear_int8_workspace`` bytes of its own for calls that may overlap."""
+    code, device = _first("linear_int8", "out", out)
+    dtype = out.dtype
+    i8, f32 = _types["int8"], _types[FP32]
+    xs = _look("linear_int8", "x", x, 2, i8, device)
+    ws = _look("linear_int8", "weights", weights, 2, i8, device)
+    os = _look("linear_int8", "out", out, 2, dtype, device)
+    _look("linear_int8", "x_scales", x_scales, 1, f32, device)
+    _look("linear_int8", "weight_scales", weight_scales, 1, f32, device)
+    rows, in_c = x.shape
+    out_c, w_in = weights.shape
+    if w_in != in_c:
+        _invalid(f"linear_int8: weights have {w_in} input channels, x has {in_c}")
+    _sizes("linear_int8", rows, in_c, out_c)
+    _shape("linear_int8", "out", out, rows, out_c)
+    _shape("linear_int8", "x_scales", x_scales, rows)
+    _shape("linear_int8", "weight_scales", weight_scales, out_c)
+    act = ACTIVATIONS.get(activation or "identity")
+    if act is None:
+        _invalid(f"linear_int8: unknown activation {activation!r}")
+    bp = None
+    rs = space = (None, 0)
+    if bias is not None:
+        _look("linear_int8", "bias", bias, 1, f32, device)
+        _shape("linear_int8", "bias", bias, out_c)
+        bp = bias.data_ptr()
+    if residual is not None:
+        rs = (residual.data_ptr(), _look("linear_int8", "residual", residual, 2, dtype, device)[0])
+        _shape("linear_int8", "residual", residual, rows, out_c)
+    if workspace is not None:
+        space = _workspace("linear_int8", workspace, device)
+    _no_gradients("linear_int8", x_scales, weight_scales, out, bias, residual)
+    p = _LinearInt8Params(code, act, rows, in_c, out_c, x.data_ptr(), xs[0], x_scales.data_ptr(), weights.data_ptr(), ws[0], weight_scales.data_ptr(),
+                          bp, *rs, out.data_ptr(), os[0], *space)
+    hip_check((_lib or _library()).kgh_linear_int8(device, p, _stream(out, device) if stream is None else stream))
+    return out
+
+
+def _norm_start(op, x, groups, activation):
+    """What both directions' parameters begin with, and the device."""
+    code, device = _first(op, "x", x)
+    xs = _look(op, "x", x, 3, x.dtype, device)
+    batch, positions, channels = x.shape
+    _sizes(op, batch, positions, channels)
+    if groups < 1 or channels % groups != 0:
+        _invalid(f"{op}: groups must divide channels")
+    act = ACTIVATIONS.get(activation or "identity")
+    if act is None:
+        _invalid(f"{op}: unknown activation {activation!r}")
+    return (code, act, batch, positions, channels, groups), xs[:2], device
+
+
+def _norm_inputs(op, p, device, weight, bias, lengths, mask):
+    """The arguments that both directions may have."""
+    if weight is not None:
+        _look(op, "weight", weight, 1, _types[FP32], device)
+        _shape(op, "weight", weight, p.channels)
+        p.weight = weight.data_ptr()
+    if bias is not None:
+        _look(op, "bias", bias, 1, _types[FP32], device)
+        _shape(op, "bias", bias, p.channels)
+        p.bias = bias.data_ptr()
+    if lengths is not None:
+        _look(op, "lengths", lengths, 1, _types["int32"], device)
+        _shape(op, "lengths", lengths, p.batch)
+        p.lengths = lengths.data_ptr()
+    if mask is not None:
+        kind = _code(op, "mask", mask)
+        ms = _look(op, "mask", mask, 2, _types[kind if kind in ("uint8", "bool") else "uint8"], device)
+        _shape(op, "mask", mask, p.batch, p.positions)
+        p.mask, p.mask_stride = mask.data_ptr(), ms[0]
+
+
+def _whole(op, name, t, shape, device):
+    """The pointer of a contiguous float32 tensor."""
+    strides = _look(op, name, t, len(shape), _types[FP32], device)
+    _shape(op, name, t, *shape)
+    n = 1
+    for size, stride in zip(reversed(shape), reversed(strides)):
+        if stride != n and size > 1:
+            _invalid(f"{op}: {name} is not contiguous")
+        n *= size
+    return t.data_ptr()
+
+
+def group_norm_workspace(x, out, groups) -> int:
+    """kgh_group_norm_workspace: bytes of workspace that ``group_norm`` needs for
+    tensors of these shapes and types (0: none). A larger one serves too."""
+    start, xs, device = _norm_start("group_norm", x, groups, None)
+    p = _GroupNormParams(*start)
+    if _code("group_norm", "out", out) == "int8":
+        p.out_scales = 4
+    n = ctypes.c_uint64()
+    hip_check((_lib or _library()).kgh_group_norm_workspace(device, p, n))
+    return n.value
+
+
+def group_norm(x, out, groups, weight=None, bias=None, eps=1e-5, activation=None, lengths=None, mask=None, out_scales=None, stats=None,
+               workspace=None, stream=None):
+    """kgh_group_norm: activation((x - mean) / sqrt(variance + eps) * weight + bias),
+    mean and variance of each item over a group's channels at the positions that take
+    part.
+
+    x [batch, positions, channels] (float32, float16, bfloat16), out of the same shape
+    and type, any strides but that of the last axis; or out int8 and out_scales [batch,
+    positions] float32, contiguous: rows in 8 bits as ``quantize_rows`` makes them.
+    groups runs of channels; weight and bias [channels] float32; activation one of
+    ``ACTIVATIONS``. lengths [batch] int32: positions from there on take no part; mask
+    [batch, positions] uint8 or bool: nor do those with 0. What x holds there is not
+    used, and out is zero. stats [batch, groups, 2] float32, contiguous, takes mean and
+    1 / sqrt(variance + eps) for ``group_norm_backward``. out may be x itself. workspace:
+    at least ``group_norm_workspace`` bytes, of its own for calls that may overlap."""
+    start, xs, device = _norm_start("group_norm", x, groups, activation)
+    p = _GroupNormParams(*start, eps, x.data_ptr(), xs)
+    _norm_inputs("group_norm", p, device, weight, bias, lengths, mask)
+    if out_scales is not None:
+        p.out_scales = _whole("group_norm", "out_scales", out_scales, (p.batch, p.positions), device)
+    p.out_strides = _look("group_norm", "out", out, 3, x.dtype if out_scales is None else _types["int8"], device)[:2]
+    _shape("group_norm", "out", out, p.batch, p.positions, p.channels)
+    p.out = out.data_ptr()
+    if stats is not None:
+        p.statistics = _whole("group_norm", "stats", stats, (p.batch, groups, 2), device)
+    _no_gradients("group_norm", x, out, weight, bias)
+    if workspace is not None:
+        p.workspace, p.workspace_bytes = _workspace("group_norm", workspace, device)
+    hip_check((_lib or _library()).kgh_group_norm(device, p, _stream(x, device) if stream is None else stream))
+    return out
+
+
+def group_norm_backward_workspace(x, groups) -> int:
+    """kgh_group_norm_backward_workspace: bytes of workspace that
+    ``group_norm_backward`` needs for a tensor of this shape and type (0: none). A larger
+    one serves too."""
+    start, xs, device = _norm_start("group_norm_backward", x, groups, None)
+    n = ctypes.c_uint64()
+    hip_check((_lib or _library()).kgh_group_norm_backward_workspace(device, _GroupNormBackwardParams(*start), n))
+    return n.value
+
+
+def group_norm_backward(x, grad_out, stats, grad_x, groups, weight=None, bias=None, activation=None, lengths=None, mask=None, grad_weight=None,
+                        grad_bias=None, workspace=None, stream=None):
+    """kgh_group_norm_backward: the gradients of ``group_norm`` for x (into grad_x,
+    which is returned), and where they are given for weight (grad_weight) and bias
+    (grad_bias).
+
+    x, grad_out and grad_x [batch, positions, channels] of one type, any strides but
+    that of the last axis; stats [batch, groups, 2] of the forward call; weight, bias,
+    activation, lengths and mask as they were there; grad_weight and grad_bias [channels]
+    float32. grad_x is zero at positions that take no part. workspace: at least
+    ``group_norm_backward_workspace`` bytes, of its own for calls that may overlap."""
+    op = "group_norm_backward"
+    start, xs, device = _norm_start(op, x, groups, activation)
+    p = _GroupNormBackwardParams(*start, x.data_ptr(), xs)
+    _norm_inputs(op, p, device, weight, bias, lengths, mask)
+    p.grad_out_strides = _look(op, "grad_out", grad_out, 3, x.dtype, device)[:2]
+    p.grad_x_strides = _look(op, "grad_x", grad_x, 3, x.dtype, device)[:2]
+    _shape(op, "grad_out", grad_out, p.batch, p.positions, p.channels)
+    _shape(op, "grad_x", grad_x, p.batch, p.positions, p.channels)
+    p.grad_out, p.grad_x = grad_out.data_ptr(), grad_x.data_ptr()
+    p.statistics = _whole(op, "stats", stats, (p.batch, groups, 2), device)
+    if grad_weight is not None:
+        p.grad_weight = _whole(op, "grad_weight", grad_weight, (p.channels,), device)
+    if grad_bias is not None:
+        p.grad_bias = _whole(op, "grad_bias", grad_bias, (p.channels,), device)
+    _no_gradients(op, x, grad_out, grad_x, weight, bias, grad_weight, grad_bias)
+    if workspace is not None:
+        p.workspace, p.workspace_bytes = _workspace(op, workspace, device)
+    hip_check((_lib or _library()).kgh_group_norm_backward(device, p, _stream(x, device) if stream is None else stream))
+    return grad_x
