@@ -44,7 +44,7 @@ ORACLE_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-mavx2", "-mfma", "-Wall"]
 
 HIP_SOURCES = ["kgh_conv.hip", "kgh_conv_split.hip", "kgh_conv_stream.hip", "kgh_kernels.hip", "kgh_transformer.hip",
                "kgh_op_linear.hip", "kgh_op_rope.hip", "kgh_op_attention.hip", "kgh_op_quantize.hip",
-               "kgh_op_linear_int8.hip", "kgh_op_norm.hip", "kgh_api.hip"]
+               "kgh_op_linear_int8.hip", "kgh_op_norm.hip", "kgh_op_norm_backward.hip", "kgh_api.hip"]
 HOST_SOURCES = [
     "host/core/global.cpp",
     "host/neuralnet/desc.cpp",

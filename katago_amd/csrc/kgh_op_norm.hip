@@ -1,227 +1,615 @@
-// Group norm with an activation, channels last, and its gradient (kgh_group_norm,
-// kgh_group_norm_backward).
-#include "kgh_op_quantize_device.h"
+// Group norm with an activation, channels last (kgh_group_norm).
+#include "kgh_op_norm_device.h"
 
-#include <algorithm>
 #include <cfloat>
 
 namespace {
 
-constexpr int NORM_MAX_LEN = 1 << 30, NORM_MAX_CHANNELS = 1 << 20;
-
-// What both directions read. Strides count elements.
-struct NormArgs {
-  const void* x;
-  const float* weight;
-  const float* bias;
-  const int32_t* lengths;
-  const uint8_t* mask;
-  int64_t xB, xP, maskB;
-  int batch, positions, channels, groups, per;  // per: channels of a group
-  float eps;
-};
-
-__device__ __forceinline__ int validLength(const NormArgs& a, int b) {
-  return a.lengths == nullptr ? a.positions : min(max(a.lengths[b], 0), a.positions);
-}
-__device__ __forceinline__ bool takesPart(const NormArgs& a, int b, int p, int len) { return p < len && (a.mask == nullptr || a.mask[b * a.maskB + p] != 0); }
-
-// The sum over a workgroup of 256, for all of its threads.
-__device__ __forceinline__ double sumAll(double v, double* lds) {
-#pragma unroll
-  for(int w = 32; w > 0; w >>= 1) v += __shfl_xor(v, w);
-  __syncthreads();
-  if((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
-}
-
-// Mean and 1 / sqrt(variance + eps) of a group of an item.
-template<typename T>
-__global__ __launch_bounds__(256) void normStatsKernel(NormArgs a, float* stats) {
-  __shared__ double lds[4];
-  for(int64_t i = blockIdx.x; i < (int64_t)a.batch * a.groups; i += gridDim.x) {
-  const int b = (int)(i / a.groups), g = (int)(i - (int64_t)b * a.groups);
-  const T* x = (const T*)a.x + b * a.xB + g * a.per;
-  const int len = validLength(a, b);
-  double sum = 0.0, count = 0.0;
-  for(int64_t e = threadIdx.x; e < (int64_t)len * a.per; e += 256) {
-    const int p = (int)(e / a.per);
-    if(!takesPart(a, b, p, len)) continue;
-    sum += (double)(float)x[p * a.xP + (e - (int64_t)p * a.per)];
-    count += 1.0;
-  }
-  count = sumAll(count, lds);
-  const double mean = sumAll(sum, lds) / fmax(count, 1.0);
-  double squares = 0.0;
-  for(int64_t e = threadIdx.x; e < (int64_t)len * a.per; e += 256) {
-    const int p = (int)(e / a.per);
-    if(!takesPart(a, b, p, len)) continue;
-    const double d = (double)(float)x[p * a.xP + (e - (int64_t)p * a.per)] - mean;
-    squares += d * d;
-  }
-  const double var = sumAll(squares, lds) / fmax(count, 1.0);
-  if(threadIdx.x == 0) {
-    float* s = stats + ((int64_t)b * a.groups + g) * 2;
-    s[0] = count == 0.0 ? 0.0f : (float)mean;
-    s[1] = count == 0.0 ? 0.0f : (float)(1.0 / sqrt(var + (double)a.eps));
-  }
-  }
-}
-
-// A row (item, position).
-template<typename T, int ACT>
-__global__ __launch_bounds__(256) void normApplyKernel(NormArgs a, const float* stats, void* out, int64_t oB, int64_t oP, float* scales) {
-  __shared__ unsigned tops[4];
-  for(int i = blockIdx.x; i < a.batch * a.positions; i += gridDim.x) {
-  const int p = i % a.positions, b = i / a.positions;
-  const T* x = (const T*)a.x + b * a.xB + p * a.xP;
-  const bool on = takesPart(a, b, p, validLength(a, b));
-  const int64_t at = b * oB + p * oP;
-  auto value = [&](int c) {
-    if(!on) return 0.0f;
-    const float* s = stats + ((int64_t)b * a.groups + c / a.per) * 2;
-    const float h = ((float)x[c] - s[0]) * s[1];
-    return activate<T, ACT>(fmaf(h, a.weight != nullptr ? a.weight[c] : 1.0f, a.bias != nullptr ? a.bias[c] : 0.0f));
-  };
-  if(scales == nullptr) {
-    for(int c = threadIdx.x; c < a.channels; c += 256) ((T*)out)[at + c] = (T)value(c);
-    continue;
-  }
-  unsigned top = 0;
-  for(int c = threadIdx.x; c < a.channels; c += 256) top = max(top, magnitudeBits(value(c)));
-#pragma unroll
-  for(int w = 32; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
-  if((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  const RowScale s(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
-  for(int c = threadIdx.x; c < a.channels; c += 256) ((int8_t*)out)[at + c] = (int8_t)s.quantized(value(c));
-  if(threadIdx.x == 0) scales[(int64_t)b * a.positions + p] = s.scale;
-  __syncthreads();
-  }
-}
-
-// The activations' derivatives, by the accurate functions.
-template<int ACT>
-__device__ __forceinline__ float slope(float v) {
-  if constexpr(ACT == KGH_ACT_IDENTITY) return 1.0f;
-  else if constexpr(ACT == KGH_ACT_RELU) return v > 0.0f ? 1.0f : v != v ? v : 0.0f;
-  else if constexpr(ACT == KGH_ACT_SILU) {
-    const float s = 1.0f / (1.0f + expf(-v));
-    return s * fmaf(v, 1.0f - s, 1.0f);
-  }
-  else if constexpr(ACT == KGH_ACT_MISH) {
-    const float e = expf(fminf(v, 20.0f)), n = e * (e + 2.0f), w = 1.0f / (n + 2.0f);
-    return v > 20.0f ? 1.0f : w * fmaf(4.0f * v * e * (1.0f + e), w, n);
-  }
-  else return fmaf(0.5f, erfcf(-0.70710678118654752f * v), v * expf(-0.5f * v * v) * 0.39894228040143268f);
-}
-
-struct NormBackArgs {
-  const void* grad;
-  int64_t gB, gP;
-  const float* stats;
+struct NormOut {
   void* out;
   int64_t oB, oP;
-  float* gradWeight;
-  float* gradBias;
-  float* sums;  // [batch][channels][2]: of u and u h over an item's positions
+  float* scales;  // of rows in 8 bits, or null
+  float* stats;   // [batch][groups][2]: mean and 1 / sqrt(variance + eps), or null
 };
 
-template<typename T, int ACT>
-__device__ __forceinline__ void backValues(const NormArgs& a, const NormBackArgs& k, int b, int p, int c, float& u, float& h, float& rstd) {
-  const float* s = k.stats + ((int64_t)b * a.groups + c / a.per) * 2;
-  rstd = s[1];
-  h = ((float)((const T*)a.x)[b * a.xB + p * a.xP + c] - s[0]) * rstd;
-  const float z = fmaf(h, a.weight != nullptr ? a.weight[c] : 1.0f, a.bias != nullptr ? a.bias[c] : 0.0f);
-  u = (float)((const T*)k.grad)[b * k.gB + p * k.gP + c] * slope<ACT>(z);
+// ---------------------------------------------------------------------------
+// Sums of a group's values are of differences from a reference point, 0 at first: n,
+// sum d and sum d^2 give mean and variance, and rounding costs them little where the
+// reference lies within two deviations of the mean. Where it does not, they are taken
+// once more from the mean found so far; where they pass the largest float, once more of
+// values 2^-80 times as large. A group is done after three turns at most, almost every
+// one after the first.
+constexpr int NORM_TURNS = 3;
+constexpr float NORM_SMALL = 0x1p-80f;
+
+struct GroupTurn {
+  float ref, factor;
+};
+struct GroupSums {
+  float mean, var;  // var in units of the factor's square
+  GroupTurn next;
+  bool again;
+};
+
+// What a turn's sums over n values say.
+__device__ __forceinline__ GroupSums groupSums(float n, float sum, float squares, GroupTurn turn, int turns) {
+  GroupSums r;
+  r.next = turn;
+  r.again = false;
+  const float m = sum / n;
+  r.mean = turn.ref + m / turn.factor;
+  r.var = fmaf(-m, m, squares / n);
+  if(!(fabsf(sum) <= FLT_MAX && squares <= FLT_MAX)) {
+    r.var = __builtin_nanf("");
+    r.again = turn.factor == 1.0f;
+    r.next = GroupTurn{0.0f, NORM_SMALL};
+  }
+  else {
+    r.var = fmaxf(r.var, 0.0f);
+    r.again = turn.ref == 0.0f && m * m > 4.0f * r.var;
+    r.next.ref = r.mean;
+  }
+  if(turns + 1 >= NORM_TURNS || n == 0.0f) r.again = false;
+  if(!r.again) r.next = turn;
+  return r;
 }
 
-template<typename T, int ACT>
-__global__ __launch_bounds__(256) void normBackSumsKernel(NormArgs a, NormBackArgs k) {
-  __shared__ double lds[4];
-  for(int64_t i = blockIdx.x; i < (int64_t)a.batch * a.channels; i += gridDim.x) {
-  const int b = (int)(i / a.channels), c = (int)(i - (int64_t)b * a.channels);
-  const int len = validLength(a, b);
-  double s0 = 0.0, s1 = 0.0;
-  for(int p = threadIdx.x; p < len; p += 256) {
-    if(!takesPart(a, b, p, len)) continue;
-    float u, h, rstd;
-    backValues<T, ACT>(a, k, b, p, c, u, h, rstd);
-    s0 += u;
-    s1 += (double)u * h;
-  }
-  s0 = sumAll(s0, lds);
-  s1 = sumAll(s1, lds);
-  if(threadIdx.x == 0) {
-    k.sums[((int64_t)b * a.channels + c) * 2] = (float)s0;
-    k.sums[((int64_t)b * a.channels + c) * 2 + 1] = (float)s1;
-  }
-  }
+__device__ __forceinline__ float reciprocalDeviation(const GroupSums& r, float eps) {
+  if(r.next.factor == 1.0f) return 1.0f / sqrtf(r.var + eps);
+  return (float)(1.0 / sqrt((double)r.var * 0x1p160 + (double)eps));
 }
 
-template<typename T, int ACT>
-__global__ __launch_bounds__(256) void normBackApplyKernel(NormArgs a, NormBackArgs k) {
-  __shared__ double lds[4];
-  for(int64_t i = blockIdx.x; i < (int64_t)a.batch * a.groups; i += gridDim.x) {
-  const int b = (int)(i / a.groups), g = (int)(i - (int64_t)b * a.groups);
+// (x - mean) / deviation, weight, bias and activation of VEC channels.
+template<typename T, int ACT, int VEC>
+__device__ __forceinline__ void normalise(float (&y)[VEC], const Values<T>& x, const float (&mean)[VEC], const float (&scale)[VEC], const float (&bias)[VEC]) {
+#pragma unroll
+  for(int j = 0; j < VEC; j++) y[j] = activate<T, ACT>(fmaf(x.f[j] - mean[j], scale[j], bias[j]));
+}
+
+// ---------------------------------------------------------------------------
+// An item's run of channels lies in a unit's registers from its one way in to its way
+// out: sums over a thread's positions for each of its channels, over the unit's threads
+// in LDS, then norm and activation of the same registers. Positions that take no part
+// read the item's first one, which is in a cache. QUANT: rows in 8 bits, a unit being an
+// item with all of its channels.
+template<typename T, int ACT, int NV, bool QUANT>
+__global__ __launch_bounds__(NV == 2 ? 1024 : 512) void normSlabKernel(NormArgs a, NormOut o, NormSlab s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ float2 lds[];
+  __shared__ int counts[4];
+  const int unit = s.units == 1 ? 0 : threadIdx.x >> 6;
+  const int tt = threadIdx.x - unit * s.threads;
+  const int row = tt / s.cols, col = tt - row * s.cols;
+  const int inRun = s.run / a.per;
+  float2* part = lds + unit * s.ldsPairs;
+  float2* state = part + s.ldsPairs - 2 * inRun;  // a group's reference and factor
+  float2* result = state + inRun;                 // its mean and reciprocal deviation
+  const int64_t id = s.first + (int64_t)xcdContiguousTile() * s.units + unit;
+  const bool live = id < s.count;  // (units of the last workgroup that have no work go along)
+  const int64_t mine = live ? id : s.count - 1;
+  const int b = (int)(mine / s.runs), r = (int)(mine - (int64_t)b * s.runs);
+  const int c1 = r * s.run, c0 = c1 + col * VEC;
+  const bool on = row < s.rowLanes && c0 < min(c1 + s.run, a.channels);
+  const Window<VEC> win(c0, a.channels);
+  const int groups = min(inRun, a.groups - r * inRun);
   const int len = validLength(a, b);
-  double count = 0.0, m1 = 0.0, m2 = 0.0;
-  for(int p = threadIdx.x; p < len; p += 256) count += takesPart(a, b, p, len) ? 1.0 : 0.0;
-  for(int c = threadIdx.x; c < a.per; c += 256) {
-    const float* s = k.sums + ((int64_t)b * a.channels + g * a.per + c) * 2;
-    const double w = a.weight != nullptr ? a.weight[g * a.per + c] : 1.0;
-    m1 += s[0] * w;
-    m2 += s[1] * w;
+  const T* x = (const T*)a.x + b * a.xB + win.at;
+  unsigned bits = 0;  // positions of this thread that take part
+  if(a.mask == nullptr) {
+#pragma unroll
+    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len ? 1u << i : 0u;
   }
-  count = fmax(sumAll(count, lds) * a.per, 1.0);
-  const float a1 = (float)(sumAll(m1, lds) / count), a2 = (float)(sumAll(m2, lds) / count);
-  for(int64_t e = threadIdx.x; e < (int64_t)a.positions * a.per; e += 256) {
-    const int p = (int)(e / a.per), c = g * a.per + (int)(e - (int64_t)p * a.per);
-    float y = 0.0f;
-    if(takesPart(a, b, p, len)) {
-      float u, h, rstd;
-      backValues<T, ACT>(a, k, b, p, c, u, h, rstd);
-      y = rstd * (u * (a.weight != nullptr ? a.weight[c] : 1.0f) - a1 - h * a2);
+  else {
+    if(tt == 0) counts[unit] = 0;
+    const uint8_t* mask = a.mask + b * a.maskB;
+    uint8_t m[NV];
+#pragma unroll
+    for(int i = 0; i < NV; i++) m[i] = mask[min(row + i * s.rowLanes, a.positions - 1)];
+#pragma unroll
+    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len && m[i] != 0 ? 1u << i : 0u;
+  }
+  u32x4_t v[NV];
+#pragma unroll
+  for(int i = 0; i < NV; i++)
+    if(i < s.nv) __builtin_memcpy(&v[i], x + ((bits >> i) & 1 ? row + i * s.rowLanes : 0) * a.xP, 16);
+  if(a.mask != nullptr) {
+    __syncthreads();
+    if(col == 0 && bits != 0) atomicAdd(&counts[unit], __popc(bits));
+  }
+
+  {
+    float s1[VEC], s2[VEC];
+#pragma unroll
+    for(int j = 0; j < VEC; j++) s1[j] = s2[j] = 0.0f;
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+      if(i < s.nv) {
+        const u32x4_t zero = {0, 0, 0, 0};
+        v[i] = (bits >> i) & 1 ? v[i] : zero;
+        const Values<T> d(v[i]);
+#pragma unroll
+        for(int j = 0; j < VEC; j++) {
+          s1[j] += d.f[j];
+          s2[j] = fmaf(d.f[j], d.f[j], s2[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    if(on) {
+      float2* p = part + row * s.entries + col * s.pv;
+      if(s.pv == 1) {
+#pragma unroll
+        for(int j = 1; j < VEC; j++) s1[0] += s1[j], s2[0] += s2[j];
+        *p = make_float2(s1[0], s2[0]);
+      }
+      else {
+#pragma unroll
+        for(int j = 0; j < VEC; j++)
+          if(j >= win.skip) p[j - win.skip] = make_float2(s1[j], s2[j]);
+      }
     }
-    ((T*)k.out)[b * k.oB + p * k.oP + c] = (T)y;
+    __syncthreads();
   }
+  for(int turns = 0;; turns++) {
+    const float2* red = addRows(part, s, tt);
+    if(s.rowLanes > 1) __syncthreads();
+    const int entries = s.pv == 1 ? a.per / VEC : a.per;
+    const int sub = tt & (s.lanes - 1);
+    const float n = (float)(a.mask != nullptr ? counts[unit] : len) * (float)a.per;
+    bool again = false;
+    for(int q = tt / s.lanes; q < groups; q += s.threads / s.lanes) {
+      float sum = 0.0f, squares = 0.0f;
+      for(int k = sub; k < entries * s.segments; k += s.lanes) {
+        const int seg = k / entries;
+        const float2 u = red[seg * s.entries + q * entries + (k - seg * entries)];
+        sum += u.x;
+        squares += u.y;
+      }
+      for(int k = s.lanes >> 1; k > 0; k >>= 1) {
+        sum += __shfl_xor(sum, k);
+        squares += __shfl_xor(squares, k);
+      }
+      const GroupSums t = groupSums(n, sum, squares, turns == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turns);
+      again |= t.again;
+      if(sub == 0) {
+        const float rd = reciprocalDeviation(t, a.eps);
+        state[q] = make_float2(t.next.ref, t.next.factor);
+        result[q] = n == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(t.mean, rd);
+      }
+    }
+    if(!__syncthreads_or(again)) break;
+    // Channel by channel: few registers, for few units.
+    int first = win.at - c1;
+    asm volatile("" : "+v"(first));
+    float2 all = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      const float2 t = state[min(max(first + j, 0) / a.per, groups - 1)];
+      const float ref = t.x * t.y;
+      float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for(int i = 0; i < NV; i++) {
+        renew(v[i]);
+        const float d = fmaf(Values<T>(v[i]).f[j], t.y, -ref);
+        if((bits >> i) & 1) {
+          sum.x += d;
+          sum.y = fmaf(d, d, sum.y);
+        }
+      }
+      all.x += sum.x;
+      all.y += sum.y;
+      if(s.pv > 1 && on && j >= win.skip) part[row * s.entries + col * VEC + j - win.skip] = sum;
+    }
+    if(s.pv == 1 && on) part[row * s.entries + col] = all;
+    __syncthreads();
+  }
+
+  if(o.stats != nullptr && live)
+    for(int q = tt; q < groups; q += s.threads) *(float2*)(o.stats + 2 * ((int64_t)b * a.groups + r * inRun + q)) = result[q];
+  float scale[VEC], bias[VEC], mean[VEC];
+  loadFloats(scale, a.weight == nullptr ? nullptr : a.weight + win.at, VEC, 1.0f);
+  loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + win.at, VEC, 0.0f);
+#pragma unroll
+  for(int j = 0; j < VEC; j++) {
+    const float2 t = result[min(max(win.at + j - c1, 0) / a.per, groups - 1)];
+    mean[j] = t.x;
+    scale[j] *= t.y;
+  }
+  if constexpr(!QUANT) {
+    T* out = (T*)o.out + b * o.oB + win.at;
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+      if(i < s.nv) {
+        const int p = row + i * s.rowLanes;
+        float y[VEC];
+        renew(v[i]);
+        normalise<T, ACT>(y, Values<T>(v[i]), mean, scale, bias);
+        const uint4 u = packed<T>(y), zero = make_uint4(0, 0, 0, 0);
+        if(on && live && p < a.positions) storeWindow(out + p * o.oP, (bits >> i) & 1 ? u : zero, win.skip);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+  else {
+    unsigned* tops = (unsigned*)part;
+    for(int p = tt; p < a.positions; p += s.threads) tops[p] = 0;
+    __syncthreads();
+    float y[NV][VEC];
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+      if(i < s.nv) {
+        renew(v[i]);
+        normalise<T, ACT>(y[i], Values<T>(v[i]), mean, scale, bias);
+        unsigned top = 0;
+#pragma unroll
+        for(int j = 0; j < VEC; j++) top = max(top, j >= win.skip ? magnitudeBits(y[i][j]) : 0);
+        if((bits >> i) & 1) atomicMax(&tops[row + i * s.rowLanes], top);
+      }
+    __syncthreads();
+    int8_t* out = (int8_t*)o.out + b * o.oB + win.at;
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+      if(i < s.nv) {
+        const int p = row + i * s.rowLanes;
+        if(on && live && p < a.positions) {
+          const RowScale rs(tops[p]);
+          const uint2 q = quantized(y[i], rs);
+          storeBytes<VEC>(out + p * o.oP, (bits >> i) & 1 ? q : make_uint2(0, 0), win.skip, VEC);
+          if(col == 0) o.scales[(int64_t)b * a.positions + p] = rs.scale;
+        }
+      }
   }
 }
 
-__global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackArgs k) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if(c >= a.channels) return;
-  double s0 = 0.0, s1 = 0.0;
-  for(int b = 0; b < a.batch; b++) {
-    s0 += k.sums[((int64_t)b * a.channels + c) * 2];
-    s1 += k.sums[((int64_t)b * a.channels + c) * 2 + 1];
+// ---------------------------------------------------------------------------
+// Items that no workgroup's registers hold: their positions in `chunks` of chunkRows,
+// their columns in `blocks` of `cols`, each a workgroup. A part's groups have their
+// number of values, mean, sum of squares about it and that sum's factor in
+// parts[item][chunk][block][slot], slot 0 being the block's first group.
+struct NormParts {
+  float4* parts;
+  int chunks, chunkRows, blocks, cols, rowLanes, slots, lanes;  // lanes: threads that add up a group
+};
+
+constexpr int PARTS_AHEAD = 4;  // rows of a thread under way
+
+template<typename T>
+__global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  __shared__ float2 part[256 * VEC];
+  __shared__ float2 state[256 * VEC];
+  __shared__ int counted;
+  const int row = threadIdx.x / k.cols, col = threadIdx.x - row * k.cols;
+  const int64_t all = (int64_t)a.batch * k.chunks * k.blocks;
+  for(int64_t id = blockIdx.x; id < all; id += gridDim.x) {
+    const int64_t itemChunk = id / k.blocks;
+    const int block = (int)(id - itemChunk * k.blocks);
+    const int b = (int)(itemChunk / k.chunks), chunk = (int)(itemChunk - (int64_t)b * k.chunks);
+    const int from = block * k.cols * VEC, to = min(from + k.cols * VEC, a.channels);
+    const int c0 = from + col * VEC, nc = min(to - c0, VEC);
+    const bool on = row < k.rowLanes && nc > 0;
+    const int firstGroup = from / a.per, groups = (to - 1) / a.per - firstGroup + 1;
+    const int len = validLength(a, b);
+    const int p0 = chunk * k.chunkRows, p1 = min(p0 + k.chunkRows, len);
+    const RowGroup<T, false> g((on ? c0 : 0) / VEC, a.channels);
+    const T* x = (const T*)a.x + b * a.xB;
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.maskB;
+    if(threadIdx.x == 0) counted = 0;
+    __syncthreads();
+    auto groupOf = [&](int j) { return (c0 + max(min(j, nc - 1), 0)) / a.per - firstGroup; };
+    int rows = 0;
+    for(int turns = 0;; turns++) {
+      float s1[VEC], s2[VEC], ref[VEC], factor[VEC];
+#pragma unroll
+      for(int j = 0; j < VEC; j++) {
+        s1[j] = s2[j] = ref[j] = 0.0f;
+        factor[j] = 1.0f;
+        if(turns > 0 && on) {
+          const float2 t = state[groupOf(j)];
+          factor[j] = t.y;
+          ref[j] = t.x * t.y;
+        }
+      }
+      rows = 0;
+      if(on) {
+        for(int p = p0 + row; p < p1; p += PARTS_AHEAD * k.rowLanes) {
+          u32x4_t v[PARTS_AHEAD];
+          bool take[PARTS_AHEAD];
+#pragma unroll
+          for(int i = 0; i < PARTS_AHEAD; i++) {
+            const int q = p + i * k.rowLanes;
+            take[i] = q < p1 && (mask == nullptr || mask[q] != 0);
+          }
+#pragma unroll
+          for(int i = 0; i < PARTS_AHEAD; i++) v[i] = g.load(x + (take[i] ? p + i * k.rowLanes : p) * a.xP);
+#pragma unroll
+          for(int i = 0; i < PARTS_AHEAD; i++) {
+            rows += take[i] ? 1 : 0;
+            const u32x4_t zero = {0, 0, 0, 0};
+            const Values<T> u(take[i] ? g.place(v[i]) : zero);
+#pragma unroll
+            for(int j = 0; j < VEC; j++) {
+              const float d = turns == 0 ? u.f[j] : take[i] && j < nc ? fmaf(u.f[j], factor[j], -ref[j]) : 0.0f;
+              s1[j] += d;
+              s2[j] = fmaf(d, d, s2[j]);
+            }
+          }
+        }
+      }
+      if(turns == 0 && on && col == 0 && rows > 0) atomicAdd(&counted, rows);
+      if(row < k.rowLanes) {
+#pragma unroll
+        for(int j = 0; j < VEC; j++) part[(row * k.cols + col) * VEC + j] = make_float2(s1[j], s2[j]);
+      }
+      __syncthreads();
+      // A group's channels in this block, over the rows, by `lanes` threads.
+      const int sub = threadIdx.x & (k.lanes - 1);
+      bool again = false;
+      for(int q = threadIdx.x / k.lanes; q < groups; q += 256 / k.lanes) {
+        const int e0 = max((firstGroup + q) * a.per - from, 0), e1 = min((firstGroup + q + 1) * a.per, to) - from;
+        float sum = 0.0f, squares = 0.0f;
+        for(int i = sub; i < (e1 - e0) * k.rowLanes; i += k.lanes) {
+          const int r = i / (e1 - e0);
+          const float2 u = part[r * k.cols * VEC + e0 + (i - r * (e1 - e0))];
+          sum += u.x;
+          squares += u.y;
+        }
+        for(int w = k.lanes >> 1; w > 0; w >>= 1) {
+          sum += __shfl_xor(sum, w);
+          squares += __shfl_xor(squares, w);
+        }
+        const float n = (float)counted * (float)(e1 - e0);
+        const GroupSums t = groupSums(n, sum, squares, turns == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turns);
+        again |= t.again;
+        if(sub == 0) {
+          state[q] = make_float2(t.next.ref, t.next.factor);
+          k.parts[id * k.slots + q] = n == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 1.0f) : make_float4(n, t.mean, t.var, t.next.factor);
+        }
+      }
+      if(!__syncthreads_or(again)) break;
+    }
   }
-  if(k.gradBias != nullptr) k.gradBias[c] = (float)s0;
-  if(k.gradWeight != nullptr) k.gradWeight[c] = (float)s1;
 }
 
-// Rows (item, position) of a tensor that is written lie apart.
-void checkApartRows(const char* op, const char* name, int64_t batchStride, int64_t positionStride, int batch, int positions, int channels) {
-  const bool positionsInside = (positions == 1 || positionStride >= channels) && (batch == 1 || batchStride >= (positions - 1) * positionStride + channels);
-  const bool itemsInside = (batch == 1 || batchStride >= channels) && (positions == 1 || positionStride >= (batch - 1) * batchStride + channels);
-  if(!positionsInside && !itemsInside) kgh::opInvalid(op, std::string("the strides of ") + name + " make its rows overlap");
+// The parts of a group in one: mean, then the squares about it, in 64 bits (numbers are
+// few, and may be any fp32's square). A wave a group of an item.
+__global__ __launch_bounds__(256) void normJoinKernel(NormArgs a, NormParts k, float* stats, int vec) {
+  const int lane = threadIdx.x & 63;
+  for(int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < (int64_t)a.batch * a.groups; i += (int64_t)gridDim.x * 4) {
+    const int b = (int)(i / a.groups), g = (int)(i - (int64_t)b * a.groups);
+    const int width = k.cols * vec;
+    const int block0 = g * a.per / width, block1 = ((g + 1) * a.per - 1) / width;
+    const int64_t parts = (int64_t)k.chunks * (block1 - block0 + 1);
+    auto part = [&](int64_t e) {
+      const int chunk = (int)(e / (block1 - block0 + 1)), block = block0 + (int)(e - (int64_t)chunk * (block1 - block0 + 1));
+      return k.parts[(((int64_t)b * k.chunks + chunk) * k.blocks + block) * k.slots + g - block * width / a.per];
+    };
+    double n = 0.0, sum = 0.0, squares = 0.0;
+    for(int64_t e = lane; e < parts; e += 64) {
+      const float4 v = part(e);
+      n += v.x;
+      sum += (double)v.x * v.y;
+    }
+#pragma unroll
+    for(int w = 32; w > 0; w >>= 1) {
+      n += __shfl_xor(n, w);
+      sum += __shfl_xor(sum, w);
+    }
+    const double mean = n == 0.0 ? 0.0 : sum / n;
+    for(int64_t e = lane; e < parts; e += 64) {
+      const float4 v = part(e);
+      const double d = v.y - mean;
+      squares += v.x == 0.0f ? 0.0 : v.x * ((v.w == 1.0f ? (double)v.z : v.z * 0x1p160) + d * d);
+    }
+#pragma unroll
+    for(int w = 32; w > 0; w >>= 1) squares += __shfl_xor(squares, w);
+    if(lane == 0) {
+      stats[i * 2] = (float)mean;
+      stats[i * 2 + 1] = n == 0.0 ? 0.0f : (float)(1.0 / sqrt(squares / n + (double)a.eps));
+    }
+  }
 }
 
-template<typename P>
-void checkNormSizes(const char* op, const P& p) {
-  kgh::opCheckDtype(op, p.dtype);
-  kgh::opCheckActivation(op, p.activation);
-  if(p.batch < 0 || p.positions < 0 || (int64_t)p.batch * p.positions > NORM_MAX_LEN)
-    kgh::opInvalid(op, "batch and positions must be 0 or more, their product at most " + std::to_string(NORM_MAX_LEN));
-  if(p.channels < 1 || p.channels > NORM_MAX_CHANNELS) kgh::opInvalid(op, "channels must be in 1.." + std::to_string(NORM_MAX_CHANNELS));
-  if(p.groups < 1 || p.channels % p.groups != 0) kgh::opInvalid(op, "groups must divide channels");
+// Norm and activation of what normJoinKernel has the statistics of: the same chunks and
+// blocks, a thread with a column's constants in registers.
+template<typename T, int ACT>
+__global__ __launch_bounds__(256) void normApplyKernel(NormArgs a, NormOut o, NormParts k) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int row = threadIdx.x / k.cols, col = threadIdx.x - row * k.cols;
+  const int64_t all = (int64_t)a.batch * k.chunks * k.blocks;
+  if(row >= k.rowLanes) return;
+  for(int64_t id = blockIdx.x; id < all; id += gridDim.x) {
+    const int64_t itemChunk = id / k.blocks;
+    const int block = (int)(id - itemChunk * k.blocks);
+    const int b = (int)(itemChunk / k.chunks), chunk = (int)(itemChunk - (int64_t)b * k.chunks);
+    const int c0 = (block * k.cols + col) * VEC, nc = min(a.channels - c0, VEC);
+    if(nc <= 0) continue;
+    const int len = validLength(a, b);
+    const int p0 = chunk * k.chunkRows, p1 = min(p0 + k.chunkRows, a.positions);
+    const RowGroup<T, false> g(c0 / VEC, a.channels);
+    const T* x = (const T*)a.x + b * a.xB;
+    T* out = (T*)o.out + b * o.oB + c0;
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.maskB;
+    float mean[VEC], scale[VEC], bias[VEC];
+    loadFloats(scale, a.weight == nullptr ? nullptr : a.weight + c0, nc, 1.0f);
+    loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + c0, nc, 0.0f);
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      const float* t = o.stats + 2 * ((int64_t)b * a.groups + (c0 + min(j, nc - 1)) / a.per);
+      mean[j] = t[0];
+      scale[j] *= t[1];
+    }
+    for(int p = p0 + row; p < p1; p += PARTS_AHEAD * k.rowLanes) {
+      u32x4_t v[PARTS_AHEAD];
+      bool take[PARTS_AHEAD];
+#pragma unroll
+      for(int i = 0; i < PARTS_AHEAD; i++) {
+        const int q = min(p + i * k.rowLanes, p1 - 1);
+        take[i] = q < len && (mask == nullptr || mask[q] != 0);
+      }
+#pragma unroll
+      for(int i = 0; i < PARTS_AHEAD; i++) v[i] = g.load(x + (take[i] ? min(p + i * k.rowLanes, p1 - 1) : 0) * a.xP);
+#pragma unroll
+      for(int i = 0; i < PARTS_AHEAD; i++) {
+        const int q = p + i * k.rowLanes;
+        float y[VEC];
+        normalise<T, ACT>(y, Values<T>(g.place(v[i])), mean, scale, bias);
+        const uint4 u = packed<T>(y), zero = make_uint4(0, 0, 0, 0);
+        if(q < p1) storeGroup(out + q * o.oP, take[i] ? u : zero, nc);
+      }
+    }
+  }
 }
 
-template<typename P>
-NormArgs normArgs(const P& p, float eps) {
-  return NormArgs{p.x, p.weight, p.bias, p.lengths, p.mask, p.x_batch_stride, p.x_position_stride, p.mask_stride,
-                  p.batch, p.positions, p.channels, p.groups, p.channels / p.groups, eps};
+// The same in 8 bits: a row's columns by `lanes` threads, K each.
+template<typename T, int ACT, int K>
+__global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, int lanes, int chunks, int chunkRows) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  __shared__ unsigned tops[2][4];
+  const int sub = threadIdx.x & (lanes - 1), row = threadIdx.x / lanes, rows = 256 / lanes;
+  for(int64_t id = blockIdx.x; id < (int64_t)a.batch * chunks; id += gridDim.x) {
+    const int b = (int)(id / chunks), chunk = (int)(id - (int64_t)b * chunks);
+    const int len = validLength(a, b);
+    const int p0 = chunk * chunkRows, p1 = min(p0 + chunkRows, a.positions);
+    const T* x = (const T*)a.x + b * a.xB;
+    int8_t* out = (int8_t*)o.out + b * o.oB;
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.maskB;
+    float mean[K][VEC], scale[K][VEC], bias[K][VEC];
+#pragma unroll
+    for(int i = 0; i < K; i++) {
+      const int c0 = (sub + i * lanes) * VEC, nc = a.channels - c0;
+      loadFloats(scale[i], a.weight == nullptr ? nullptr : a.weight + c0, nc, 1.0f);
+      loadFloats(bias[i], a.bias == nullptr ? nullptr : a.bias + c0, nc, 0.0f);
+#pragma unroll
+      for(int j = 0; j < VEC; j++) {
+        const float* t = o.stats + 2 * ((int64_t)b * a.groups + min(c0 + j, a.channels - 1) / a.per);
+        mean[i][j] = t[0];
+        scale[i][j] *= t[1];
+      }
+    }
+    int turn = 0;
+    for(int p = p0 + row; p - row < p1; p += rows, turn ^= 1) {
+      const int q = min(p, p1 - 1);
+      const bool take = p < p1 && q < len && (mask == nullptr || mask[q] != 0);
+      u32x4_t v[K];
+#pragma unroll
+      for(int i = 0; i < K; i++) v[i] = RowGroup<T, false>(min(sub + i * lanes, (a.channels - 1) / VEC), a.channels).load(x + (take ? q : 0) * a.xP);
+      float y[K][VEC];
+      unsigned top = 0;
+#pragma unroll
+      for(int i = 0; i < K; i++) {
+        const int nc = a.channels - (sub + i * lanes) * VEC;
+        normalise<T, ACT>(y[i], Values<T>(RowGroup<T, false>(min(sub + i * lanes, (a.channels - 1) / VEC), a.channels).place(v[i])), mean[i], scale[i], bias[i]);
+#pragma unroll
+        for(int j = 0; j < VEC; j++) top = max(top, j < nc && take ? magnitudeBits(y[i][j]) : 0);
+      }
+      top = rowTop(top, lanes, tops[turn]);
+      const RowScale rs(top);
+      if(p < p1) {
+#pragma unroll
+        for(int i = 0; i < K; i++) {
+          const int c0 = (sub + i * lanes) * VEC, nc = a.channels - c0;
+          if(nc <= 0) continue;
+          storeBytes<VEC>(out + q * o.oP + c0, take ? quantized(y[i], rs) : make_uint2(0, 0), 0, nc);
+        }
+        if(sub == 0) o.scales[(int64_t)b * a.positions + q] = rs.scale;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Rows of any length in 8 bits: each value computed twice.
+template<typename T, int ACT>
+__global__ __launch_bounds__(256) void normQuantLongKernel(NormArgs a, NormOut o) {
+  __shared__ unsigned tops[4];
+  for(int i = blockIdx.x; i < a.batch * a.positions; i += gridDim.x) {
+    const int b = i / a.positions, p = i - b * a.positions;
+    const T* x = (const T*)a.x + b * a.xB + p * a.xP;
+    int8_t* out = (int8_t*)o.out + b * o.oB + p * o.oP;
+    const bool take = p < validLength(a, b) && (a.mask == nullptr || a.mask[b * a.maskB + p] != 0);
+    auto value = [&](int c) {
+      const float* t = o.stats + 2 * ((int64_t)b * a.groups + c / a.per);
+      const float scale = (a.weight != nullptr ? a.weight[c] : 1.0f) * t[1];
+      return activate<T, ACT>(fmaf((float)x[c] - t[0], scale, a.bias != nullptr ? a.bias[c] : 0.0f));
+    };
+    unsigned top = 0;
+    if(take)
+      for(int c = threadIdx.x; c < a.channels; c += 256) top = max(top, magnitudeBits(value(c)));
+    const RowScale rs(rowTop(top, 256, tops));
+    for(int c = threadIdx.x; c < a.channels; c += 256) out[c] = (int8_t)(take ? rs.quantized(value(c)) : 0);
+    if(threadIdx.x == 0) o.scales[i] = rs.scale;
+    __syncthreads();
+  }
+}
+
+struct NormPlan {
+  NormSlab slab;    // threads 0: parts
+  NormParts parts;
+  uint64_t partsBytes, statsBytes;
+};
+
+NormPlan planNorm(const kgh_group_norm_params& p) {
+  const int size = (int)kgh::opElemBytes(p.dtype), vec = 16 / size;
+  const bool quant = p.out_scales != nullptr;
+  NormPlan plan{};
+  // One position of an item, or few: more threads with less each.
+  plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 96, false, 2, 1024, quant, 2);
+  if(plan.slab.threads == 0 && !quant) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 96, false, 16, 512, false, 2);
+  if(plan.slab.threads != 0) return plan;
+  NormParts& k = plan.parts;
+  const int cols = (p.channels + vec - 1) / vec, per = p.channels / p.groups;
+  k.cols = std::min(cols, 256);
+  k.blocks = (cols + k.cols - 1) / k.cols;
+  k.rowLanes = std::min(256 / k.cols, p.positions);
+  // A thread's rows are added one after the other: at most 128.
+  const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(128, (int64_t)p.batch * p.positions * k.blocks / k.rowLanes / 1024));
+  k.chunkRows = (int)std::min<int64_t>(p.positions, (rows + PARTS_AHEAD - 1) / PARTS_AHEAD * PARTS_AHEAD * k.rowLanes);
+  k.chunks = (p.positions + k.chunkRows - 1) / k.chunkRows;
+  k.slots = (k.cols * vec + per - 2) / per + 1;
+  k.lanes = 64;
+  while(k.lanes > 1 && k.lanes * k.slots > 256) k.lanes /= 2;
+  plan.partsBytes = (uint64_t)p.batch * k.chunks * k.blocks * k.slots * sizeof(float4);
+  plan.statsBytes = (uint64_t)p.batch * p.groups * 8;
+  return plan;
+}
+
+template<typename T, int ACT>
+void launchNorm(const NormPlan& plan, const NormArgs& a, NormOut o, void* workspace, hipStream_t stream) {
+  const bool quant = o.scales != nullptr;
+  if(plan.slab.threads != 0) {
+    forUnits(plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
+      if(quant) normSlabKernel<T, ACT, 2, true><<<grid, threads, bytes, stream>>>(a, o, s);
+      else if(s.nv <= 2) normSlabKernel<T, ACT, 2, false><<<grid, threads, bytes, stream>>>(a, o, s);
+      else if(s.nv <= 8) normSlabKernel<T, ACT, 8, false><<<grid, threads, bytes, stream>>>(a, o, s);
+      else normSlabKernel<T, ACT, 16, false><<<grid, threads, bytes, stream>>>(a, o, s);
+      KGH_CHECK_LAUNCH();
+    });
+    return;
+  }
+  NormParts k = plan.parts;
+  k.parts = (float4*)workspace;
+  if(o.stats == nullptr) o.stats = (float*)((char*)workspace + plan.partsBytes);
+  const unsigned grid = normGrid((int64_t)a.batch * k.chunks * k.blocks);
+  normPartsKernel<T><<<grid, 256, 0, stream>>>(a, k);
+  KGH_CHECK_LAUNCH();
+  normJoinKernel<<<normGrid(((int64_t)a.batch * a.groups + 3) / 4), 256, 0, stream>>>(a, k, o.stats, 16 / (int)sizeof(T));
+  KGH_CHECK_LAUNCH();
+  if(!quant) normApplyKernel<T, ACT><<<grid, 256, 0, stream>>>(a, o, k);
+  else {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const RowLanes r = rowLanes((a.channels + VEC - 1) / VEC, 4);
+    if(r.lanes == 0) normQuantLongKernel<T, ACT><<<normGrid((int64_t)a.batch * a.positions), 256, 0, stream>>>(a, o);
+    else {
+      const int rows = 256 / r.lanes;
+      const int chunkRows = (int)std::min<int64_t>((int64_t)a.positions, std::max<int64_t>(1, (int64_t)a.batch * a.positions / rows / 2048) * rows);
+      const int chunks = (a.positions + chunkRows - 1) / chunkRows;
+      const unsigned g = normGrid((int64_t)a.batch * chunks);
+      if(r.each == 1) normQuantKernel<T, ACT, 1><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+      else if(r.each == 2) normQuantKernel<T, ACT, 2><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+      else if(r.each == 3) normQuantKernel<T, ACT, 3><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+      else normQuantKernel<T, ACT, 4><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+    }
+  }
+  KGH_CHECK_LAUNCH();
 }
 
 }  // namespace
@@ -253,69 +641,20 @@ void checkGroupNorm(const kgh_group_norm_params& p, bool pointers) {
   opCheckWorkspace(op, p.workspace, p.workspace_bytes, groupNormWorkspace(p));
 }
 
-uint64_t groupNormWorkspace(const kgh_group_norm_params& p) { return (uint64_t)p.batch * p.groups * 8; }
+uint64_t groupNormWorkspace(const kgh_group_norm_params& p) {
+  if(p.batch == 0 || p.positions == 0) return 0;
+  const NormPlan plan = planNorm(p);
+  return plan.partsBytes + plan.statsBytes;
+}
 
 void launchGroupNorm(const kgh_group_norm_params& p, hipStream_t stream) {
   if(p.batch == 0 || p.positions == 0) return;
+  const NormPlan plan = planNorm(p);
   const NormArgs a = normArgs(p, p.eps);
-  float* stats = p.statistics != nullptr ? p.statistics : (float*)p.workspace;
+  const NormOut o{p.out, p.out_batch_stride, p.out_position_stride, p.out_scales, p.statistics};
   withDtype(p.dtype, [&](auto t) {
-    typedef decltype(t) T;
-    normStatsKernel<T><<<dim3((unsigned)std::min<int64_t>((int64_t)p.groups * p.batch, 1 << 20)), 256, 0, stream>>>(a, stats);
-    KGH_CHECK_LAUNCH();
-    withActivation(p.activation, [&](auto act) {
-      normApplyKernel<T, decltype(act)::value><<<dim3((unsigned)std::min<int64_t>(p.batch * p.positions, 1 << 20)), 256, 0, stream>>>(a, stats, p.out, p.out_batch_stride,
-                                                                                                             p.out_position_stride, p.out_scales);
-    });
-    KGH_CHECK_LAUNCH();
+    withActivation(p.activation, [&](auto act) { launchNorm<decltype(t), decltype(act)::value>(plan, a, o, p.workspace, stream); });
   });
-}
-
-void checkGroupNormBackward(const kgh_group_norm_backward_params& p, bool pointers) {
-  const char* op = "kgh_group_norm_backward";
-  checkNormSizes(op, p);
-  if(!pointers) return;
-  for(int64_t s : {p.x_batch_stride, p.x_position_stride, p.mask_stride, p.grad_out_batch_stride, p.grad_out_position_stride, p.grad_x_batch_stride,
-                   p.grad_x_position_stride})
-    if(s < 0) opInvalid(op, "negative stride");
-  if(p.grad_weight != nullptr) opCheckPointer(op, "grad_weight", p.grad_weight, 4);
-  if(p.grad_bias != nullptr) opCheckPointer(op, "grad_bias", p.grad_bias, 4);
-  if(p.grad_weight != nullptr && p.grad_weight == p.grad_bias) opInvalid(op, "grad_weight is grad_bias itself");
-  if(p.batch == 0 || p.positions == 0) return;
-  checkApartRows(op, "grad_x", p.grad_x_batch_stride, p.grad_x_position_stride, p.batch, p.positions, p.channels);
-  const size_t e = opElemBytes(p.dtype);
-  opCheckPointer(op, "x", p.x, e);
-  opCheckPointer(op, "grad_out", p.grad_out, e);
-  opCheckPointer(op, "grad_x", p.grad_x, e);
-  opCheckPointer(op, "statistics", p.statistics, 4);
-  if(p.weight != nullptr) opCheckPointer(op, "weight", p.weight, 4);
-  if(p.bias != nullptr) opCheckPointer(op, "bias", p.bias, 4);
-  if(p.lengths != nullptr) opCheckPointer(op, "lengths", p.lengths, 4);
-  if(p.x == p.grad_x) opInvalid(op, "grad_x is x itself");
-  if(p.grad_out == p.grad_x) opInvalid(op, "grad_x is grad_out itself");
-  opCheckWorkspace(op, p.workspace, p.workspace_bytes, groupNormBackwardWorkspace(p));
-}
-
-uint64_t groupNormBackwardWorkspace(const kgh_group_norm_backward_params& p) { return (uint64_t)p.batch * p.channels * 8; }
-
-void launchGroupNormBackward(const kgh_group_norm_backward_params& p, hipStream_t stream) {
-  NormArgs a = normArgs(p, 0.0f);
-  if(p.positions == 0) a.batch = 0;
-  const NormBackArgs k{p.grad_out, p.grad_out_batch_stride, p.grad_out_position_stride, p.statistics, p.grad_x, p.grad_x_batch_stride,
-                       p.grad_x_position_stride, p.grad_weight, p.grad_bias, (float*)p.workspace};
-  if(p.batch > 0 && p.positions > 0)
-    withDtype(p.dtype, [&](auto t) {
-      typedef decltype(t) T;
-      withActivation(p.activation, [&](auto act) {
-        normBackSumsKernel<T, decltype(act)::value><<<dim3((unsigned)std::min<int64_t>((int64_t)p.channels * p.batch, 1 << 20)), 256, 0, stream>>>(a, k);
-        KGH_CHECK_LAUNCH();
-        normBackApplyKernel<T, decltype(act)::value><<<dim3((unsigned)std::min<int64_t>((int64_t)p.groups * p.batch, 1 << 20)), 256, 0, stream>>>(a, k);
-        KGH_CHECK_LAUNCH();
-      });
-    });
-  if(p.grad_weight == nullptr && p.grad_bias == nullptr) return;
-  normBackJoinKernel<<<dim3((unsigned)((p.channels + 255) / 256)), 256, 0, stream>>>(a, k);
-  KGH_CHECK_LAUNCH();
 }
 
 }  // namespace kgh

@@ -1,0 +1,500 @@
+// The gradient of group norm with an activation (kgh_group_norm_backward).
+#include "kgh_op_norm_device.h"
+
+namespace {
+
+// The activations' slopes. In 16 bits by the hardware's exponential and reciprocal, to
+// within 2^-18 of 1; in fp32 by the accurate functions, to within 2^-20.
+//   silu: s (1 + v (1 - s)), s = 1 / (1 + e^-v);
+//   mish: with n = e^v (e^v + 2): n w + 4 v e^v (1 + e^v) w^2, w = 1 / (n + 2);
+//   gelu: Phi(v) + v phi(v).
+template<typename T, int ACT>
+__device__ __forceinline__ float slope(float v) {
+  if constexpr(ACT == KGH_ACT_IDENTITY) return 1.0f;
+  else if constexpr(ACT == KGH_ACT_RELU) return v > 0.0f ? 1.0f : v != v ? v : 0.0f;
+  else if constexpr(ACT == KGH_ACT_SILU) {
+    float s;
+    if constexpr(sizeof(T) == 4) s = 1.0f / (1.0f + expf(-v));
+    else s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -ACT_LOG2E));
+    return s * fmaf(v, 1.0f - s, 1.0f);
+  }
+  else if constexpr(ACT == KGH_ACT_MISH) {
+    const float c = v > 20.0f ? 20.0f : v;  // NaN stays NaN
+    float e, w;
+    if constexpr(sizeof(T) == 4) e = expf(c);
+    else e = __builtin_amdgcn_exp2f(c * ACT_LOG2E);
+    const float n = fmaf(e, e, 2.0f * e);
+    if constexpr(sizeof(T) == 4) w = 1.0f / (n + 2.0f);
+    else w = __builtin_amdgcn_rcpf(n + 2.0f);
+    return w * fmaf(4.0f * c * fmaf(e, e, e), w, n);
+  }
+  else if constexpr(sizeof(T) == 4) return fmaf(0.5f, erfcf(-0.70710678118654752f * v), v * expf(-0.5f * v * v) * 0.39894228040143268f);
+  else {
+    // erfc(|v| / sqrt(2)) / 2 as in activateFast, which gives e^(-v^2 / 2) too.
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.435f * 0.70710678118654752f, fabsf(v), 1.0f));
+    float poly = fmaf(t, 0.5f * -0.15086693f, 0.5f * 0.38131212f);
+    poly = fmaf(t, poly, 0.5f * 0.01284851f);
+    poly = fmaf(t, poly, 0.5f * 0.27344433f);
+    poly = fmaf(t, poly, 0.5f * 0.23733569f);
+    poly = fmaf(t, poly, 0.5f * 0.24592536f);
+    const float e = __builtin_amdgcn_exp2f(v * v * (-0.5f * ACT_LOG2E));
+    const float q = t * poly * e;
+    return fmaf(v, e * 0.39894228040143268f, v < 0.0f ? q : 1.0f - q);
+  }
+}
+
+struct NormBackArgs {
+  const void* grad;
+  int64_t gB, gP;
+  const float* stats;
+  void* out;
+  int64_t oB, oP;
+  float* gradWeight;
+  float* gradBias;
+  float2* sums;  // [batch][channels]: of u and u h over an item's positions
+};
+
+// u (the gradient behind the activation) and h (the normalised input) of VEC channels.
+template<typename T, int ACT, int VEC>
+__device__ __forceinline__ void backward(float (&u)[VEC], float (&h)[VEC], const Values<T>& x, const Values<T>& grad, const float (&mean)[VEC],
+                                         const float (&rstd)[VEC], const float (&weight)[VEC], const float (&bias)[VEC]) {
+#pragma unroll
+  for(int j = 0; j < VEC; j++) {
+    h[j] = (x.f[j] - mean[j]) * rstd[j];
+    u[j] = grad.f[j] * slope<T, ACT>(fmaf(h[j], weight[j], bias[j]));
+  }
+}
+
+// The gradient by the group's means a.x of u weight and a.y of u weight h.
+__device__ __forceinline__ float backwardX(float u, float h, float weight, float rstd, float2 a) { return rstd * (fmaf(u, weight, -a.x) - h * a.y); }
+
+// A thread's channels' constants.
+template<int VEC>
+struct BackChannels {
+  float weight[VEC], bias[VEC], mean[VEC], rstd[VEC];
+  __device__ __forceinline__ BackChannels(const NormArgs& a, const float* stats, int b, int c0, int nc) {
+    loadFloats(weight, a.weight == nullptr ? nullptr : a.weight + c0, nc, 1.0f);
+    loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + c0, nc, 0.0f);
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      const float* t = stats + 2 * ((int64_t)b * a.groups + min(c0 + j, a.channels - 1) / a.per);
+      mean[j] = t[0];
+      rstd[j] = t[1];
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// An item's run of channels in a unit's registers, as in the forward pass: x as it came
+// and u in fp32 (its slope is most of the work, and is computed once).
+template<typename T, int ACT, int NV>
+__global__ __launch_bounds__(512) void normBackSlabKernel(NormArgs a, NormBackArgs k, NormSlab s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ float2 lds[];
+  __shared__ int counts[4];
+  const int unit = s.units == 1 ? 0 : threadIdx.x >> 6;
+  const int tt = threadIdx.x - unit * s.threads;
+  const int row = tt / s.cols, col = tt - row * s.cols;
+  const int inRun = s.run / a.per;
+  float2* part = lds + unit * s.ldsPairs;
+  float2* means = part + s.ldsPairs - inRun;
+  const int64_t id = s.first + (int64_t)xcdContiguousTile() * s.units + unit;
+  const bool live = id < s.count;
+  const int64_t mine = live ? id : s.count - 1;
+  const int b = (int)(mine / s.runs), r = (int)(mine - (int64_t)b * s.runs);
+  const int c1 = r * s.run, c0 = c1 + col * VEC;
+  const bool on = row < s.rowLanes && c0 < min(c1 + s.run, a.channels);
+  const Window<VEC> win(c0, a.channels);
+  const int groups = min(inRun, a.groups - r * inRun);
+  const int len = validLength(a, b);
+  const T* x = (const T*)a.x + b * a.xB + win.at;
+  const T* grad = (const T*)k.grad + b * k.gB + win.at;
+  unsigned bits = 0;
+  if(a.mask == nullptr) {
+#pragma unroll
+    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len ? 1u << i : 0u;
+  }
+  else {
+    if(tt == 0) counts[unit] = 0;
+    const uint8_t* mask = a.mask + b * a.maskB;
+    uint8_t m[NV];
+#pragma unroll
+    for(int i = 0; i < NV; i++) m[i] = mask[min(row + i * s.rowLanes, a.positions - 1)];
+#pragma unroll
+    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len && m[i] != 0 ? 1u << i : 0u;
+  }
+  u32x4_t v[NV], d[NV];
+#pragma unroll
+  for(int i = 0; i < NV; i++)
+    if(i < s.nv) {
+      const int64_t p = (bits >> i) & 1 ? row + i * s.rowLanes : 0;
+      __builtin_memcpy(&v[i], x + p * a.xP, 16);
+      __builtin_memcpy(&d[i], grad + p * k.gP, 16);
+    }
+  const BackChannels<VEC> ch(a, k.stats, b, win.at, VEC);
+  if(a.mask != nullptr) {
+    __syncthreads();
+    if(col == 0 && bits != 0) atomicAdd(&counts[unit], __popc(bits));
+  }
+  float u[NV][VEC], s0[VEC], s1[VEC];
+#pragma unroll
+  for(int j = 0; j < VEC; j++) s0[j] = s1[j] = 0.0f;
+#pragma unroll
+  for(int i = 0; i < NV; i++)
+    if(i < s.nv) {
+      float h[VEC];
+      backward<T, ACT>(u[i], h, Values<T>(v[i]), Values<T>(d[i]), ch.mean, ch.rstd, ch.weight, ch.bias);
+      if((bits >> i) & 1) {
+#pragma unroll
+        for(int j = 0; j < VEC; j++) {
+          s0[j] += u[i][j];
+          s1[j] = fmaf(u[i][j], h[j], s1[j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  if(on) {
+    float2* p = part + row * s.entries + col * VEC;
+#pragma unroll
+    for(int j = 0; j < VEC; j++)
+      if(j >= win.skip) p[j - win.skip] = make_float2(s0[j], s1[j]);
+  }
+  __syncthreads();
+  const float2* red = addRows(part, s, tt);
+  if(s.rowLanes > 1) __syncthreads();
+  // Channels' sums for the weight's and bias's gradients.
+  if(live)
+    for(int e = tt; e < min(s.run, a.channels - c1); e += s.threads) {
+      float2 t = red[e];
+      for(int q = 1; q < s.segments; q++) {
+        t.x += red[q * s.entries + e].x;
+        t.y += red[q * s.entries + e].y;
+      }
+      k.sums[(int64_t)b * a.channels + c1 + e] = t;
+    }
+  const int sub = tt & (s.lanes - 1);
+  const float n = (float)(a.mask != nullptr ? counts[unit] : len) * (float)a.per;
+  for(int q = tt / s.lanes; q < groups; q += s.threads / s.lanes) {
+    float m1 = 0.0f, m2 = 0.0f;
+    for(int i = sub; i < a.per * s.segments; i += s.lanes) {
+      const int seg = i / a.per, e = q * a.per + (i - seg * a.per);
+      const float2 t = red[seg * s.entries + e];
+      const float w = a.weight == nullptr ? 1.0f : a.weight[c1 + e];
+      m1 = fmaf(t.x, w, m1);
+      m2 = fmaf(t.y, w, m2);
+    }
+    for(int w = s.lanes >> 1; w > 0; w >>= 1) {
+      m1 += __shfl_xor(m1, w);
+      m2 += __shfl_xor(m2, w);
+    }
+    if(sub == 0) means[q] = make_float2(m1 / n, m2 / n);
+  }
+  __syncthreads();
+  float2 mean2[VEC];
+#pragma unroll
+  for(int j = 0; j < VEC; j++) mean2[j] = means[min(max(win.at + j - c1, 0) / a.per, groups - 1)];
+  T* out = (T*)k.out + b * k.oB + win.at;
+#pragma unroll
+  for(int i = 0; i < NV; i++)
+    if(i < s.nv) {
+      const int p = row + i * s.rowLanes;
+      renew(v[i]);
+      const Values<T> xv(v[i]);
+      float y[VEC];
+#pragma unroll
+      for(int j = 0; j < VEC; j++) y[j] = backwardX(u[i][j], (xv.f[j] - ch.mean[j]) * ch.rstd[j], ch.weight[j], ch.rstd[j], mean2[j]);
+      const uint4 o = packed<T>(y), zero = make_uint4(0, 0, 0, 0);
+      if(on && live && p < a.positions) storeWindow(out + p * k.oP, (bits >> i) & 1 ? o : zero, win.skip);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Items that do not fit: chunks of positions and blocks of columns, each a workgroup.
+// parts[item][chunk][channel]: sums of u and u h. counts[item][chunk]: positions that
+// take part.
+struct BackParts {
+  float2* parts;
+  int* counts;
+  float2* means;  // [item][group]
+  int chunks, chunkRows, blocks, cols, rowLanes, segments;
+};
+
+constexpr int BACK_AHEAD = 2;  // rows of a thread under way
+
+template<typename T, int ACT, bool APPLY>
+__global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackArgs k, BackParts s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  __shared__ float2 part[APPLY ? 1 : 256 * VEC];
+  __shared__ int counted;
+  const int row = threadIdx.x / s.cols, col = threadIdx.x - row * s.cols;
+  const int64_t all = (int64_t)a.batch * s.chunks * s.blocks;
+  for(int64_t id = blockIdx.x; id < all; id += gridDim.x) {
+    const int64_t itemChunk = id / s.blocks;
+    const int block = (int)(id - itemChunk * s.blocks);
+    const int b = (int)(itemChunk / s.chunks), chunk = (int)(itemChunk - (int64_t)b * s.chunks);
+    const int from = block * s.cols * VEC;
+    const int c0 = from + col * VEC, nc = min(a.channels - c0, VEC);
+    const bool on = row < s.rowLanes && nc > 0;
+    const int len = validLength(a, b);
+    const int p0 = chunk * s.chunkRows, p1 = min(p0 + s.chunkRows, a.positions);
+    const RowGroup<T, false> g((on ? c0 : 0) / VEC, a.channels);
+    const T* x = (const T*)a.x + b * a.xB;
+    const T* grad = (const T*)k.grad + b * k.gB;
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.maskB;
+    const BackChannels<VEC> ch(a, k.stats, b, min(c0, a.channels - 1), nc);
+    float s0[VEC], s1[VEC];
+    float2 mean2[VEC];
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      s0[j] = s1[j] = 0.0f;
+      mean2[j] = APPLY ? s.means[(int64_t)b * a.groups + min(c0 + j, a.channels - 1) / a.per] : make_float2(0.0f, 0.0f);
+    }
+    if(!APPLY) {
+      if(threadIdx.x == 0) counted = 0;
+      __syncthreads();
+    }
+    int rows = 0;
+    if(on) {
+      for(int p = p0 + row; p < p1; p += BACK_AHEAD * s.rowLanes) {
+        u32x4_t v[BACK_AHEAD], d[BACK_AHEAD];
+        bool take[BACK_AHEAD];
+#pragma unroll
+        for(int i = 0; i < BACK_AHEAD; i++) {
+          const int q = p + i * s.rowLanes;
+          take[i] = q < p1 && q < len && (mask == nullptr || mask[q] != 0);
+        }
+#pragma unroll
+        for(int i = 0; i < BACK_AHEAD; i++) {
+          const int64_t q = take[i] ? p + i * s.rowLanes : 0;
+          v[i] = g.load(x + q * a.xP);
+          d[i] = g.load(grad + q * k.gP);
+        }
+#pragma unroll
+        for(int i = 0; i < BACK_AHEAD; i++) {
+          float u[VEC], h[VEC];
+          backward<T, ACT>(u, h, Values<T>(g.place(v[i])), Values<T>(g.place(d[i])), ch.mean, ch.rstd, ch.weight, ch.bias);
+          if constexpr(APPLY) {
+            const int q = p + i * s.rowLanes;
+            float y[VEC];
+#pragma unroll
+            for(int j = 0; j < VEC; j++) y[j] = backwardX(u[j], h[j], ch.weight[j], ch.rstd[j], mean2[j]);
+            const uint4 o = packed<T>(y), zero = make_uint4(0, 0, 0, 0);
+            if(q < p1) storeGroup((T*)k.out + b * k.oB + q * k.oP + c0, take[i] ? o : zero, nc);
+          }
+          else if(take[i]) {
+            rows++;
+#pragma unroll
+            for(int j = 0; j < VEC; j++) {
+              s0[j] += u[j];
+              s1[j] = fmaf(u[j], h[j], s1[j]);
+            }
+          }
+        }
+      }
+    }
+    if constexpr(!APPLY) {
+      if(col == 0 && rows > 0) atomicAdd(&counted, rows);
+      if(row < s.rowLanes) {
+#pragma unroll
+        for(int j = 0; j < VEC; j++) part[(row * s.cols + col) * VEC + j] = make_float2(s0[j], s1[j]);
+      }
+      __syncthreads();
+      const int width = s.cols * VEC;
+      for(int e = threadIdx.x; e < min(width, a.channels - from); e += 256) {
+        float2 t = make_float2(0.0f, 0.0f);
+        for(int q = 0; q < s.rowLanes; q++) {
+          t.x += part[q * width + e].x;
+          t.y += part[q * width + e].y;
+        }
+        s.parts[itemChunk * a.channels + from + e] = t;
+      }
+      if(threadIdx.x == 0 && block == 0) s.counts[itemChunk] = counted;
+      __syncthreads();
+    }
+  }
+}
+
+// The chunks' sums of an item's group: its channels' sums and its means. Threads are
+// (chunk slice, channel); channels of long groups in turns.
+__global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackArgs k, BackParts s) {
+  __shared__ float2 part[256];
+  __shared__ float2 total[4];
+  __shared__ int counted;
+  const int width = min(a.per, 64), slices = 256 / width;
+  const int slice = threadIdx.x / width, c = threadIdx.x - slice * width;
+  for(int64_t i = blockIdx.x; i < (int64_t)a.batch * a.groups; i += gridDim.x) {
+    const int b = (int)(i / a.groups), g = (int)(i - (int64_t)b * a.groups);
+    if(threadIdx.x == 0) counted = 0;
+    __syncthreads();
+    int rows = 0;
+    for(int q = threadIdx.x; q < s.chunks; q += 256) rows += s.counts[(int64_t)b * s.chunks + q];
+    if(rows > 0) atomicAdd(&counted, rows);
+    float m1 = 0.0f, m2 = 0.0f;
+    for(int from = 0; from < a.per; from += width) {
+      const bool on = slice < slices && from + c < a.per;
+      const int ch = g * a.per + from + c;
+      float2 t = make_float2(0.0f, 0.0f);
+      if(on)
+#pragma unroll 4
+        for(int q = slice; q < s.chunks; q += slices) {
+          const float2 v = s.parts[((int64_t)b * s.chunks + q) * a.channels + ch];
+          t.x += v.x;
+          t.y += v.y;
+        }
+      part[threadIdx.x] = t;
+      __syncthreads();
+      if(slice == 0 && on) {
+        for(int q = 1; q < slices; q++) {
+          t.x += part[q * width + c].x;
+          t.y += part[q * width + c].y;
+        }
+        k.sums[(int64_t)b * a.channels + ch] = t;
+        const float w = a.weight == nullptr ? 1.0f : a.weight[ch];
+        m1 = fmaf(t.x, w, m1);
+        m2 = fmaf(t.y, w, m2);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for(int w = 32; w > 0; w >>= 1) {
+      m1 += __shfl_xor(m1, w);
+      m2 += __shfl_xor(m2, w);
+    }
+    if((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = make_float2(m1, m2);
+    __syncthreads();
+    if(threadIdx.x == 0) {
+      const float n = (float)counted * (float)a.per;
+      s.means[i] = make_float2(((total[0].x + total[1].x) + (total[2].x + total[3].x)) / n, ((total[0].y + total[1].y) + (total[2].y + total[3].y)) / n);
+    }
+    __syncthreads();
+  }
+}
+
+// The items' sums: the gradients of weight and bias. 32 channels a workgroup.
+__global__ __launch_bounds__(256) void normBackWeightsKernel(NormArgs a, NormBackArgs k) {
+  __shared__ float2 part[256];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  float2 t = make_float2(0.0f, 0.0f);
+  if(c < a.channels)
+#pragma unroll 8
+    for(int b = slice; b < a.batch; b += 8) {
+      const float2 v = k.sums[(int64_t)b * a.channels + c];
+      t.x += v.x;
+      t.y += v.y;
+    }
+  part[threadIdx.x] = t;
+  __syncthreads();
+  if(slice != 0 || c >= a.channels) return;
+#pragma unroll
+  for(int q = 1; q < 8; q++) {
+    t.x += part[q * 32 + threadIdx.x].x;
+    t.y += part[q * 32 + threadIdx.x].y;
+  }
+  if(k.gradBias != nullptr) k.gradBias[c] = t.x;
+  if(k.gradWeight != nullptr) k.gradWeight[c] = t.y;
+}
+
+struct NormBackPlan {
+  NormSlab slab;  // threads 0: parts
+  BackParts parts;
+  uint64_t sumsBytes, partsBytes, countsBytes, meansBytes;
+};
+
+NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
+  const int size = (int)kgh::opElemBytes(p.dtype), vec = 16 / size;
+  const auto round16 = [](uint64_t n) { return (n + 15) / 16 * 16; };
+  NormBackPlan plan{};
+  plan.sumsBytes = round16((uint64_t)p.batch * p.channels * 8);
+  plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 96, true, 8, 512, false, 1);
+  if(plan.slab.threads != 0) return plan;
+  BackParts& s = plan.parts;
+  const int cols = (p.channels + vec - 1) / vec;
+  s.cols = std::min(cols, 256);
+  s.blocks = (cols + s.cols - 1) / s.cols;
+  s.rowLanes = std::min(256 / s.cols, p.positions);
+  const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(64, (int64_t)p.batch * p.positions * s.blocks / s.rowLanes / 1024));
+  s.chunkRows = (int)std::min<int64_t>(p.positions, (rows + BACK_AHEAD - 1) / BACK_AHEAD * BACK_AHEAD * s.rowLanes);
+  s.chunks = (p.positions + s.chunkRows - 1) / s.chunkRows;
+  plan.partsBytes = round16((uint64_t)p.batch * s.chunks * p.channels * 8);
+  plan.countsBytes = round16((uint64_t)p.batch * s.chunks * 4);
+  plan.meansBytes = round16((uint64_t)p.batch * p.groups * 8);
+  return plan;
+}
+
+template<typename T, int ACT>
+void launchBackward(const NormBackPlan& plan, const NormArgs& a, const NormBackArgs& k, hipStream_t stream) {
+  if(plan.slab.threads != 0) {
+    forUnits(plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
+      if(s.nv <= 2) normBackSlabKernel<T, ACT, 2><<<grid, threads, bytes, stream>>>(a, k, s);
+      else normBackSlabKernel<T, ACT, 8><<<grid, threads, bytes, stream>>>(a, k, s);
+      KGH_CHECK_LAUNCH();
+    });
+    return;
+  }
+  BackParts parts = plan.parts;
+  char* at = (char*)k.sums + plan.sumsBytes;
+  parts.parts = (float2*)at;
+  parts.counts = (int*)(at + plan.partsBytes);
+  parts.means = (float2*)(at + plan.partsBytes + plan.countsBytes);
+  const unsigned grid = normGrid((int64_t)a.batch * parts.chunks * parts.blocks);
+  normBackPartsKernel<T, ACT, false><<<grid, 256, 0, stream>>>(a, k, parts);
+  KGH_CHECK_LAUNCH();
+  normBackJoinKernel<<<normGrid((int64_t)a.batch * a.groups), 256, 0, stream>>>(a, k, parts);
+  KGH_CHECK_LAUNCH();
+  normBackPartsKernel<T, ACT, true><<<grid, 256, 0, stream>>>(a, k, parts);
+  KGH_CHECK_LAUNCH();
+}
+
+}  // namespace
+
+namespace kgh {
+
+void checkGroupNormBackward(const kgh_group_norm_backward_params& p, bool pointers) {
+  const char* op = "kgh_group_norm_backward";
+  checkNormSizes(op, p);
+  if(!pointers) return;
+  for(int64_t s : {p.x_batch_stride, p.x_position_stride, p.mask_stride, p.grad_out_batch_stride, p.grad_out_position_stride, p.grad_x_batch_stride,
+                   p.grad_x_position_stride})
+    if(s < 0) opInvalid(op, "negative stride");
+  if(p.grad_weight != nullptr) opCheckPointer(op, "grad_weight", p.grad_weight, 4);
+  if(p.grad_bias != nullptr) opCheckPointer(op, "grad_bias", p.grad_bias, 4);
+  if(p.grad_weight != nullptr && p.grad_weight == p.grad_bias) opInvalid(op, "grad_weight is grad_bias itself");
+  if(p.batch == 0 || p.positions == 0) return;
+  checkApartRows(op, "grad_x", p.grad_x_batch_stride, p.grad_x_position_stride, p.batch, p.positions, p.channels);
+  const size_t e = opElemBytes(p.dtype);
+  opCheckPointer(op, "x", p.x, e);
+  opCheckPointer(op, "grad_out", p.grad_out, e);
+  opCheckPointer(op, "grad_x", p.grad_x, e);
+  opCheckPointer(op, "statistics", p.statistics, 4);
+  if(p.weight != nullptr) opCheckPointer(op, "weight", p.weight, 4);
+  if(p.bias != nullptr) opCheckPointer(op, "bias", p.bias, 4);
+  if(p.lengths != nullptr) opCheckPointer(op, "lengths", p.lengths, 4);
+  if(p.x == p.grad_x) opInvalid(op, "grad_x is x itself");
+  if(p.grad_out == p.grad_x) opInvalid(op, "grad_x is grad_out itself");
+  opCheckWorkspace(op, p.workspace, p.workspace_bytes, groupNormBackwardWorkspace(p));
+}
+
+uint64_t groupNormBackwardWorkspace(const kgh_group_norm_backward_params& p) {
+  if(p.batch == 0 || p.positions == 0) return 0;
+  const NormBackPlan plan = planBackward(p);
+  return plan.sumsBytes + plan.partsBytes + plan.countsBytes + plan.meansBytes;
+}
+
+void launchGroupNormBackward(const kgh_group_norm_backward_params& p, hipStream_t stream) {
+  NormArgs a = normArgs(p, 0.0f);
+  const NormBackArgs k{p.grad_out, p.grad_out_batch_stride, p.grad_out_position_stride, p.statistics, p.grad_x, p.grad_x_batch_stride,
+                       p.grad_x_position_stride, p.grad_weight, p.grad_bias, (float2*)p.workspace};
+  if(p.batch > 0 && p.positions > 0) {
+    const NormBackPlan plan = planBackward(p);
+    withDtype(p.dtype, [&](auto t) {
+      withActivation(p.activation, [&](auto act) { launchBackward<decltype(t), decltype(act)::value>(plan, a, k, stream); });
+    });
+  }
+  else a.batch = 0;  // no sums: the gradients of weight and bias are zeros
+  if(p.grad_weight == nullptr && p.grad_bias == nullptr) return;
+  normBackWeightsKernel<<<dim3((unsigned)((p.channels + 31) / 32)), 256, 0, stream>>>(a, k);
+  KGH_CHECK_LAUNCH();
+}
+
+}  // namespace kgh

@@ -1,0 +1,184 @@
+// What group norm and its gradient share: arguments, layouts of threads, sums.
+#ifndef KGH_OP_NORM_DEVICE_H
+#define KGH_OP_NORM_DEVICE_H
+
+#include "kgh_op_quantize_device.h"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int NORM_MAX_LEN = 1 << 30, NORM_MAX_CHANNELS = 1 << 20;
+constexpr int NORM_MAX_GRID = 1 << 20;  // workgroups of a launch
+
+// What both directions read. Strides count elements.
+struct NormArgs {
+  const void* x;
+  const float* weight;
+  const float* bias;
+  const int32_t* lengths;
+  const uint8_t* mask;
+  int64_t xB, xP, maskB;
+  int batch, positions, channels, groups, per;  // per: channels of a group
+  float eps;
+};
+
+__device__ __forceinline__ int validLength(const NormArgs& a, int b) {
+  return a.lengths == nullptr ? a.positions : min(max(a.lengths[b], 0), a.positions);
+}
+
+// A unit's threads: an item's run of `run` channels (whole groups), `cols` 16-byte
+// columns of it side by side in `rowLanes` rows of threads; a thread has positions row,
+// row + rowLanes, ..., `nv` of them. `units` units share a workgroup.
+// Sums go through LDS as pairs: `pv` a column (one where a group is whole columns, else
+// one a channel), `entries` = cols pv a row; `segments` runs of rows are added first,
+// then a group's entries by `lanes` threads.
+struct NormSlab {
+  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, segments, lanes;
+  int64_t count, first;  // units in all, and the first one of this launch
+  int ldsPairs;   // a unit's LDS, in pairs of floats: sums, then groups' state
+};
+
+// 16 bytes that the compiler is to take for new ones: it would otherwise keep the floats
+// of a unit's registers from one use to the next, twice as many registers.
+__device__ __forceinline__ void renew(u32x4_t& v) { asm volatile("" : "+v"(v)); }
+
+template<typename T>
+__device__ __forceinline__ uint4 packed(const float (&y)[16 / sizeof(T)]) {
+  T e[16 / sizeof(T)];
+#pragma unroll
+  for(int j = 0; j < 16 / (int)sizeof(T); j++) e[j] = (T)y[j];
+  uint4 u;
+  __builtin_memcpy(&u, e, 16);
+  return u;
+}
+
+// A thread's 16 bytes of a row of `channels` (at least VEC): those of channels c0..
+// where they end in the row, else the row's last ones, the first `skip` of which are
+// another thread's.
+template<int VEC>
+struct Window {
+  int at, skip;
+  __device__ __forceinline__ Window(int c0, int channels) {
+    at = max(0, min(c0, channels - VEC));
+    skip = min(c0 - at, VEC);
+  }
+};
+// The window's own elements to p, the address of its first one.
+template<typename T>
+__device__ __forceinline__ void storeWindow(T* p, uint4 v, int skip) {
+  if(skip == 0) __builtin_memcpy(p, &v, 16);
+  else {
+#pragma unroll 1
+    for(int j = 0; j < 16 / (int)sizeof(T); j++) {
+      T e;
+      __builtin_memcpy(&e, &v.x, sizeof(T));
+      if(j >= skip) p[j] = e;
+      v = shiftDown<T>(v);
+    }
+  }
+}
+
+// n of the VEC floats from p on, `other` where p is null or behind them.
+template<int VEC>
+__device__ __forceinline__ void loadFloats(float (&f)[VEC], const float* p, int n, float other) {
+  if(p != nullptr && n >= VEC) __builtin_memcpy(f, p, sizeof(f));
+  else {
+#pragma unroll
+    for(int j = 0; j < VEC; j++) f[j] = p != nullptr && j < n ? p[j] : other;
+  }
+}
+
+// A unit's pairs of sums [rowLanes][entries], added over the rows in `segments` runs:
+// [segments][entries] behind them (the rows themselves where there is one).
+__device__ __forceinline__ const float2* addRows(float2* part, const NormSlab& s, int tt) {
+  if(s.rowLanes == 1) return part;
+  float2* red = part + s.rowLanes * s.entries;
+  for(int i = tt; i < s.entries * s.segments; i += s.threads) {
+    const int seg = i / s.entries, e = i - seg * s.entries;
+    float2 v = make_float2(0.0f, 0.0f);
+    for(int r = seg; r < s.rowLanes; r += s.segments) {
+      const float2 u = part[r * s.entries + e];
+      v.x += u.x;
+      v.y += u.y;
+    }
+    red[i] = v;
+  }
+  return red;
+}
+
+// Rows (item, position) of a tensor that is written lie apart.
+inline void checkApartRows(const char* op, const char* name, int64_t batchStride, int64_t positionStride, int batch, int positions, int channels) {
+  const bool positionsInside = (positions == 1 || positionStride >= channels) && (batch == 1 || batchStride >= (positions - 1) * positionStride + channels);
+  const bool itemsInside = (batch == 1 || batchStride >= channels) && (positions == 1 || positionStride >= (batch - 1) * batchStride + channels);
+  if(!positionsInside && !itemsInside) kgh::opInvalid(op, std::string("the strides of ") + name + " make its rows overlap");
+}
+
+template<typename P>
+void checkNormSizes(const char* op, const P& p) {
+  kgh::opCheckDtype(op, p.dtype);
+  kgh::opCheckActivation(op, p.activation);
+  if(p.batch < 0 || p.positions < 0 || (int64_t)p.batch * p.positions > NORM_MAX_LEN)
+    kgh::opInvalid(op, "batch and positions must be 0 or more, their product at most " + std::to_string(NORM_MAX_LEN));
+  if(p.channels < 1 || p.channels > NORM_MAX_CHANNELS) kgh::opInvalid(op, "channels must be in 1.." + std::to_string(NORM_MAX_CHANNELS));
+  if(p.groups < 1 || p.channels % p.groups != 0) kgh::opInvalid(op, "groups must divide channels");
+}
+
+template<typename P>
+NormArgs normArgs(const P& p, float eps) {
+  return NormArgs{p.x, p.weight, p.bias, p.lengths, p.mask, p.x_batch_stride, p.x_position_stride, p.mask_stride,
+                  p.batch, p.positions, p.channels, p.groups, p.channels / p.groups, eps};
+}
+
+inline unsigned normGrid(int64_t blocks) { return (unsigned)std::min<int64_t>(blocks, NORM_MAX_GRID); }
+
+// Launches f(slab, grid, threads, bytes of LDS) for all units.
+template<typename F>
+void forUnits(NormSlab s, F&& f) {
+  for(s.first = 0; s.first < s.count; s.first += (int64_t)NORM_MAX_GRID * s.units)
+    f(s, normGrid((s.count - s.first + s.units - 1) / s.units), (unsigned)(s.threads * s.units), (size_t)s.ldsPairs * 8 * s.units);
+}
+
+// The layout of a unit's threads: at most `most` positions a thread and `wide` threads;
+// threads is 0 where there is none. Runs of at least `bytes` a row, or (wholeRows) of all
+// channels. perChannel: sums of each channel are wanted. What a group has in LDS beside
+// the sums: `state` pairs.
+inline NormSlab planSlab(int64_t batch, int positions, int channels, int groups, int size, int bytes, bool perChannel, int most, int wide, bool wholeRows,
+                         int state) {
+  const int vec = 16 / size, per = channels / groups;
+  NormSlab none{};
+  if(channels < vec) return none;
+  int64_t base = per;
+  while(base % vec != 0) base += per;
+  int64_t run = wholeRows ? channels : (bytes + base * size - 1) / (base * size) * base;
+  if(run > channels) run = channels;
+  for(int nv : {std::min(most, 8), most})
+    for(int threads = 64; threads <= wide; threads += 64) {
+      NormSlab s{};
+      s.run = (int)run;
+      s.runs = (int)((channels + run - 1) / run);
+      s.cols = (int)((run + vec - 1) / vec);
+      s.threads = threads;
+      s.units = threads == 64 ? 4 : 1;
+      s.count = batch * s.runs;
+      if(s.cols > threads) continue;
+      s.rowLanes = std::min(threads / s.cols, positions);
+      s.nv = (positions + s.rowLanes - 1) / s.rowLanes;
+      if(s.nv > nv) continue;
+      s.pv = !perChannel && per % vec == 0 ? 1 : vec;
+      s.entries = s.cols * s.pv;
+      s.segments = s.rowLanes == 1 ? 1 : std::max(1, std::min(s.rowLanes, threads / s.entries));
+      s.ldsPairs = (s.rowLanes == 1 ? 1 : s.rowLanes + s.segments) * s.entries;
+      const int inRun = s.run / per;
+      s.lanes = 64;
+      while(s.lanes > 1 && s.lanes * inRun > threads) s.lanes /= 2;
+      s.ldsPairs += state * inRun;
+      if((int64_t)s.ldsPairs * 8 * s.units > 60000) continue;
+      return s;
+    }
+  return none;
+}
+
+}  // namespace
+
+#endif

@@ -16,23 +16,66 @@ struct QuantArgs {
   int channels;
 };
 
-template<typename T>
-__global__ __launch_bounds__(256) void quantizeRowsKernel(QuantArgs a) {
-  __shared__ unsigned tops[4];
-  for(int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-  const T* x = (const T*)a.x + row * a.ldx;
-  int8_t* out = a.out + row * a.ldo;
-  unsigned top = 0;
-  for(int c = threadIdx.x; c < a.channels; c += 256) top = max(top, magnitudeBits((float)x[c]));
+// A row by `lanes` threads side by side, K 16-byte groups each, which stay in registers
+// between the largest value and the whole numbers: bound by the row's way in and out.
+template<typename T, int K>
+__global__ __launch_bounds__(256) void quantizeRowsKernel(QuantArgs a, int lanes) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  __shared__ unsigned tops[2][4];
+  const int sub = threadIdx.x & (lanes - 1), perBlock = 256 / lanes;
+  const int64_t row0 = threadIdx.x / lanes;
+  int turn = 0;
+  for(int64_t base = (int64_t)blockIdx.x * perBlock; base < a.rows; base += (int64_t)gridDim.x * perBlock, turn ^= 1) {
+    const int64_t row = min(base + row0, a.rows - 1);
+    const T* x = (const T*)a.x + row * a.ldx;
+    u32x4_t v[K];
 #pragma unroll
-  for(int w = 32; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
-  if((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-  const RowScale s(top);
-  for(int c = threadIdx.x; c < a.channels; c += 256) out[c] = (int8_t)s.quantized((float)x[c]);
-  if(threadIdx.x == 0) a.scales[row] = s.scale;
-  __syncthreads();
+    for(int i = 0; i < K; i++) v[i] = RowGroup<T, false>(min(sub + i * lanes, (a.channels - 1) / VEC), a.channels).load(x);
+    unsigned top = 0;
+#pragma unroll
+    for(int i = 0; i < K; i++) {
+      v[i] = RowGroup<T, false>(min(sub + i * lanes, (a.channels - 1) / VEC), a.channels).place(v[i]);
+      const Values<T> f(v[i]);
+#pragma unroll
+      for(int j = 0; j < VEC; j++) top = max(top, magnitudeBits(f.f[j]));
+    }
+    const RowScale s(rowTop(top, lanes, tops[turn]));
+    if(base + row0 >= a.rows) continue;
+    int8_t* out = a.out + row * a.ldo;
+#pragma unroll
+    for(int i = 0; i < K; i++) {
+      const int c = (sub + i * lanes) * VEC;
+      if(c < a.channels) storeBytes<VEC>(out + c, quantized(Values<T>(v[i]).f, s), 0, a.channels - c);
+    }
+    if(sub == 0) a.scales[row] = s.scale;
+  }
+}
+
+// Rows of any length, read twice.
+template<typename T>
+__global__ __launch_bounds__(256) void quantizeRowsLongKernel(QuantArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  __shared__ unsigned tops[2][4];
+  int turn = 0;
+  for(int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T* x = (const T*)a.x + row * a.ldx;
+    int8_t* out = a.out + row * a.ldo;
+    const int groups = (a.channels + VEC - 1) / VEC;
+    unsigned top = 0;
+#pragma unroll 4
+    for(int g = threadIdx.x; g < groups; g += 256) {
+      const RowGroup<T, false> r(g, a.channels);
+      const Values<T> f(r.place(r.load(x)));
+#pragma unroll
+      for(int j = 0; j < VEC; j++) top = max(top, magnitudeBits(f.f[j]));
+    }
+    const RowScale s(rowTop(top, 256, tops[turn]));
+#pragma unroll 4
+    for(int g = threadIdx.x; g < groups; g += 256) {
+      const RowGroup<T, false> r(g, a.channels);
+      storeBytes<VEC>(out + g * VEC, quantized(Values<T>(r.place(r.load(x))).f, s), 0, a.channels - g * VEC);
+    }
+    if(threadIdx.x == 0) a.scales[row] = s.scale;
   }
 }
 
@@ -59,7 +102,19 @@ void checkQuantize(const kgh_quantize_params& p) {
 void launchQuantize(const kgh_quantize_params& p, hipStream_t stream) {
   if(p.rows == 0) return;
   const QuantArgs a{p.x, p.out, p.scales, p.x_stride, p.out_stride, p.rows, p.channels};
-  withDtype(p.dtype, [&](auto t) { quantizeRowsKernel<decltype(t)><<<dim3((unsigned)std::min<int64_t>(p.rows, 1 << 20)), 256, 0, stream>>>(a); });
+  withDtype(p.dtype, [&](auto t) {
+    typedef decltype(t) T;
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const RowLanes r = rowLanes((p.channels + VEC - 1) / VEC, 8);
+    const int64_t perBlock = r.lanes == 0 ? 1 : 256 / r.lanes;
+    const dim3 grid((unsigned)std::min<int64_t>((p.rows + perBlock - 1) / perBlock, 1 << 20));
+    if(r.lanes == 0) quantizeRowsLongKernel<T><<<grid, 256, 0, stream>>>(a);
+    else if(r.each <= 1) quantizeRowsKernel<T, 1><<<grid, 256, 0, stream>>>(a, r.lanes);
+    else if(r.each <= 2) quantizeRowsKernel<T, 2><<<grid, 256, 0, stream>>>(a, r.lanes);
+    else if(r.each <= 3) quantizeRowsKernel<T, 3><<<grid, 256, 0, stream>>>(a, r.lanes);
+    else if(r.each <= 4) quantizeRowsKernel<T, 4><<<grid, 256, 0, stream>>>(a, r.lanes);
+    else quantizeRowsKernel<T, 8><<<grid, 256, 0, stream>>>(a, r.lanes);
+  });
   KGH_CHECK_LAUNCH();
 }
 

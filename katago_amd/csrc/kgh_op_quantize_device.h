@@ -6,6 +6,28 @@
 
 namespace {
 
+// Elements of a 16-byte group as floats.
+template<typename T>
+struct Values {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  float f[VEC];
+  __device__ __forceinline__ explicit Values(u32x4_t v) {
+    if constexpr(__is_same(T, bf16_t)) {
+#pragma unroll
+      for(int i = 0; i < 4; i++) {
+        f[2 * i] = __uint_as_float(v[i] << 16);
+        f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+      }
+    }
+    else {
+      T e[VEC];
+      __builtin_memcpy(e, &v, 16);
+#pragma unroll
+      for(int j = 0; j < VEC; j++) f[j] = (float)e[j];
+    }
+  }
+};
+
 // A number's bits without its sign: ordered as magnitudes, infinity above every
 // number and NaN above infinity.
 __device__ __forceinline__ unsigned magnitudeBits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -26,6 +48,54 @@ struct RowScale {
   // 0 where the factor is: also of infinities and NaN.
   __device__ __forceinline__ int quantized(float v) const { return factor == 0.0f ? 0 : (int)rintf(v * factor); }
 };
+
+// The largest of a row that `lanes` threads side by side have (a power of two up to 64,
+// or a workgroup of 256, whose waves meet in lds).
+__device__ __forceinline__ unsigned rowTop(unsigned top, int lanes, unsigned* lds) {
+  for(int w = min(lanes, 64) >> 1; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
+  if(lanes <= 64) return top;
+  if((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
+  __syncthreads();
+  return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+}
+
+// How threads share a row of `groups` 16-byte groups, at most `most` each: the power of
+// two in a wave, or the workgroup of 256, that leaves the fewest idle; lanes is 0 where
+// the row is longer.
+struct RowLanes {
+  int lanes, each;
+};
+inline RowLanes rowLanes(int groups, int most) {
+  RowLanes best{0, 0};
+  for(int lanes : {64, 32, 16, 8, 256}) {
+    const int each = (groups + lanes - 1) / lanes;
+    if(each <= most && (best.lanes == 0 || lanes * each < best.lanes * best.each)) best = RowLanes{lanes, each};
+  }
+  return best;
+}
+
+// Bytes [from, to) of VEC (4 or 8), to p + from and on.
+template<int VEC>
+__device__ __forceinline__ void storeBytes(int8_t* p, uint2 v, int from, int to) {
+  if(from == 0 && to >= VEC) __builtin_memcpy(p, &v, VEC);
+  else {
+#pragma unroll 1
+    for(int j = 0; j < VEC; j++) {
+      if(j >= from && j < to) p[j] = (int8_t)(v.x & 0xff);
+      v.x = __builtin_amdgcn_alignbit(v.y, v.x, 8);
+      v.y >>= 8;
+    }
+  }
+}
+
+// VEC values in 8 bits.
+template<int VEC>
+__device__ __forceinline__ uint2 quantized(const float (&y)[VEC], const RowScale& s) {
+  unsigned w[2] = {0, 0};
+#pragma unroll
+  for(int j = 0; j < VEC; j++) w[j >> 2] |= (unsigned)(s.quantized(y[j]) & 0xff) << (8 * (j & 3));
+  return make_uint2(w[0], w[1]);
+}
 
 }  // namespace
 
