@@ -1,9 +1,6 @@
 // Matrix product of 8-bit integers with scales for rows and channels
 // (kgh_linear_int8).
-#include "kgh_conv_device.h"
-#include "kgh_ops_device.h"
-
-#include <algorithm>
+#include "kgh_op_linear_device.h"
 
 namespace {
 
@@ -11,77 +8,348 @@ namespace {
 // launch counts its threads in 32 bits.
 constexpr int64_t LIN8_MAX = 1 << 30, LIN8_MAX_OUT = 1 << 26;
 
-typedef int intx4 __attribute__((ext_vector_type(4)));
-typedef int intx16 __attribute__((ext_vector_type(16)));
-
-struct Linear8Args {
-  const int8_t* x;
-  const int8_t* w;
-  const float* xScales;
-  const float* wScales;
-  const float* bias;
-  const void* residual;
-  void* out;
-  int64_t ldx, ldw, ldr, ldo;
-  int M, N, K;
+struct Scales {
+  const float* x;
+  const float* w;
 };
 
-// 16 bytes of k per lane half times the other operand's: 32 x 32 results, laid out
-// as mma32's.
-__device__ __forceinline__ intx16 mma32(intx4 a, intx4 b, intx16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
-
-// Elements [0, n) of the 16 bytes at p, zeros behind them.
+// Bytes [0, n) of the 16 at p, zeros behind them.
 __device__ __forceinline__ u32x4_t loadBytes(const int8_t* p, int n) {
   u32x4_t v = {0, 0, 0, 0};
   if(n >= 16) __builtin_memcpy(&v, p, 16);
   else
-    for(int j = 0; j < n; j++) v[j >> 2] |= (unsigned)(uint8_t)p[j] << (8 * (j & 3));
+#pragma unroll 1
+    for(int j = 0; j < 16; j++) {  // byte j enters at the top and moves down to its place
+      v[0] = __builtin_amdgcn_alignbit(v[1], v[0], 8);
+      v[1] = __builtin_amdgcn_alignbit(v[2], v[1], 8);
+      v[2] = __builtin_amdgcn_alignbit(v[3], v[2], 8);
+      v[3] = v[3] >> 8 | (j < n ? (unsigned)(uint8_t)p[j] << 24 : 0);
+    }
   return v;
 }
 
-template<typename T, int ACT>
-__device__ __forceinline__ T finish(const Linear8Args& a, int sum, int m, int n) {
-  float v = (float)sum * a.xScales[m] * a.wScales[n];
-  v = activate<T, ACT>(v + (a.bias != nullptr ? a.bias[n] : 0.0f));
-  if(a.residual != nullptr) v += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n];
-  return (T)v;
+// A sum's value: one rounding of its own, two of the products.
+__device__ __forceinline__ float scaled(int sum, float x, float w) { return (float)sum * x * w; }
+
+// storeTile of sums: by their scales, or as they are where K is split.
+template<typename T, int RB, int CB, int ACT>
+__device__ __forceinline__ void storeSums(const LinearArgs& a, const Scales& s, const intx16 (&sums)[RB][CB], int m, int n) {
+  const int lane = threadIdx.x & 63, laneRow = lane & 31, half = lane >> 5;
+  floatx16 acc[RB][CB];
+  if(a.part != nullptr) {
+#pragma unroll
+    for(int i = 0; i < RB; i++)
+#pragma unroll
+      for(int j = 0; j < CB; j++) acc[i][j] = __builtin_bit_cast(floatx16, sums[i][j]);
+  }
+  else {
+    float x[RB];
+#pragma unroll
+    for(int i = 0; i < RB; i++) x[i] = s.x[min(m + i * 32 + laneRow, a.M - 1)];
+#pragma unroll
+    for(int j = 0; j < CB; j++)
+#pragma unroll
+      for(int q = 0; q < 4; q++) {
+        const int c = n + j * 32 + q * 8 + half * 4;
+        const uint4 u = loadGroupSmall(s.w + min(c, a.N - 1), c < a.N ? a.N - c : 1);
+        const floatx4 w = *(const floatx4*)&u;
+#pragma unroll
+        for(int i = 0; i < RB; i++)
+#pragma unroll
+          for(int e = 0; e < 4; e++) acc[i][j][4 * q + e] = scaled(sums[i][j][4 * q + e], x[i], w[e]);
+      }
+  }
+  storeTile<T, RB, CB, ACT>(a, acc, m, n);
 }
 
-// Any sizes, strides and alignment: 64 x 64 tiles of four waves, steps of 128 bytes
-// of K through LDS.
-template<typename T, int ACT>
-__global__ __launch_bounds__(256) void linear8TileKernel(Linear8Args a, int rowTiles, int colTiles) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[128 * 128];
+// ---------------------------------------------------------------------------
+// Rows that are 16-byte aligned: dmaTile's loop, 128 k a step.
+template<typename T, int WM, int WN, int RB, int CB, int PER_CU, int ACT>
+__global__ __launch_bounds__(64 * WM * WN, PER_CU * WM * WN / 4) void linear8DmaKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
+  intx16 acc[RB][CB];
+  int m, n;
+  if(dmaTile<int8_t, WM, WN, 1, RB, CB>(a, rowTiles, colTiles, acc, m, n)) storeSums<T, RB, CB, ACT>(a, s, acc, m, n);
+}
+
+// ---------------------------------------------------------------------------
+// Any strides and alignment: tiles of 2 x 2 waves of 32 RB x 32 CB, steps of 128 bytes
+// of K, loaded into registers two steps ahead, put into one LDS buffer while the other
+// one's products run.
+template<typename T, int RB, int CB, int ACT>
+__global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
+  constexpr int STEP = 128, BM = 64 * RB, BN = 64 * CB, LOADS = 2 * (RB + CB);
+  __shared__ __attribute__((aligned(16))) unsigned char lds0[(BM + BN) * 128];
+  __shared__ __attribute__((aligned(16))) unsigned char lds1[(BM + BN) * 128];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int laneRow = lane & 31, half = lane >> 5;
   int rowTile, colTile;
   blockedTile(rowTiles, colTiles, rowTile, colTile);
-  const int m0 = rowTile * 64, n0 = colTile * 64;
+  const int m0 = rowTile * BM, n0 = colTile * BN;
+  const int kBegin = blockIdx.y * a.chunk, kEnd = min(kBegin + a.chunk, a.K);
+  const int whole = (kEnd - kBegin) / STEP;
+  // Thread t loads group t & 7 of rows t >> 3, + 32, ...
   const int lr = tid >> 3, lg = tid & 7;
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-  intx16 acc;
+  const int8_t* src[LOADS];
 #pragma unroll
-  for(int r = 0; r < 16; r++) acc[r] = 0;
-  for(int k = 0; k < a.K; k += 128) {
-    __syncthreads();
+  for(int i = 0; i < 2 * RB; i++) src[i] = (const int8_t*)a.x + (int64_t)min(m0 + lr + 32 * i, a.M - 1) * a.ldx + kBegin + lg * 16;
 #pragma unroll
-    for(int i = 0; i < 4; i++) {
-      const int row = lr + 32 * i;
-      const int8_t* src = row < 64 ? a.x + (int64_t)min(m0 + row, a.M - 1) * a.ldx : a.w + (int64_t)min(n0 + row - 64, a.N - 1) * a.ldw;
-      *(u32x4_t*)(lds + swizzled128(row, lg)) = loadBytes(src + k + lg * 16, a.K - k - lg * 16);
+  for(int i = 0; i < 2 * CB; i++) src[2 * RB + i] = (const int8_t*)a.w + (int64_t)min(n0 + lr + 32 * i, a.N - 1) * a.ldw + kBegin + lg * 16;
+  struct Rows {
+    u32x4_t v[LOADS];
+  };
+  // Steps past the last whole one read that one again, into a buffer that nobody reads.
+  auto fetch = [&](int step, Rows& r) {
+    const int k = min(step, whole - 1) * STEP;
+#pragma unroll
+    for(int i = 0; i < LOADS; i++) __builtin_memcpy(&r.v[i], src[i] + k, 16);
+  };
+  auto stage = [&](unsigned char* lds, const Rows& r) {
+#pragma unroll
+    for(int i = 0; i < LOADS; i++) *(u32x4_t*)(lds + swizzled128(lr + 32 * i, lg)) = r.v[i];
+  };
+  intx16 acc[RB][CB];
+#pragma unroll
+  for(int i = 0; i < RB; i++)
+#pragma unroll
+    for(int j = 0; j < CB; j++)
+#pragma unroll
+      for(int r = 0; r < 16; r++) acc[i][j][r] = 0;
+  const int wm = (wave >> 1) * 32 * RB, wn = (wave & 1) * 32 * CB;
+  auto products = [&](const unsigned char* lds) {
+    intx4 af[4][RB], bf[4][CB];
+#pragma unroll
+    for(int p = 0; p < 4; p++) {
+#pragma unroll
+      for(int i = 0; i < RB; i++) af[p][i] = *(const intx4*)(lds + swizzled128(wm + i * 32 + laneRow, 2 * p + half));
+#pragma unroll
+      for(int j = 0; j < CB; j++) bf[p][j] = *(const intx4*)(lds + swizzled128(BM + wn + j * 32 + laneRow, 2 * p + half));
     }
-    __syncthreads();
 #pragma unroll
-    for(int s = 0; s < 4; s++)
-      acc = mma32(*(const intx4*)(lds + swizzled128(64 + wn + laneRow, 2 * s + half)), *(const intx4*)(lds + swizzled128(wm + laneRow, 2 * s + half)), acc);
+    for(int p = 0; p < 4; p++)
+#pragma unroll
+      for(int i = 0; i < RB; i++)
+#pragma unroll
+        for(int j = 0; j < CB; j++) acc[i][j] = mma32(bf[p][j], af[p][i], acc[i][j]);
+  };
+  if(whole > 0) {
+    auto step = [&](const unsigned char* now, unsigned char* then, Rows& use, Rows& load, int at) {
+      fetch(at + 2, load);
+      __builtin_amdgcn_sched_barrier(0);
+      products(now);
+      stage(then, use);
+      barrierLds();
+    };
+    Rows r0, r1;
+    fetch(0, r0);
+    fetch(1, r1);
+    stage(lds0, r0);
+    barrierLds();
+    int at = 0;
+    for(; at + 2 <= whole; at += 2) {
+      step(lds0, lds1, r1, r0, at);
+      step(lds1, lds0, r0, r1, at + 1);
+    }
+    if(at < whole) step(lds0, lds1, r1, r0, at);
   }
-  const int m = m0 + wm + laneRow;
+  const int left = kEnd - kBegin - whole * STEP;
+  if(left > 0) {
+    Rows r;
+#pragma unroll
+    for(int i = 0; i < LOADS; i++) r.v[i] = loadBytes(src[i] + whole * STEP, left - lg * 16);
+    stage(lds0, r);
+    barrierLds();
+    products(lds0);
+  }
+  storeSums<T, RB, CB, ACT>(a, s, acc, m0 + wm, n0 + wn);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (at most 16 MT), any strides and alignment: the weights are read once. A
+// workgroup has 16 NT output channels; its waves take units of 128 bytes of K in turn
+// (every wave's loads of UNROLL units are issued before the first product), and their
+// sums meet in LDS.
+template<typename T, int MT, int NT, int WAVES, int UNROLL, int ACT>
+__global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, Scales s) {
+  constexpr int UNIT = 128;
+  __shared__ int sums[WAVES][MT * NT][4][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, quad = lane >> 4;
+  const int n0 = blockIdx.x * 16 * NT;
+  const int8_t* wRow[NT];
+  const int8_t* xRow[MT];
+#pragma unroll
+  for(int j = 0; j < NT; j++) wRow[j] = (const int8_t*)a.w + (int64_t)min(n0 + j * 16 + l16, a.N - 1) * a.ldw + quad * 16;
+#pragma unroll
+  for(int i = 0; i < MT; i++) xRow[i] = (const int8_t*)a.x + (int64_t)min(i * 16 + l16, a.M - 1) * a.ldx + quad * 16;
+  intx4 acc[MT][NT];
+#pragma unroll
+  for(int i = 0; i < MT; i++)
+#pragma unroll
+    for(int j = 0; j < NT; j++) acc[i][j] = intx4{0, 0, 0, 0};
+  const int kEnd = min((int)(blockIdx.y + 1) * a.chunk, a.K);
+  auto run = [&](int k0, auto units, auto whole) {
+    constexpr int U = decltype(units)::value;
+    u32x4_t wv[U][2][NT], xv[U][2][MT];
+#pragma unroll
+    for(int u = 0; u < U; u++)
+#pragma unroll
+      for(int p = 0; p < 2; p++) {
+        const int k = k0 + (u * WAVES * 2 + p) * 64;
+#pragma unroll
+        for(int j = 0; j < NT; j++) {
+          if constexpr(decltype(whole)::value) __builtin_memcpy(&wv[u][p][j], wRow[j] + k, 16);
+          else wv[u][p][j] = loadBytes(wRow[j] + k, kEnd - quad * 16 - k);
+        }
+#pragma unroll
+        for(int i = 0; i < MT; i++) {
+          if constexpr(decltype(whole)::value) __builtin_memcpy(&xv[u][p][i], xRow[i] + k, 16);
+          else xv[u][p][i] = loadBytes(xRow[i] + k, kEnd - quad * 16 - k);
+        }
+      }
+#pragma unroll
+    for(int u = 0; u < U; u++)
+#pragma unroll
+      for(int p = 0; p < 2; p++)
+#pragma unroll
+        for(int i = 0; i < MT; i++)
+#pragma unroll
+          for(int j = 0; j < NT; j++) acc[i][j] = mma16(*(const intx4*)&wv[u][p][j], *(const intx4*)&xv[u][p][i], acc[i][j]);
+  };
+  int k = blockIdx.y * a.chunk + wave * UNIT;
+  // (a second loop of one unit each would be the same sums)
+  for(; k + (UNROLL - 1) * WAVES * UNIT + UNIT <= kEnd; k += UNROLL * WAVES * UNIT) run(k, std::integral_constant<int, UNROLL>(), std::true_type());
+  for(; k + UNIT <= kEnd; k += WAVES * UNIT) run(k, std::integral_constant<int, 1>(), std::true_type());
+  if(k < kEnd) run(k, std::integral_constant<int, 1>(), std::false_type());
+
+#pragma unroll
+  for(int i = 0; i < MT; i++)
+#pragma unroll
+    for(int j = 0; j < NT; j++)
+#pragma unroll
+      for(int r = 0; r < 4; r++) sums[wave][i * NT + j][r][lane] = acc[i][j][r];
+  __syncthreads();
+  for(int o = tid; o < 256 * MT * NT; o += 64 * WAVES) {
+    const int c = o % (16 * NT), m = o / (16 * NT);
+    const int n = n0 + c;
+    if(n >= a.N || m >= a.M) continue;
+    int sum = 0;
+#pragma unroll
+    for(int w = 0; w < WAVES; w++) sum += sums[w][(m >> 4) * NT + (c >> 4)][c & 3][((c & 15) >> 2) * 16 + (m & 15)];
+    if(a.part != nullptr) {
+      ((int*)a.part)[((int64_t)blockIdx.y * a.M + m) * a.N + n] = sum;
+      continue;
+    }
+    float v = activate<T, ACT>(scaled(sum, s.x[m], s.w[n]) + (a.bias != nullptr ? a.bias[n] : 0.0f));
+    if(a.residual != nullptr) v += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n];
+    ((T*)a.out)[(int64_t)m * a.ldo + n] = (T)v;
+  }
+}
+
+// The sums of K's splits, and the epilogue; a thread takes four columns.
+template<typename T, int ACT>
+__global__ __launch_bounds__(256) void linear8JoinKernel(LinearArgs a, Scales s, int splits) {
+  const int cols = (a.N + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(id / cols), n = (int)(id - (int64_t)m * cols) * 4;
   if(m >= a.M) return;
-#pragma unroll
-  for(int r = 0; r < 16; r++) {
-    const int n = n0 + wn + (r >> 2) * 8 + half * 4 + (r & 3);
-    if(n < a.N) ((T*)a.out)[(int64_t)m * a.ldo + n] = finish<T, ACT>(a, acc[r], m, n);
+  const int count = min(4, a.N - n);
+  int v[4] = {0, 0, 0, 0};
+  const int* p = (const int*)a.part + (int64_t)m * a.N + n;
+#pragma unroll 4
+  for(int i = 0; i < splits; i++) {
+    const uint4 u = loadGroup((const float*)(p + (int64_t)i * a.M * a.N), count);
+    v[0] += (int)u.x;
+    v[1] += (int)u.y;
+    v[2] += (int)u.z;
+    v[3] += (int)u.w;
   }
+  const float x = s.x[m];
+#pragma unroll
+  for(int j = 0; j < 4; j++) {
+    if(j >= count) break;
+    float y = activate<T, ACT>(scaled(v[j], x, s.w[n + j]) + (a.bias != nullptr ? a.bias[n + j] : 0.0f));
+    if(a.residual != nullptr) y += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n + j];
+    ((T*)a.out)[(int64_t)m * a.ldo + n + j] = (T)y;
+  }
+}
+
+template<typename T, int WM, int WN, int RB, int CB, int PER_CU, int ACT>
+void launchDma(const LinearArgs& a, const Scales& s, int splits, hipStream_t stream) {
+  constexpr int BM = 32 * RB * WM, BN = 32 * CB * WN;
+  const int rowTiles = (a.M + BM - 1) / BM, colTiles = (a.N + BN - 1) / BN;
+  linear8DmaKernel<T, WM, WN, RB, CB, PER_CU, ACT><<<dim3((unsigned)(rowTiles * colTiles), (unsigned)splits), 64 * WM * WN, 0, stream>>>(a, s, rowTiles, colTiles);
+}
+
+template<typename T, int RB, int CB, int ACT>
+void launchTile(const LinearArgs& a, const Scales& s, int splits, hipStream_t stream) {
+  const int rowTiles = (a.M + 64 * RB - 1) / (64 * RB), colTiles = (a.N + 64 * CB - 1) / (64 * CB);
+  linear8TileKernel<T, RB, CB, ACT><<<dim3((unsigned)(rowTiles * colTiles), (unsigned)splits), 256, 0, stream>>>(a, s, rowTiles, colTiles);
+}
+
+template<typename T, int MT, int NT, int WAVES, int UNROLL, int ACT>
+void launchSkinny(const LinearArgs& a, const Scales& s, int splits, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)splits);
+  linear8SkinnyKernel<T, MT, NT, WAVES, UNROLL, ACT><<<grid, 64 * WAVES, 0, stream>>>(a, s);
+}
+
+enum Linear8Kernel { LIN8_SKINNY, LIN8_DMA_256, LIN8_DMA_128, LIN8_DMA_64, LIN8_TILE_128, LIN8_TILE_64 };
+struct Linear8Plan {
+  Linear8Kernel kernel;
+  int splits;  // of K
+  int chunk;   // k of a split
+};
+
+// Which kernel runs, and in how many splits of K with `bytes` of workspace.
+Linear8Plan planLinear8(const kgh_linear_int8_params& p, bool aligned, uint64_t bytes) {
+  const auto tiles = [&](int64_t side) { return (p.rows + side - 1) / side * ((p.out_channels + side - 1) / side); };
+  const int64_t K = p.in_channels, big = tiles(256);
+  Linear8Plan plan;
+  int64_t most = 1;  // splits worth their sums' way through memory and a second launch
+  if(p.rows <= 64) {
+    plan.kernel = LIN8_SKINNY;
+    if(K >= 12288) most = std::min<int64_t>(256 / ((p.out_channels + 15) / 16), K / 4096);
+  }
+  else if(aligned && K >= 1024 && big * 10 >= (big + 255) / 256 * 256 * 7) plan.kernel = LIN8_DMA_256;
+  else if(tiles(128) >= 224) plan.kernel = aligned ? LIN8_DMA_128 : LIN8_TILE_128;
+  else {
+    plan.kernel = aligned ? LIN8_DMA_64 : LIN8_TILE_64;
+    if(K >= 4096) most = std::min<int64_t>(512 / tiles(64), K / 1024);
+  }
+  const uint64_t one = (uint64_t)p.rows * p.out_channels * 4;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)std::min<uint64_t>(bytes / one, 1024)));
+  plan.chunk = (int)((K + splits * 128 - 1) / (splits * 128) * 128);
+  plan.splits = (int)((K + plan.chunk - 1) / plan.chunk);
+  return plan;
+}
+
+template<typename T, int ACT>
+void runLinear8(const Linear8Plan& plan, const LinearArgs& a, const Scales& scales, hipStream_t stream) {
+  const int s = plan.splits;
+  if(plan.kernel == LIN8_SKINNY) {
+    const bool wide = a.N >= 8192;
+    if(a.M <= 16) launchSkinny<T, 1, 1, 8, 4, ACT>(a, scales, s, stream);
+    else if(a.M <= 32 && wide) launchSkinny<T, 2, 2, 8, 4, ACT>(a, scales, s, stream);
+    else if(a.M <= 32) launchSkinny<T, 2, 1, 8, 4, ACT>(a, scales, s, stream);
+    else if(wide) launchSkinny<T, 4, 2, 8, 2, ACT>(a, scales, s, stream);
+    else launchSkinny<T, 4, 1, 8, 2, ACT>(a, scales, s, stream);
+  }
+  else if(plan.kernel == LIN8_TILE_128) launchTile<T, 2, 2, ACT>(a, scales, s, stream);
+  else if(plan.kernel == LIN8_TILE_64) launchTile<T, 1, 1, ACT>(a, scales, s, stream);
+  else if(plan.kernel == LIN8_DMA_256) launchDma<T, 2, 4, 4, 2, 1, ACT>(a, scales, s, stream);
+  else if(plan.kernel == LIN8_DMA_128) launchDma<T, 2, 2, 2, 2, 2, ACT>(a, scales, s, stream);
+  else launchDma<T, 2, 2, 1, 1, 4, ACT>(a, scales, s, stream);
+  KGH_CHECK_LAUNCH();
+  if(s > 1) {
+    const int64_t threads = (int64_t)a.M * ((a.N + 3) / 4);
+    linear8JoinKernel<T, ACT><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, stream>>>(a, scales, s);
+    KGH_CHECK_LAUNCH();
+  }
+}
+
+bool linear8Aligned(const kgh_linear_int8_params& p) {
+  return (((uintptr_t)p.x | (uintptr_t)p.weights) & 15) == 0 && p.in_channels % 16 == 0 && p.x_stride % 16 == 0 && p.weights_stride % 16 == 0 &&
+         p.x_stride < LIN_DMA_STRIDE && p.weights_stride < LIN_DMA_STRIDE;
 }
 
 }  // namespace
@@ -118,19 +386,22 @@ void checkLinearInt8(const kgh_linear_int8_params& p, bool pointers) {
   if(p.residual == p.out && p.rows > 1 && p.residual_stride != p.out_stride) opInvalid(op, "in place, residual_stride must be out_stride");
 }
 
-uint64_t linearInt8Workspace(const kgh_linear_int8_params&) { return 0; }
+// By the sizes alone: as if the rows were aligned.
+uint64_t linearInt8Workspace(const kgh_linear_int8_params& p) {
+  if(p.rows == 0) return 0;
+  const Linear8Plan plan = planLinear8(p, true, UINT64_MAX);
+  return plan.splits > 1 ? (uint64_t)plan.splits * p.rows * p.out_channels * 4 : 0;
+}
 
 void launchLinearInt8(const kgh_linear_int8_params& p, hipStream_t stream) {
   if(p.rows == 0) return;
-  const Linear8Args a{p.x, p.weights, p.x_scales, p.weight_scales, p.bias, p.residual, p.out, p.x_stride, p.weights_stride, p.residual_stride,
-                      p.out_stride, (int)p.rows, p.out_channels, p.in_channels};
-  const int rowTiles = (a.M + 63) / 64, colTiles = (a.N + 63) / 64;
+  const Linear8Plan plan = planLinear8(p, linear8Aligned(p), p.workspace != nullptr ? p.workspace_bytes : 0);
+  const LinearArgs a{p.x, p.weights, p.bias, p.residual, p.out, p.x_stride, p.weights_stride, p.residual_stride, p.out_stride,
+                     (int)p.rows, p.out_channels, p.in_channels, plan.splits > 1 ? (float*)p.workspace : nullptr, plan.chunk};
+  const Scales s{p.x_scales, p.weight_scales};
   withDtype(p.dtype, [&](auto t) {
-    withActivation(p.activation, [&](auto act) {
-      linear8TileKernel<decltype(t), decltype(act)::value><<<dim3((unsigned)(rowTiles * colTiles)), 256, 0, stream>>>(a, rowTiles, colTiles);
-    });
+    withActivation(p.activation, [&](auto act) { runLinear8<decltype(t), decltype(act)::value>(plan, a, s, stream); });
   });
-  KGH_CHECK_LAUNCH();
 }
 
 }  // namespace kgh

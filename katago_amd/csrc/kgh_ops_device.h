@@ -15,6 +15,9 @@ template<typename T> struct Vec16;
 template<> struct Vec16<half_t> { typedef half8_t V; };
 template<> struct Vec16<bf16_t> { typedef bf16x8_t V; };
 template<> struct Vec16<float> { typedef floatx4 V; };
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
+template<> struct Vec16<int8_t> { typedef intx4 V; };
 
 // Elements [0, n) of the 16-byte group at p, zeros behind them; p need not be
 // aligned to more than an element (the memory takes any alignment).
@@ -151,6 +154,10 @@ __device__ __forceinline__ floatx4 mma16(floatx4 a, floatx4 b, floatx4 c) {
   for(int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
   return c;
 }
+
+// The same of 8-bit integers, 16 consecutive k a lane half (quarter): exact sums.
+__device__ __forceinline__ intx16 mma32(intx4 a, intx4 b, intx16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ intx4 mma16(intx4 a, intx4 b, intx4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
 // The activations: a result is rounded to its type once, so what a value left of 0
 // keeps of itself (e^v or erfc) has to be right relative to itself, down to the type's
