@@ -69,63 +69,44 @@ __device__ __forceinline__ void normalise(float (&y)[VEC], const Values<T>& x, c
 // ---------------------------------------------------------------------------
 // An item's run of channels lies in a unit's registers from its one way in to its way
 // out: sums over a thread's positions for each of its channels, over the unit's threads
-// in LDS, then norm and activation of the same registers. Positions that take no part
-// read the item's first one, which is in a cache. QUANT: rows in 8 bits, a unit being an
-// item with all of its channels.
+// in LDS, then norm and activation of the same registers. Positions that take no part are
+// neither read nor computed: threads have places in a list of those that do. QUANT: rows
+// in 8 bits, a unit being an item with all of its channels.
 template<typename T, int ACT, int NV, bool QUANT>
-__global__ __launch_bounds__(NV == 2 ? 1024 : 512) void normSlabKernel(NormArgs a, NormOut o, NormSlab s) {
+__global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSlabKernel(NormArgs a, NormOut o, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   extern __shared__ float2 lds[];
-  __shared__ int counts[4];
-  const int unit = s.units == 1 ? 0 : threadIdx.x >> 6;
-  const int tt = threadIdx.x - unit * s.threads;
-  const int row = tt / s.cols, col = tt - row * s.cols;
+  const SlabThread<VEC> th(a, s);
   const int inRun = s.run / a.per;
-  float2* part = lds + unit * s.ldsPairs;
+  float2* part = lds + th.unit * s.ldsPairs;
   float2* state = part + s.ldsPairs - 2 * inRun;  // a group's reference and factor
   float2* result = state + inRun;                 // its mean and reciprocal deviation
-  const int64_t id = s.first + (int64_t)xcdContiguousTile() * s.units + unit;
-  const bool live = id < s.count;  // (units of the last workgroup that have no work go along)
-  const int64_t mine = live ? id : s.count - 1;
-  const int b = (int)(mine / s.runs), r = (int)(mine - (int64_t)b * s.runs);
-  const int c1 = r * s.run, c0 = c1 + col * VEC;
-  const bool on = row < s.rowLanes && c0 < min(c1 + s.run, a.channels);
-  const Window<VEC> win(c0, a.channels);
-  const int groups = min(inRun, a.groups - r * inRun);
-  const int len = validLength(a, b);
-  const T* x = (const T*)a.x + b * a.xB + win.at;
-  unsigned bits = 0;  // positions of this thread that take part
-  if(a.mask == nullptr) {
-#pragma unroll
-    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len ? 1u << i : 0u;
+  unsigned short* list = (unsigned short*)((char*)lds + s.listAt) + th.unit * (listBytes(a.positions) / 2);
+  const T* x = (const T*)a.x + th.b * a.xB + th.at;
+  int count = validLength(a, th.b);  // places that take part
+  if(a.mask != nullptr) {
+    count = listPositions(a, s, th.b, th.tt, count, list);
+    __syncthreads();
   }
-  else {
-    if(tt == 0) counts[unit] = 0;
-    const uint8_t* mask = a.mask + b * a.maskB;
-    uint8_t m[NV];
-#pragma unroll
-    for(int i = 0; i < NV; i++) m[i] = mask[min(row + i * s.rowLanes, a.positions - 1)];
-#pragma unroll
-    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len && m[i] != 0 ? 1u << i : 0u;
-  }
+  count = __builtin_amdgcn_readfirstlane(count);
+  auto position = [&](int place) -> unsigned { return a.mask != nullptr ? list[place] : place; };
   u32x4_t v[NV];
 #pragma unroll
-  for(int i = 0; i < NV; i++)
-    if(i < s.nv) __builtin_memcpy(&v[i], x + ((bits >> i) & 1 ? row + i * s.rowLanes : 0) * a.xP, 16);
-  if(a.mask != nullptr) {
-    __syncthreads();
-    if(col == 0 && bits != 0) atomicAdd(&counts[unit], __popc(bits));
-  }
+  for(int i = 0, from = 0; i < NV; i++, from += s.rowLanes)
+    if(from < count) __builtin_memcpy(&v[i], x + (uint64_t)position(min(th.row + from, a.positions - 1)) * a.xP, 16);
 
   {
+    const int rowLanes = fresh(s.rowLanes);
     float s1[VEC], s2[VEC];
 #pragma unroll
     for(int j = 0; j < VEC; j++) s1[j] = s2[j] = 0.0f;
 #pragma unroll
-    for(int i = 0; i < NV; i++)
-      if(i < s.nv) {
-        const u32x4_t zero = {0, 0, 0, 0};
-        v[i] = (bits >> i) & 1 ? v[i] : zero;
+    for(int i = 0, from = 0; i < NV; i++, from += rowLanes)
+      if(from < count) {
+        if(from + rowLanes > count) {  // the last places that take part
+          const u32x4_t zero = {0, 0, 0, 0};
+          v[i] = th.row + from < count ? v[i] : zero;
+        }
         const Values<T> d(v[i]);
 #pragma unroll
         for(int j = 0; j < VEC; j++) {
@@ -134,8 +115,8 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512) void normSlabKernel(NormArgs 
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-    if(on) {
-      float2* p = part + row * s.entries + col * s.pv;
+    if(th.on) {
+      float2* p = part + th.row * s.entries + th.col * s.pv;
       if(s.pv == 1) {
 #pragma unroll
         for(int j = 1; j < VEC; j++) s1[0] += s1[j], s2[0] += s2[j];
@@ -144,118 +125,142 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512) void normSlabKernel(NormArgs 
       else {
 #pragma unroll
         for(int j = 0; j < VEC; j++)
-          if(j >= win.skip) p[j - win.skip] = make_float2(s1[j], s2[j]);
+          if(j >= th.skip) p[j - th.skip] = make_float2(s1[j], s2[j]);
       }
     }
     __syncthreads();
   }
-  for(int turns = 0;; turns++) {
-    const float2* red = addRows(part, s, tt);
+  // The groups' mean and deviation by a turn's sums; whether one needs another turn.
+  auto finish = [&](int turn) {
+    const float2* red = addRows(part, s, th.tt);
     if(s.rowLanes > 1) __syncthreads();
-    const int entries = s.pv == 1 ? a.per / VEC : a.per;
-    const int sub = tt & (s.lanes - 1);
-    const float n = (float)(a.mask != nullptr ? counts[unit] : len) * (float)a.per;
+    const float n = (float)count * (float)a.per;
     bool again = false;
-    for(int q = tt / s.lanes; q < groups; q += s.threads / s.lanes) {
+    for(int q = th.tt >> s.lanesLog; q < th.groups; q += s.threads >> s.lanesLog) {
       float sum = 0.0f, squares = 0.0f;
-      for(int k = sub; k < entries * s.segments; k += s.lanes) {
-        const int seg = k / entries;
-        const float2 u = red[seg * s.entries + q * entries + (k - seg * entries)];
+      eachEntry(red, s, q, th.tt, [&](float2 u, int) {
         sum += u.x;
         squares += u.y;
-      }
-      for(int k = s.lanes >> 1; k > 0; k >>= 1) {
+      });
+      for(int k = (1 << s.lanesLog) >> 1; k > 0; k >>= 1) {
         sum += __shfl_xor(sum, k);
         squares += __shfl_xor(squares, k);
       }
-      const GroupSums t = groupSums(n, sum, squares, turns == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turns);
+      const GroupSums t = groupSums(n, sum, squares, turn == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turn);
       again |= t.again;
-      if(sub == 0) {
+      if((th.tt & ((1 << s.lanesLog) - 1)) == 0) {
         const float rd = reciprocalDeviation(t, a.eps);
         state[q] = make_float2(t.next.ref, t.next.factor);
         result[q] = n == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(t.mean, rd);
       }
     }
-    if(!__syncthreads_or(again)) break;
-    // Channel by channel: few registers, for few units.
-    int first = win.at - c1;
-    asm volatile("" : "+v"(first));
-    float2 all = make_float2(0.0f, 0.0f);
+    return __syncthreads_or(again);
+  };
+  if(finish(0)) {
+    // Other turns read x again, from a cache: in the registers' copy they would cost
+    // every unit a quarter of its workgroups a CU.
+#pragma unroll 1
+    for(int turn = 1;; turn++) {
+      // (four channels at a time, for the same reason)
+      float2 all = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+      for(int j0 = 0; j0 < VEC; j0 += 4) {
+        float s1[4], s2[4], ref[4], factor[4];
 #pragma unroll
-    for(int j = 0; j < VEC; j++) {
-      const float2 t = state[min(max(first + j, 0) / a.per, groups - 1)];
-      const float ref = t.x * t.y;
-      float2 sum = make_float2(0.0f, 0.0f);
+        for(int j = 0; j < 4; j++) {
+          const float2 t = state[min((th.channel + max(j0 + j - th.skip, 0)) / a.per, th.groups - 1)];
+          s1[j] = s2[j] = 0.0f;
+          ref[j] = t.x * t.y;
+          factor[j] = t.y;
+        }
+#pragma unroll 1
+        for(int place = th.row; place < count; place += s.rowLanes) {
+          T e[4];
+          __builtin_memcpy(e, x + j0 + (uint64_t)position(place) * a.xP, sizeof(e));
 #pragma unroll
-      for(int i = 0; i < NV; i++) {
-        renew(v[i]);
-        const float d = fmaf(Values<T>(v[i]).f[j], t.y, -ref);
-        if((bits >> i) & 1) {
-          sum.x += d;
-          sum.y = fmaf(d, d, sum.y);
+          for(int j = 0; j < 4; j++) {
+            const float d = fmaf((float)e[j], factor[j], -ref[j]);
+            s1[j] += d;
+            s2[j] = fmaf(d, d, s2[j]);
+          }
+        }
+#pragma unroll
+        for(int j = 0; j < 4; j++) {
+          all.x += s1[j];
+          all.y += s2[j];
+          if(s.pv > 1 && th.on && j0 + j >= th.skip) part[th.row * s.entries + th.channel + j0 + j - th.skip] = make_float2(s1[j], s2[j]);
         }
       }
-      all.x += sum.x;
-      all.y += sum.y;
-      if(s.pv > 1 && on && j >= win.skip) part[row * s.entries + col * VEC + j - win.skip] = sum;
+      if(s.pv == 1 && th.on) part[th.row * s.entries + th.col] = all;
+      __syncthreads();
+      if(!finish(turn)) break;
     }
-    if(s.pv == 1 && on) part[row * s.entries + col] = all;
-    __syncthreads();
   }
 
-  if(o.stats != nullptr && live)
-    for(int q = tt; q < groups; q += s.threads) *(float2*)(o.stats + 2 * ((int64_t)b * a.groups + r * inRun + q)) = result[q];
+  if(o.stats != nullptr && th.live)
+    for(int q = th.tt; q < th.groups; q += s.threads) *(float2*)(o.stats + 2 * ((int64_t)th.b * a.groups + th.c1 / a.per + q)) = result[q];
   float scale[VEC], bias[VEC], mean[VEC];
-  loadFloats(scale, a.weight == nullptr ? nullptr : a.weight + win.at, VEC, 1.0f);
-  loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + win.at, VEC, 0.0f);
-#pragma unroll
-  for(int j = 0; j < VEC; j++) {
-    const float2 t = result[min(max(win.at + j - c1, 0) / a.per, groups - 1)];
+  loadFloats(scale, a.weight == nullptr ? nullptr : a.weight + th.at, VEC, 1.0f);
+  loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + th.at, VEC, 0.0f);
+  th.eachGroup(a, [&](int j, int q) {
+    const float2 t = result[q];
     mean[j] = t.x;
     scale[j] *= t.y;
-  }
+  });
+  const bool stores = th.on && th.live;
   if constexpr(!QUANT) {
-    T* out = (T*)o.out + b * o.oB + win.at;
+    if(!stores) return;
+    T* out = (T*)o.out + th.b * o.oB + th.at;
+    const int rowLanes = fresh(s.rowLanes);
 #pragma unroll
-    for(int i = 0; i < NV; i++)
-      if(i < s.nv) {
-        const int p = row + i * s.rowLanes;
-        float y[VEC];
-        renew(v[i]);
-        normalise<T, ACT>(y, Values<T>(v[i]), mean, scale, bias);
-        const uint4 u = packed<T>(y), zero = make_uint4(0, 0, 0, 0);
-        if(on && live && p < a.positions) storeWindow(out + p * o.oP, (bits >> i) & 1 ? u : zero, win.skip);
+    for(int i = 0, from = 0; i < NV; i++, from += rowLanes)
+      if(from < a.positions) {
+        const int place = th.row + from;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if(from < count) {
+          float y[VEC];
+          renew(v[i]);
+          normalise<T, ACT>(y, Values<T>(v[i]), mean, scale, bias);
+          u = packed<T>(y);
+          if(from + rowLanes > count && place >= count) u = make_uint4(0, 0, 0, 0);
+        }
+        if(place < a.positions) {
+          T* p = out + (uint64_t)position(place) * o.oP;
+          if(a.channels % VEC == 0) __builtin_memcpy(p, &u, 16);
+          else storeWindow(p, u, th.skip);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
   }
   else {
-    unsigned* tops = (unsigned*)part;
-    for(int p = tt; p < a.positions; p += s.threads) tops[p] = 0;
+    unsigned* tops = (unsigned*)part;  // of places
+    for(int p = th.tt; p < a.positions; p += s.threads) tops[p] = 0;
     __syncthreads();
     float y[NV][VEC];
 #pragma unroll
     for(int i = 0; i < NV; i++)
-      if(i < s.nv) {
+      if(i * s.rowLanes < count) {
+        const int place = th.row + i * s.rowLanes;
         renew(v[i]);
         normalise<T, ACT>(y[i], Values<T>(v[i]), mean, scale, bias);
         unsigned top = 0;
 #pragma unroll
-        for(int j = 0; j < VEC; j++) top = max(top, j >= win.skip ? magnitudeBits(y[i][j]) : 0);
-        if((bits >> i) & 1) atomicMax(&tops[row + i * s.rowLanes], top);
+        for(int j = 0; j < VEC; j++) top = max(top, j >= th.skip ? magnitudeBits(y[i][j]) : 0);
+        if(th.on && place < count) atomicMax(&tops[place], top);
       }
     __syncthreads();
-    int8_t* out = (int8_t*)o.out + b * o.oB + win.at;
+    int8_t* out = (int8_t*)o.out + th.b * o.oB + th.at;
 #pragma unroll
-    for(int i = 0; i < NV; i++)
-      if(i < s.nv) {
-        const int p = row + i * s.rowLanes;
-        if(on && live && p < a.positions) {
-          const RowScale rs(tops[p]);
-          const uint2 q = quantized(y[i], rs);
-          storeBytes<VEC>(out + p * o.oP, (bits >> i) & 1 ? q : make_uint2(0, 0), win.skip, VEC);
-          if(col == 0) o.scales[(int64_t)b * a.positions + p] = rs.scale;
-        }
+    for(int i = 0; i < NV; i++) {
+      const int place = th.row + i * s.rowLanes;
+      if(stores && place < a.positions) {
+        const unsigned p = position(place);
+        const RowScale rs(tops[place]);
+        const uint2 q = quantized(y[i], rs);
+        storeBytes<VEC>(out + (uint64_t)p * o.oP, place < count ? q : make_uint2(0, 0), th.skip, VEC);
+        if(th.col == 0) o.scales[(int64_t)th.b * a.positions + p] = rs.scale;
       }
+    }
   }
 }
 
@@ -269,7 +274,7 @@ struct NormParts {
   int chunks, chunkRows, blocks, cols, rowLanes, slots, lanes;  // lanes: threads that add up a group
 };
 
-constexpr int PARTS_AHEAD = 4;  // rows of a thread under way
+constexpr int PARTS_AHEAD = 8;  // rows of a thread under way
 
 template<typename T>
 __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) {
@@ -459,12 +464,13 @@ __global__ __launch_bounds__(256) void normApplyKernel(NormArgs a, NormOut o, No
   }
 }
 
-// The same in 8 bits: a row's columns by `lanes` threads, K each.
-template<typename T, int ACT, int K>
+// The same in 8 bits: a row's columns by `lanes` threads, K each, and R rows at a time.
+template<typename T, int ACT, int K, int R>
 __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, int lanes, int chunks, int chunkRows) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  __shared__ unsigned tops[2][4];
+  __shared__ unsigned tops[2][R][4];
   const int sub = threadIdx.x & (lanes - 1), row = threadIdx.x / lanes, rows = 256 / lanes;
+  const int groups = (a.channels + VEC - 1) / VEC;
   for(int64_t id = blockIdx.x; id < (int64_t)a.batch * chunks; id += gridDim.x) {
     const int b = (int)(id / chunks), chunk = (int)(id - (int64_t)b * chunks);
     const int len = validLength(a, b);
@@ -486,31 +492,41 @@ __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, in
       }
     }
     int turn = 0;
-    for(int p = p0 + row; p - row < p1; p += rows, turn ^= 1) {
-      const int q = min(p, p1 - 1);
-      const bool take = p < p1 && q < len && (mask == nullptr || mask[q] != 0);
-      u32x4_t v[K];
+    for(int from = p0; from < p1; from += R * rows, turn ^= 1) {
+      u32x4_t v[R][K];
+      bool take[R];
 #pragma unroll
-      for(int i = 0; i < K; i++) v[i] = RowGroup<T, false>(min(sub + i * lanes, (a.channels - 1) / VEC), a.channels).load(x + (take ? q : 0) * a.xP);
-      float y[K][VEC];
-      unsigned top = 0;
-#pragma unroll
-      for(int i = 0; i < K; i++) {
-        const int nc = a.channels - (sub + i * lanes) * VEC;
-        normalise<T, ACT>(y[i], Values<T>(RowGroup<T, false>(min(sub + i * lanes, (a.channels - 1) / VEC), a.channels).place(v[i])), mean[i], scale[i], bias[i]);
-#pragma unroll
-        for(int j = 0; j < VEC; j++) top = max(top, j < nc && take ? magnitudeBits(y[i][j]) : 0);
+      for(int r = 0; r < R; r++) {
+        const int p = from + r * rows + row;
+        take[r] = p < min(p1, len) && (mask == nullptr || mask[p] != 0);
       }
-      top = rowTop(top, lanes, tops[turn]);
-      const RowScale rs(top);
-      if(p < p1) {
+#pragma unroll
+      for(int r = 0; r < R; r++)
+#pragma unroll
+        for(int i = 0; i < K; i++)
+          v[r][i] = RowGroup<T, false>(min(sub + i * lanes, groups - 1), a.channels).load(x + (uint64_t)(unsigned)(take[r] ? from + r * rows + row : 0) * a.xP);
+#pragma unroll
+      for(int r = 0; r < R; r++) {
+        const int p = from + r * rows + row;
+        float y[K][VEC];
+        unsigned top = 0;
 #pragma unroll
         for(int i = 0; i < K; i++) {
-          const int c0 = (sub + i * lanes) * VEC, nc = a.channels - c0;
-          if(nc <= 0) continue;
-          storeBytes<VEC>(out + q * o.oP + c0, take ? quantized(y[i], rs) : make_uint2(0, 0), 0, nc);
+          const int nc = a.channels - (sub + i * lanes) * VEC;
+          normalise<T, ACT>(y[i], Values<T>(RowGroup<T, false>(min(sub + i * lanes, groups - 1), a.channels).place(v[r][i])), mean[i], scale[i], bias[i]);
+#pragma unroll
+          for(int j = 0; j < VEC; j++) top = max(top, j < nc ? magnitudeBits(y[i][j]) : 0);
         }
-        if(sub == 0) o.scales[(int64_t)b * a.positions + q] = rs.scale;
+        top = rowTop(take[r] ? top : 0, lanes, tops[turn][r]);
+        const RowScale rs(top);
+        if(p < p1) {
+#pragma unroll
+          for(int i = 0; i < K; i++) {
+            const int c0 = (sub + i * lanes) * VEC, nc = a.channels - c0;
+            if(nc > 0) storeBytes<VEC>(out + (uint64_t)(unsigned)p * o.oP + c0, take[r] ? quantized(y[i], rs) : make_uint2(0, 0), 0, nc);
+          }
+          if(sub == 0) o.scales[(int64_t)b * a.positions + p] = rs.scale;
+        }
       }
     }
     __syncthreads();
@@ -541,6 +557,9 @@ __global__ __launch_bounds__(256) void normQuantLongKernel(NormArgs a, NormOut o
   }
 }
 
+constexpr int NORM_QUANT_EACH = 4;  // 16-byte groups of a thread
+constexpr int NORM_RUN_BYTES = 96;  // of a unit's rows at least
+
 struct NormPlan {
   NormSlab slab;    // threads 0: parts
   NormParts parts;
@@ -551,9 +570,19 @@ NormPlan planNorm(const kgh_group_norm_params& p) {
   const int size = (int)kgh::opElemBytes(p.dtype), vec = 16 / size;
   const bool quant = p.out_scales != nullptr;
   NormPlan plan{};
-  // One position of an item, or few: more threads with less each.
-  plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 96, false, 2, 1024, quant, 2);
-  if(plan.slab.threads == 0 && !quant) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 96, false, 16, 512, false, 2);
+  // Few units: many threads with little each.
+  const auto slab = [&](int bytes, int most, int wide) {
+    if(plan.slab.threads == 0) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, bytes, false, most, wide, quant, 2);
+  };
+  const int64_t rowBytes = (int64_t)p.batch * p.channels * size;
+  if(quant || rowBytes <= 256 * NORM_RUN_BYTES) slab(NORM_RUN_BYTES, 2, 1024);
+  if(!quant) {
+    if(rowBytes <= 512 * NORM_RUN_BYTES) slab(NORM_RUN_BYTES, 4, 512);
+    slab(NORM_RUN_BYTES, 12, 512);
+    slab(NORM_RUN_BYTES, 16, 512);
+    slab(32, 16, 512);
+    slab(32, 2, 1024);
+  }
   if(plan.slab.threads != 0) return plan;
   NormParts& k = plan.parts;
   const int cols = (p.channels + vec - 1) / vec, per = p.channels / p.groups;
@@ -576,10 +605,11 @@ template<typename T, int ACT>
 void launchNorm(const NormPlan& plan, const NormArgs& a, NormOut o, void* workspace, hipStream_t stream) {
   const bool quant = o.scales != nullptr;
   if(plan.slab.threads != 0) {
-    forUnits(plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
+    forUnits(a, plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
       if(quant) normSlabKernel<T, ACT, 2, true><<<grid, threads, bytes, stream>>>(a, o, s);
       else if(s.nv <= 2) normSlabKernel<T, ACT, 2, false><<<grid, threads, bytes, stream>>>(a, o, s);
-      else if(s.nv <= 8) normSlabKernel<T, ACT, 8, false><<<grid, threads, bytes, stream>>>(a, o, s);
+      else if(s.nv <= 4) normSlabKernel<T, ACT, 4, false><<<grid, threads, bytes, stream>>>(a, o, s);
+      else if(s.nv <= 12) normSlabKernel<T, ACT, 12, false><<<grid, threads, bytes, stream>>>(a, o, s);
       else normSlabKernel<T, ACT, 16, false><<<grid, threads, bytes, stream>>>(a, o, s);
       KGH_CHECK_LAUNCH();
     });
@@ -596,17 +626,16 @@ void launchNorm(const NormPlan& plan, const NormArgs& a, NormOut o, void* worksp
   if(!quant) normApplyKernel<T, ACT><<<grid, 256, 0, stream>>>(a, o, k);
   else {
     constexpr int VEC = 16 / (int)sizeof(T);
-    const RowLanes r = rowLanes((a.channels + VEC - 1) / VEC, 4);
+    const RowLanes r = rowLanes((a.channels + VEC - 1) / VEC, NORM_QUANT_EACH);
     if(r.lanes == 0) normQuantLongKernel<T, ACT><<<normGrid((int64_t)a.batch * a.positions), 256, 0, stream>>>(a, o);
     else {
-      const int rows = 256 / r.lanes;
+      const int rows = 256 / r.lanes * (r.each == 1 ? 2 : 1);
       const int chunkRows = (int)std::min<int64_t>((int64_t)a.positions, std::max<int64_t>(1, (int64_t)a.batch * a.positions / rows / 2048) * rows);
       const int chunks = (a.positions + chunkRows - 1) / chunkRows;
       const unsigned g = normGrid((int64_t)a.batch * chunks);
-      if(r.each == 1) normQuantKernel<T, ACT, 1><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
-      else if(r.each == 2) normQuantKernel<T, ACT, 2><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
-      else if(r.each == 3) normQuantKernel<T, ACT, 3><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
-      else normQuantKernel<T, ACT, 4><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+      if(r.each == 1) normQuantKernel<T, ACT, 1, 2><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+      else if(r.each == 2) normQuantKernel<T, ACT, 2, 1><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
+      else normQuantKernel<T, ACT, 4, 1><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);
     }
   }
   KGH_CHECK_LAUNCH();

@@ -88,63 +88,51 @@ struct BackChannels {
 // An item's run of channels in a unit's registers, as in the forward pass: x as it came
 // and u in fp32 (its slope is most of the work, and is computed once).
 template<typename T, int ACT, int NV>
-__global__ __launch_bounds__(512) void normBackSlabKernel(NormArgs a, NormBackArgs k, NormSlab s) {
+__global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormArgs a, NormBackArgs k, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   extern __shared__ float2 lds[];
-  __shared__ int counts[4];
-  const int unit = s.units == 1 ? 0 : threadIdx.x >> 6;
-  const int tt = threadIdx.x - unit * s.threads;
-  const int row = tt / s.cols, col = tt - row * s.cols;
+  const SlabThread<VEC> th(a, s);
   const int inRun = s.run / a.per;
-  float2* part = lds + unit * s.ldsPairs;
+  float2* part = lds + th.unit * s.ldsPairs;
   float2* means = part + s.ldsPairs - inRun;
-  const int64_t id = s.first + (int64_t)xcdContiguousTile() * s.units + unit;
-  const bool live = id < s.count;
-  const int64_t mine = live ? id : s.count - 1;
-  const int b = (int)(mine / s.runs), r = (int)(mine - (int64_t)b * s.runs);
-  const int c1 = r * s.run, c0 = c1 + col * VEC;
-  const bool on = row < s.rowLanes && c0 < min(c1 + s.run, a.channels);
-  const Window<VEC> win(c0, a.channels);
-  const int groups = min(inRun, a.groups - r * inRun);
-  const int len = validLength(a, b);
-  const T* x = (const T*)a.x + b * a.xB + win.at;
-  const T* grad = (const T*)k.grad + b * k.gB + win.at;
-  unsigned bits = 0;
-  if(a.mask == nullptr) {
-#pragma unroll
-    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len ? 1u << i : 0u;
+  unsigned short* list = (unsigned short*)((char*)lds + s.listAt) + th.unit * (listBytes(a.positions) / 2);
+  const T* x = (const T*)a.x + th.b * a.xB + th.at;
+  const T* grad = (const T*)k.grad + th.b * k.gB + th.at;
+  int count = validLength(a, th.b);
+  if(a.mask != nullptr) {
+    count = listPositions(a, s, th.b, th.tt, count, list);
+    __syncthreads();
   }
-  else {
-    if(tt == 0) counts[unit] = 0;
-    const uint8_t* mask = a.mask + b * a.maskB;
-    uint8_t m[NV];
-#pragma unroll
-    for(int i = 0; i < NV; i++) m[i] = mask[min(row + i * s.rowLanes, a.positions - 1)];
-#pragma unroll
-    for(int i = 0; i < NV; i++) bits |= on && i < s.nv && row + i * s.rowLanes < len && m[i] != 0 ? 1u << i : 0u;
-  }
+  count = __builtin_amdgcn_readfirstlane(count);
+  auto position = [&](int i) -> unsigned {
+    const int place = th.row + i * s.rowLanes;
+    return a.mask != nullptr ? list[min(place, a.positions - 1)] : min(place, a.positions - 1);
+  };
   u32x4_t v[NV], d[NV];
 #pragma unroll
   for(int i = 0; i < NV; i++)
-    if(i < s.nv) {
-      const int64_t p = (bits >> i) & 1 ? row + i * s.rowLanes : 0;
+    if(i * s.rowLanes < count) {
+      const uint64_t p = position(i);
       __builtin_memcpy(&v[i], x + p * a.xP, 16);
       __builtin_memcpy(&d[i], grad + p * k.gP, 16);
     }
-  const BackChannels<VEC> ch(a, k.stats, b, win.at, VEC);
-  if(a.mask != nullptr) {
-    __syncthreads();
-    if(col == 0 && bits != 0) atomicAdd(&counts[unit], __popc(bits));
-  }
+  float weight[VEC], bias[VEC], mean[VEC], rstd[VEC];
+  loadFloats(weight, a.weight == nullptr ? nullptr : a.weight + th.at, VEC, 1.0f);
+  loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + th.at, VEC, 0.0f);
+  const float* stats = k.stats + 2 * ((int64_t)th.b * a.groups + th.c1 / a.per);
+  th.eachGroup(a, [&](int j, int q) {
+    mean[j] = stats[2 * q];
+    rstd[j] = stats[2 * q + 1];
+  });
   float u[NV][VEC], s0[VEC], s1[VEC];
 #pragma unroll
   for(int j = 0; j < VEC; j++) s0[j] = s1[j] = 0.0f;
 #pragma unroll
   for(int i = 0; i < NV; i++)
-    if(i < s.nv) {
+    if(i * s.rowLanes < count) {
       float h[VEC];
-      backward<T, ACT>(u[i], h, Values<T>(v[i]), Values<T>(d[i]), ch.mean, ch.rstd, ch.weight, ch.bias);
-      if((bits >> i) & 1) {
+      backward<T, ACT>(u[i], h, Values<T>(v[i]), Values<T>(d[i]), mean, rstd, weight, bias);
+      if(th.row + i * s.rowLanes < count) {
 #pragma unroll
         for(int j = 0; j < VEC; j++) {
           s0[j] += u[i][j];
@@ -153,58 +141,58 @@ __global__ __launch_bounds__(512) void normBackSlabKernel(NormArgs a, NormBackAr
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-  if(on) {
-    float2* p = part + row * s.entries + col * VEC;
+  if(th.on) {
+    float2* p = part + th.row * s.entries + th.channel;
 #pragma unroll
     for(int j = 0; j < VEC; j++)
-      if(j >= win.skip) p[j - win.skip] = make_float2(s0[j], s1[j]);
+      if(j >= th.skip) p[j - th.skip] = make_float2(s0[j], s1[j]);
   }
   __syncthreads();
-  const float2* red = addRows(part, s, tt);
+  const float2* red = addRows(part, s, th.tt);
   if(s.rowLanes > 1) __syncthreads();
   // Channels' sums for the weight's and bias's gradients.
-  if(live)
-    for(int e = tt; e < min(s.run, a.channels - c1); e += s.threads) {
+  if(th.live)
+    for(int e = th.tt; e < min(s.run, a.channels - th.c1); e += s.threads) {
       float2 t = red[e];
       for(int q = 1; q < s.segments; q++) {
         t.x += red[q * s.entries + e].x;
         t.y += red[q * s.entries + e].y;
       }
-      k.sums[(int64_t)b * a.channels + c1 + e] = t;
+      k.sums[(int64_t)th.b * a.channels + th.c1 + e] = t;
     }
-  const int sub = tt & (s.lanes - 1);
-  const float n = (float)(a.mask != nullptr ? counts[unit] : len) * (float)a.per;
-  for(int q = tt / s.lanes; q < groups; q += s.threads / s.lanes) {
+  const float n = (float)count * (float)a.per;
+  for(int q = th.tt >> s.lanesLog; q < th.groups; q += s.threads >> s.lanesLog) {
     float m1 = 0.0f, m2 = 0.0f;
-    for(int i = sub; i < a.per * s.segments; i += s.lanes) {
-      const int seg = i / a.per, e = q * a.per + (i - seg * a.per);
-      const float2 t = red[seg * s.entries + e];
-      const float w = a.weight == nullptr ? 1.0f : a.weight[c1 + e];
+    eachEntry(red, s, q, th.tt, [&](float2 t, int e) {
+      const float w = a.weight == nullptr ? 1.0f : a.weight[th.c1 + e];
       m1 = fmaf(t.x, w, m1);
       m2 = fmaf(t.y, w, m2);
-    }
-    for(int w = s.lanes >> 1; w > 0; w >>= 1) {
+    });
+    for(int w = (1 << s.lanesLog) >> 1; w > 0; w >>= 1) {
       m1 += __shfl_xor(m1, w);
       m2 += __shfl_xor(m2, w);
     }
-    if(sub == 0) means[q] = make_float2(m1 / n, m2 / n);
+    if((th.tt & ((1 << s.lanesLog) - 1)) == 0) means[q] = make_float2(m1 / n, m2 / n);
   }
   __syncthreads();
   float2 mean2[VEC];
-#pragma unroll
-  for(int j = 0; j < VEC; j++) mean2[j] = means[min(max(win.at + j - c1, 0) / a.per, groups - 1)];
-  T* out = (T*)k.out + b * k.oB + win.at;
+  th.eachGroup(a, [&](int j, int q) { mean2[j] = means[q]; });
+  T* out = (T*)k.out + th.b * k.oB + th.at;
 #pragma unroll
   for(int i = 0; i < NV; i++)
-    if(i < s.nv) {
-      const int p = row + i * s.rowLanes;
-      renew(v[i]);
-      const Values<T> xv(v[i]);
-      float y[VEC];
+    if(i * s.rowLanes < a.positions) {
+      const int place = th.row + i * s.rowLanes;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if(i * s.rowLanes < count) {
+        renew(v[i]);
+        const Values<T> xv(v[i]);
+        float y[VEC];
 #pragma unroll
-      for(int j = 0; j < VEC; j++) y[j] = backwardX(u[i][j], (xv.f[j] - ch.mean[j]) * ch.rstd[j], ch.weight[j], ch.rstd[j], mean2[j]);
-      const uint4 o = packed<T>(y), zero = make_uint4(0, 0, 0, 0);
-      if(on && live && p < a.positions) storeWindow(out + p * k.oP, (bits >> i) & 1 ? o : zero, win.skip);
+        for(int j = 0; j < VEC; j++) y[j] = backwardX(u[i][j], (xv.f[j] - mean[j]) * rstd[j], weight[j], rstd[j], mean2[j]);
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        w = place < count ? packed<T>(y) : zero;
+      }
+      if(th.on && th.live && place < a.positions) storeWindow(out + (uint64_t)position(i) * k.oP, w, th.skip);
       __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -406,7 +394,14 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
   const auto round16 = [](uint64_t n) { return (n + 15) / 16 * 16; };
   NormBackPlan plan{};
   plan.sumsBytes = round16((uint64_t)p.batch * p.channels * 8);
-  plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 96, true, 8, 512, false, 1);
+  const auto slab = [&](int bytes, int most, int wide) {
+    if(plan.slab.threads == 0) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, bytes, true, most, wide, false, 1);
+  };
+  const int64_t rowBytes = (int64_t)p.batch * p.channels * size;
+  if(rowBytes <= 512 * 96) slab(96, 2, 512);
+  slab(48, 6, 256);
+  slab(48, 6, 512);
+  slab(16, 6, 512);
   if(plan.slab.threads != 0) return plan;
   BackParts& s = plan.parts;
   const int cols = (p.channels + vec - 1) / vec;
@@ -425,9 +420,10 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
 template<typename T, int ACT>
 void launchBackward(const NormBackPlan& plan, const NormArgs& a, const NormBackArgs& k, hipStream_t stream) {
   if(plan.slab.threads != 0) {
-    forUnits(plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
+    forUnits(a, plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
       if(s.nv <= 2) normBackSlabKernel<T, ACT, 2><<<grid, threads, bytes, stream>>>(a, k, s);
-      else normBackSlabKernel<T, ACT, 8><<<grid, threads, bytes, stream>>>(a, k, s);
+      else if(s.nv <= 4) normBackSlabKernel<T, ACT, 4><<<grid, threads, bytes, stream>>>(a, k, s);
+      else normBackSlabKernel<T, ACT, 6><<<grid, threads, bytes, stream>>>(a, k, s);
       KGH_CHECK_LAUNCH();
     });
     return;

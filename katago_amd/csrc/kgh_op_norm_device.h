@@ -28,20 +28,31 @@ __device__ __forceinline__ int validLength(const NormArgs& a, int b) {
 }
 
 // A unit's threads: an item's run of `run` channels (whole groups), `cols` 16-byte
-// columns of it side by side in `rowLanes` rows of threads; a thread has positions row,
-// row + rowLanes, ..., `nv` of them. `units` units share a workgroup.
+// columns of it side by side in `rowLanes` rows of threads; a thread has places row,
+// row + rowLanes, ..., `nv` of them, in the list of the item's positions that begins
+// with those that take part. `units` units share a workgroup.
 // Sums go through LDS as pairs: `pv` a column (one where a group is whole columns, else
 // one a channel), `entries` = cols pv a row; `segments` runs of rows are added first,
-// then a group's entries by `lanes` threads.
+// then a group's entries by 2^lanesLog threads, whose steps over the runs' entries are
+// stepSegments runs and stepEntries entries.
 struct NormSlab {
-  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, segments, lanes;
-  int64_t count, first;  // units in all, and the first one of this launch
-  int ldsPairs;   // a unit's LDS, in pairs of floats: sums, then groups' state
+  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, segments, groupEntries, lanesLog, stepSegments, stepEntries;
+  int ldsPairs;  // a unit's LDS, in pairs of floats: sums, then groups' state
+  int listAt;    // its list of positions (16 bits each) behind the pairs of all units, in bytes; only where there is a mask
+  int64_t count;             // of units
+  int firstItem, launched;   // of this launch: its first item and its number of units
 };
 
 // 16 bytes that the compiler is to take for new ones: it would otherwise keep the floats
 // of a unit's registers from one use to the next, twice as many registers.
 __device__ __forceinline__ void renew(u32x4_t& v) { asm volatile("" : "+v"(v)); }
+
+// The same of a number that all threads have: products of it are not kept from one loop
+// to the next.
+__device__ __forceinline__ int fresh(int n) {
+  asm volatile("" : "+s"(n));
+  return n;
+}
 
 template<typename T>
 __device__ __forceinline__ uint4 packed(const float (&y)[16 / sizeof(T)]) {
@@ -89,6 +100,86 @@ __device__ __forceinline__ void loadFloats(float (&f)[VEC], const float* p, int 
   }
 }
 
+// What a thread of a unit is.
+template<int VEC>
+struct SlabThread {
+  int unit, tt, row, col;
+  int b, r, c1, groups;  // its item, run, first channel and groups
+  int channel;           // its own first channel in the run
+  int at, skip;          // see Window
+  bool live, on;         // (units of the last workgroup that have no work go along)
+  __device__ __forceinline__ SlabThread(const NormArgs& a, const NormSlab& s) {
+    unit = s.units == 1 ? 0 : threadIdx.x >> 6;
+    tt = threadIdx.x - unit * s.threads;
+    row = tt / s.cols;
+    col = tt - row * s.cols;
+    const unsigned id = xcdContiguousTile() * s.units + unit;
+    live = id < (unsigned)s.launched;
+    const unsigned mine = live ? id : s.launched - 1;
+    const unsigned item = mine / (unsigned)s.runs;
+    b = s.firstItem + (int)item;
+    r = (int)(mine - item * s.runs);
+    c1 = r * s.run;
+    groups = min(s.run / a.per, a.groups - c1 / a.per);
+    channel = col * VEC;
+    on = row < s.rowLanes && channel < min(s.run, a.channels - c1);
+    const Window<VEC> win(c1 + channel, a.channels);
+    at = win.at;
+    skip = win.skip;
+  }
+  // f(j, q) for its channels j and their groups q in the run.
+  template<typename F>
+  __device__ __forceinline__ void eachGroup(const NormArgs& a, F&& f) const {
+    int q = channel / a.per, rest = channel - q * a.per;
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      f(j, min(q, groups - 1));
+      rest += j >= skip ? 1 : 0;
+      if(rest >= a.per) {
+        rest = 0;
+        q++;
+      }
+    }
+  }
+};
+
+// The positions that take part, in order, then the others: list[0..positions). Returns
+// how many take part. Threads of a unit; a barrier has to follow.
+__device__ __forceinline__ int listPositions(const NormArgs& a, const NormSlab& s, int b, int tt, int len, unsigned short* list) {
+  __shared__ int found[2][16];
+  constexpr int AHEAD = 4;
+  const uint8_t* mask = a.mask + b * a.maskB;
+  const int lane = tt & 63, wave = tt >> 6, waves = s.threads >> 6;
+  int count = 0, turn = 0;
+  for(int from = 0; from < a.positions; from += AHEAD * s.threads) {
+    uint8_t m[AHEAD];
+#pragma unroll
+    for(int i = 0; i < AHEAD; i++) m[i] = mask[min(from + i * s.threads + tt, a.positions - 1)];
+#pragma unroll
+    for(int i = 0; i < AHEAD; i++) {
+      const int p = from + i * s.threads + tt;
+      if(from + i * s.threads >= a.positions) break;
+      const bool on = p < len && m[i] != 0;
+      const unsigned long long bits = __ballot(on);
+      int before = 0, all = __popcll(bits);
+      if(s.units == 1) {
+        if(lane == 0) found[turn][wave] = all;
+        __syncthreads();
+        all = 0;
+        for(int w = 0; w < waves; w++) {
+          before += w < wave ? found[turn][w] : 0;
+          all += found[turn][w];
+        }
+        turn ^= 1;
+      }
+      const int at = count + before + __popcll(bits & ((1ull << lane) - 1));
+      if(p < a.positions) list[on ? at : a.positions - 1 - (p - at)] = (unsigned short)p;
+      count += all;
+    }
+  }
+  return count;
+}
+
 // A unit's pairs of sums [rowLanes][entries], added over the rows in `segments` runs:
 // [segments][entries] behind them (the rows themselves where there is one).
 __device__ __forceinline__ const float2* addRows(float2* part, const NormSlab& s, int tt) {
@@ -105,6 +196,26 @@ __device__ __forceinline__ const float2* addRows(float2* part, const NormSlab& s
     red[i] = v;
   }
   return red;
+}
+
+// f(pair, entry of the run) of this thread's part of group q.
+template<typename F>
+__device__ __forceinline__ void eachEntry(const float2* red, const NormSlab& s, int q, int tt, F&& f) {
+  int seg = 0, e = tt & ((1 << s.lanesLog) - 1);
+  if(e >= s.groupEntries) {
+    seg = e / s.groupEntries;
+    e -= seg * s.groupEntries;
+  }
+  while(seg < s.segments) {
+    const int at = q * s.groupEntries + e;
+    f(red[seg * s.entries + at], at);
+    seg += s.stepSegments;
+    e += s.stepEntries;
+    if(e >= s.groupEntries) {
+      e -= s.groupEntries;
+      seg++;
+    }
+  }
 }
 
 // Rows (item, position) of a tensor that is written lie apart.
@@ -130,52 +241,63 @@ NormArgs normArgs(const P& p, float eps) {
                   p.batch, p.positions, p.channels, p.groups, p.channels / p.groups, eps};
 }
 
+__host__ __device__ __forceinline__ int listBytes(int positions) { return (positions * 2 + 15) / 16 * 16; }
 inline unsigned normGrid(int64_t blocks) { return (unsigned)std::min<int64_t>(blocks, NORM_MAX_GRID); }
 
 // Launches f(slab, grid, threads, bytes of LDS) for all units.
 template<typename F>
-void forUnits(NormSlab s, F&& f) {
-  for(s.first = 0; s.first < s.count; s.first += (int64_t)NORM_MAX_GRID * s.units)
-    f(s, normGrid((s.count - s.first + s.units - 1) / s.units), (unsigned)(s.threads * s.units), (size_t)s.ldsPairs * 8 * s.units);
+void forUnits(const NormArgs& a, NormSlab s, F&& f) {
+  const int64_t items = std::max<int64_t>(1, (int64_t)NORM_MAX_GRID * s.units / s.runs);
+  for(int64_t item = 0; item < a.batch; item += items) {
+    s.firstItem = (int)item;
+    s.launched = (int)(std::min(items, a.batch - item) * s.runs);
+    s.listAt = s.ldsPairs * 8 * s.units;
+    f(s, (unsigned)((s.launched + s.units - 1) / s.units), (unsigned)(s.threads * s.units),
+      (size_t)s.listAt + (a.mask != nullptr ? (size_t)listBytes(a.positions) * s.units : 0));
+  }
 }
 
-// The layout of a unit's threads: at most `most` positions a thread and `wide` threads;
-// threads is 0 where there is none. Runs of at least `bytes` a row, or (wholeRows) of all
-// channels. perChannel: sums of each channel are wanted. What a group has in LDS beside
-// the sums: `state` pairs.
+// The layout of a unit's threads for items of these sizes: at most `most` positions a
+// thread and `wide` threads; threads is 0 where there is none. Runs of at least `bytes` a
+// row, or (wholeRows) of all channels. perChannel: sums of each channel are wanted. What a
+// group has in LDS beside the sums: `state` pairs.
 inline NormSlab planSlab(int64_t batch, int positions, int channels, int groups, int size, int bytes, bool perChannel, int most, int wide, bool wholeRows,
                          int state) {
   const int vec = 16 / size, per = channels / groups;
   NormSlab none{};
-  if(channels < vec) return none;
+  if(channels < vec || positions > 65536) return none;
   int64_t base = per;
   while(base % vec != 0) base += per;
   int64_t run = wholeRows ? channels : (bytes + base * size - 1) / (base * size) * base;
   if(run > channels) run = channels;
-  for(int nv : {std::min(most, 8), most})
-    for(int threads = 64; threads <= wide; threads += 64) {
-      NormSlab s{};
-      s.run = (int)run;
-      s.runs = (int)((channels + run - 1) / run);
-      s.cols = (int)((run + vec - 1) / vec);
-      s.threads = threads;
-      s.units = threads == 64 ? 4 : 1;
-      s.count = batch * s.runs;
-      if(s.cols > threads) continue;
-      s.rowLanes = std::min(threads / s.cols, positions);
-      s.nv = (positions + s.rowLanes - 1) / s.rowLanes;
-      if(s.nv > nv) continue;
-      s.pv = !perChannel && per % vec == 0 ? 1 : vec;
-      s.entries = s.cols * s.pv;
-      s.segments = s.rowLanes == 1 ? 1 : std::max(1, std::min(s.rowLanes, threads / s.entries));
-      s.ldsPairs = (s.rowLanes == 1 ? 1 : s.rowLanes + s.segments) * s.entries;
-      const int inRun = s.run / per;
-      s.lanes = 64;
-      while(s.lanes > 1 && s.lanes * inRun > threads) s.lanes /= 2;
-      s.ldsPairs += state * inRun;
-      if((int64_t)s.ldsPairs * 8 * s.units > 60000) continue;
-      return s;
-    }
+  // (whole rounds of the four SIMDs: waves that one of them has more of hold the others up)
+  for(int threads : {64, 128, 256, 512, 768, 1024}) {
+    NormSlab s{};
+    if(threads > wide) break;
+    s.run = (int)run;
+    s.runs = (int)((channels + run - 1) / run);
+    s.cols = (int)((run + vec - 1) / vec);
+    s.threads = threads;
+    s.units = threads == 64 ? 4 : 1;
+    s.count = batch * s.runs;
+    if(s.cols > threads) continue;
+    s.rowLanes = std::min(threads / s.cols, positions);
+    s.nv = (positions + s.rowLanes - 1) / s.rowLanes;
+    if(s.nv > most) continue;
+    s.pv = !perChannel && per % vec == 0 ? 1 : vec;
+    s.entries = s.cols * s.pv;
+    s.groupEntries = s.pv == 1 ? per / vec : per;
+    s.segments = s.rowLanes == 1 ? 1 : std::max(1, std::min(s.rowLanes, threads / s.entries));
+    s.ldsPairs = (s.rowLanes == 1 ? 1 : s.rowLanes + s.segments) * s.entries;
+    const int inRun = s.run / per;
+    s.lanesLog = 6;
+    while(s.lanesLog > 0 && (inRun << s.lanesLog) > threads) s.lanesLog--;
+    s.stepSegments = (1 << s.lanesLog) / s.groupEntries;
+    s.stepEntries = (1 << s.lanesLog) - s.stepSegments * s.groupEntries;
+    s.ldsPairs += state * inRun;
+    if(((int64_t)s.ldsPairs * 8 + listBytes(positions)) * s.units > 60000) continue;
+    return s;
+  }
   return none;
 }
 

@@ -111,7 +111,6 @@ void launchQuantize(const kgh_quantize_params& p, hipStream_t stream) {
     if(r.lanes == 0) quantizeRowsLongKernel<T><<<grid, 256, 0, stream>>>(a);
     else if(r.each <= 1) quantizeRowsKernel<T, 1><<<grid, 256, 0, stream>>>(a, r.lanes);
     else if(r.each <= 2) quantizeRowsKernel<T, 2><<<grid, 256, 0, stream>>>(a, r.lanes);
-    else if(r.each <= 3) quantizeRowsKernel<T, 3><<<grid, 256, 0, stream>>>(a, r.lanes);
     else if(r.each <= 4) quantizeRowsKernel<T, 4><<<grid, 256, 0, stream>>>(a, r.lanes);
     else quantizeRowsKernel<T, 8><<<grid, 256, 0, stream>>>(a, r.lanes);
   });

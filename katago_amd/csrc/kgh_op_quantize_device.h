@@ -59,19 +59,19 @@ __device__ __forceinline__ unsigned rowTop(unsigned top, int lanes, unsigned* ld
   return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
 }
 
-// How threads share a row of `groups` 16-byte groups, at most `most` each: the power of
-// two in a wave, or the workgroup of 256, that leaves the fewest idle; lanes is 0 where
-// the row is longer.
+// How threads share a row of `groups` 16-byte groups, at most `most` each: by the fewest
+// a thread that a wave manages with, in the power of two that leaves the fewest threads
+// idle; by a workgroup of 256 above; lanes is 0 where the row is longer.
 struct RowLanes {
   int lanes, each;
 };
 inline RowLanes rowLanes(int groups, int most) {
-  RowLanes best{0, 0};
-  for(int lanes : {64, 32, 16, 8, 256}) {
-    const int each = (groups + lanes - 1) / lanes;
-    if(each <= most && (best.lanes == 0 || lanes * each < best.lanes * best.each)) best = RowLanes{lanes, each};
-  }
-  return best;
+  for(int each = 1; each <= most; each *= 2)
+    for(int lanes : {8, 16, 32, 64})
+      if(lanes * each >= groups) return RowLanes{lanes, each};
+  for(int each = 1; each <= most; each *= 2)
+    if(256 * each >= groups) return RowLanes{256, each};
+  return RowLanes{0, 0};
 }
 
 // Bytes [from, to) of VEC (4 or 8), to p + from and on.
