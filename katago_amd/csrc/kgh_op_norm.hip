@@ -36,9 +36,9 @@ __device__ __forceinline__ GroupSums groupSums(float n, float sum, float squares
   GroupSums r;
   r.next = turn;
   r.again = false;
-  const float m = sum / n;
-  r.mean = turn.ref + m / turn.factor;
-  r.var = fmaf(-m, m, squares / n);
+  const float share = 1.0f / n, m = sum * share;
+  r.mean = fmaf(m, turn.factor == 1.0f ? 1.0f : 1.0f / NORM_SMALL, turn.ref);
+  r.var = fmaf(-m, m, squares * share);
   if(!(fabsf(sum) <= FLT_MAX && squares <= FLT_MAX)) {
     r.var = __builtin_nanf("");
     r.again = turn.factor == 1.0f;
@@ -76,6 +76,8 @@ template<typename T, int ACT, int NV, bool QUANT>
 __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSlabKernel(NormArgs a, NormOut o, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   extern __shared__ float2 lds[];
+  __shared__ int again;  // the last turn that a group needs
+  if(threadIdx.x == 0) again = 0;
   const SlabThread<VEC> th(a, s);
   const int inRun = s.run / a.per;
   float2* part = lds + th.unit * s.ldsPairs;
@@ -84,10 +86,7 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSl
   unsigned short* list = (unsigned short*)((char*)lds + s.listAt) + th.unit * (listBytes(a.positions) / 2);
   const T* x = (const T*)a.x + th.b * a.xB + th.at;
   int count = validLength(a, th.b);  // places that take part
-  if(a.mask != nullptr) {
-    count = listPositions(a, s, th.b, th.tt, count, list);
-    __syncthreads();
-  }
+  if(a.mask != nullptr) count = listPositions(a, th.b, count, list);
   count = __builtin_amdgcn_readfirstlane(count);
   auto position = [&](int place) -> unsigned { return a.mask != nullptr ? list[place] : place; };
   u32x4_t v[NV];
@@ -132,29 +131,24 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSl
   }
   // The groups' mean and deviation by a turn's sums; whether one needs another turn.
   auto finish = [&](int turn) {
-    const float2* red = addRows(part, s, th.tt);
-    if(s.rowLanes > 1) __syncthreads();
     const float n = (float)count * (float)a.per;
-    bool again = false;
     for(int q = th.tt >> s.lanesLog; q < th.groups; q += s.threads >> s.lanesLog) {
-      float sum = 0.0f, squares = 0.0f;
-      eachEntry(red, s, q, th.tt, [&](float2 u, int) {
-        sum += u.x;
-        squares += u.y;
+      float2 sums = make_float2(0.0f, 0.0f);
+      eachEntry(part, s, q, th.tt, [&](float2 u, int) {
+        sums.x += u.x;
+        sums.y += u.y;
       });
-      for(int k = (1 << s.lanesLog) >> 1; k > 0; k >>= 1) {
-        sum += __shfl_xor(sum, k);
-        squares += __shfl_xor(squares, k);
-      }
-      const GroupSums t = groupSums(n, sum, squares, turn == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turn);
-      again |= t.again;
+      sums = addLanes(sums, s.lanesLog);
+      const GroupSums t = groupSums(n, sums.x, sums.y, turn == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turn);
       if((th.tt & ((1 << s.lanesLog) - 1)) == 0) {
         const float rd = reciprocalDeviation(t, a.eps);
         state[q] = make_float2(t.next.ref, t.next.factor);
         result[q] = n == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(t.mean, rd);
+        if(t.again) again = turn + 1;
       }
     }
-    return __syncthreads_or(again);
+    __syncthreads();
+    return again == turn + 1;
   };
   if(finish(0)) {
     // Other turns read x again, from a cache: in the registers' copy they would cost
@@ -265,8 +259,8 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSl
 }
 
 // ---------------------------------------------------------------------------
-// Items that no workgroup's registers hold: their positions in `chunks` of chunkRows,
-// their columns in `blocks` of `cols`, each a workgroup. A part's groups have their
+// Items that no workgroup's registers hold: their positions in `chunks`, their columns in
+// `blocks` of `cols`, each a workgroup. A part's groups have their
 // number of values, mean, sum of squares about it and that sum's factor in
 // parts[item][chunk][block][slot], slot 0 being the block's first group.
 struct NormParts {
@@ -274,7 +268,7 @@ struct NormParts {
   int chunks, chunkRows, blocks, cols, rowLanes, slots, lanes;  // lanes: threads that add up a group
 };
 
-constexpr int PARTS_AHEAD = 8;  // rows of a thread under way
+constexpr int PARTS_AHEAD = 8, APPLY_AHEAD = 8;  // rows of a thread under way
 
 template<typename T>
 __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) {
@@ -293,7 +287,7 @@ __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) 
     const bool on = row < k.rowLanes && nc > 0;
     const int firstGroup = from / a.per, groups = (to - 1) / a.per - firstGroup + 1;
     const int len = validLength(a, b);
-    const int p0 = chunk * k.chunkRows, p1 = min(p0 + k.chunkRows, len);
+    const int step = k.chunks * k.rowLanes;
     const RowGroup<T, false> g((on ? c0 : 0) / VEC, a.channels);
     const T* x = (const T*)a.x + b * a.xB;
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.maskB;
@@ -315,16 +309,16 @@ __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) 
       }
       rows = 0;
       if(on) {
-        for(int p = p0 + row; p < p1; p += PARTS_AHEAD * k.rowLanes) {
+        for(int p = chunk * k.rowLanes + row; p < len; p += PARTS_AHEAD * step) {
           u32x4_t v[PARTS_AHEAD];
           bool take[PARTS_AHEAD];
 #pragma unroll
           for(int i = 0; i < PARTS_AHEAD; i++) {
-            const int q = p + i * k.rowLanes;
-            take[i] = q < p1 && (mask == nullptr || mask[q] != 0);
+            const int q = p + i * step;
+            take[i] = q < len && (mask == nullptr || mask[q] != 0);
           }
 #pragma unroll
-          for(int i = 0; i < PARTS_AHEAD; i++) v[i] = g.load(x + (take[i] ? p + i * k.rowLanes : p) * a.xP);
+          for(int i = 0; i < PARTS_AHEAD; i++) v[i] = g.load(x + (uint64_t)(unsigned)(take[i] ? p + i * step : p) * a.xP);
 #pragma unroll
           for(int i = 0; i < PARTS_AHEAD; i++) {
             rows += take[i] ? 1 : 0;
@@ -442,18 +436,18 @@ __global__ __launch_bounds__(256) void normApplyKernel(NormArgs a, NormOut o, No
       mean[j] = t[0];
       scale[j] *= t[1];
     }
-    for(int p = p0 + row; p < p1; p += PARTS_AHEAD * k.rowLanes) {
-      u32x4_t v[PARTS_AHEAD];
-      bool take[PARTS_AHEAD];
+    for(int p = p0 + row; p < p1; p += APPLY_AHEAD * k.rowLanes) {
+      u32x4_t v[APPLY_AHEAD];
+      bool take[APPLY_AHEAD];
 #pragma unroll
-      for(int i = 0; i < PARTS_AHEAD; i++) {
+      for(int i = 0; i < APPLY_AHEAD; i++) {
         const int q = min(p + i * k.rowLanes, p1 - 1);
         take[i] = q < len && (mask == nullptr || mask[q] != 0);
       }
 #pragma unroll
-      for(int i = 0; i < PARTS_AHEAD; i++) v[i] = g.load(x + (take[i] ? min(p + i * k.rowLanes, p1 - 1) : 0) * a.xP);
+      for(int i = 0; i < APPLY_AHEAD; i++) v[i] = g.load(x + (take[i] ? min(p + i * k.rowLanes, p1 - 1) : 0) * a.xP);
 #pragma unroll
-      for(int i = 0; i < PARTS_AHEAD; i++) {
+      for(int i = 0; i < APPLY_AHEAD; i++) {
         const int q = p + i * k.rowLanes;
         float y[VEC];
         normalise<T, ACT>(y, Values<T>(g.place(v[i])), mean, scale, bias);

@@ -99,20 +99,14 @@ __global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormA
   const T* x = (const T*)a.x + th.b * a.xB + th.at;
   const T* grad = (const T*)k.grad + th.b * k.gB + th.at;
   int count = validLength(a, th.b);
-  if(a.mask != nullptr) {
-    count = listPositions(a, s, th.b, th.tt, count, list);
-    __syncthreads();
-  }
+  if(a.mask != nullptr) count = listPositions(a, th.b, count, list);
   count = __builtin_amdgcn_readfirstlane(count);
-  auto position = [&](int i) -> unsigned {
-    const int place = th.row + i * s.rowLanes;
-    return a.mask != nullptr ? list[min(place, a.positions - 1)] : min(place, a.positions - 1);
-  };
+  auto position = [&](int place) -> unsigned { return a.mask != nullptr ? list[place] : place; };
   u32x4_t v[NV], d[NV];
 #pragma unroll
-  for(int i = 0; i < NV; i++)
-    if(i * s.rowLanes < count) {
-      const uint64_t p = position(i);
+  for(int i = 0, from = 0; i < NV; i++, from += s.rowLanes)
+    if(from < count) {
+      const uint64_t p = position(min(th.row + from, a.positions - 1));
       __builtin_memcpy(&v[i], x + p * a.xP, 16);
       __builtin_memcpy(&d[i], grad + p * k.gP, 16);
     }
@@ -148,52 +142,55 @@ __global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormA
       if(j >= th.skip) p[j - th.skip] = make_float2(s0[j], s1[j]);
   }
   __syncthreads();
-  const float2* red = addRows(part, s, th.tt);
-  if(s.rowLanes > 1) __syncthreads();
-  // Channels' sums for the weight's and bias's gradients.
-  if(th.live)
-    for(int e = th.tt; e < min(s.run, a.channels - th.c1); e += s.threads) {
-      float2 t = red[e];
-      for(int q = 1; q < s.segments; q++) {
-        t.x += red[q * s.entries + e].x;
-        t.y += red[q * s.entries + e].y;
-      }
-      k.sums[(int64_t)th.b * a.channels + th.c1 + e] = t;
-    }
   const float n = (float)count * (float)a.per;
   for(int q = th.tt >> s.lanesLog; q < th.groups; q += s.threads >> s.lanesLog) {
-    float m1 = 0.0f, m2 = 0.0f;
-    eachEntry(red, s, q, th.tt, [&](float2 t, int e) {
+    float2 m = make_float2(0.0f, 0.0f);
+    eachEntry(part, s, q, th.tt, [&](float2 t, int e) {
       const float w = a.weight == nullptr ? 1.0f : a.weight[th.c1 + e];
-      m1 = fmaf(t.x, w, m1);
-      m2 = fmaf(t.y, w, m2);
+      m.x = fmaf(t.x, w, m.x);
+      m.y = fmaf(t.y, w, m.y);
     });
-    for(int w = (1 << s.lanesLog) >> 1; w > 0; w >>= 1) {
-      m1 += __shfl_xor(m1, w);
-      m2 += __shfl_xor(m2, w);
-    }
-    if((th.tt & ((1 << s.lanesLog) - 1)) == 0) means[q] = make_float2(m1 / n, m2 / n);
+    m = addLanes(m, s.lanesLog);
+    if((th.tt & ((1 << s.lanesLog) - 1)) == 0) means[q] = make_float2(m.x / n, m.y / n);
   }
   __syncthreads();
   float2 mean2[VEC];
   th.eachGroup(a, [&](int j, int q) { mean2[j] = means[q]; });
   T* out = (T*)k.out + th.b * k.oB + th.at;
+  const bool stores = th.on && th.live;
+  const int rowLanes = fresh(s.rowLanes);
 #pragma unroll
-  for(int i = 0; i < NV; i++)
-    if(i * s.rowLanes < a.positions) {
-      const int place = th.row + i * s.rowLanes;
+  for(int i = 0, from = 0; i < NV; i++, from += rowLanes)
+    if(from < a.positions) {
+      const int place = th.row + from;
       uint4 w = make_uint4(0, 0, 0, 0);
-      if(i * s.rowLanes < count) {
+      if(from < count) {
         renew(v[i]);
         const Values<T> xv(v[i]);
         float y[VEC];
 #pragma unroll
         for(int j = 0; j < VEC; j++) y[j] = backwardX(u[i][j], (xv.f[j] - mean[j]) * rstd[j], weight[j], rstd[j], mean2[j]);
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        w = place < count ? packed<T>(y) : zero;
+        w = packed<T>(y);
+        if(from + rowLanes > count && place >= count) w = make_uint4(0, 0, 0, 0);
       }
-      if(th.on && th.live && place < a.positions) storeWindow(out + (uint64_t)position(i) * k.oP, w, th.skip);
+      if(stores && place < a.positions) {
+        T* p = out + (uint64_t)position(place) * k.oP;
+        if(a.channels % VEC == 0) __builtin_memcpy(p, &w, 16);
+        else storeWindow(p, w, th.skip);
+      }
       __builtin_amdgcn_sched_barrier(0);
+    }
+  // Channels' sums, for the weight's and bias's gradients.
+  if(th.live)
+    for(int e = th.tt; e < min(s.run, a.channels - th.c1); e += s.threads) {
+      float2 t = part[e];
+#pragma unroll 8
+      for(int r = 1; r < s.rowLanes; r++) {
+        const float2 w = part[r * s.entries + e];
+        t.x += w.x;
+        t.y += w.y;
+      }
+      k.sums[(int64_t)th.b * a.channels + th.c1 + e] = t;
     }
 }
 

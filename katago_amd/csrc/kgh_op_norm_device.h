@@ -32,11 +32,10 @@ __device__ __forceinline__ int validLength(const NormArgs& a, int b) {
 // row + rowLanes, ..., `nv` of them, in the list of the item's positions that begins
 // with those that take part. `units` units share a workgroup.
 // Sums go through LDS as pairs: `pv` a column (one where a group is whole columns, else
-// one a channel), `entries` = cols pv a row; `segments` runs of rows are added first,
-// then a group's entries by 2^lanesLog threads, whose steps over the runs' entries are
-// stepSegments runs and stepEntries entries.
+// one a channel), `entries` = cols pv a row; a group's are added by 2^lanesLog threads,
+// whose steps are stepRows rows and stepEntries entries.
 struct NormSlab {
-  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, segments, groupEntries, lanesLog, stepSegments, stepEntries;
+  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, groupEntries, lanesLog, stepRows, stepEntries;
   int ldsPairs;  // a unit's LDS, in pairs of floats: sums, then groups' state
   int listAt;    // its list of positions (16 bits each) behind the pairs of all units, in bytes; only where there is a mask
   int64_t count;             // of units
@@ -144,76 +143,83 @@ struct SlabThread {
 };
 
 // The positions that take part, in order, then the others: list[0..positions). Returns
-// how many take part. Threads of a unit; a barrier has to follow.
-__device__ __forceinline__ int listPositions(const NormArgs& a, const NormSlab& s, int b, int tt, int len, unsigned short* list) {
-  __shared__ int found[2][16];
-  constexpr int AHEAD = 4;
+// how many take part. Every wave of a unit writes the whole list by itself, the same
+// numbers in the same places, so that it need not wait for another one to read it.
+__device__ __forceinline__ int listPositions(const NormArgs& a, int b, int len, unsigned short* list) {
+  constexpr int AHEAD = 8;
   const uint8_t* mask = a.mask + b * a.maskB;
-  const int lane = tt & 63, wave = tt >> 6, waves = s.threads >> 6;
-  int count = 0, turn = 0;
-  for(int from = 0; from < a.positions; from += AHEAD * s.threads) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for(int from = 0; from < a.positions; from += 64 * AHEAD) {
     uint8_t m[AHEAD];
 #pragma unroll
-    for(int i = 0; i < AHEAD; i++) m[i] = mask[min(from + i * s.threads + tt, a.positions - 1)];
+    for(int i = 0; i < AHEAD; i++) m[i] = mask[min(from + i * 64 + lane, a.positions - 1)];
 #pragma unroll
     for(int i = 0; i < AHEAD; i++) {
-      const int p = from + i * s.threads + tt;
-      if(from + i * s.threads >= a.positions) break;
+      const int p = from + i * 64 + lane;
+      if(from + i * 64 >= a.positions) break;
       const bool on = p < len && m[i] != 0;
       const unsigned long long bits = __ballot(on);
-      int before = 0, all = __popcll(bits);
-      if(s.units == 1) {
-        if(lane == 0) found[turn][wave] = all;
-        __syncthreads();
-        all = 0;
-        for(int w = 0; w < waves; w++) {
-          before += w < wave ? found[turn][w] : 0;
-          all += found[turn][w];
-        }
-        turn ^= 1;
-      }
-      const int at = count + before + __popcll(bits & ((1ull << lane) - 1));
+      const int at = count + __popcll(bits & ((1ull << lane) - 1));
       if(p < a.positions) list[on ? at : a.positions - 1 - (p - at)] = (unsigned short)p;
-      count += all;
+      count += __popcll(bits);
     }
   }
+  asm volatile("" ::: "memory");  // a wave's LDS accesses run in order
   return count;
 }
 
-// A unit's pairs of sums [rowLanes][entries], added over the rows in `segments` runs:
-// [segments][entries] behind them (the rows themselves where there is one).
-__device__ __forceinline__ const float2* addRows(float2* part, const NormSlab& s, int tt) {
-  if(s.rowLanes == 1) return part;
-  float2* red = part + s.rowLanes * s.entries;
-  for(int i = tt; i < s.entries * s.segments; i += s.threads) {
-    const int seg = i / s.entries, e = i - seg * s.entries;
-    float2 v = make_float2(0.0f, 0.0f);
-    for(int r = seg; r < s.rowLanes; r += s.segments) {
-      const float2 u = part[r * s.entries + e];
-      v.x += u.x;
-      v.y += u.y;
-    }
-    red[i] = v;
+// The sum of v over the 2^log threads side by side that share it, for all of them: within
+// sixteen by rotations, without LDS.
+__device__ __forceinline__ float rotated(float v, std::integral_constant<int, 8>) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true)); }
+__device__ __forceinline__ float rotated(float v, std::integral_constant<int, 4>) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, true)); }
+__device__ __forceinline__ float rotated(float v, std::integral_constant<int, 2>) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, true)); }
+__device__ __forceinline__ float rotated(float v, std::integral_constant<int, 1>) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, true)); }
+__device__ __forceinline__ float2 addLanes(float2 v, int log) {
+  if(log >= 4) {
+    const auto add = [&](auto n) {
+      v.x += rotated(v.x, n);
+      v.y += rotated(v.y, n);
+    };
+    add(std::integral_constant<int, 8>());
+    add(std::integral_constant<int, 4>());
+    add(std::integral_constant<int, 2>());
+    add(std::integral_constant<int, 1>());
   }
-  return red;
+  else
+    for(int k = (1 << log) >> 1; k > 0; k >>= 1) {
+      v.x += __shfl_xor(v.x, k);
+      v.y += __shfl_xor(v.y, k);
+    }
+  if(log >= 5) {
+    v.x += __shfl_xor(v.x, 16);
+    v.y += __shfl_xor(v.y, 16);
+  }
+  if(log >= 6) {
+    v.x += __shfl_xor(v.x, 32);
+    v.y += __shfl_xor(v.y, 32);
+  }
+  return v;
 }
 
-// f(pair, entry of the run) of this thread's part of group q.
+// f(pair, entry of the run) of this thread's part of group q: of a unit's pairs of sums
+// [rowLanes][entries].
 template<typename F>
-__device__ __forceinline__ void eachEntry(const float2* red, const NormSlab& s, int q, int tt, F&& f) {
-  int seg = 0, e = tt & ((1 << s.lanesLog) - 1);
+__device__ __forceinline__ void eachEntry(const float2* part, const NormSlab& s, int q, int tt, F&& f) {
+  int row = 0, e = tt & ((1 << s.lanesLog) - 1);
   if(e >= s.groupEntries) {
-    seg = e / s.groupEntries;
-    e -= seg * s.groupEntries;
+    row = e / s.groupEntries;
+    e -= row * s.groupEntries;
   }
-  while(seg < s.segments) {
+#pragma unroll 4
+  while(row < s.rowLanes) {
     const int at = q * s.groupEntries + e;
-    f(red[seg * s.entries + at], at);
-    seg += s.stepSegments;
+    f(part[row * s.entries + at], at);
+    row += s.stepRows;
     e += s.stepEntries;
     if(e >= s.groupEntries) {
       e -= s.groupEntries;
-      seg++;
+      row++;
     }
   }
 }
@@ -287,13 +293,12 @@ inline NormSlab planSlab(int64_t batch, int positions, int channels, int groups,
     s.pv = !perChannel && per % vec == 0 ? 1 : vec;
     s.entries = s.cols * s.pv;
     s.groupEntries = s.pv == 1 ? per / vec : per;
-    s.segments = s.rowLanes == 1 ? 1 : std::max(1, std::min(s.rowLanes, threads / s.entries));
-    s.ldsPairs = (s.rowLanes == 1 ? 1 : s.rowLanes + s.segments) * s.entries;
+    s.ldsPairs = s.rowLanes * s.entries;
     const int inRun = s.run / per;
     s.lanesLog = 6;
     while(s.lanesLog > 0 && (inRun << s.lanesLog) > threads) s.lanesLog--;
-    s.stepSegments = (1 << s.lanesLog) / s.groupEntries;
-    s.stepEntries = (1 << s.lanesLog) - s.stepSegments * s.groupEntries;
+    s.stepRows = (1 << s.lanesLog) / s.groupEntries;
+    s.stepEntries = (1 << s.lanesLog) - s.stepRows * s.groupEntries;
     s.ldsPairs += state * inRun;
     if(((int64_t)s.ldsPairs * 8 + listBytes(positions)) * s.units > 60000) continue;
     return s;
