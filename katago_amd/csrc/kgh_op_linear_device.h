@@ -160,9 +160,14 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
 // over the step's border too: the barrier stands before a step's last part, whose
 // fragments every wave then holds. The buffers are arrays of their own, so that the
 // compiler does not make a fragment read wait for a load in flight to another one.
+// early(column tile's first column, this wave's row and column) is called while the
+// first steps' loads are under way; a barrier follows before the loop.
 // Returns whether this wave has a block of the result, at row m and column n.
-template<typename T, int WM, int WN, int KW, int RB, int CB, typename Acc>
-__device__ __forceinline__ bool dmaTile(const LinearArgs& a, int rowTiles, int colTiles, Acc (&acc)[RB][CB], int& m, int& n) {
+struct NothingEarly {
+  __device__ __forceinline__ void operator()(int, int, int) const {}
+};
+template<typename T, int WM, int WN, int KW, int RB, int CB, typename Acc, typename Early = NothingEarly>
+__device__ __forceinline__ bool dmaTile(const LinearArgs& a, int rowTiles, int colTiles, Acc (&acc)[RB][CB], int& m, int& n, Early early = Early()) {
   typedef typename Vec16<T>::V V;
   constexpr int SIZE = (int)sizeof(T), VEC = 16 / SIZE, STEP = 128 / SIZE;
   constexpr int WAVES = WM * WN * KW, PARTS = 4 / KW;  // a wave's 32-byte parts of a step
@@ -274,6 +279,7 @@ __device__ __forceinline__ bool dmaTile(const LinearArgs& a, int rowTiles, int c
   };
   load(B0(), 0);
   load(B1(), 1);
+  early(n0, m0 + wm, n0 + wn);
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrierNoFence();
   read(a0s, b0s, 0, f);

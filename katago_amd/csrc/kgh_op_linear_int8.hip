@@ -28,12 +28,18 @@ __device__ __forceinline__ u32x4_t loadBytes(const int8_t* p, int n) {
   return v;
 }
 
-// A sum's value: one rounding of its own, two of the products.
-__device__ __forceinline__ float scaled(int sum, float x, float w) { return (float)sum * x * w; }
+// A sum's value with its bias: the sum's conversion, a product, and a product and sum
+// rounded once, in every kernel (the compiler would else round some of them to 16 bits
+// without the 32 between, and a call's bits would depend on its workspace).
+__device__ __forceinline__ float scaled(int sum, float x, float w, float bias) {
+  float v = fmaf((float)sum * x, w, bias);
+  asm("" : "+v"(v));
+  return v;
+}
 
 // storeTile of sums: by their scales, or as they are where K is split.
 template<typename T, int RB, int CB, int ACT>
-__device__ __forceinline__ void storeSums(const LinearArgs& a, const Scales& s, const intx16 (&sums)[RB][CB], int m, int n) {
+__device__ __forceinline__ void storeSums(LinearArgs a, const Scales& s, const intx16 (&sums)[RB][CB], int m, int n) {
   const int lane = threadIdx.x & 63, laneRow = lane & 31, half = lane >> 5;
   floatx16 acc[RB][CB];
   if(a.part != nullptr) {
@@ -50,16 +56,70 @@ __device__ __forceinline__ void storeSums(const LinearArgs& a, const Scales& s, 
     for(int j = 0; j < CB; j++)
 #pragma unroll
       for(int q = 0; q < 4; q++) {
-        const int c = n + j * 32 + q * 8 + half * 4;
-        const uint4 u = loadGroupSmall(s.w + min(c, a.N - 1), c < a.N ? a.N - c : 1);
-        const floatx4 w = *(const floatx4*)&u;
+        const int c = n + j * 32 + q * 8 + half * 4, at = min(c, a.N - 1), count = c < a.N ? a.N - c : 1;
+        const uint4 u = loadGroupSmall(s.w + at, count);
+        const uint4 v = a.bias != nullptr ? loadGroupSmall(a.bias + at, count) : make_uint4(0, 0, 0, 0);
+        const floatx4 w = *(const floatx4*)&u, b = *(const floatx4*)&v;
 #pragma unroll
         for(int i = 0; i < RB; i++)
 #pragma unroll
-          for(int e = 0; e < 4; e++) acc[i][j][4 * q + e] = scaled(sums[i][j][4 * q + e], x[i], w[e]);
+          for(int e = 0; e < 4; e++) acc[i][j][4 * q + e] = scaled(sums[i][j][4 * q + e], x[i], w[e], b[e]);
       }
+    a.bias = nullptr;
   }
   storeTile<T, RB, CB, ACT>(a, acc, m, n);
+}
+
+// What a wave's block of the result needs beside the sums, for blocks that lie inside it
+// (in 16 bits): loaded while the first steps are under way, the columns' scales and biases
+// into LDS.
+template<typename T, int RB, int CB>
+struct EarlyLoads {
+  float x[RB];
+  u32x4_t residual[RB][CB][2];
+};
+
+// Two groups of four columns to the 16 bytes of the same columns, as finishGroup.
+template<typename T, int ACT, bool RES>
+__device__ __forceinline__ uint4 finishSums(const int (&s0)[4], const int (&s1)[4], float x, floatx4 w0, floatx4 w1, floatx4 b0, floatx4 b1, u32x4_t res) {
+  union Four {
+    uint2 v;
+    T e[4];
+  } ra[2], oa[2];
+  if constexpr(RES) {
+    const uint2 r01 = swapHalves(res.x, res.z), r23 = swapHalves(res.y, res.w);
+    ra[0].v = make_uint2(r01.x, r23.x);
+    ra[1].v = make_uint2(r01.y, r23.y);
+  }
+#pragma unroll
+  for(int e = 0; e < 4; e++) {
+    const float v0 = activate<T, ACT>(scaled(s0[e], x, w0[e], b0[e])), v1 = activate<T, ACT>(scaled(s1[e], x, w1[e], b1[e]));
+    oa[0].e[e] = (T)(RES ? v0 + (float)ra[0].e[e] : v0);
+    oa[1].e[e] = (T)(RES ? v1 + (float)ra[1].e[e] : v1);
+  }
+  const uint2 o01 = swapHalves(oa[0].v.x, oa[1].v.x), o23 = swapHalves(oa[0].v.y, oa[1].v.y);
+  return make_uint4(o01.x, o23.x, o01.y, o23.y);
+}
+
+// columns: scales of this wave's columns, their biases BN behind them.
+template<typename T, int RB, int CB, int ACT, bool RES, int BN>
+__device__ __forceinline__ void storeInside(const LinearArgs& a, const intx16 (&sums)[RB][CB], const EarlyLoads<T, RB, CB>& early, const float* columns, int m, int n) {
+  const int lane = threadIdx.x & 63, laneRow = lane & 31, half = lane >> 5;
+  T* out = (T*)a.out + (int64_t)(m + laneRow) * a.ldo + n;
+#pragma unroll
+  for(int j = 0; j < CB; j++)
+#pragma unroll
+    for(int p = 0; p < 2; p++) {
+      const float* c = columns + j * 32 + p * 16 + half * 4;
+      const floatx4 w0 = *(const floatx4*)c, w1 = *(const floatx4*)(c + 8), b0 = *(const floatx4*)(c + BN), b1 = *(const floatx4*)(c + BN + 8);
+#pragma unroll
+      for(int i = 0; i < RB; i++) {
+        const intx16& t = sums[i][j];
+        const int s0[4] = {t[8 * p], t[8 * p + 1], t[8 * p + 2], t[8 * p + 3]}, s1[4] = {t[8 * p + 4], t[8 * p + 5], t[8 * p + 6], t[8 * p + 7]};
+        const uint4 o = finishSums<T, ACT, RES>(s0, s1, early.x[i], w0, w1, b0, b1, RES ? early.residual[i][j][p] : u32x4_t{0, 0, 0, 0});
+        __builtin_memcpy(out + (int64_t)i * 32 * a.ldo + j * 32 + (2 * p + half) * 8, &o, 16);
+      }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -68,7 +128,44 @@ template<typename T, int WM, int WN, int RB, int CB, int PER_CU, int ACT>
 __global__ __launch_bounds__(64 * WM * WN, PER_CU * WM * WN / 4) void linear8DmaKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
   intx16 acc[RB][CB];
   int m, n;
-  if(dmaTile<int8_t, WM, WN, 1, RB, CB>(a, rowTiles, colTiles, acc, m, n)) storeSums<T, RB, CB, ACT>(a, s, acc, m, n);
+  // (blocks of more registers leave no room for what is loaded early)
+  if constexpr(sizeof(T) == 2 && RB * CB <= 4) {
+    constexpr int BN = 32 * CB * WN;
+    __shared__ __attribute__((aligned(16))) float columns[2 * BN];  // scales, biases
+    const int lane = threadIdx.x & 63, laneRow = lane & 31, half = lane >> 5;
+    EarlyLoads<T, RB, CB> early;
+    int column = 0;
+    bool inside = false;
+    dmaTile<int8_t, WM, WN, 1, RB, CB>(a, rowTiles, colTiles, acc, m, n, [&](int n0, int row, int col) {
+      inside = a.part == nullptr && row + 32 * RB <= a.M && col + 32 * CB <= a.N;
+      column = col - n0;
+#pragma unroll
+      for(int i = 0; i < RB; i++) early.x[i] = s.x[min(row + i * 32 + laneRow, a.M - 1)];
+      if(inside && a.residual != nullptr) {
+        const T* res = (const T*)a.residual + (int64_t)(row + laneRow) * a.ldr + col;
+#pragma unroll
+        for(int i = 0; i < RB; i++)
+#pragma unroll
+          for(int j = 0; j < CB; j++)
+#pragma unroll
+            for(int p = 0; p < 2; p++) __builtin_memcpy(&early.residual[i][j][p], res + (int64_t)i * 32 * a.ldr + j * 32 + (2 * p + half) * 8, 16);
+      }
+      for(int c = threadIdx.x; c < BN; c += 64 * WM * WN) {
+        const int at = min(n0 + c, a.N - 1);
+        columns[c] = s.w[at];
+        columns[BN + c] = a.bias != nullptr ? a.bias[at] : 0.0f;
+      }
+    });
+    if(inside) {
+      if(a.residual != nullptr) storeInside<T, RB, CB, ACT, true, BN>(a, acc, early, columns + column, m, n);
+      else storeInside<T, RB, CB, ACT, false, BN>(a, acc, early, columns + column, m, n);
+    }
+    else storeSums<T, RB, CB, ACT>(a, s, acc, m, n);
+  }
+  else {
+    dmaTile<int8_t, WM, WN, 1, RB, CB>(a, rowTiles, colTiles, acc, m, n);
+    storeSums<T, RB, CB, ACT>(a, s, acc, m, n);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -240,7 +337,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, 
       ((int*)a.part)[((int64_t)blockIdx.y * a.M + m) * a.N + n] = sum;
       continue;
     }
-    float v = activate<T, ACT>(scaled(sum, s.x[m], s.w[n]) + (a.bias != nullptr ? a.bias[n] : 0.0f));
+    float v = activate<T, ACT>(scaled(sum, s.x[m], s.w[n], a.bias != nullptr ? a.bias[n] : 0.0f));
     if(a.residual != nullptr) v += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n];
     ((T*)a.out)[(int64_t)m * a.ldo + n] = (T)v;
   }
@@ -268,7 +365,7 @@ __global__ __launch_bounds__(256) void linear8JoinKernel(LinearArgs a, Scales s,
 #pragma unroll
   for(int j = 0; j < 4; j++) {
     if(j >= count) break;
-    float y = activate<T, ACT>(scaled(v[j], x, s.w[n + j]) + (a.bias != nullptr ? a.bias[n + j] : 0.0f));
+    float y = activate<T, ACT>(scaled(v[j], x, s.w[n + j], a.bias != nullptr ? a.bias[n + j] : 0.0f));
     if(a.residual != nullptr) y += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n + j];
     ((T*)a.out)[(int64_t)m * a.ldo + n + j] = (T)y;
   }
@@ -310,7 +407,7 @@ Linear8Plan planLinear8(const kgh_linear_int8_params& p, bool aligned, uint64_t 
     plan.kernel = LIN8_SKINNY;
     if(K >= 12288) most = std::min<int64_t>(256 / ((p.out_channels + 15) / 16), K / 4096);
   }
-  else if(aligned && K >= 1024 && big * 10 >= (big + 255) / 256 * 256 * 7) plan.kernel = LIN8_DMA_256;
+  else if(aligned && K >= 2048 && big * 10 >= (big + 255) / 256 * 256 * 7) plan.kernel = LIN8_DMA_256;
   else if(tiles(128) >= 224) plan.kernel = aligned ? LIN8_DMA_128 : LIN8_TILE_128;
   else {
     plan.kernel = aligned ? LIN8_DMA_64 : LIN8_TILE_64;
