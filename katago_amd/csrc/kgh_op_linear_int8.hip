@@ -13,18 +13,26 @@ struct Scales {
   const float* w;
 };
 
-// Bytes [0, n) of the 16 at p, zeros behind them.
-__device__ __forceinline__ u32x4_t loadBytes(const int8_t* p, int n) {
+// Bytes [k, end) of a row, up to 16 of them, zeros behind them: 16 bytes that lie in the
+// row wherever it ends, moved to their places.
+__device__ __forceinline__ u32x4_t loadBytes(const int8_t* row, int k, int end) {
   u32x4_t v = {0, 0, 0, 0};
-  if(n >= 16) __builtin_memcpy(&v, p, 16);
-  else
+  if(end >= 16) {
+    const int at = min(k, end - 16), excess = min(k - at, 16);
+    __builtin_memcpy(&v, row + at, 16);
+    if(excess & 8) v = u32x4_t{v[2], v[3], 0, 0};
+    if(excess & 4) v = u32x4_t{v[1], v[2], v[3], 0};
+    const unsigned n = excess & 3;
+    v = u32x4_t{__builtin_amdgcn_alignbyte(v[1], v[0], n), __builtin_amdgcn_alignbyte(v[2], v[1], n), __builtin_amdgcn_alignbyte(v[3], v[2], n), v[3] >> (8 * n)};
+    return excess >= 16 ? u32x4_t{0, 0, 0, 0} : v;
+  }
 #pragma unroll 1
-    for(int j = 0; j < 16; j++) {  // byte j enters at the top and moves down to its place
-      v[0] = __builtin_amdgcn_alignbit(v[1], v[0], 8);
-      v[1] = __builtin_amdgcn_alignbit(v[2], v[1], 8);
-      v[2] = __builtin_amdgcn_alignbit(v[3], v[2], 8);
-      v[3] = v[3] >> 8 | (j < n ? (unsigned)(uint8_t)p[j] << 24 : 0);
-    }
+  for(int j = 0; j < 16; j++) {  // byte j enters at the top and moves down to its place
+    v[0] = __builtin_amdgcn_alignbit(v[1], v[0], 8);
+    v[1] = __builtin_amdgcn_alignbit(v[2], v[1], 8);
+    v[2] = __builtin_amdgcn_alignbit(v[3], v[2], 8);
+    v[3] = v[3] >> 8 | (k + j < end ? (unsigned)(uint8_t)row[k + j] << 24 : 0);
+  }
   return v;
 }
 
@@ -186,17 +194,17 @@ __global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s,
   const int whole = (kEnd - kBegin) / STEP;
   // Thread t loads group t & 7 of rows t >> 3, + 32, ...
   const int lr = tid >> 3, lg = tid & 7;
-  const int8_t* src[LOADS];
+  const int8_t* src[LOADS];  // the rows' first bytes of this part of K
 #pragma unroll
-  for(int i = 0; i < 2 * RB; i++) src[i] = (const int8_t*)a.x + (int64_t)min(m0 + lr + 32 * i, a.M - 1) * a.ldx + kBegin + lg * 16;
+  for(int i = 0; i < 2 * RB; i++) src[i] = (const int8_t*)a.x + (int64_t)min(m0 + lr + 32 * i, a.M - 1) * a.ldx + kBegin;
 #pragma unroll
-  for(int i = 0; i < 2 * CB; i++) src[2 * RB + i] = (const int8_t*)a.w + (int64_t)min(n0 + lr + 32 * i, a.N - 1) * a.ldw + kBegin + lg * 16;
+  for(int i = 0; i < 2 * CB; i++) src[2 * RB + i] = (const int8_t*)a.w + (int64_t)min(n0 + lr + 32 * i, a.N - 1) * a.ldw + kBegin;
   struct Rows {
     u32x4_t v[LOADS];
   };
   // Steps past the last whole one read that one again, into a buffer that nobody reads.
   auto fetch = [&](int step, Rows& r) {
-    const int k = min(step, whole - 1) * STEP;
+    const int k = min(step, whole - 1) * STEP + lg * 16;
 #pragma unroll
     for(int i = 0; i < LOADS; i++) __builtin_memcpy(&r.v[i], src[i] + k, 16);
   };
@@ -248,11 +256,10 @@ __global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s,
     }
     if(at < whole) step(lds0, lds1, r1, r0, at);
   }
-  const int left = kEnd - kBegin - whole * STEP;
-  if(left > 0) {
+  if(kBegin + whole * STEP < kEnd) {
     Rows r;
 #pragma unroll
-    for(int i = 0; i < LOADS; i++) r.v[i] = loadBytes(src[i] + whole * STEP, left - lg * 16);
+    for(int i = 0; i < LOADS; i++) r.v[i] = loadBytes(src[i], whole * STEP + lg * 16, kEnd - kBegin);
     stage(lds0, r);
     barrierLds();
     products(lds0);
@@ -276,9 +283,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, 
   const int8_t* wRow[NT];
   const int8_t* xRow[MT];
 #pragma unroll
-  for(int j = 0; j < NT; j++) wRow[j] = (const int8_t*)a.w + (int64_t)min(n0 + j * 16 + l16, a.N - 1) * a.ldw + quad * 16;
+  for(int j = 0; j < NT; j++) wRow[j] = (const int8_t*)a.w + (int64_t)min(n0 + j * 16 + l16, a.N - 1) * a.ldw;
 #pragma unroll
-  for(int i = 0; i < MT; i++) xRow[i] = (const int8_t*)a.x + (int64_t)min(i * 16 + l16, a.M - 1) * a.ldx + quad * 16;
+  for(int i = 0; i < MT; i++) xRow[i] = (const int8_t*)a.x + (int64_t)min(i * 16 + l16, a.M - 1) * a.ldx;
   intx4 acc[MT][NT];
 #pragma unroll
   for(int i = 0; i < MT; i++)
@@ -292,16 +299,16 @@ __global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, 
     for(int u = 0; u < U; u++)
 #pragma unroll
       for(int p = 0; p < 2; p++) {
-        const int k = k0 + (u * WAVES * 2 + p) * 64;
+        const int k = k0 + (u * WAVES * 2 + p) * 64 + quad * 16;
 #pragma unroll
         for(int j = 0; j < NT; j++) {
           if constexpr(decltype(whole)::value) __builtin_memcpy(&wv[u][p][j], wRow[j] + k, 16);
-          else wv[u][p][j] = loadBytes(wRow[j] + k, kEnd - quad * 16 - k);
+          else wv[u][p][j] = loadBytes(wRow[j], k, kEnd);
         }
 #pragma unroll
         for(int i = 0; i < MT; i++) {
           if constexpr(decltype(whole)::value) __builtin_memcpy(&xv[u][p][i], xRow[i] + k, 16);
-          else xv[u][p][i] = loadBytes(xRow[i] + k, kEnd - quad * 16 - k);
+          else xv[u][p][i] = loadBytes(xRow[i], k, kEnd);
         }
       }
 #pragma unroll

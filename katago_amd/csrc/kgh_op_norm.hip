@@ -59,7 +59,9 @@ __device__ __forceinline__ float reciprocalDeviation(const GroupSums& r, float e
   return (float)(1.0 / sqrt((double)r.var * 0x1p160 + (double)eps));
 }
 
-// (x - mean) / deviation, weight, bias and activation of VEC channels.
+// (x - mean) / deviation, weight, bias and activation of VEC channels. (With the mean in
+// the bias, one operation less, a group of equal values would not be its bias exactly; it
+// was no faster.)
 template<typename T, int ACT, int VEC>
 __device__ __forceinline__ void normalise(float (&y)[VEC], const Values<T>& x, const float (&mean)[VEC], const float (&scale)[VEC], const float (&bias)[VEC]) {
 #pragma unroll
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSl
     const float n = (float)count * (float)a.per;
     for(int q = th.tt >> s.lanesLog; q < th.groups; q += s.threads >> s.lanesLog) {
       float2 sums = make_float2(0.0f, 0.0f);
-      eachEntry(part, s, q, th.tt, [&](float2 u, int) {
+      eachEntry(part, s, s.rowLanes, q, th.tt, [&](float2 u, int) {
         sums.x += u.x;
         sums.y += u.y;
       });
@@ -265,7 +267,7 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSl
 // parts[item][chunk][block][slot], slot 0 being the block's first group.
 struct NormParts {
   float4* parts;
-  int chunks, chunkRows, blocks, cols, rowLanes, slots, lanes;  // lanes: threads that add up a group
+  int chunks, chunkRows, blocks, cols, rowLanes, slots, lanes, pv;  // lanes: threads that add up a group; pv: see NormSlab
 };
 
 constexpr int PARTS_AHEAD = 8, APPLY_AHEAD = 8;  // rows of a thread under way
@@ -335,19 +337,28 @@ __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) 
       }
       if(turns == 0 && on && col == 0 && rows > 0) atomicAdd(&counted, rows);
       if(row < k.rowLanes) {
+        if(k.pv == 1) {
 #pragma unroll
-        for(int j = 0; j < VEC; j++) part[(row * k.cols + col) * VEC + j] = make_float2(s1[j], s2[j]);
+          for(int j = 1; j < VEC; j++) s1[0] += s1[j], s2[0] += s2[j];
+          part[row * k.cols + col] = make_float2(s1[0], s2[0]);
+        }
+        else {
+#pragma unroll
+          for(int j = 0; j < VEC; j++) part[(row * k.cols + col) * VEC + j] = make_float2(s1[j], s2[j]);
+        }
       }
       __syncthreads();
-      // A group's channels in this block, over the rows, by `lanes` threads.
+      // A group's entries in this block, over the rows, by `lanes` threads.
       const int sub = threadIdx.x & (k.lanes - 1);
       bool again = false;
       for(int q = threadIdx.x / k.lanes; q < groups; q += 256 / k.lanes) {
-        const int e0 = max((firstGroup + q) * a.per - from, 0), e1 = min((firstGroup + q + 1) * a.per, to) - from;
+        const int c0 = max((firstGroup + q) * a.per - from, 0), c1 = min((firstGroup + q + 1) * a.per, to) - from;
+        const int e0 = k.pv == 1 ? c0 / VEC : c0, e1 = k.pv == 1 ? c1 / VEC : c1;
         float sum = 0.0f, squares = 0.0f;
+#pragma unroll 4
         for(int i = sub; i < (e1 - e0) * k.rowLanes; i += k.lanes) {
           const int r = i / (e1 - e0);
-          const float2 u = part[r * k.cols * VEC + e0 + (i - r * (e1 - e0))];
+          const float2 u = part[r * k.cols * k.pv + e0 + (i - r * (e1 - e0))];
           sum += u.x;
           squares += u.y;
         }
@@ -355,7 +366,7 @@ __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) 
           sum += __shfl_xor(sum, w);
           squares += __shfl_xor(squares, w);
         }
-        const float n = (float)counted * (float)(e1 - e0);
+        const float n = (float)counted * (float)(c1 - c0);
         const GroupSums t = groupSums(n, sum, squares, turns == 0 ? GroupTurn{0.0f, 1.0f} : GroupTurn{state[q].x, state[q].y}, turns);
         again |= t.again;
         if(sub == 0) {
@@ -369,35 +380,46 @@ __global__ __launch_bounds__(256) void normPartsKernel(NormArgs a, NormParts k) 
 }
 
 // The parts of a group in one: mean, then the squares about it, in 64 bits (numbers are
-// few, and may be any fp32's square). A wave a group of an item.
+// few, and may be any fp32's square). A wave a group of an item; up to 64 JOIN_AHEAD
+// parts are all under way at a time and stay in registers between the two.
+constexpr int JOIN_AHEAD = 8;
+
 __global__ __launch_bounds__(256) void normJoinKernel(NormArgs a, NormParts k, float* stats, int vec) {
   const int lane = threadIdx.x & 63;
   for(int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < (int64_t)a.batch * a.groups; i += (int64_t)gridDim.x * 4) {
     const int b = (int)(i / a.groups), g = (int)(i - (int64_t)b * a.groups);
     const int width = k.cols * vec;
-    const int block0 = g * a.per / width, block1 = ((g + 1) * a.per - 1) / width;
-    const int64_t parts = (int64_t)k.chunks * (block1 - block0 + 1);
+    const int block0 = g * a.per / width, blocks = ((g + 1) * a.per - 1) / width - block0 + 1;
+    const int64_t parts = (int64_t)k.chunks * blocks, first = (int64_t)b * k.chunks;
     auto part = [&](int64_t e) {
-      const int chunk = (int)(e / (block1 - block0 + 1)), block = block0 + (int)(e - (int64_t)chunk * (block1 - block0 + 1));
-      return k.parts[(((int64_t)b * k.chunks + chunk) * k.blocks + block) * k.slots + g - block * width / a.per];
+      const int64_t chunk = blocks == 1 ? e : e / blocks;
+      const int block = block0 + (int)(e - chunk * blocks);
+      return k.parts[((first + chunk) * k.blocks + block) * k.slots + g - block * width / a.per];
     };
+    float4 v[JOIN_AHEAD];
+#pragma unroll
+    for(int q = 0; q < JOIN_AHEAD; q++) v[q] = lane + 64 * q < parts ? part(lane + 64 * q) : make_float4(0.0f, 0.0f, 0.0f, 1.0f);
     double n = 0.0, sum = 0.0, squares = 0.0;
-    for(int64_t e = lane; e < parts; e += 64) {
-      const float4 v = part(e);
-      n += v.x;
-      sum += (double)v.x * v.y;
-    }
+    const auto add = [&](float4 t) {
+      n += t.x;
+      sum += (double)t.x * t.y;
+    };
+#pragma unroll
+    for(int q = 0; q < JOIN_AHEAD; q++) add(v[q]);
+    for(int64_t e = lane + 64 * JOIN_AHEAD; e < parts; e += 64) add(part(e));
 #pragma unroll
     for(int w = 32; w > 0; w >>= 1) {
       n += __shfl_xor(n, w);
       sum += __shfl_xor(sum, w);
     }
     const double mean = n == 0.0 ? 0.0 : sum / n;
-    for(int64_t e = lane; e < parts; e += 64) {
-      const float4 v = part(e);
-      const double d = v.y - mean;
-      squares += v.x == 0.0f ? 0.0 : v.x * ((v.w == 1.0f ? (double)v.z : v.z * 0x1p160) + d * d);
-    }
+    const auto square = [&](float4 t) {
+      const double d = t.y - mean;
+      squares += t.x == 0.0f ? 0.0 : t.x * ((t.w == 1.0f ? (double)t.z : t.z * 0x1p160) + d * d);
+    };
+#pragma unroll
+    for(int q = 0; q < JOIN_AHEAD; q++) square(v[q]);
+    for(int64_t e = lane + 64 * JOIN_AHEAD; e < parts; e += 64) square(part(e));
 #pragma unroll
     for(int w = 32; w > 0; w >>= 1) squares += __shfl_xor(squares, w);
     if(lane == 0) {
@@ -465,6 +487,7 @@ __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, in
   __shared__ unsigned tops[2][R][4];
   const int sub = threadIdx.x & (lanes - 1), row = threadIdx.x / lanes, rows = 256 / lanes;
   const int groups = (a.channels + VEC - 1) / VEC;
+  const bool whole = a.channels % VEC == 0;  // no thread has part of a group
   for(int64_t id = blockIdx.x; id < (int64_t)a.batch * chunks; id += gridDim.x) {
     const int b = (int)(id / chunks), chunk = (int)(id - (int64_t)b * chunks);
     const int len = validLength(a, b);
@@ -478,11 +501,16 @@ __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, in
       const int c0 = (sub + i * lanes) * VEC, nc = a.channels - c0;
       loadFloats(scale[i], a.weight == nullptr ? nullptr : a.weight + c0, nc, 1.0f);
       loadFloats(bias[i], a.bias == nullptr ? nullptr : a.bias + c0, nc, 0.0f);
+      int q = c0 / a.per, rest = c0 - q * a.per;
 #pragma unroll
       for(int j = 0; j < VEC; j++) {
-        const float* t = o.stats + 2 * ((int64_t)b * a.groups + min(c0 + j, a.channels - 1) / a.per);
-        mean[i][j] = t[0];
-        scale[i][j] *= t[1];
+        const float2 t = *(const float2*)(o.stats + 2 * ((int64_t)b * a.groups + min(q, a.groups - 1)));
+        mean[i][j] = t.x;
+        scale[i][j] *= t.y;
+        if(++rest == a.per) {
+          rest = 0;
+          q++;
+        }
       }
     }
     int turn = 0;
@@ -507,9 +535,11 @@ __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, in
 #pragma unroll
         for(int i = 0; i < K; i++) {
           const int nc = a.channels - (sub + i * lanes) * VEC;
+          const unsigned before = top;
           normalise<T, ACT>(y[i], Values<T>(RowGroup<T, false>(min(sub + i * lanes, groups - 1), a.channels).place(v[r][i])), mean[i], scale[i], bias[i]);
 #pragma unroll
-          for(int j = 0; j < VEC; j++) top = max(top, j < nc ? magnitudeBits(y[i][j]) : 0);
+          for(int j = 0; j < VEC; j++) top = max(top, whole || j < nc ? magnitudeBits(y[i][j]) : 0);
+          if(whole && nc <= 0) top = before;
         }
         top = rowTop(take[r] ? top : 0, lanes, tops[turn][r]);
         const RowScale rs(top);
@@ -545,7 +575,7 @@ __global__ __launch_bounds__(256) void normQuantLongKernel(NormArgs a, NormOut o
     if(take)
       for(int c = threadIdx.x; c < a.channels; c += 256) top = max(top, magnitudeBits(value(c)));
     const RowScale rs(rowTop(top, 256, tops));
-    for(int c = threadIdx.x; c < a.channels; c += 256) out[c] = (int8_t)(take ? rs.quantized(value(c)) : 0);
+    for(int c = threadIdx.x; c < a.channels; c += 256) out[c] = (int8_t)(take ? rs.quantized(value(c)) & 0xff : 0);
     if(threadIdx.x == 0) o.scales[i] = rs.scale;
     __syncthreads();
   }
@@ -588,6 +618,7 @@ NormPlan planNorm(const kgh_group_norm_params& p) {
   k.chunkRows = (int)std::min<int64_t>(p.positions, (rows + PARTS_AHEAD - 1) / PARTS_AHEAD * PARTS_AHEAD * k.rowLanes);
   k.chunks = (p.positions + k.chunkRows - 1) / k.chunkRows;
   k.slots = (k.cols * vec + per - 2) / per + 1;
+  k.pv = per % vec == 0 ? 1 : vec;
   k.lanes = 64;
   while(k.lanes > 1 && k.lanes * k.slots > 256) k.lanes /= 2;
   plan.partsBytes = (uint64_t)p.batch * k.chunks * k.blocks * k.slots * sizeof(float4);
@@ -624,7 +655,7 @@ void launchNorm(const NormPlan& plan, const NormArgs& a, NormOut o, void* worksp
     if(r.lanes == 0) normQuantLongKernel<T, ACT><<<normGrid((int64_t)a.batch * a.positions), 256, 0, stream>>>(a, o);
     else {
       const int rows = 256 / r.lanes * (r.each == 1 ? 2 : 1);
-      const int chunkRows = (int)std::min<int64_t>((int64_t)a.positions, std::max<int64_t>(1, (int64_t)a.batch * a.positions / rows / 2048) * rows);
+      const int chunkRows = (int)std::min<int64_t>((int64_t)a.positions, std::max<int64_t>(1, (int64_t)a.batch * a.positions / rows / 1280) * rows);
       const int chunks = (a.positions + chunkRows - 1) / chunkRows;
       const unsigned g = normGrid((int64_t)a.batch * chunks);
       if(r.each == 1) normQuantKernel<T, ACT, 1, 2><<<g, 256, 0, stream>>>(a, o, r.lanes, chunks, chunkRows);

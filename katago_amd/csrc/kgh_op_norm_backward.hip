@@ -51,7 +51,7 @@ struct NormBackArgs {
   int64_t oB, oP;
   float* gradWeight;
   float* gradBias;
-  float2* sums;  // [batch][channels]: of u and u h over an item's positions
+  float2* sums;  // [item or slice][channels]: of u and u h
 };
 
 // u (the gradient behind the activation) and h (the normalised input) of VEC channels.
@@ -86,7 +86,8 @@ struct BackChannels {
 
 // ---------------------------------------------------------------------------
 // An item's run of channels in a unit's registers, as in the forward pass: x as it came
-// and u in fp32 (its slope is most of the work, and is computed once).
+// and u in fp32 (its slope is most of the work, and is computed once). sums has a row for
+// each item.
 template<typename T, int ACT, int NV>
 __global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormArgs a, NormBackArgs k, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -142,10 +143,24 @@ __global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormA
       if(j >= th.skip) p[j - th.skip] = make_float2(s0[j], s1[j]);
   }
   __syncthreads();
+  // The rows' sums in `segments` parts, which are kept for the weight's and bias's gradients.
+  float2* red = part + s.rowLanes * s.entries;
+  for(int i = th.tt; i < s.segments * s.entries; i += s.threads) {
+    const int seg = i / s.entries, e = i - seg * s.entries;
+    float2 t = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for(int r = seg; r < s.rowLanes; r += s.segments) {
+      const float2 w = part[r * s.entries + e];
+      t.x += w.x;
+      t.y += w.y;
+    }
+    red[i] = t;
+  }
+  __syncthreads();
   const float n = (float)count * (float)a.per;
   for(int q = th.tt >> s.lanesLog; q < th.groups; q += s.threads >> s.lanesLog) {
     float2 m = make_float2(0.0f, 0.0f);
-    eachEntry(part, s, q, th.tt, [&](float2 t, int e) {
+    eachEntry(red, s, s.segments, q, th.tt, [&](float2 t, int e) {
       const float w = a.weight == nullptr ? 1.0f : a.weight[th.c1 + e];
       m.x = fmaf(t.x, w, m.x);
       m.y = fmaf(t.y, w, m.y);
@@ -180,15 +195,12 @@ __global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormA
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-  // Channels' sums, for the weight's and bias's gradients.
   if(th.live)
     for(int e = th.tt; e < min(s.run, a.channels - th.c1); e += s.threads) {
-      float2 t = part[e];
-#pragma unroll 8
-      for(int r = 1; r < s.rowLanes; r++) {
-        const float2 w = part[r * s.entries + e];
-        t.x += w.x;
-        t.y += w.y;
+      float2 t = red[e];
+      for(int r = 1; r < s.segments; r++) {
+        t.x += red[r * s.entries + e].x;
+        t.y += red[r * s.entries + e].y;
       }
       k.sums[(int64_t)th.b * a.channels + th.c1 + e] = t;
     }
@@ -300,6 +312,103 @@ __global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackA
   }
 }
 
+// Many items of few positions, a thread one: a workgroup has a run of channels of every
+// `slices`-th item, and its channels' sums in registers all the while; sums has a row for
+// each slice (a row for each item would be as many bytes as the tensors).
+template<typename T, int ACT>
+__global__ __launch_bounds__(512) void normBackItemsKernel(NormArgs a, NormBackArgs k, NormSlab s, int slices) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ float2 lds[];
+  const int run = blockIdx.x % s.runs, slice = blockIdx.x / s.runs;
+  const int row = threadIdx.x / s.cols, col = threadIdx.x - row * s.cols;
+  const int c1 = run * s.run, channel = col * VEC;
+  const int groups = min(s.run / a.per, a.groups - c1 / a.per);
+  const bool on = row < s.rowLanes && channel < min(s.run, a.channels - c1);
+  const Window<VEC> win(c1 + channel, a.channels);
+  float2* part = lds;
+  float2* means = part + s.ldsPairs - s.run / a.per;
+  float weight[VEC], bias[VEC], all0[VEC], all1[VEC];
+  int group[VEC];
+  loadFloats(weight, a.weight == nullptr ? nullptr : a.weight + win.at, VEC, 1.0f);
+  loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + win.at, VEC, 0.0f);
+#pragma unroll
+  for(int j = 0; j < VEC; j++) {
+    all0[j] = all1[j] = 0.0f;
+    group[j] = min((channel + max(j - win.skip, 0)) / a.per, groups - 1);
+  }
+  for(int b = slice; b < a.batch; b += slices) {
+    const int len = validLength(a, b);
+    const T* x = (const T*)a.x + b * a.xB + win.at;
+    const T* grad = (const T*)k.grad + b * k.gB + win.at;
+    int count = len;
+    if(a.mask != nullptr) {
+      count = 0;
+      for(int p = 0; p < len; p++) count += a.mask[b * a.maskB + p] != 0 ? 1 : 0;
+    }
+    const int p = min(row, a.positions - 1);
+    const bool take = row < len && (a.mask == nullptr || a.mask[b * a.maskB + p] != 0);
+    u32x4_t v, d;
+    __builtin_memcpy(&v, x + (uint64_t)(unsigned)p * a.xP, 16);
+    __builtin_memcpy(&d, grad + (uint64_t)(unsigned)p * k.gP, 16);
+    const float* stats = k.stats + 2 * ((int64_t)b * a.groups + c1 / a.per);
+    float mean[VEC], rstd[VEC], u[VEC], h[VEC];
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      mean[j] = stats[2 * group[j]];
+      rstd[j] = stats[2 * group[j] + 1];
+    }
+    backward<T, ACT>(u, h, Values<T>(v), Values<T>(d), mean, rstd, weight, bias);
+    __syncthreads();  // the item before has read its means
+    float2 m = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for(int j = 0; j < VEC; j++) {
+      const float s0 = take ? u[j] : 0.0f, s1 = take ? u[j] * h[j] : 0.0f;
+      all0[j] += s0;
+      all1[j] += s1;
+      if(s.pv == 1) {
+        m.x = fmaf(s0, weight[j], m.x);
+        m.y = fmaf(s1, weight[j], m.y);
+      }
+      else if(on && j >= win.skip) part[row * s.entries + channel + j - win.skip] = make_float2(s0 * weight[j], s1 * weight[j]);
+    }
+    if(s.pv == 1 && on) part[row * s.entries + col] = m;
+    __syncthreads();
+    const float n = (float)count * (float)a.per;
+    const int lanes = 1 << s.lanesLog, sub = threadIdx.x & (lanes - 1);
+    for(int q = threadIdx.x >> s.lanesLog; q < groups; q += s.threads >> s.lanesLog) {
+      float2 t = make_float2(0.0f, 0.0f);
+      eachEntry(part, s, s.rowLanes, q, threadIdx.x, [&](float2 w, int) {
+        t.x += w.x;
+        t.y += w.y;
+      });
+      t = addLanes(t, s.lanesLog);
+      if(sub == 0) means[q] = make_float2(t.x / n, t.y / n);
+    }
+    __syncthreads();
+    T* out = (T*)k.out + b * k.oB + win.at;
+    float y[VEC];
+#pragma unroll
+    for(int j = 0; j < VEC; j++) y[j] = take ? backwardX(u[j], h[j], weight[j], rstd[j], means[group[j]]) : 0.0f;
+    if(on && row < a.positions) storeWindow(out + (uint64_t)(unsigned)row * k.oP, packed<T>(y), win.skip);
+  }
+  // The channels' sums over the rows of threads.
+  for(int turn = 0; turn < s.rowLanes; turn++) {
+    __syncthreads();
+    if(row == turn && on) {
+#pragma unroll
+      for(int j = 0; j < VEC; j++)
+        if(j >= win.skip) {
+          float2& t = k.sums[(int64_t)slice * a.channels + c1 + channel + j - win.skip];
+          if(turn == 0) t = make_float2(all0[j], all1[j]);
+          else {
+            t.x += all0[j];
+            t.y += all1[j];
+          }
+        }
+    }
+  }
+}
+
 // The chunks' sums of an item's group: its channels' sums and its means. Threads are
 // (chunk slice, channel); channels of long groups in turns.
 __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackArgs k, BackParts s) {
@@ -321,7 +430,7 @@ __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackAr
       const int ch = g * a.per + from + c;
       float2 t = make_float2(0.0f, 0.0f);
       if(on)
-#pragma unroll 4
+#pragma unroll 8
         for(int q = slice; q < s.chunks; q += slices) {
           const float2 v = s.parts[((int64_t)b * s.chunks + q) * a.channels + ch];
           t.x += v.x;
@@ -356,32 +465,34 @@ __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackAr
   }
 }
 
-// The items' sums: the gradients of weight and bias. 32 channels a workgroup.
-__global__ __launch_bounds__(256) void normBackWeightsKernel(NormArgs a, NormBackArgs k) {
-  __shared__ float2 part[256];
+// The items' (or slices') sums: the gradients of weight and bias. 32 channels a workgroup;
+// rows may be many, so in 64 bits.
+__global__ __launch_bounds__(1024) void normBackWeightsKernel(NormBackArgs k, int channels, int rows) {
+  __shared__ double2 part[1024];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-  float2 t = make_float2(0.0f, 0.0f);
-  if(c < a.channels)
+  double2 t = make_double2(0.0, 0.0);
+  if(c < channels)
 #pragma unroll 8
-    for(int b = slice; b < a.batch; b += 8) {
-      const float2 v = k.sums[(int64_t)b * a.channels + c];
+    for(int b = slice; b < rows; b += 32) {
+      const float2 v = k.sums[(int64_t)b * channels + c];
       t.x += v.x;
       t.y += v.y;
     }
   part[threadIdx.x] = t;
   __syncthreads();
-  if(slice != 0 || c >= a.channels) return;
-#pragma unroll
-  for(int q = 1; q < 8; q++) {
+  if(slice != 0 || c >= channels) return;
+#pragma unroll 8
+  for(int q = 1; q < 32; q++) {
     t.x += part[q * 32 + threadIdx.x].x;
     t.y += part[q * 32 + threadIdx.x].y;
   }
-  if(k.gradBias != nullptr) k.gradBias[c] = t.x;
-  if(k.gradWeight != nullptr) k.gradWeight[c] = t.y;
+  if(k.gradBias != nullptr) k.gradBias[c] = (float)t.x;
+  if(k.gradWeight != nullptr) k.gradWeight[c] = (float)t.y;
 }
 
 struct NormBackPlan {
   NormSlab slab;  // threads 0: parts
+  int slices;     // 0: a row of sums for each item
   BackParts parts;
   uint64_t sumsBytes, partsBytes, countsBytes, meansBytes;
 };
@@ -390,6 +501,17 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
   const int size = (int)kgh::opElemBytes(p.dtype), vec = 16 / size;
   const auto round16 = [](uint64_t n) { return (n + 15) / 16 * 16; };
   NormBackPlan plan{};
+  // 8192 x 1 x 4096 bf16, one group: 321 us with a row of sums for each item.
+  if(p.positions <= 4 && p.batch >= 1024) {
+    plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 1024, false, 1, 512, false, 1);
+    if(plan.slab.threads != 0) {
+      // At most 64 items a slice, sums' terms one after the other, where the launch has room.
+      const int64_t most = std::max<int64_t>(1, NORM_MAX_GRID / plan.slab.runs);
+      plan.slices = (int)std::min(most, std::max<int64_t>(std::max(1, 1024 / plan.slab.runs), p.batch / 64));
+      plan.sumsBytes = round16((uint64_t)plan.slices * p.channels * 8);
+      return plan;
+    }
+  }
   plan.sumsBytes = round16((uint64_t)p.batch * p.channels * 8);
   const auto slab = [&](int bytes, int most, int wide) {
     if(plan.slab.threads == 0) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, bytes, true, most, wide, false, 1);
@@ -416,6 +538,12 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
 
 template<typename T, int ACT>
 void launchBackward(const NormBackPlan& plan, const NormArgs& a, const NormBackArgs& k, hipStream_t stream) {
+  if(plan.slices > 0) {
+    const NormSlab& s = plan.slab;
+    normBackItemsKernel<T, ACT><<<(unsigned)(plan.slices * s.runs), (unsigned)s.threads, (size_t)s.ldsPairs * 8, stream>>>(a, k, s, plan.slices);
+    KGH_CHECK_LAUNCH();
+    return;
+  }
   if(plan.slab.threads != 0) {
     forUnits(a, plan.slab, [&](const NormSlab& s, unsigned grid, unsigned threads, size_t bytes) {
       if(s.nv <= 2) normBackSlabKernel<T, ACT, 2><<<grid, threads, bytes, stream>>>(a, k, s);
@@ -475,18 +603,19 @@ uint64_t groupNormBackwardWorkspace(const kgh_group_norm_backward_params& p) {
 }
 
 void launchGroupNormBackward(const kgh_group_norm_backward_params& p, hipStream_t stream) {
-  NormArgs a = normArgs(p, 0.0f);
+  const NormArgs a = normArgs(p, 0.0f);
   const NormBackArgs k{p.grad_out, p.grad_out_batch_stride, p.grad_out_position_stride, p.statistics, p.grad_x, p.grad_x_batch_stride,
                        p.grad_x_position_stride, p.grad_weight, p.grad_bias, (float2*)p.workspace};
+  int rows = 0;  // of sums; without any the gradients of weight and bias are zeros
   if(p.batch > 0 && p.positions > 0) {
     const NormBackPlan plan = planBackward(p);
+    rows = plan.slices > 0 ? std::min(plan.slices, p.batch) : p.batch;
     withDtype(p.dtype, [&](auto t) {
       withActivation(p.activation, [&](auto act) { launchBackward<decltype(t), decltype(act)::value>(plan, a, k, stream); });
     });
   }
-  else a.batch = 0;  // no sums: the gradients of weight and bias are zeros
   if(p.grad_weight == nullptr && p.grad_bias == nullptr) return;
-  normBackWeightsKernel<<<dim3((unsigned)((p.channels + 31) / 32)), 256, 0, stream>>>(a, k);
+  normBackWeightsKernel<<<dim3((unsigned)((p.channels + 31) / 32)), 1024, 0, stream>>>(k, p.channels, rows);
   KGH_CHECK_LAUNCH();
 }
 

@@ -33,9 +33,10 @@ __device__ __forceinline__ int validLength(const NormArgs& a, int b) {
 // with those that take part. `units` units share a workgroup.
 // Sums go through LDS as pairs: `pv` a column (one where a group is whole columns, else
 // one a channel), `entries` = cols pv a row; a group's are added by 2^lanesLog threads,
-// whose steps are stepRows rows and stepEntries entries.
+// whose steps are stepRows rows and stepEntries entries; where channels' sums are wanted,
+// `segments` threads add up the rows of an entry before that.
 struct NormSlab {
-  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, groupEntries, lanesLog, stepRows, stepEntries;
+  int threads, units, run, runs, cols, rowLanes, nv, pv, entries, segments, groupEntries, lanesLog, stepRows, stepEntries;
   int ldsPairs;  // a unit's LDS, in pairs of floats: sums, then groups' state
   int listAt;    // its list of positions (16 bits each) behind the pairs of all units, in bytes; only where there is a mask
   int64_t count;             // of units
@@ -202,17 +203,17 @@ __device__ __forceinline__ float2 addLanes(float2 v, int log) {
   return v;
 }
 
-// f(pair, entry of the run) of this thread's part of group q: of a unit's pairs of sums
-// [rowLanes][entries].
+// f(pair, entry of the run) of this thread's part of group q: of pairs of sums
+// [rows][entries].
 template<typename F>
-__device__ __forceinline__ void eachEntry(const float2* part, const NormSlab& s, int q, int tt, F&& f) {
+__device__ __forceinline__ void eachEntry(const float2* part, const NormSlab& s, int rows, int q, int tt, F&& f) {
   int row = 0, e = tt & ((1 << s.lanesLog) - 1);
   if(e >= s.groupEntries) {
     row = e / s.groupEntries;
     e -= row * s.groupEntries;
   }
 #pragma unroll 4
-  while(row < s.rowLanes) {
+  while(row < rows) {
     const int at = q * s.groupEntries + e;
     f(part[row * s.entries + at], at);
     row += s.stepRows;
@@ -293,7 +294,8 @@ inline NormSlab planSlab(int64_t batch, int positions, int channels, int groups,
     s.pv = !perChannel && per % vec == 0 ? 1 : vec;
     s.entries = s.cols * s.pv;
     s.groupEntries = s.pv == 1 ? per / vec : per;
-    s.ldsPairs = s.rowLanes * s.entries;
+    s.segments = std::min(std::max(threads / s.entries, 1), s.rowLanes);
+    s.ldsPairs = (s.rowLanes + (perChannel ? s.segments : 0)) * s.entries;
     const int inRun = s.run / per;
     s.lanesLog = 6;
     while(s.lanesLog > 0 && (inRun << s.lanesLog) > threads) s.lanesLog--;

@@ -45,14 +45,29 @@ struct RowScale {
     factor = none ? 0.0f : __fdiv_rn(127.0f, t);
     scale = top >= QUANT_INFINITE_BITS ? __builtin_nanf("") : none ? 0.0f : __fdiv_rn(t, 127.0f);
   }
-  // 0 where the factor is: also of infinities and NaN.
-  __device__ __forceinline__ int quantized(float v) const { return factor == 0.0f ? 0 : (int)rintf(v * factor); }
+  // The whole number nearest to v's product with the factor, in the lowest byte: of that
+  // number and 1.5 * 2^23, whose steps are 1 (of NaN, which an infinity becomes too where
+  // the factor is 0, that byte is 0).
+  __device__ __forceinline__ unsigned quantized(float v) const {
+    float p = v * factor;
+    asm("" : "+v"(p));  // rounded by itself
+    return __float_as_uint(p + 12582912.0f);
+  }
 };
 
 // The largest of a row that `lanes` threads side by side have (a power of two up to 64,
 // or a workgroup of 256, whose waves meet in lds).
 __device__ __forceinline__ unsigned rowTop(unsigned top, int lanes, unsigned* lds) {
-  for(int w = min(lanes, 64) >> 1; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
+  if(lanes >= 16) {  // within sixteen threads by rotations
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xf, 0xf, true));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x124, 0xf, 0xf, true));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x122, 0xf, 0xf, true));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x121, 0xf, 0xf, true));
+    if(lanes >= 32) top = max(top, (unsigned)__shfl_xor((int)top, 16));
+    if(lanes >= 64) top = max(top, (unsigned)__shfl_xor((int)top, 32));
+  }
+  else
+    for(int w = lanes >> 1; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
   if(lanes <= 64) return top;
   if((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
   __syncthreads();
@@ -93,7 +108,11 @@ template<int VEC>
 __device__ __forceinline__ uint2 quantized(const float (&y)[VEC], const RowScale& s) {
   unsigned w[2] = {0, 0};
 #pragma unroll
-  for(int j = 0; j < VEC; j++) w[j >> 2] |= (unsigned)(s.quantized(y[j]) & 0xff) << (8 * (j & 3));
+  for(int j = 0; j < VEC; j += 4) {
+    const unsigned low = __builtin_amdgcn_perm(s.quantized(y[j + 1]), s.quantized(y[j]), 0x0c0c0400);
+    const unsigned high = __builtin_amdgcn_perm(s.quantized(y[j + 3]), s.quantized(y[j + 2]), 0x04000c0c);
+    w[j >> 2] = low | high;
+  }
   return make_uint2(w[0], w[1]);
 }
 

@@ -161,7 +161,7 @@ def test_linear_int8_sizes(dtype, m, k, n):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("pad,shift", [(16, 0), (1, 0), (0, 1), (3, 5), (8, 8), (16, 4)])
-@pytest.mark.parametrize("m,k,n", [(5, 80, 40), (40, 160, 264), (70, 208, 96), (1800, 150, 1900), (1800, 160, 1900)], ids=ids)
+@pytest.mark.parametrize("m,k,n", [(5, 80, 40), (40, 160, 264), (70, 208, 96), (1800, 150, 1900), (1800, 160, 1900), (3, 15, 20), (90, 11, 70), (90, 131, 70), (9, 149, 40)], ids=ids)
 def test_linear_int8_strides(dtype, pad, shift, m, k, n):
     x, w = _bytes(m, k, pad=pad, shift=shift), _bytes(n, k, seed=1, pad=pad, shift=shift)
     xs, ws = torch.rand(m, device="cuda"), torch.rand(n, device="cuda") * 1e-3
@@ -525,6 +525,33 @@ def test_backward_strides(dtype, pad, shift, p, c, groups):
     check(_backward(x, dy, stats, dx, groups, activation="gelu"), want)
     one = dy[:1, :1].expand(3, p, c)  # a gradient that is the same everywhere, as of a sum
     check(_backward(x, one, stats, dx, groups, activation="gelu"), ref.group_norm_backward(x, one, stats, groups, act="gelu")[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("kind", ["none", "lengths", "both"])
+@pytest.mark.parametrize("b,p,c,groups", [(1024, 1, 384, 1), (5003, 1, 40, 5), (1500, 4, 33, 3), (2000, 3, 1000, 8), (1027, 2, 2048, 1), (70001, 1, 24, 1), (1100, 1, 9000, 3),
+                                          (1031, 4, 7, 7), (1030, 1, 4000, 1000)], ids=ids)
+def test_backward_of_many_items(dtype, kind, b, p, c, groups):
+    """Items of a few positions, whose sums a workgroup has for many of them."""
+    lengths, mask = _masks(kind, b, p, _seeded(p, c)) if kind != "none" else (None, None)
+    x, dy = _rand(b, p, c, dtype=dtype, shift=0.3), _rand(b, p, c, dtype=dtype, seed=5, pad=1)
+    w, bias = _rand(c, dtype=torch.float32, seed=1, shift=1.0, scale=0.3), _rand(c, dtype=torch.float32, seed=2)
+    stats = _forward_statistics(x, groups, eps=1e-3, lengths=lengths, mask=mask)
+    want = ref.group_norm_backward(x, dy, stats, groups, w, bias, "gelu", lengths, mask)
+    if kind != "none":
+        on = ref.valid(x, lengths, mask).cuda()
+        x.masked_fill_(~on[..., None], float("nan"))
+        dy.masked_fill_(~on[..., None], float("inf"))
+    dx, untouched = _guarded(b, p, c, dtype=dtype)
+    dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    kw = dict(weight=w, bias=bias, activation="gelu", lengths=lengths, mask=mask)
+    _backward(x, dy, stats, dx, groups, grad_weight=dw, grad_bias=db, **kw)
+    for got, to, what in zip((dx, dw, db), want, ("x", "weight", "bias")):
+        check(got, to, what)
+    untouched()
+    again = torch.empty(c, device="cuda")
+    _backward(x, dy, stats, dx, groups, grad_weight=again, **kw)
+    assert torch.equal(dw, again), "not the same bits again"
 
 
 @pytest.mark.parametrize("act", [a for a in ops.ACTIVATIONS if a != "relu"])
