@@ -72,17 +72,17 @@ class _LinearInt8Params(ctypes.Structure):
 class _GroupNormParams(ctypes.Structure):
     """kgh_group_norm_params."""
     _fields_ = [("dtype", _i32), ("activation", _i32), ("batch", _i32), ("positions", _i32), ("channels", _i32), ("groups", _i32),
-                ("eps", ctypes.c_float), ("x", _ptr), ("x_strides", _i64 * 2), ("weight", _ptr), ("bias", _ptr), ("lengths", _ptr), ("mask", _ptr),
-                ("mask_stride", _i64), ("out", _ptr), ("out_strides", _i64 * 2), ("out_scales", _ptr), ("statistics", _ptr),
+                ("eps", ctypes.c_float), ("x", _ptr), ("x_batch_stride", _i64), ("x_position_stride", _i64), ("weight", _ptr), ("bias", _ptr), ("lengths", _ptr), ("mask", _ptr),
+                ("mask_stride", _i64), ("out", _ptr), ("out_batch_stride", _i64), ("out_position_stride", _i64), ("out_scales", _ptr), ("statistics", _ptr),
                 ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
 
 
 class _GroupNormBackwardParams(ctypes.Structure):
     """kgh_group_norm_backward_params."""
     _fields_ = [("dtype", _i32), ("activation", _i32), ("batch", _i32), ("positions", _i32), ("channels", _i32), ("groups", _i32),
-                ("x", _ptr), ("x_strides", _i64 * 2), ("grad_out", _ptr), ("grad_out_strides", _i64 * 2), ("statistics", _ptr),
-                ("weight", _ptr), ("bias", _ptr), ("lengths", _ptr), ("mask", _ptr), ("mask_stride", _i64), ("grad_x", _ptr),
-                ("grad_x_strides", _i64 * 2), ("grad_weight", _ptr), ("grad_bias", _ptr), ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
+                ("x", _ptr), ("x_batch_stride", _i64), ("x_position_stride", _i64), ("grad_out", _ptr), ("grad_out_batch_stride", _i64),
+                ("grad_out_position_stride", _i64), ("statistics", _ptr), ("weight", _ptr), ("bias", _ptr), ("lengths", _ptr), ("mask", _ptr),
+                ("mask_stride", _i64), ("grad_x", _ptr), ("grad_x_batch_stride", _i64), ("grad_x_position_stride", _i64), ("grad_weight", _ptr), ("grad_bias", _ptr), ("workspace", _ptr), ("workspace_bytes", ctypes.c_uint64)]
 
 
 _CALLS = {"kgh_linear": _LinearParams, "kgh_rope_axes": _RopeParams, "kgh_cross_attention": _AttentionParams, "kgh_quantize_rows": _QuantizeParams,
@@ -195,14 +195,15 @@ def _stream(t, device):
     stream does not wait for, nor it for the null stream."""
     torch = sys.modules.get("torch")
     if torch is not None and isinstance(t, torch.Tensor):
-        return torch.cuda.current_stream(device).cuda_stream
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the same without an object around it
+        return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
     return None
 
 
 def _no_gradients(op, *tensors):
     """Refuses tensors that a result's gradients would be wanted of."""
     for t in tensors:
-        if getattr(t, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
+        if t is not None and getattr(t, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
             _invalid(f"{op}: a tensor requires gradients, and the result would have none (torch.no_grad() takes it)")
 
 
@@ -212,7 +213,7 @@ def _sizes(op, *sizes):
 
 
 def _shape(op, name, t, *want):
-    if tuple(t.shape) != want:
+    if t.shape != want and tuple(t.shape) != want:
         _invalid(f"{op}: {name} has shape {tuple(t.shape)}, not {want}")
 
 
@@ -222,11 +223,15 @@ def _workspace(op, workspace, device):
         return None, 0
     if workspace.get_device() != device:
         _invalid(f"{op}: the workspace is not on the same device as the first tensor")
-    n = 1
-    for size, stride in zip(reversed(workspace.shape), reversed(workspace.stride())):
-        if stride != n and size > 1:
-            _invalid(f"{op}: the workspace is not contiguous")
-        n *= size
+    strides = workspace.stride()
+    if strides == (1,):
+        n = workspace.shape[0]
+    else:
+        n = 1
+        for size, stride in zip(reversed(workspace.shape), reversed(strides)):
+            if stride != n and size > 1:
+                _invalid(f"{op}: the workspace is not contiguous")
+            n *= size
     size = _bytes.get(workspace.dtype)
     if size is None:
         size = _bytes[workspace.dtype] = _BYTES.get(str(workspace.dtype).rsplit(".", 1)[-1], 0)
@@ -464,7 +469,7 @@ def linear_int8(x, x_scales, weights, weight_scales, out, bias=None, activation=
 
 
 def _norm_start(op, x, groups, activation):
-    """What both directions' parameters begin with, and the device."""
+    """What both directions' parameters begin with, x's strides and the device."""
     code, device = _first(op, "x", x)
     xs = _look(op, "x", x, 3, x.dtype, device)
     batch, positions, channels = x.shape
@@ -474,28 +479,31 @@ def _norm_start(op, x, groups, activation):
     act = ACTIVATIONS.get(activation or "identity")
     if act is None:
         _invalid(f"{op}: unknown activation {activation!r}")
-    return (code, act, batch, positions, channels, groups), xs[:2], device
+    return (code, act, batch, positions, channels, groups), xs, device
 
 
-def _norm_inputs(op, p, device, weight, bias, lengths, mask):
-    """The arguments that both directions may have."""
+def _norm_inputs(op, batch, positions, channels, device, weight, bias, lengths, mask):
+    """Pointers of the arguments that both directions may have, the last one's stride."""
+    wp = bp = lp = mp = None
+    ms = 0
     if weight is not None:
         _look(op, "weight", weight, 1, _types[FP32], device)
-        _shape(op, "weight", weight, p.channels)
-        p.weight = weight.data_ptr()
+        _shape(op, "weight", weight, channels)
+        wp = weight.data_ptr()
     if bias is not None:
         _look(op, "bias", bias, 1, _types[FP32], device)
-        _shape(op, "bias", bias, p.channels)
-        p.bias = bias.data_ptr()
+        _shape(op, "bias", bias, channels)
+        bp = bias.data_ptr()
     if lengths is not None:
         _look(op, "lengths", lengths, 1, _types["int32"], device)
-        _shape(op, "lengths", lengths, p.batch)
-        p.lengths = lengths.data_ptr()
+        _shape(op, "lengths", lengths, batch)
+        lp = lengths.data_ptr()
     if mask is not None:
         kind = _code(op, "mask", mask)
-        ms = _look(op, "mask", mask, 2, _types[kind if kind in ("uint8", "bool") else "uint8"], device)
-        _shape(op, "mask", mask, p.batch, p.positions)
-        p.mask, p.mask_stride = mask.data_ptr(), ms[0]
+        ms = _look(op, "mask", mask, 2, _types[kind if kind in ("uint8", "bool") else "uint8"], device)[0]
+        _shape(op, "mask", mask, batch, positions)
+        mp = mask.data_ptr()
+    return wp, bp, lp, mp, ms
 
 
 def _whole(op, name, t, shape, device):
@@ -538,18 +546,18 @@ def group_norm(x, out, groups, weight=None, bias=None, eps=1e-5, activation=None
     1 / sqrt(variance + eps) for ``group_norm_backward``. out may be x itself. workspace:
     at least ``group_norm_workspace`` bytes, of its own for calls that may overlap."""
     start, xs, device = _norm_start("group_norm", x, groups, activation)
-    p = _GroupNormParams(*start, eps, x.data_ptr(), xs)
-    _norm_inputs("group_norm", p, device, weight, bias, lengths, mask)
+    _, _, batch, positions, channels, _ = start
+    inputs = _norm_inputs("group_norm", batch, positions, channels, device, weight, bias, lengths, mask)
+    sp = tp = None
     if out_scales is not None:
-        p.out_scales = _whole("group_norm", "out_scales", out_scales, (p.batch, p.positions), device)
-    p.out_strides = _look("group_norm", "out", out, 3, x.dtype if out_scales is None else _types["int8"], device)[:2]
-    _shape("group_norm", "out", out, p.batch, p.positions, p.channels)
-    p.out = out.data_ptr()
+        sp = _whole("group_norm", "out_scales", out_scales, (batch, positions), device)
+    os = _look("group_norm", "out", out, 3, x.dtype if out_scales is None else _types["int8"], device)
+    _shape("group_norm", "out", out, batch, positions, channels)
     if stats is not None:
-        p.statistics = _whole("group_norm", "stats", stats, (p.batch, groups, 2), device)
+        tp = _whole("group_norm", "stats", stats, (batch, groups, 2), device)
     _no_gradients("group_norm", x, out, weight, bias)
-    if workspace is not None:
-        p.workspace, p.workspace_bytes = _workspace("group_norm", workspace, device)
+    space = _workspace("group_norm", workspace, device)
+    p = _GroupNormParams(*start, eps, x.data_ptr(), xs[0], xs[1], *inputs, out.data_ptr(), os[0], os[1], sp, tp, *space)
     hip_check((_lib or _library()).kgh_group_norm(device, p, _stream(x, device) if stream is None else stream))
     return out
 
@@ -577,20 +585,21 @@ def group_norm_backward(x, grad_out, stats, grad_x, groups, weight=None, bias=No
     ``group_norm_backward_workspace`` bytes, of its own for calls that may overlap."""
     op = "group_norm_backward"
     start, xs, device = _norm_start(op, x, groups, activation)
-    p = _GroupNormBackwardParams(*start, x.data_ptr(), xs)
-    _norm_inputs(op, p, device, weight, bias, lengths, mask)
-    p.grad_out_strides = _look(op, "grad_out", grad_out, 3, x.dtype, device)[:2]
-    p.grad_x_strides = _look(op, "grad_x", grad_x, 3, x.dtype, device)[:2]
-    _shape(op, "grad_out", grad_out, p.batch, p.positions, p.channels)
-    _shape(op, "grad_x", grad_x, p.batch, p.positions, p.channels)
-    p.grad_out, p.grad_x = grad_out.data_ptr(), grad_x.data_ptr()
-    p.statistics = _whole(op, "stats", stats, (p.batch, groups, 2), device)
+    _, _, batch, positions, channels, _ = start
+    inputs = _norm_inputs(op, batch, positions, channels, device, weight, bias, lengths, mask)
+    gs = _look(op, "grad_out", grad_out, 3, x.dtype, device)
+    os = _look(op, "grad_x", grad_x, 3, x.dtype, device)
+    _shape(op, "grad_out", grad_out, batch, positions, channels)
+    _shape(op, "grad_x", grad_x, batch, positions, channels)
+    tp = _whole(op, "stats", stats, (batch, groups, 2), device)
+    wp = bp = None
     if grad_weight is not None:
-        p.grad_weight = _whole(op, "grad_weight", grad_weight, (p.channels,), device)
+        wp = _whole(op, "grad_weight", grad_weight, (channels,), device)
     if grad_bias is not None:
-        p.grad_bias = _whole(op, "grad_bias", grad_bias, (p.channels,), device)
+        bp = _whole(op, "grad_bias", grad_bias, (channels,), device)
     _no_gradients(op, x, grad_out, grad_x, weight, bias, grad_weight, grad_bias)
-    if workspace is not None:
-        p.workspace, p.workspace_bytes = _workspace(op, workspace, device)
+    space = _workspace(op, workspace, device)
+    p = _GroupNormBackwardParams(*start, x.data_ptr(), xs[0], xs[1], grad_out.data_ptr(), gs[0], gs[1], tp, *inputs, grad_x.data_ptr(), os[0], os[1],
+                                 wp, bp, *space)
     hip_check((_lib or _library()).kgh_group_norm_backward(device, p, _stream(x, device) if stream is None else stream))
     return grad_x
