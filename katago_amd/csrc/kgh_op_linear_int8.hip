@@ -311,6 +311,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, 
           else xv[u][p][i] = loadBytes(xRow[i], k, kEnd);
         }
       }
+    __builtin_amdgcn_sched_barrier(0);  // every load before the first product
 #pragma unroll
     for(int u = 0; u < U; u++)
 #pragma unroll
@@ -410,7 +411,15 @@ Linear8Plan planLinear8(const kgh_linear_int8_params& p, bool aligned, uint64_t 
   const int64_t K = p.in_channels, big = tiles(256);
   Linear8Plan plan;
   int64_t most = 1;  // splits worth their sums' way through memory and a second launch
-  if(p.rows <= 64) {
+  const uint64_t one = (uint64_t)p.rows * p.out_channels * 4;
+  // Each workgroup of the kernel for few rows loads all of x: from 17 rows on that costs
+  // more than the weights do, and from some K on more than 64 x 64 tiles in splits with
+  // their join, if there is the workspace for them. us without and with: 64x16384x4096
+  // 39 and 21, 64x8192x1024 21 and 12, 32x8192x1024 13.7 and 11.2, 64x4096x8192 17.7 and
+  // 15.9, 64x8192x30000 112 and 73, but 32x4096x8192 12.1 and 14.2, 17x384x1024 3.5 and 5.1.
+  const int64_t parts = std::min<int64_t>(512 / tiles(64), K / 1024);
+  const bool tiled = aligned && p.rows > 16 && K >= (p.rows > 32 ? 4096 : 8192) && (parts <= 1 || bytes / one >= (uint64_t)(parts + 1) / 2);
+  if(p.rows <= 64 && !tiled) {
     plan.kernel = LIN8_SKINNY;
     if(K >= 12288) most = std::min<int64_t>(256 / ((p.out_channels + 15) / 16), K / 4096);
   }
@@ -418,9 +427,8 @@ Linear8Plan planLinear8(const kgh_linear_int8_params& p, bool aligned, uint64_t 
   else if(tiles(128) >= 224) plan.kernel = aligned ? LIN8_DMA_128 : LIN8_TILE_128;
   else {
     plan.kernel = aligned ? LIN8_DMA_64 : LIN8_TILE_64;
-    if(K >= 4096) most = std::min<int64_t>(512 / tiles(64), K / 1024);
+    if(K >= 4096) most = parts;
   }
-  const uint64_t one = (uint64_t)p.rows * p.out_channels * 4;
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)std::min<uint64_t>(bytes / one, 1024)));
   plan.chunk = (int)((K + splits * 128 - 1) / (splits * 128) * 128);
   plan.splits = (int)((K + plan.chunk - 1) / plan.chunk);

@@ -140,7 +140,7 @@ def test_quantize_far_and_shared_rows():
 
 LINEAR_SIZES = [(1, 1, 1), (1, 384, 1024), (3, 40, 8), (1, 4112, 24), (7, 1000, 72), (16, 256, 64), (17, 272, 40), (31, 8, 33),
                 (33, 528, 129), (64, 64, 64), (65, 96, 257), (100, 33, 31), (129, 72, 63), (200, 1040, 136), (300, 17, 520), (361, 384, 384),
-                (5, 24592, 40), (40, 16384, 24), (70, 8208, 72), (66, 4112, 65), (1900, 144, 1990), (1905, 1040, 6408), (2888, 1024, 384), (4100, 2064, 4128)]
+                (5, 24592, 40), (40, 16384, 24), (64, 8192, 1000), (33, 4096, 200), (17, 8208, 72), (32, 12304, 2100), (33, 4112, 17000), (70, 8208, 72), (66, 4112, 65), (1900, 144, 1990), (1905, 1040, 6408), (2888, 1024, 384), (4100, 2064, 4128)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
@@ -161,7 +161,7 @@ def test_linear_int8_sizes(dtype, m, k, n):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("pad,shift", [(16, 0), (1, 0), (0, 1), (3, 5), (8, 8), (16, 4)])
-@pytest.mark.parametrize("m,k,n", [(5, 80, 40), (40, 160, 264), (70, 208, 96), (1800, 150, 1900), (1800, 160, 1900), (3, 15, 20), (90, 11, 70), (90, 131, 70), (9, 149, 40)], ids=ids)
+@pytest.mark.parametrize("m,k,n", [(5, 80, 40), (40, 160, 264), (70, 208, 96), (1800, 150, 1900), (1800, 160, 1900), (3, 15, 20), (90, 11, 70), (90, 131, 70), (9, 149, 40), (9, 24592, 40), (40, 24593, 24)], ids=ids)
 def test_linear_int8_strides(dtype, pad, shift, m, k, n):
     x, w = _bytes(m, k, pad=pad, shift=shift), _bytes(n, k, seed=1, pad=pad, shift=shift)
     xs, ws = torch.rand(m, device="cuda"), torch.rand(n, device="cuda") * 1e-3
