@@ -30,13 +30,18 @@ __device__ __forceinline__ float slope(float v) {
   }
   else if constexpr(sizeof(T) == 4) return fmaf(0.5f, erfcf(-0.70710678118654752f * v), v * expf(-0.5f * v * v) * 0.39894228040143268f);
   else {
-    // erfc(|v| / sqrt(2)) / 2 as in activateFast, which gives e^(-v^2 / 2) too.
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.435f * 0.70710678118654752f, fabsf(v), 1.0f));
-    float poly = fmaf(t, 0.5f * -0.15086693f, 0.5f * 0.38131212f);
-    poly = fmaf(t, poly, 0.5f * 0.01284851f);
-    poly = fmaf(t, poly, 0.5f * 0.27344433f);
-    poly = fmaf(t, poly, 0.5f * 0.23733569f);
-    poly = fmaf(t, poly, 0.5f * 0.24592536f);
+    // erfc(|v| / sqrt(2)) / 2 = t poly(t) e^(-v^2 / 2), t = 1 / (1 + 0.4 |v| / sqrt(2)), right
+    // to 1.3e-7 of it: the gradients of weight and bias are fp32, so activateFast's 4.2e-6,
+    // which has the same sign in many values, would be seen in their sums.
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.282842712f, fabsf(v), 1.0f));
+    float poly = fmaf(t, 0.025129477f, -0.0914449404f);
+    poly = fmaf(t, poly, 0.0845342149f);
+    poly = fmaf(t, poly, -0.00279735801f);
+    poly = fmaf(t, poly, 0.0707130809f);
+    poly = fmaf(t, poly, 0.084271567f);
+    poly = fmaf(t, poly, 0.103921288f);
+    poly = fmaf(t, poly, 0.112834802f);
+    poly = fmaf(t, poly, 0.112837931f);
     const float e = __builtin_amdgcn_exp2f(v * v * (-0.5f * ACT_LOG2E));
     const float q = t * poly * e;
     return fmaf(v, e * 0.39894228040143268f, v < 0.0f ? q : 1.0f - q);
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackA
 // `slices`-th item, and its channels' sums in registers all the while; sums has a row for
 // each slice (a row for each item would be as many bytes as the tensors).
 template<typename T, int ACT>
-__global__ __launch_bounds__(512) void normBackItemsKernel(NormArgs a, NormBackArgs k, NormSlab s, int slices) {
+__global__ __launch_bounds__(1024) void normBackItemsKernel(NormArgs a, NormBackArgs k, NormSlab s, int slices) {
   constexpr int VEC = 16 / (int)sizeof(T);
   extern __shared__ float2 lds[];
   const int run = blockIdx.x % s.runs, slice = blockIdx.x / s.runs;
@@ -328,15 +333,19 @@ __global__ __launch_bounds__(512) void normBackItemsKernel(NormArgs a, NormBackA
   float2* part = lds;
   float2* means = part + s.ldsPairs - s.run / a.per;
   float weight[VEC], bias[VEC], all0[VEC], all1[VEC];
-  int group[VEC];
+  unsigned pair[VEC / 2];  // channels' groups, 16 bits each: registers are what a second workgroup a CU wants
   loadFloats(weight, a.weight == nullptr ? nullptr : a.weight + win.at, VEC, 1.0f);
   loadFloats(bias, a.bias == nullptr ? nullptr : a.bias + win.at, VEC, 0.0f);
 #pragma unroll
   for(int j = 0; j < VEC; j++) {
     all0[j] = all1[j] = 0.0f;
-    group[j] = min((channel + max(j - win.skip, 0)) / a.per, groups - 1);
+    const unsigned q = min((channel + max(j - win.skip, 0)) / a.per, groups - 1);
+    pair[j / 2] = j & 1 ? pair[j / 2] | q << 16 : q;
   }
+  const auto group = [&](int j) { return j & 1 ? pair[j / 2] >> 16 : pair[j / 2] & 0xffff; };
   for(int b = slice; b < a.batch; b += slices) {
+#pragma unroll
+    for(int i = 0; i < VEC / 2; i++) asm volatile("" : "+v"(pair[i]));  // (else they are taken apart before the loop)
     const int len = validLength(a, b);
     const T* x = (const T*)a.x + b * a.xB + win.at;
     const T* grad = (const T*)k.grad + b * k.gB + win.at;
@@ -354,10 +363,12 @@ __global__ __launch_bounds__(512) void normBackItemsKernel(NormArgs a, NormBackA
     float mean[VEC], rstd[VEC], u[VEC], h[VEC];
 #pragma unroll
     for(int j = 0; j < VEC; j++) {
-      mean[j] = stats[2 * group[j]];
-      rstd[j] = stats[2 * group[j] + 1];
+      const float2 t = ((const float2*)stats)[group(j)];
+      mean[j] = t.x;
+      rstd[j] = t.y;
     }
     backward<T, ACT>(u, h, Values<T>(v), Values<T>(d), mean, rstd, weight, bias);
+    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();  // the item before has read its means
     float2 m = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -388,7 +399,7 @@ __global__ __launch_bounds__(512) void normBackItemsKernel(NormArgs a, NormBackA
     T* out = (T*)k.out + b * k.oB + win.at;
     float y[VEC];
 #pragma unroll
-    for(int j = 0; j < VEC; j++) y[j] = take ? backwardX(u[j], h[j], weight[j], rstd[j], means[group[j]]) : 0.0f;
+    for(int j = 0; j < VEC; j++) y[j] = take ? backwardX(u[j], h[j], weight[j], rstd[j], means[group(j)]) : 0.0f;
     if(on && row < a.positions) storeWindow(out + (uint64_t)(unsigned)row * k.oP, packed<T>(y), win.skip);
   }
   // The channels' sums over the rows of threads.
@@ -501,13 +512,21 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
   const int size = (int)kgh::opElemBytes(p.dtype), vec = 16 / size;
   const auto round16 = [](uint64_t n) { return (n + 15) / 16 * 16; };
   NormBackPlan plan{};
-  // 8192 x 1 x 4096 bf16, one group: 321 us with a row of sums for each item.
-  if(p.positions <= 4 && p.batch >= 1024) {
-    plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 1024, false, 1, 512, false, 1);
+  // Few positions an item: us with a row of sums for each item and with one for a slice
+  // (bf16) 8192 x 1 x 4096 600 and 75, 64 x 1 x 4096 54 and 12, 1024 x 1 x 384 15 and 12,
+  // 1 x 1 x 384 9.2 and 7.2, 4096 x 2 x 256 70 and 21, 1024 x 4 x 384 29 and 20; but
+  // 256 x 4 x 1024 14 and 19, 1024 x 8 x 384 29 and 64.
+  if(p.positions == 1 || (p.positions <= 4 && p.batch >= 1024)) {
+    plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 1024, false, 1, 1024, false, 1);
     if(plan.slab.threads != 0) {
-      // At most 64 items a slice, sums' terms one after the other, where the launch has room.
+      // Slices that fill the card: of 512 threads two a CU (8192 x 1 x 4096 SiLU: 256 slices
+      // 114 us, one workgroup a CU; 512 82), of few threads more (8192 x 1 x 384: 512 38 us,
+      // 1024 27). Of two items at least where there are many (512 x 1 x 4096: 27 us with one,
+      // 20 with two; 64 x 1 x 4096: 12 and 13.5), of at most 64, sums' terms one after the
+      // other, where the launch has room.
+      const int64_t room = std::min(1024, 262144 / plan.slab.threads) / plan.slab.runs;
       const int64_t most = std::max<int64_t>(1, NORM_MAX_GRID / plan.slab.runs);
-      plan.slices = (int)std::min(most, std::max<int64_t>(std::max(1, 1024 / plan.slab.runs), p.batch / 64));
+      plan.slices = (int)std::min(most, std::max<int64_t>({1, std::min<int64_t>(room, p.batch <= 256 ? p.batch : p.batch / 2), p.batch / 64}));
       plan.sumsBytes = round16((uint64_t)plan.slices * p.channels * 8);
       return plan;
     }
@@ -516,8 +535,7 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
   const auto slab = [&](int bytes, int most, int wide) {
     if(plan.slab.threads == 0) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, bytes, true, most, wide, false, 1);
   };
-  const int64_t rowBytes = (int64_t)p.batch * p.channels * size;
-  if(rowBytes <= 512 * 96) slab(96, 2, 512);
+  // us of 128 x 361 x 384 bf16 in 32 groups: runs of 48 bytes 45, of 96 53, in parts 61.
   slab(48, 6, 256);
   slab(48, 6, 512);
   slab(16, 6, 512);
@@ -609,7 +627,7 @@ void launchGroupNormBackward(const kgh_group_norm_backward_params& p, hipStream_
   int rows = 0;  // of sums; without any the gradients of weight and bias are zeros
   if(p.batch > 0 && p.positions > 0) {
     const NormBackPlan plan = planBackward(p);
-    rows = plan.slices > 0 ? std::min(plan.slices, p.batch) : p.batch;
+    rows = plan.slices > 0 ? plan.slices : p.batch;
     withDtype(p.dtype, [&](auto t) {
       withActivation(p.activation, [&](auto act) { launchBackward<decltype(t), decltype(act)::value>(plan, a, k, stream); });
     });

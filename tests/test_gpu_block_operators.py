@@ -530,7 +530,7 @@ def test_backward_strides(dtype, pad, shift, p, c, groups):
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("kind", ["none", "lengths", "both"])
 @pytest.mark.parametrize("b,p,c,groups", [(1024, 1, 384, 1), (5003, 1, 40, 5), (1500, 4, 33, 3), (2000, 3, 1000, 8), (1027, 2, 2048, 1), (70001, 1, 24, 1), (1100, 1, 9000, 3),
-                                          (1031, 4, 7, 7), (1030, 1, 4000, 1000)], ids=ids)
+                                          (1031, 4, 7, 7), (1030, 1, 4000, 1000), (3, 1, 384, 1), (63, 1, 4096, 2), (300, 1, 50, 5), (3, 1, 8200, 1)], ids=ids)
 def test_backward_of_many_items(dtype, kind, b, p, c, groups):
     """Items of a few positions, whose sums a workgroup has for many of them."""
     lengths, mask = _masks(kind, b, p, _seeded(p, c)) if kind != "none" else (None, None)
@@ -552,6 +552,37 @@ def test_backward_of_many_items(dtype, kind, b, p, c, groups):
     again = torch.empty(c, device="cuda")
     _backward(x, dy, stats, dx, groups, grad_weight=again, **kw)
     assert torch.equal(dw, again), "not the same bits again"
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("act", [a for a in ops.ACTIVATIONS if a != "relu"])
+@pytest.mark.parametrize("b,p,c", [(3, 120, 96), (2, 6000, 96), (300, 1, 96)], ids=ids)
+def test_sums_of_slopes(dtype, act, b, p, c):
+    """grad_weight and grad_bias are fp32 whatever x is: 1e-6 of their norm is what rounding
+    in fp32 may cost them (16 roundings of 2^-24 of a term, each of random sign), not what
+    rounding to 16 bits would (2^-11)."""
+    x, dy = _rand(b, p, c, dtype=dtype), _rand(b, p, c, dtype=dtype, seed=5)
+    w, bias = _rand(c, dtype=torch.float32, seed=1, shift=1.0, scale=0.2), _rand(c, dtype=torch.float32, seed=2, scale=0.2)
+    stats, dx = _forward_statistics(x, 8), torch.empty_like(x)
+    dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    _backward(x, dy, stats, dx, 8, weight=w, bias=bias, activation=act, grad_weight=dw, grad_bias=db)
+    want = ref.group_norm_backward(x, dy, stats, 8, w, bias, act)
+    for got, (to, _) in zip((dw, db), want[1:]):
+        to = to.to(got.device).double()
+        assert float((got.double() - to).norm() / to.norm()) < 1e-6
+
+
+@pytest.mark.parametrize("b,p,c,groups", [(3, 20, 24, 3), (2, 9000, 24, 3), (40, 1, 24, 3)], ids=ids)
+def test_statistics_anywhere(b, p, c, groups):
+    """Statistics at an address that no pair of numbers begins at."""
+    x, dy = _rand(b, p, c, dtype=torch.float16, shift=0.3), _rand(b, p, c, dtype=torch.float16, seed=5)
+    stats = torch.empty(b * groups * 2 + 1, device="cuda")[1:].view(b, groups, 2)
+    _norm(x, torch.empty_like(x), groups, stats=stats)
+    there = _forward_statistics(x, groups)
+    assert torch.equal(stats, there)
+    dx, want = torch.empty_like(x), torch.empty_like(x)
+    _backward(x, dy, stats, dx, groups)
+    assert torch.equal(dx, _backward(x, dy, there, want, groups))
 
 
 @pytest.mark.parametrize("act", [a for a in ops.ACTIVATIONS if a != "relu"])
