@@ -131,7 +131,12 @@ __device__ __forceinline__ void storeInside(const LinearArgs& a, const intx16 (&
 }
 
 // ---------------------------------------------------------------------------
-// Rows that are 16-byte aligned: dmaTile's loop, 128 k a step.
+// Rows that are 16-byte aligned: dmaTile's loop, 128 k a step. 8192 x 4096 x 8192 bf16 on
+// 256 x 256 tiles: 277 us, 1987 TOP/s (the library's product, without scales, 267), at
+// the clock that the power limit leaves (1.66 GHz); GELU and a residual add 50, a tile's
+// end which nothing covers on one workgroup a CU. 46208 x 1024 x 384 fp16 with a residual
+// on 128 x 128: 42 us, 2.8 TB/s, a tile's first loads and stores around eight steps; with
+// the epilogue's own loads behind the steps 54.
 template<typename T, int WM, int WN, int RB, int CB, int PER_CU, int ACT>
 __global__ __launch_bounds__(64 * WM * WN, PER_CU * WM * WN / 4) void linear8DmaKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
   intx16 acc[RB][CB];
@@ -179,7 +184,8 @@ __global__ __launch_bounds__(64 * WM * WN, PER_CU * WM * WN / 4) void linear8Dma
 // ---------------------------------------------------------------------------
 // Any strides and alignment: tiles of 2 x 2 waves of 32 RB x 32 CB, steps of 128 bytes
 // of K, loaded into registers two steps ahead, put into one LDS buffer while the other
-// one's products run.
+// one's products run. Loads that straddle cache lines bound it: 8192 x 4096 x 8192 bf16,
+// rows 7 bytes apart, 617 us, 46208 x 1000 x 384 fp16 67.
 template<typename T, int RB, int CB, int ACT>
 __global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
   constexpr int STEP = 128, BM = 64 * RB, BN = 64 * CB, LOADS = 2 * (RB + CB);
@@ -270,8 +276,10 @@ __global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s,
 // ---------------------------------------------------------------------------
 // Few rows (at most 16 MT), any strides and alignment: the weights are read once. A
 // workgroup has 16 NT output channels; its waves take units of 128 bytes of K in turn
-// (every wave's loads of UNROLL units are issued before the first product), and their
-// sums meet in LDS.
+// (every wave's loads of UNROLL units are issued before the first product: 32 x 4096 x
+// 8192 12.1 us, 15.4 where the compiler spreads them), and their sums meet in LDS. 1 x
+// 4096 x 8192 bf16: 8.4 us, 4.0 TB/s; x, which every workgroup loads, costs the more the
+// more rows it has: 8 rows 9.4, 16 10.6.
 template<typename T, int MT, int NT, int WAVES, int UNROLL, int ACT>
 __global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, Scales s) {
   constexpr int UNIT = 128;
@@ -423,7 +431,13 @@ Linear8Plan planLinear8(const kgh_linear_int8_params& p, bool aligned, uint64_t 
     plan.kernel = LIN8_SKINNY;
     if(K >= 12288) most = std::min<int64_t>(256 / ((p.out_channels + 15) / 16), K / 4096);
   }
+  // 256 x 256 tiles move half the bytes into LDS, one workgroup a CU; 128 x 128 tiles, two a
+  // CU, cover each other's starts and ends, which weigh more the fewer steps there are. us on
+  // 256 and 128: 8192x4096x8192 with GELU and residual 327 and 355, 2888x4096x4096 55 and 61,
+  // 5776x1024x4096 44 and 39, 46208x1024x384 59 and 44. (0.7: their rounds of 256 CUs full.)
   else if(aligned && K >= 2048 && big * 10 >= (big + 255) / 256 * 256 * 7) plan.kernel = LIN8_DMA_256;
+  // us on 128 x 128 and on 64 x 64: 2888x1024x1024 (184 tiles of 128) 11.7 and 9.8,
+  // 2888x384x384 8.0 and 5.7, 128x4096x1024 14.5 and 11; 1000x4096x4096 (256) 28 on 128.
   else if(tiles(128) >= 224) plan.kernel = aligned ? LIN8_DMA_128 : LIN8_TILE_128;
   else {
     plan.kernel = aligned ? LIN8_DMA_64 : LIN8_TILE_64;

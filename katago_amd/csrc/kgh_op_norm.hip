@@ -74,6 +74,11 @@ __device__ __forceinline__ void normalise(float (&y)[VEC], const Values<T>& x, c
 // in LDS, then norm and activation of the same registers. Positions that take no part are
 // neither read nor computed: threads have places in a list of those that do. QUANT: rows
 // in 8 bits, a unit being an item with all of its channels.
+// 256 x 361 x 384 fp16, 32 groups, mish: 50 us of 142 MB (2.9 TB/s), with 54% of the
+// positions 42; vector instructions are 0.65 of the cycles, and a CU's four workgroups
+// come in two rounds that overlap in part. Registers decide: with 12 vectors a thread
+// four workgroups of 256 threads a CU, where the floats of x beside them, or another
+// turn from registers, left three or spilled.
 template<typename T, int ACT, int NV, bool QUANT>
 __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSlabKernel(NormArgs a, NormOut o, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -264,7 +269,10 @@ __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSl
 // Items that no workgroup's registers hold: their positions in `chunks`, their columns in
 // `blocks` of `cols`, each a workgroup. A part's groups have their
 // number of values, mean, sum of squares about it and that sum's factor in
-// parts[item][chunk][block][slot], slot 0 being the block's first group.
+// parts[item][chunk][block][slot], slot 0 being the block's first group. A chunk's rows
+// are every chunks-th `rowLanes` rows, so that the card reads one stretch at a time; with
+// eight rows of a thread under way 4 x 16384 x 512 bf16 takes 22 us (3.0 TB/s of reads;
+// reading alone reaches 4.0), 24 for the results behind it and 4 for the join.
 struct NormParts {
   float4* parts;
   int chunks, chunkRows, blocks, cols, rowLanes, slots, lanes, pv;  // lanes: threads that add up a group; pv: see NormSlab
@@ -481,6 +489,7 @@ __global__ __launch_bounds__(256) void normApplyKernel(NormArgs a, NormOut o, No
 }
 
 // The same in 8 bits: a row's columns by `lanes` threads, K each, and R rows at a time.
+// 46208 x 384 bf16, SiLU: 27 us (2.0 TB/s); vector instructions bound it.
 template<typename T, int ACT, int K, int R>
 __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, int lanes, int chunks, int chunkRows) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -582,7 +591,7 @@ __global__ __launch_bounds__(256) void normQuantLongKernel(NormArgs a, NormOut o
 }
 
 constexpr int NORM_QUANT_EACH = 4;  // 16-byte groups of a thread
-constexpr int NORM_RUN_BYTES = 96;  // of a unit's rows at least
+constexpr int NORM_RUN_BYTES = 96;  // of a unit's rows at least; see planNorm
 
 struct NormPlan {
   NormSlab slab;    // threads 0: parts

@@ -92,7 +92,8 @@ struct BackChannels {
 // ---------------------------------------------------------------------------
 // An item's run of channels in a unit's registers, as in the forward pass: x as it came
 // and u in fp32 (its slope is most of the work, and is computed once). sums has a row for
-// each item.
+// each item. 128 x 361 x 384 bf16, mish: 40 us of 107 MB (2.7 TB/s), with 54% of the
+// positions 34; vector instructions are 0.58 of the cycles.
 template<typename T, int ACT, int NV>
 __global__ __launch_bounds__(512, NV == 2 ? 4 : 3) void normBackSlabKernel(NormArgs a, NormBackArgs k, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -224,6 +225,10 @@ struct BackParts {
 
 constexpr int BACK_AHEAD = 2;  // rows of a thread under way
 
+// Items that no workgroup's registers hold: first the sums of chunks of positions, then,
+// behind their join, the results of the same chunks, u computed in both (kept, it would be
+// as many bytes again as x in fp32, twice as many in 16 bits). 8 x 4096 x 320 fp32, SiLU:
+// 26 us (3.2 TB/s) and 25 (5.0), the joins 8 and 4.
 template<typename T, int ACT, bool APPLY>
 __global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackArgs k, BackParts s) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -319,7 +324,9 @@ __global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackA
 
 // Many items of few positions, a thread one: a workgroup has a run of channels of every
 // `slices`-th item, and its channels' sums in registers all the while; sums has a row for
-// each slice (a row for each item would be as many bytes as the tensors).
+// each slice (a row for each item would be more bytes than the tensors). 8192 x 4096 bf16:
+// 71 us (2.8 TB/s); an item's way through three barriers bounds it, beside that of the
+// CU's other workgroup: 128 registers a thread leave room for two of 512 threads.
 template<typename T, int ACT>
 __global__ __launch_bounds__(1024) void normBackItemsKernel(NormArgs a, NormBackArgs k, NormSlab s, int slices) {
   constexpr int VEC = 16 / (int)sizeof(T);

