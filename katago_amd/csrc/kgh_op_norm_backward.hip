@@ -6,7 +6,8 @@ namespace {
 // The activations' slopes. In 16 bits by the hardware's exponential and reciprocal, to
 // within 2^-18 of 1; in fp32 by the accurate functions, to within 2^-20.
 //   silu: s (1 + v (1 - s)), s = 1 / (1 + e^-v);
-//   mish: with n = e^v (e^v + 2): n w + 4 v e^v (1 + e^v) w^2, w = 1 / (n + 2);
+//   mish: with n = e^v (e^v + 2): n w + 4 v e^v (1 + e^v) w^2, w = 1 / (n + 2) (v e^v
+//         before anything else: it is 0 where 4 v would pass the largest float);
 //   gelu: Phi(v) + v phi(v).
 template<typename T, int ACT>
 __device__ __forceinline__ float slope(float v) {
@@ -26,7 +27,7 @@ __device__ __forceinline__ float slope(float v) {
     const float n = fmaf(e, e, 2.0f * e);
     if constexpr(sizeof(T) == 4) w = 1.0f / (n + 2.0f);
     else w = __builtin_amdgcn_rcpf(n + 2.0f);
-    return w * fmaf(4.0f * c * fmaf(e, e, e), w, n);
+    return w * fmaf(c * e * fmaf(e, 4.0f, 4.0f), w, n);
   }
   else if constexpr(sizeof(T) == 4) return fmaf(0.5f, erfcf(-0.70710678118654752f * v), v * expf(-0.5f * v * v) * 0.39894228040143268f);
   else {
