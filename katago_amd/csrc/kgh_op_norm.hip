@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256) void normQuantLongKernel(NormArgs a, NormOut o
     if(take)
       for(int c = threadIdx.x; c < a.channels; c += 256) top = max(top, magnitudeBits(value(c)));
     const RowScale rs(rowTop(top, 256, tops));
-    for(int c = threadIdx.x; c < a.channels; c += 256) out[c] = (int8_t)(take ? rs.quantized(value(c)) & 0xff : 0);
+    for(int c = threadIdx.x; c < a.channels; c += 256) out[c] = (int8_t)(take ? rs.quantized(value(c)) & rs.keep & 0xff : 0);
     if(threadIdx.x == 0) o.scales[i] = rs.scale;
     __syncthreads();
   }

@@ -39,15 +39,17 @@ constexpr unsigned QUANT_INFINITE_BITS = 0x7f800000u;
 // rounded once, so that a plain fp32 form of the definition has the same bits.
 struct RowScale {
   float scale, factor;
+  unsigned keep;  // of the whole numbers' bytes: none where the row's are zeros
   __device__ __forceinline__ explicit RowScale(unsigned top) {
     const float t = __uint_as_float(top);
     const bool none = top < QUANT_LEAST_BITS || top >= QUANT_INFINITE_BITS;
     factor = none ? 0.0f : __fdiv_rn(127.0f, t);
+    keep = none ? 0u : ~0u;
     scale = top >= QUANT_INFINITE_BITS ? __builtin_nanf("") : none ? 0.0f : __fdiv_rn(t, 127.0f);
   }
   // The whole number nearest to v's product with the factor, in the lowest byte: of that
-  // number and 1.5 * 2^23, whose steps are 1 (of NaN, which an infinity becomes too where
-  // the factor is 0, that byte is 0).
+  // number and 1.5 * 2^23, whose steps are 1. Of a NaN that byte is any (arithmetic hands
+  // on a NaN's own lower bits): what is stored goes through `keep`.
   __device__ __forceinline__ unsigned quantized(float v) const {
     float p = v * factor;
     asm("" : "+v"(p));  // rounded by itself
@@ -113,7 +115,7 @@ __device__ __forceinline__ uint2 quantized(const float (&y)[VEC], const RowScale
     const unsigned high = __builtin_amdgcn_perm(s.quantized(y[j + 3]), s.quantized(y[j + 2]), 0x04000c0c);
     w[j >> 2] = low | high;
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint2(w[0] & s.keep, w[1] & s.keep);
 }
 
 }  // namespace

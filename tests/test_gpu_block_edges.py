@@ -36,3 +36,36 @@ def test_slopes_at_the_far_ends(dtype, act, b, p):
             assert not db[0] and not db[17] and not dw[0]
         for got, want in zip(results[-1], results[0]):
             assert torch.equal(got, want), size
+
+
+def _nans():
+    """NaN of several bits: fp32 arithmetic hands on the bits below the first."""
+    return torch.tensor([0x7FC00001, -1, 0x7F800001, 0x7FC000FF, -0x3FFFFE], dtype=torch.int32, device="cuda").view(torch.float32)
+
+
+@pytest.mark.parametrize("channels", [5, 64, 700, 9000, 40003])
+def test_quantize_nan_of_any_bits(channels):
+    x = _rand(12, channels, dtype=torch.float32)
+    for i, nan in enumerate(_nans()):
+        x[2 * i, [0, channels - 1, channels // 2, 1, 3][i]] = nan
+    x[8] = _nans()[1]  # memory filled with ones
+    q, scales = torch.full((12, channels), 9, dtype=torch.int8, device="cuda"), torch.empty(12, device="cuda")
+    ops.quantize_rows(x, q, scales)
+    bad = torch.arange(12, device="cuda") % 2 == 0
+    bad[10] = False
+    assert torch.equal(torch.isnan(scales), bad)
+    assert not q[bad].any()
+    want, want_scales = ref.quantize(x[~bad])
+    assert torch.equal(q[~bad].cpu(), want) and torch.equal(scales[~bad].cpu(), want_scales)
+
+
+@pytest.mark.parametrize("p,c,groups", [(1, 512, 4), (300, 24, 2), (9001, 40, 5), (2, 70000, 1)], ids=ids)
+def test_group_norm_rows_with_nan_of_any_bits(p, c, groups):
+    for act in ("identity", "relu", "gelu"):
+        for nan in _nans():
+            x = _rand(3, p, c, dtype=torch.float32)
+            x[1, p - 1, c // groups - 1] = nan
+            q, scales = torch.full((3, p, c), 9, dtype=torch.int8, device="cuda"), torch.empty(3, p, device="cuda")
+            _norm(x, q, groups, activation=act, out_scales=scales)
+            assert bool(torch.isnan(scales[1]).all()) and not torch.isnan(scales[0]).any() and not torch.isnan(scales[2]).any()
+            assert not q[1].any(), act
