@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (RB == 2 ? 2 : 4) : 1) void l
       }
     }
   }
-  storeTile<T, RB, CB, ACT>(a, acc, m0 + wm, n0 + wn);
+  storeTile<T, RB, CB, LinearFinish<T, ACT>>(a, acc, m0 + wm, n0 + wn);
 }
 
 // ---------------------------------------------------------------------------
@@ -257,7 +257,7 @@ template<typename T, int WM, int WN, int KW, int RB, int CB, int PER_CU, int ACT
 __global__ __launch_bounds__(64 * WM * WN * KW, PER_CU * WM * WN * KW / 4) void linearDmaKernel(LinearArgs a, int rowTiles, int colTiles) {
   floatx16 acc[RB][CB];
   int m, n;
-  if(dmaTile<T, WM, WN, KW, RB, CB>(a, rowTiles, colTiles, acc, m, n)) storeTile<T, RB, CB, ACT>(a, acc, m, n);
+  if(dmaTile<T, WM, WN, KW, RB, CB>(a, rowTiles, colTiles, acc, m, n)) storeTile<T, RB, CB, LinearFinish<T, ACT>>(a, acc, m, n);
 }
 
 template<typename T, int WM, int WN, int KW, int RB, int CB, int PER_CU, int ACT>

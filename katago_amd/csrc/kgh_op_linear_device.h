@@ -27,9 +27,17 @@ struct LinearArgs {
   int chunk;
 };
 
+// What becomes of a sum, and the bits of a residual that is not there.
+template<typename T, int ACT>
+struct LinearFinish {
+  static constexpr unsigned NO_RESIDUAL = 0;
+  static __device__ __forceinline__ float activated(float sum, float bias) { return activate<T, ACT>(sum + bias); }
+  static __device__ __forceinline__ float added(float y, float residual) { return y + residual; }
+};
+
 // Two groups of four columns, bias and activation, and the residual's 16 bytes of
 // this lane's columns, to the 16 bytes of the same columns.
-template<typename T, int ACT>
+template<typename T, typename Finish>
 __device__ __forceinline__ uint4 finishGroup(floatx4 v0, floatx4 v1, floatx4 b0, floatx4 b1, uint4 res) {
   const uint2 r01 = swapHalves(res.x, res.z), r23 = swapHalves(res.y, res.w);
   union Four {
@@ -40,8 +48,8 @@ __device__ __forceinline__ uint4 finishGroup(floatx4 v0, floatx4 v1, floatx4 b0,
   ra[1].v = make_uint2(r01.y, r23.y);
 #pragma unroll
   for(int e = 0; e < 4; e++) {
-    oa[0].e[e] = (T)(activate<T, ACT>(v0[e] + b0[e]) + (float)ra[0].e[e]);
-    oa[1].e[e] = (T)(activate<T, ACT>(v1[e] + b1[e]) + (float)ra[1].e[e]);
+    oa[0].e[e] = (T)Finish::added(Finish::activated(v0[e], b0[e]), (float)ra[0].e[e]);
+    oa[1].e[e] = (T)Finish::added(Finish::activated(v1[e], b1[e]), (float)ra[1].e[e]);
   }
   const uint2 o01 = swapHalves(oa[0].v.x, oa[1].v.x), o23 = swapHalves(oa[0].v.y, oa[1].v.y);
   return make_uint4(o01.x, o23.x, o01.y, o23.y);
@@ -51,9 +59,10 @@ __device__ __forceinline__ uint4 finishGroup(floatx4 v0, floatx4 v1, floatx4 b0,
 // are the products' row operand, so a lane has four consecutive columns of row
 // laneRow, and its partner lane ^ 32 the four behind them; in 16 bits two such
 // groups of both swap halves into 16 consecutive bytes a lane.
-template<typename T, int RB, int CB, int ACT>
+template<typename T, int RB, int CB, typename Finish>
 __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&acc)[RB][CB], int mBase, int nBase) {
   const int lane = threadIdx.x & 63, laneRow = lane & 31, half = lane >> 5;
+  constexpr unsigned NONE = Finish::NO_RESIDUAL;
   const T* res = (const T*)a.residual;
   T* out = (T*)a.out;
   if constexpr(sizeof(T) == 2) {
@@ -67,7 +76,7 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
         for(int j = 0; j < CB; j++)
 #pragma unroll
           for(int p = 0; p < 2; p++) {
-            rv[i][j][p] = u32x4_t{0, 0, 0, 0};
+            rv[i][j][p] = u32x4_t{NONE, NONE, NONE, NONE};
             if(res != nullptr)
               __builtin_memcpy(&rv[i][j][p], res + (int64_t)(mBase + i * 32 + laneRow) * a.ldr + nBase + j * 32 + (2 * p + half) * 8, 16);
           }
@@ -87,7 +96,7 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
             const u32x4_t r = rv[i][j][p];
             const floatx4 v0 = {acc[i][j][8 * p], acc[i][j][8 * p + 1], acc[i][j][8 * p + 2], acc[i][j][8 * p + 3]};
             const floatx4 v1 = {acc[i][j][8 * p + 4], acc[i][j][8 * p + 5], acc[i][j][8 * p + 6], acc[i][j][8 * p + 7]};
-            const uint4 o = finishGroup<T, ACT>(v0, v1, bias[2 * p], bias[2 * p + 1], make_uint4(r.x, r.y, r.z, r.w));
+            const uint4 o = finishGroup<T, Finish>(v0, v1, bias[2 * p], bias[2 * p + 1], make_uint4(r.x, r.y, r.z, r.w));
             __builtin_memcpy(out + (int64_t)(mBase + i * 32 + laneRow) * a.ldo + nj + (2 * p + half) * 8, &o, 16);
           }
       }
@@ -121,7 +130,7 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
             continue;
           }
 #pragma unroll
-          for(int e = 0; e < 4; e++) v[e] = activate<T, ACT>(v[e] + bias[q][e]);
+          for(int e = 0; e < 4; e++) v[e] = Finish::activated(v[e], bias[q][e]);
           if(res != nullptr) {
             const uint4 r = loadGroupSmall((const float*)a.residual + (int64_t)m * a.ldr + n, a.N - n);
             v += *(const floatx4*)&r;
@@ -134,14 +143,14 @@ __device__ __forceinline__ void storeTile(const LinearArgs& a, const floatx16 (&
 #pragma unroll
         for(int p = 0; p < 2; p++) {
           const int n = nj + (2 * p + half) * 8;
-          rv[p] = make_uint4(0, 0, 0, 0);
+          rv[p] = make_uint4(NONE, NONE, NONE, NONE);
           if(res != nullptr && m < a.M && n < a.N) rv[p] = loadGroupSmall(res + (int64_t)m * a.ldr + n, a.N - n);
         }
 #pragma unroll
         for(int p = 0; p < 2; p++) {
           const floatx4 v0 = {acc[i][j][8 * p], acc[i][j][8 * p + 1], acc[i][j][8 * p + 2], acc[i][j][8 * p + 3]};
           const floatx4 v1 = {acc[i][j][8 * p + 4], acc[i][j][8 * p + 5], acc[i][j][8 * p + 6], acc[i][j][8 * p + 7]};
-          const uint4 o = finishGroup<T, ACT>(v0, v1, bias[2 * p], bias[2 * p + 1], rv[p]);
+          const uint4 o = finishGroup<T, Finish>(v0, v1, bias[2 * p], bias[2 * p + 1], rv[p]);
           const int n = nj + (2 * p + half) * 8;
           if(m < a.M && n < a.N) storeGroup(out + (int64_t)m * a.ldo + n, o, a.N - n);
         }

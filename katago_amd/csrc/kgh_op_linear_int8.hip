@@ -36,14 +36,24 @@ __device__ __forceinline__ u32x4_t loadBytes(const int8_t* row, int k, int end) 
   return v;
 }
 
-// A sum's value with its bias: the sum's conversion, a product, and a product and sum
-// rounded once, in every kernel (the compiler would else round some of them to 16 bits
-// without the 32 between, and a call's bits would depend on its workspace).
-__device__ __forceinline__ float scaled(int sum, float x, float w, float bias) {
-  float v = fmaf((float)sum * x, w, bias);
+// A result's steps, each rounded by itself and to 32 bits in every kernel, so that a
+// call's bits depend on neither kernel nor workspace: the compiler would else take the
+// activation's last product and the residual into one operation, or into the conversion
+// to 16 bits, in some kernels and not in others.
+__device__ __forceinline__ float rounded(float v) {
   asm("" : "+v"(v));
   return v;
 }
+// A sum's value with its bias: the sum's conversion, a product, and a product and sum
+// rounded once.
+__device__ __forceinline__ float scaled(int sum, float x, float w, float bias) { return rounded(fmaf((float)sum * x, w, bias)); }
+// (a residual that is not there is -0: it leaves every number as it is, -0 too)
+template<typename T, int ACT>
+struct Int8Finish {
+  static constexpr unsigned NO_RESIDUAL = 0x80008000u;
+  static __device__ __forceinline__ float activated(float scaled, float) { return rounded(activate<T, ACT>(scaled)); }
+  static __device__ __forceinline__ float added(float y, float residual) { return rounded(y + residual); }
+};
 
 // storeTile of sums: by their scales, or as they are where K is split.
 template<typename T, int RB, int CB, int ACT>
@@ -75,7 +85,7 @@ __device__ __forceinline__ void storeSums(LinearArgs a, const Scales& s, const i
       }
     a.bias = nullptr;
   }
-  storeTile<T, RB, CB, ACT>(a, acc, m, n);
+  storeTile<T, RB, CB, Int8Finish<T, ACT>>(a, acc, m, n);
 }
 
 // What a wave's block of the result needs beside the sums, for blocks that lie inside it
@@ -90,6 +100,7 @@ struct EarlyLoads {
 // Two groups of four columns to the 16 bytes of the same columns, as finishGroup.
 template<typename T, int ACT, bool RES>
 __device__ __forceinline__ uint4 finishSums(const int (&s0)[4], const int (&s1)[4], float x, floatx4 w0, floatx4 w1, floatx4 b0, floatx4 b1, u32x4_t res) {
+  typedef Int8Finish<T, ACT> Finish;
   union Four {
     uint2 v;
     T e[4];
@@ -101,9 +112,9 @@ __device__ __forceinline__ uint4 finishSums(const int (&s0)[4], const int (&s1)[
   }
 #pragma unroll
   for(int e = 0; e < 4; e++) {
-    const float v0 = activate<T, ACT>(scaled(s0[e], x, w0[e], b0[e])), v1 = activate<T, ACT>(scaled(s1[e], x, w1[e], b1[e]));
-    oa[0].e[e] = (T)(RES ? v0 + (float)ra[0].e[e] : v0);
-    oa[1].e[e] = (T)(RES ? v1 + (float)ra[1].e[e] : v1);
+    const float v0 = Finish::activated(scaled(s0[e], x, w0[e], b0[e]), 0.0f), v1 = Finish::activated(scaled(s1[e], x, w1[e], b1[e]), 0.0f);
+    oa[0].e[e] = (T)(RES ? Finish::added(v0, (float)ra[0].e[e]) : v0);
+    oa[1].e[e] = (T)(RES ? Finish::added(v1, (float)ra[1].e[e]) : v1);
   }
   const uint2 o01 = swapHalves(oa[0].v.x, oa[1].v.x), o23 = swapHalves(oa[0].v.y, oa[1].v.y);
   return make_uint4(o01.x, o23.x, o01.y, o23.y);
@@ -353,8 +364,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear8SkinnyKernel(LinearArgs a, 
       ((int*)a.part)[((int64_t)blockIdx.y * a.M + m) * a.N + n] = sum;
       continue;
     }
-    float v = activate<T, ACT>(scaled(sum, s.x[m], s.w[n], a.bias != nullptr ? a.bias[n] : 0.0f));
-    if(a.residual != nullptr) v += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n];
+    float v = Int8Finish<T, ACT>::activated(scaled(sum, s.x[m], s.w[n], a.bias != nullptr ? a.bias[n] : 0.0f), 0.0f);
+    if(a.residual != nullptr) v = Int8Finish<T, ACT>::added(v, (float)((const T*)a.residual)[(int64_t)m * a.ldr + n]);
     ((T*)a.out)[(int64_t)m * a.ldo + n] = (T)v;
   }
 }
@@ -381,8 +392,8 @@ __global__ __launch_bounds__(256) void linear8JoinKernel(LinearArgs a, Scales s,
 #pragma unroll
   for(int j = 0; j < 4; j++) {
     if(j >= count) break;
-    float y = activate<T, ACT>(scaled(v[j], x, s.w[n + j], a.bias != nullptr ? a.bias[n + j] : 0.0f));
-    if(a.residual != nullptr) y += (float)((const T*)a.residual)[(int64_t)m * a.ldr + n + j];
+    float y = Int8Finish<T, ACT>::activated(scaled(v[j], x, s.w[n + j], a.bias != nullptr ? a.bias[n + j] : 0.0f), 0.0f);
+    if(a.residual != nullptr) y = Int8Finish<T, ACT>::added(y, (float)((const T*)a.residual)[(int64_t)m * a.ldr + n + j]);
     ((T*)a.out)[(int64_t)m * a.ldo + n + j] = (T)y;
   }
 }

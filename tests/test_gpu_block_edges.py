@@ -14,6 +14,11 @@ CURVED = [a for a in ops.ACTIVATIONS if a not in ("identity", "relu")]
 LARGEST = torch.finfo(torch.float32).max
 
 
+def _same_bits(a, b):
+    kind = torch.int32 if a.dtype == torch.float32 else torch.int16
+    return torch.equal(a.contiguous().view(kind), b.contiguous().view(kind))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("act", CURVED)
 @pytest.mark.parametrize("b,p", [(3, 49), (2, 9001), (40, 1), (1100, 3)], ids=ids)
@@ -69,3 +74,30 @@ def test_group_norm_rows_with_nan_of_any_bits(p, c, groups):
             _norm(x, q, groups, activation=act, out_scales=scales)
             assert bool(torch.isnan(scales[1]).all()) and not torch.isnan(scales[0]).any() and not torch.isnan(scales[2]).any()
             assert not q[1].any(), act
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("m,k,n", [(5, 24592, 40), (40, 16384, 24), (64, 8192, 1000), (70, 8208, 72), (66, 4112, 65), (128, 4096, 1024), (361, 384, 384),
+                                   (2000, 1040, 1990), (4000, 2048, 3800)], ids=ids)
+def test_linear_int8_bits_of_every_kernel(dtype, m, k, n):
+    """The same bits with a workspace, without one, from rows of any alignment and among
+    other rows, whatever follows the sum."""
+    x, w = _bytes(m, k), _bytes(n, k, seed=1)
+    x_apart, w_apart = _laid(x.cpu(), pad=1, shift=1), _laid(w.cpu(), pad=1, shift=1)
+    xs, ws = torch.rand(m, device="cuda") / 73, (torch.rand(n, device="cuda") + 0.5) * k ** -0.5 / 73
+    far = torch.linspace(-12, 12, n, device="cuda")
+    far[::9] *= 10
+    res = _rand(m, n, dtype=dtype, seed=3)
+    for act in ops.ACTIVATIONS:
+        for bias in (None, far):
+            for residual in (None, res):
+                kw = dict(bias=bias, activation=act)
+                new = lambda rows=m: torch.empty(rows, n, dtype=dtype, device="cuda")
+                want = _linear(x, xs, w, ws, new(), residual=residual, **kw)
+                others = {"no workspace": ops.linear_int8(x, xs, w, ws, new(), residual=residual, **kw),
+                          "apart": _linear(x_apart, xs, w_apart, ws, new(), residual=residual, **kw)}
+                for rows in (1, 30, 60, 300, 2000):
+                    if rows < m:
+                        others[rows] = _linear(x[:rows], xs[:rows], w, ws, new(rows), residual=None if residual is None else residual[:rows], **kw)
+                for name, got in others.items():
+                    assert _same_bits(got, want[:got.shape[0]]), (act, bias is None, residual is None, name)
