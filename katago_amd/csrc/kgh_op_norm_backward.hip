@@ -310,12 +310,12 @@ __global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackA
       __syncthreads();
       const int width = s.cols * VEC;
       for(int e = threadIdx.x; e < min(width, a.channels - from); e += 256) {
-        float2 t = make_float2(0.0f, 0.0f);
+        double2 t = make_double2(0.0, 0.0);  // rows of threads may be 256
         for(int q = 0; q < s.rowLanes; q++) {
           t.x += part[q * width + e].x;
           t.y += part[q * width + e].y;
         }
-        s.parts[itemChunk * a.channels + from + e] = t;
+        s.parts[itemChunk * a.channels + from + e] = make_float2((float)t.x, (float)t.y);
       }
       if(threadIdx.x == 0 && block == 0) s.counts[itemChunk] = counted;
       __syncthreads();
@@ -428,11 +428,13 @@ __global__ __launch_bounds__(1024) void normBackItemsKernel(NormArgs a, NormBack
   }
 }
 
-// The chunks' sums of an item's group: its channels' sums and its means. Threads are
-// (chunk slice, channel); channels of long groups in turns.
+// The chunks' sums of an item's group: its channels' sums and its means, in 64 bits
+// (chunks may be thousands, and roundings of terms of one sign add up: 262144 positions of
+// 1024 channels that are all the same were 7e-6 off in fp32). Threads are (chunk slice,
+// channel); channels of long groups in turns.
 __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackArgs k, BackParts s) {
-  __shared__ float2 part[256];
-  __shared__ float2 total[4];
+  __shared__ double2 part[256];
+  __shared__ double2 total[4];
   __shared__ int counted;
   const int width = min(a.per, 64), slices = 256 / width;
   const int slice = threadIdx.x / width, c = threadIdx.x - slice * width;
@@ -443,11 +445,11 @@ __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackAr
     int rows = 0;
     for(int q = threadIdx.x; q < s.chunks; q += 256) rows += s.counts[(int64_t)b * s.chunks + q];
     if(rows > 0) atomicAdd(&counted, rows);
-    float m1 = 0.0f, m2 = 0.0f;
+    double m1 = 0.0, m2 = 0.0;
     for(int from = 0; from < a.per; from += width) {
       const bool on = slice < slices && from + c < a.per;
       const int ch = g * a.per + from + c;
-      float2 t = make_float2(0.0f, 0.0f);
+      double2 t = make_double2(0.0, 0.0);
       if(on)
 #pragma unroll 8
         for(int q = slice; q < s.chunks; q += slices) {
@@ -462,10 +464,10 @@ __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackAr
           t.x += part[q * width + c].x;
           t.y += part[q * width + c].y;
         }
-        k.sums[(int64_t)b * a.channels + ch] = t;
-        const float w = a.weight == nullptr ? 1.0f : a.weight[ch];
-        m1 = fmaf(t.x, w, m1);
-        m2 = fmaf(t.y, w, m2);
+        k.sums[(int64_t)b * a.channels + ch] = make_float2((float)t.x, (float)t.y);
+        const double w = a.weight == nullptr ? 1.0 : a.weight[ch];
+        m1 = fma(t.x, w, m1);
+        m2 = fma(t.y, w, m2);
       }
       __syncthreads();
     }
@@ -474,11 +476,11 @@ __global__ __launch_bounds__(256) void normBackJoinKernel(NormArgs a, NormBackAr
       m1 += __shfl_xor(m1, w);
       m2 += __shfl_xor(m2, w);
     }
-    if((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = make_float2(m1, m2);
+    if((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = make_double2(m1, m2);
     __syncthreads();
     if(threadIdx.x == 0) {
-      const float n = (float)counted * (float)a.per;
-      s.means[i] = make_float2(((total[0].x + total[1].x) + (total[2].x + total[3].x)) / n, ((total[0].y + total[1].y) + (total[2].y + total[3].y)) / n);
+      const double n = (double)counted * a.per;
+      s.means[i] = make_float2((float)(((total[0].x + total[1].x) + (total[2].x + total[3].x)) / n), (float)(((total[0].y + total[1].y) + (total[2].y + total[3].y)) / n));
     }
     __syncthreads();
   }

@@ -101,3 +101,23 @@ def test_linear_int8_bits_of_every_kernel(dtype, m, k, n):
                         others[rows] = _linear(x[:rows], xs[:rows], w, ws, new(rows), residual=None if residual is None else residual[:rows], **kw)
                 for name, got in others.items():
                     assert _same_bits(got, want[:got.shape[0]]), (act, bias is None, residual is None, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("p,c", [(1 << 18, 1024), (1 << 18, 8), (200001, 264)], ids=ids)
+def test_backward_sums_of_very_many_terms(dtype, p, c):
+    """Every position the same, so that roundings of a sum go one way: a sum over them is
+    `p` times a position's. In fp32 a thread adds at most 64 of them, and 8 roundings are
+    left for what is done with these sums in 64 bits and for the terms' own."""
+    depth = 64 + 8
+    one, grad = _rand(1, 1, c, dtype=dtype), _rand(1, 1, c, dtype=dtype, seed=1).abs() + 0.25
+    x, dy = one.expand(1, p, c), grad.expand(1, p, c)
+    w = _rand(c, dtype=torch.float32, seed=2, shift=1.0, scale=0.3)
+    stats = _forward_statistics(one, 1)
+    dx, dw, db = torch.empty(1, p, c, dtype=dtype, device="cuda"), torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    _backward(x, dy, stats, dx, 1, weight=w, grad_weight=dw, grad_bias=db)
+    want_x, want_w, want_b = ref.group_norm_backward(one, grad, stats, 1, weight=w)
+    for got, (y, off), what in ((dw, want_w, "weight"), (db, want_b, "bias")):
+        check(got, (p * y, p * (off + (depth - ref.DEPTH) * U32 * y.abs())), what)  # the reference's own depth is taken out
+    assert torch.equal(dx, dx[:, :1].expand_as(dx))
+    check(dx[:, :1], want_x)
