@@ -14,10 +14,15 @@ __device__ __forceinline__ float slope(float v) {
   if constexpr(ACT == KGH_ACT_IDENTITY) return 1.0f;
   else if constexpr(ACT == KGH_ACT_RELU) return v > 0.0f ? 1.0f : v != v ? v : 0.0f;
   else if constexpr(ACT == KGH_ACT_SILU) {
-    float s;
-    if constexpr(sizeof(T) == 4) s = 1.0f / (1.0f + expf(-v));
-    else s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -ACT_LOG2E));
-    return s * fmaf(v, 1.0f - s, 1.0f);
+    if constexpr(sizeof(T) == 4) {
+      // (1 - s of an s next to 1 would have lost the bits that v multiplies)
+      const float e = expf(-fabsf(v)), most = 1.0f / (1.0f + e), least = e * most;
+      return (v < 0.0f ? least : most) * fmaf(v, v < 0.0f ? most : least, 1.0f);
+    }
+    else {
+      const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -ACT_LOG2E));
+      return s * fmaf(v, 1.0f - s, 1.0f);
+    }
   }
   else if constexpr(ACT == KGH_ACT_MISH) {
     const float c = v > 20.0f ? 20.0f : v;  // NaN stays NaN
