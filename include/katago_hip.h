@@ -232,8 +232,8 @@ int kgh_memcpy_dtoh(void* dst, const void* src, size_t bytes);
  *  - Sums and statistics are kept in fp32, and a result is rounded to the
  *    tensors' type once (kgh_cross_attention says what it rounds before). Results do not depend on what ran before, and the
  *    same call gives the same bits.
- *  - An axis of length zero (rows, tokens, batch, queries) makes the call a
- *    no-op. Unless stated otherwise the output overlaps no input.
+ *  - An axis of length zero (rows, tokens, batch, positions, queries) makes the
+ *    call a no-op, where nothing else is said. Unless stated otherwise the output overlaps no input.
  *  - A workspace may be NULL where nothing else is said. Calls that may overlap need workspaces of their
  *    own; so do captured graphs that may replay at the same time. Its contents
  *    need no initialisation and mean nothing after the call. */
@@ -417,7 +417,8 @@ int kgh_linear_int8(int32_t device, const kgh_linear_int8_params* params, void* 
  * int8: rows (b, p) over all channels as kgh_quantize_rows makes them of the results
  * before they are rounded, and their scales.
  * statistics, where not NULL, takes mean and 1 / sqrt(variance + eps) of each item's
- * groups for kgh_group_norm_backward (0 and 0 of an item without a position). */
+ * groups for kgh_group_norm_backward (0 and 0 of an item without a position, also where
+ * `positions` is 0). */
 typedef struct kgh_group_norm_params {
   int32_t dtype;      /* KGH_DTYPE_* of x, and of out without out_scales */
   int32_t activation; /* KGH_ACTIVATION_* */

@@ -590,6 +590,11 @@ __global__ __launch_bounds__(256) void normQuantLongKernel(NormArgs a, NormOut o
   }
 }
 
+// The statistics of items without positions, where there is nothing else.
+__global__ __launch_bounds__(256) void normNothingKernel(float* stats, int64_t n) {
+  for(int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) stats[i] = 0.0f;
+}
+
 constexpr int NORM_QUANT_EACH = 4;  // 16-byte groups of a thread
 constexpr int NORM_RUN_BYTES = 96;  // of a unit's rows at least; see planNorm
 
@@ -609,7 +614,7 @@ NormPlan planNorm(const kgh_group_norm_params& p) {
   // pieces of lines of memory, shorter ones' units more: 48, 96 and 192 bytes take the same
   // time within 5%.
   const auto slab = [&](int bytes, int most, int wide) {
-    if(plan.slab.threads == 0) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, bytes, false, most, wide, quant, 2);
+    if(plan.slab.threads == 0) plan.slab = planSlab(p.positions, p.channels, p.groups, size, bytes, false, most, wide, quant, 2);
   };
   if(quant) slab(NORM_RUN_BYTES, 2, 1024);
   else {
@@ -691,6 +696,7 @@ void checkGroupNorm(const kgh_group_norm_params& p, bool pointers) {
   if(!(p.eps >= FLT_MIN) || p.eps > FLT_MAX) opInvalid(op, "eps must be a number of at least 2^-126");
   for(int64_t s : {p.x_batch_stride, p.x_position_stride, p.mask_stride, p.out_batch_stride, p.out_position_stride})
     if(s < 0) opInvalid(op, "negative stride");
+  if(p.batch > 0 && p.statistics != nullptr) opCheckPointer(op, "statistics", p.statistics, 4);
   if(p.batch == 0 || p.positions == 0) return;
   checkApartRows(op, "out", p.out_batch_stride, p.out_position_stride, p.batch, p.positions, p.channels);
   const size_t e = opElemBytes(p.dtype);
@@ -700,7 +706,6 @@ void checkGroupNorm(const kgh_group_norm_params& p, bool pointers) {
   if(p.bias != nullptr) opCheckPointer(op, "bias", p.bias, 4);
   if(p.lengths != nullptr) opCheckPointer(op, "lengths", p.lengths, 4);
   if(p.out_scales != nullptr) opCheckPointer(op, "out_scales", p.out_scales, 4);
-  if(p.statistics != nullptr) opCheckPointer(op, "statistics", p.statistics, 4);
   if(p.x == p.out) {
     if(p.out_scales != nullptr) opInvalid(op, "out is x itself, in another type");
     if((p.batch > 1 && p.x_batch_stride != p.out_batch_stride) || (p.positions > 1 && p.x_position_stride != p.out_position_stride))
@@ -716,6 +721,11 @@ uint64_t groupNormWorkspace(const kgh_group_norm_params& p) {
 }
 
 void launchGroupNorm(const kgh_group_norm_params& p, hipStream_t stream) {
+  if(p.batch > 0 && p.positions == 0 && p.statistics != nullptr) {
+    const int64_t n = (int64_t)p.batch * p.groups * 2;
+    normNothingKernel<<<normGrid((n + 255) / 256), 256, 0, stream>>>(p.statistics, n);
+    KGH_CHECK_LAUNCH();
+  }
   if(p.batch == 0 || p.positions == 0) return;
   const NormPlan plan = planNorm(p);
   const NormArgs a = normArgs(p, p.eps);

@@ -532,7 +532,7 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
   // 1 x 1 x 384 9.2 and 7.2, 4096 x 2 x 256 70 and 21, 1024 x 4 x 384 29 and 20; but
   // 256 x 4 x 1024 14 and 19, 1024 x 8 x 384 29 and 64.
   if(p.positions == 1 || (p.positions <= 4 && p.batch >= 1024)) {
-    plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, 1024, false, 1, 1024, false, 1);
+    plan.slab = planSlab(p.positions, p.channels, p.groups, size, 1024, false, 1, 1024, false, 1);
     if(plan.slab.threads != 0) {
       // Slices that fill the card: of 512 threads two a CU (8192 x 1 x 4096 SiLU: 256 slices
       // 114 us, one workgroup a CU; 512 82), of few threads more (8192 x 1 x 384: 512 38 us,
@@ -548,7 +548,7 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
   }
   plan.sumsBytes = round16((uint64_t)p.batch * p.channels * 8);
   const auto slab = [&](int bytes, int most, int wide) {
-    if(plan.slab.threads == 0) plan.slab = planSlab(p.batch, p.positions, p.channels, p.groups, size, bytes, true, most, wide, false, 1);
+    if(plan.slab.threads == 0) plan.slab = planSlab(p.positions, p.channels, p.groups, size, bytes, true, most, wide, false, 1);
   };
   // us of 128 x 361 x 384 bf16 in 32 groups: runs of 48 bytes 45, of 96 53, in parts 61.
   slab(48, 6, 256);

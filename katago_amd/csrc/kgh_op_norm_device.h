@@ -39,7 +39,6 @@ struct NormSlab {
   int threads, units, run, runs, cols, rowLanes, nv, pv, entries, segments, groupEntries, lanesLog, stepRows, stepEntries;
   int ldsPairs;  // a unit's LDS, in pairs of floats: sums, then groups' state
   int listAt;    // its list of positions (16 bits each) behind the pairs of all units, in bytes; only where there is a mask
-  int64_t count;             // of units
   int firstItem, launched;   // of this launch: its first item and its number of units
 };
 
@@ -268,7 +267,7 @@ void forUnits(const NormArgs& a, NormSlab s, F&& f) {
 // thread and `wide` threads; threads is 0 where there is none. Runs of at least `bytes` a
 // row, or (wholeRows) of all channels. perChannel: sums of each channel are wanted. What a
 // group has in LDS beside the sums: `state` pairs.
-inline NormSlab planSlab(int64_t batch, int positions, int channels, int groups, int size, int bytes, bool perChannel, int most, int wide, bool wholeRows,
+inline NormSlab planSlab(int positions, int channels, int groups, int size, int bytes, bool perChannel, int most, int wide, bool wholeRows,
                          int state) {
   const int vec = 16 / size, per = channels / groups;
   NormSlab none{};
@@ -286,7 +285,6 @@ inline NormSlab planSlab(int64_t batch, int positions, int channels, int groups,
     s.cols = (int)((run + vec - 1) / vec);
     s.threads = threads;
     s.units = threads == 64 ? 4 : 1;
-    s.count = batch * s.runs;
     if(s.cols > threads) continue;
     s.rowLanes = std::min(threads / s.cols, positions);
     s.nv = (positions + s.rowLanes - 1) / s.rowLanes;

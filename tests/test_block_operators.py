@@ -133,6 +133,13 @@ def test_group_norm_refuses(change, word):
     _refused(_norm(**change), word)
 
 
+def test_group_norm_of_no_positions_refuses_statistics():
+    """They are written where nothing else is."""
+    none = dict(x=Meta(2, 0, 24), out=Meta(2, 0, 24, at=2 * AT))
+    _refused(_norm(stats=Meta(2, 4, 2, at=AT + 2, **F32), **none), "statistics", "aligned")
+    _refused(_norm(stats=Meta(2, 3, 2, **F32), **none), "shape")
+
+
 def _backward(**change):
     a = dict(x=Meta(2, 9, 24), grad_out=Meta(2, 9, 24, at=2 * AT), stats=Meta(2, 4, 2, at=3 * AT, **F32), grad_x=Meta(2, 9, 24, at=4 * AT), groups=4, **WORK)
     a.update(change)

@@ -139,3 +139,13 @@ def test_slopes(dtype, act, p):
         _backward(x, dy, stats, dx, 8, weight=torch.zeros(c, device="cuda"), bias=bias.cuda(), activation=act, lengths=lengths, grad_bias=db)
         off = 2.0 ** (-20 if dtype == torch.float32 else -18)
         check(db, (ref.slope(bias.double(), act), torch.full((c,), off, dtype=torch.float64)), act)
+
+
+def test_statistics_of_no_positions():
+    """No position, no deviation: 0 and 0, as of an item whose mask leaves none."""
+    for b in (1, 3, 700):
+        x = torch.empty(b, 0, 8, dtype=torch.float16, device="cuda")
+        around = torch.full((b * 2 * 2 + 3,), 5.0, device="cuda")
+        stats = around[1:1 + b * 4].view(b, 2, 2)
+        ops.group_norm(x, torch.empty_like(x), 2, stats=stats)
+        assert not stats.any() and around[0] == 5 and bool((around[1 + b * 4:] == 5).all())
