@@ -11,8 +11,8 @@ asynchronous on ``stream``: a hipStream_t as an int, 0 for the null stream; None
 the stream that torch is on for torch tensors, and the null stream for others. The
 caller keeps the tensors alive until they have run. Nothing here records gradients:
 tensors that require them are taken under ``torch.no_grad()`` only, as in the methods
-of a torch.autograd.Function that calls ``group_norm`` and ``group_norm_backward``. Every call
-returns its output tensor. Arguments that do not fit raise ``StringError``.
+of a torch.autograd.Function that calls ``group_norm`` and ``group_norm_backward``, and
+tensors with tangents of forward mode are refused. Every call returns its output tensor. Arguments that do not fit raise ``StringError``.
 """
 from __future__ import annotations
 
@@ -202,9 +202,21 @@ def _stream(t, device):
 
 def _no_gradients(op, *tensors):
     """Refuses tensors that a result's gradients would be wanted of."""
+    torch = sys.modules.get("torch")
     for t in tensors:
-        if t is not None and getattr(t, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
+        if t is not None and getattr(t, "requires_grad", False) and torch.is_grad_enabled():
             _invalid(f"{op}: a tensor requires gradients, and the result would have none (torch.no_grad() takes it)")
+    if torch is not None and getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0:
+        _no_tangents(op, torch, tensors)
+
+
+def _no_tangents(op, torch, tensors):
+    """The same of gradients that go forward, within a dual level (but not in a
+    torch.autograd.Function's forward, whose jvp is what counts)."""
+    if torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                _invalid(f"{op}: a tensor has a tangent, and the result would have none")
 
 
 def _sizes(op, *sizes):

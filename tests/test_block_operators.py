@@ -249,3 +249,36 @@ def test_gradients_are_taken_under_no_grad():
         _refused(_norm(x=Trained(2, 9, 24), out=Meta(2, 9, 24, at=0)), "null")
         _refused(_backward(x=Trained(2, 9, 24), grad_out=Meta(2, 9, 24, at=0)), "null")
         _refused(_quantize(x=Trained(4, 16), out=Meta(4, 16, at=0, **I8)), "null")
+
+
+def test_tangents_are_refused():
+    """A dual tensor's result would silently have no tangent; in a Function's forward it
+    has what the Function's jvp gives it."""
+    x = torch.randn(2, 3)
+    seen = []
+
+    class Function(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            ops._no_gradients("group_norm", x, None)
+            seen.append(True)
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, grad):
+            return grad * 2
+
+        @staticmethod
+        def jvp(ctx, tangent):
+            return tangent * 2
+
+    ops._no_gradients("group_norm", x, None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        ops._no_gradients("group_norm", x, None, Meta(4, 16))
+        for tensors in ((dual,), (x, None, dual)):
+            _refused(lambda: ops._no_gradients("group_norm", *tensors), "group_norm", "tangent")
+            with torch.no_grad():
+                _refused(lambda: ops._no_gradients("group_norm", *tensors), "tangent")
+        assert bool((torch.autograd.forward_ad.unpack_dual(Function.apply(dual)).tangent == 2).all()) and seen
+    ops._no_gradients("group_norm", x, None)

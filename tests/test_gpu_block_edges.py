@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import block_reference as ref
-from katago_amd import ops
+from katago_amd import nn, ops
 from operator_reference import U32, check
 from test_gpu_block_operators import TYPES, _backward, _bytes, _forward_statistics, _laid, _linear, _norm, _rand, ids
 
@@ -149,3 +149,24 @@ def test_statistics_of_no_positions():
         stats = around[1:1 + b * 4].view(b, 2, 2)
         ops.group_norm(x, torch.empty_like(x), 2, stats=stats)
         assert not stats.any() and around[0] == 5 and bool((around[1 + b * 4:] == 5).all())
+
+
+def test_tangents_are_refused():
+    """By every call, and only of tensors that have one."""
+    x, f32 = _rand(2, 8, 16, dtype=torch.float32), dict(dtype=torch.float32, device="cuda")
+    q, scales = torch.empty(8, 16, dtype=torch.int8, device="cuda"), torch.empty(8, **f32)
+    ops.quantize_rows(x[0], q, scales)
+    stats = _forward_statistics(x, 4)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda x: ops.linear(x[0], torch.ones(16, 16, **f32), torch.empty(8, 16, **f32)),
+                     lambda x: ops.rope_axes(x, torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(1, 8, 1, **f32), torch.empty(2, 8, 16, **f32)),
+                     lambda x: ops.cross_attention(*(x[:, :, None],) * 3, torch.empty(2, 8, 1, 16, **f32)),
+                     lambda x: ops.quantize_rows(x[0], q, scales),
+                     lambda x: ops.linear_int8(q, scales, q, scales, torch.empty(8, 8, **f32), bias=x[0, 0, :8]),
+                     lambda x: ops.group_norm(x, torch.empty_like(x), 4),
+                     lambda x: ops.group_norm_backward(_rand(2, 8, 16, dtype=torch.float32), x, stats, torch.empty(2, 8, 16, **f32), 4,
+                                                       workspace=torch.empty(1 << 16, dtype=torch.uint8, device="cuda"))):
+            call(x)
+            with pytest.raises(nn.StringError, match="tangent"):
+                call(dual)
