@@ -538,10 +538,11 @@ NormBackPlan planBackward(const kgh_group_norm_backward_params& p) {
       // 114 us, one workgroup a CU; 512 82), of few threads more (8192 x 1 x 384: 512 38 us,
       // 1024 27). Of two items at least where there are many (512 x 1 x 4096: 27 us with one,
       // 20 with two; 64 x 1 x 4096: 12 and 13.5), of at most 64, sums' terms one after the
-      // other, where the launch has room.
+      // other (the launch's threads are counted in 32 bits: room for more bytes of items
+      // than the card holds).
       const int64_t room = std::min(1024, 262144 / plan.slab.threads) / plan.slab.runs;
-      const int64_t most = std::max<int64_t>(1, NORM_MAX_GRID / plan.slab.runs);
-      plan.slices = (int)std::min(most, std::max<int64_t>({1, std::min<int64_t>(room, p.batch <= 256 ? p.batch : p.batch / 2), p.batch / 64}));
+      const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 31) / ((int64_t)plan.slab.threads * plan.slab.runs));
+      plan.slices = (int)std::min(most, std::max<int64_t>({1, std::min<int64_t>(room, p.batch <= 256 ? p.batch : p.batch / 2), ((int64_t)p.batch + 63) / 64}));
       plan.sumsBytes = round16((uint64_t)plan.slices * p.channels * 8);
       return plan;
     }

@@ -170,3 +170,18 @@ def test_tangents_are_refused():
             call(x)
             with pytest.raises(nn.StringError, match="tangent"):
                 call(dual)
+
+
+def test_backward_sums_of_very_many_items():
+    """A thread adds at most 64 items' terms in fp32 however many there are (see
+    test_backward_sums_of_very_many_terms)."""
+    b, c, depth = 1 << 29, 8, 64 + 8
+    one, grad = _rand(1, 1, c, seed=3), _rand(1, 1, c, seed=1).abs() + 0.25
+    stats = _forward_statistics(one, 1)
+    dx, dw, db = torch.empty(b, 1, c, dtype=one.dtype, device="cuda"), torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    _backward(one.expand(b, 1, c), grad.expand(b, 1, c), stats.expand(b, 1, 2).contiguous(), dx, 1, grad_weight=dw, grad_bias=db)
+    want_x, want_w, want_b = ref.group_norm_backward(one, grad, stats, 1)
+    assert all(bool((part == dx[:1]).all()) for part in dx.split(1 << 26))
+    check(dx[:1], want_x)
+    for got, (y, off), what in ((dw, want_w, "weight"), (db, want_b, "bias")):
+        check(got, (b * y, b * (off + (depth - ref.DEPTH) * U32 * y.abs())), what)
