@@ -711,6 +711,9 @@ void checkGroupNorm(const kgh_group_norm_params& p, bool pointers) {
     if((p.batch > 1 && p.x_batch_stride != p.out_batch_stride) || (p.positions > 1 && p.x_position_stride != p.out_position_stride))
       opInvalid(op, "in place, the strides must be the same");
   }
+  checkApartFrom(op, "out", p.out, {{"weight", p.weight}, {"bias", p.bias}, {"lengths", p.lengths}, {"mask", p.mask}, {"out_scales", p.out_scales}, {"statistics", p.statistics}});
+  checkApartFrom(op, "out_scales", p.out_scales, {{"x", p.x}, {"weight", p.weight}, {"bias", p.bias}, {"lengths", p.lengths}, {"mask", p.mask}, {"statistics", p.statistics}});
+  checkApartFrom(op, "statistics", p.statistics, {{"x", p.x}, {"weight", p.weight}, {"bias", p.bias}, {"lengths", p.lengths}, {"mask", p.mask}});
   opCheckWorkspace(op, p.workspace, p.workspace_bytes, groupNormWorkspace(p));
 }
 

@@ -627,6 +627,10 @@ void checkGroupNormBackward(const kgh_group_norm_backward_params& p, bool pointe
   if(p.lengths != nullptr) opCheckPointer(op, "lengths", p.lengths, 4);
   if(p.x == p.grad_x) opInvalid(op, "grad_x is x itself");
   if(p.grad_out == p.grad_x) opInvalid(op, "grad_x is grad_out itself");
+  checkApartFrom(op, "grad_x", p.grad_x, {{"statistics", p.statistics}, {"weight", p.weight}, {"bias", p.bias}, {"lengths", p.lengths}, {"mask", p.mask}});
+  for(const auto& out : {std::make_pair("grad_weight", p.grad_weight), std::make_pair("grad_bias", p.grad_bias)})
+    checkApartFrom(op, out.first, out.second, {{"x", p.x}, {"grad_out", p.grad_out}, {"grad_x", p.grad_x}, {"statistics", p.statistics}, {"weight", p.weight}, {"bias", p.bias},
+                                               {"lengths", p.lengths}, {"mask", p.mask}});
   opCheckWorkspace(op, p.workspace, p.workspace_bytes, groupNormBackwardWorkspace(p));
 }
 

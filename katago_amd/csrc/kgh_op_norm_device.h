@@ -5,6 +5,8 @@
 #include "kgh_op_quantize_device.h"
 
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 namespace {
 
@@ -229,6 +231,12 @@ inline void checkApartRows(const char* op, const char* name, int64_t batchStride
   const bool positionsInside = (positions == 1 || positionStride >= channels) && (batch == 1 || batchStride >= (positions - 1) * positionStride + channels);
   const bool itemsInside = (batch == 1 || batchStride >= channels) && (positions == 1 || positionStride >= (batch - 1) * batchStride + channels);
   if(!positionsInside && !itemsInside) kgh::opInvalid(op, std::string("the strides of ") + name + " make its rows overlap");
+}
+
+// An output that is no other one of the call's tensors.
+inline void checkApartFrom(const char* op, const char* name, const void* out, std::initializer_list<std::pair<const char*, const void*>> others) {
+  for(const auto& o : others)
+    if(out != nullptr && out == o.second) kgh::opInvalid(op, std::string(name) + " is " + o.first + " itself");
 }
 
 template<typename P>

@@ -158,6 +158,37 @@ def test_group_norm_backward_refuses(change, word):
     _refused(_backward(**change), word)
 
 
+def _apart(**change):
+    return dict(dict(x=Meta(2, 9, 24), weight=Meta(24, at=10 * AT, **F32), bias=Meta(24, at=11 * AT, **F32), lengths=Meta(2, dtype="int32", at=12 * AT),
+                     mask=Meta(2, 9, dtype="bool", at=13 * AT)), **change)
+
+
+@pytest.mark.parametrize("name,at", [("weight", 10), ("bias", 11), ("lengths", 12), ("mask", 13)])
+def test_outputs_that_are_inputs_are_refused(name, at):
+    q = dict(out=Meta(2, 9, 24, at=2 * AT, **I8))
+    scales, stats = (lambda at: Meta(2, 9, at=at * AT, **F32)), (lambda at: Meta(2, 4, 2, at=at * AT, **F32))
+    _refused(_norm(**_apart(out=Meta(2, 9, 24, at=at * AT))), "out is " + name + " itself")
+    _refused(_norm(**_apart(out_scales=scales(at), **q)), "out_scales is " + name + " itself")
+    _refused(_norm(**_apart(stats=stats(at))), "statistics is " + name + " itself")
+    _refused(_backward(**_apart(grad_x=Meta(2, 9, 24, at=at * AT))), "grad_x is " + name + " itself")
+    for grad in ("grad_weight", "grad_bias"):
+        _refused(_backward(**_apart(**{grad: Meta(24, at=at * AT, **F32)})), grad + " is " + name + " itself")
+
+
+def test_outputs_that_are_each_other_are_refused():
+    f32 = lambda *shape, at: Meta(*shape, at=at * AT, **F32)
+    q = dict(out=Meta(2, 9, 24, at=2 * AT, **I8))
+    _refused(_norm(**_apart(out_scales=f32(2, 9, at=2), **q)), "out is out_scales itself")
+    _refused(_norm(**_apart(stats=f32(2, 4, 2, at=2))), "out is statistics itself")
+    _refused(_norm(**_apart(out_scales=f32(2, 9, at=5), stats=f32(2, 4, 2, at=5), **q)), "out_scales is statistics itself")
+    _refused(_norm(**_apart(out_scales=f32(2, 9, at=1), **q)), "out_scales is x itself")
+    _refused(_norm(**_apart(stats=f32(2, 4, 2, at=1))), "statistics is x itself")
+    _refused(_backward(**_apart(grad_x=Meta(2, 9, 24, at=3 * AT))), "grad_x is statistics itself")
+    for grad in ("grad_weight", "grad_bias"):
+        for name, at in (("x", 1), ("grad_out", 2), ("statistics", 3), ("grad_x", 4)):
+            _refused(_backward(**_apart(**{grad: f32(24, at=at)})), grad + " is " + name + " itself")
+
+
 def test_workspaces_that_are_needed():
     """A call that needs a workspace names the bytes."""
     x, q = Meta(3, 16384, 512), Meta(3, 16384, 512, at=2 * AT, **I8)
