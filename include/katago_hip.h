@@ -373,8 +373,9 @@ int kgh_quantize_rows(int32_t device, const kgh_quantize_params* params, void* h
  * channel:
  *   out[m][n] = act(S * x_scales[m] * weight_scales[n] + bias[n]) + residual[m][n],
  *   S = sum_k x[m][k] weights[n][k].
- * S is exact; from there on the arithmetic is fp32's, and the result is rounded to its
- * type once. residual may be out itself (with its stride). in_channels is at most
+ * S is exact; from there on each step is rounded to fp32, the same in every kernel (S *
+ * x_scales[m] first: past the largest float it is infinite), and the result is rounded to
+ * its type once. residual may be out itself (with its stride). in_channels is at most
  * KGH_LINEAR_INT8_MAX_IN (S then fits 32 bits whatever the bytes are). Activations are
  * those of kgh_linear. Rows of x and weights that are 16-byte aligned, in_channels and
  * strides among them, are read fastest. */
@@ -411,8 +412,9 @@ int kgh_linear_int8(int32_t device, const kgh_linear_int8_params* params, void* 
  * Positions p < lengths[b] with mask[b][p] != 0 take part (either may be NULL; lengths
  * are taken into 0..positions). What x holds elsewhere is not used, whatever it is, and
  * out is zero there. One group over one position is a token's layer norm. An infinity or
- * NaN that takes part makes its item's group NaN. The differences x - mean are fp32
- * numbers: one that passes the largest float is infinite; the variance may pass it.
+ * NaN that takes part makes its item's group NaN. The differences x - mean, and weight /
+ * sqrt(variance + eps), are fp32 numbers: one that passes the largest float is infinite;
+ * the variance may pass it.
  * out is of x's type, and may be x itself (with its strides). With out_scales it is
  * int8: rows (b, p) over all channels as kgh_quantize_rows makes them of the results
  * before they are rounded, and their scales.

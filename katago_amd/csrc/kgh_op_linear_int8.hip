@@ -143,8 +143,8 @@ __device__ __forceinline__ void storeInside(const LinearArgs& a, const intx16 (&
 
 // ---------------------------------------------------------------------------
 // Rows that are 16-byte aligned: dmaTile's loop, 128 k a step. 8192 x 4096 x 8192 bf16 on
-// 256 x 256 tiles: 277 us, 1987 TOP/s (the library's product, without scales, 267), at
-// the clock that the power limit leaves (1.66 GHz); GELU and a residual add 50, a tile's
+// 256 x 256 tiles: 287 us, 1915 TOP/s (the library's product, without scales, 267), at
+// the clock that the power limit leaves (1.66 GHz); GELU and a residual add 46, a tile's
 // end which nothing covers on one workgroup a CU. 46208 x 1024 x 384 fp16 with a residual
 // on 128 x 128: 42 us, 2.8 TB/s, a tile's first loads and stores around eight steps; with
 // the epilogue's own loads behind the steps 54.
@@ -195,8 +195,10 @@ __global__ __launch_bounds__(64 * WM * WN, PER_CU * WM * WN / 4) void linear8Dma
 // ---------------------------------------------------------------------------
 // Any strides and alignment: tiles of 2 x 2 waves of 32 RB x 32 CB, steps of 128 bytes
 // of K, loaded into registers two steps ahead, put into one LDS buffer while the other
-// one's products run. Loads that straddle cache lines bound it: 8192 x 4096 x 8192 bf16,
-// rows 7 bytes apart, 617 us, 46208 x 1000 x 384 fp16 67.
+// one's products run. 8192 x 4096 x 8192 bf16, rows 7 bytes apart, 612 us, 46208 x 1000 x
+// 384 bf16 66. In 16 bits 128 x 128 tiles take 257 to 272 registers a lane, so that a SIMD has one
+// wave, and nothing covers a step's wait; whether loads that straddle cache lines or that
+// bounds it is not measured.
 template<typename T, int RB, int CB, int ACT>
 __global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
   constexpr int STEP = 128, BM = 64 * RB, BN = 64 * CB, LOADS = 2 * (RB + CB);

@@ -78,7 +78,8 @@ __device__ __forceinline__ void normalise(float (&y)[VEC], const Values<T>& x, c
 // positions 42; vector instructions are 0.65 of the cycles, and a CU's four workgroups
 // come in two rounds that overlap in part. Registers decide: with 12 vectors a thread
 // four workgroups of 256 threads a CU, where the floats of x beside them, or another
-// turn from registers, left three or spilled.
+// turn from registers, left three or spilled. (Instances hold 2, 4, 12 and 16 vectors, by 76,
+// 80, 116 and 128 registers in 16 bits; ones between 4 and 12 were not tried.)
 template<typename T, int ACT, int NV, bool QUANT>
 __global__ __launch_bounds__(NV == 2 ? 1024 : 512, NV == 16 ? 3 : 4) void normSlabKernel(NormArgs a, NormOut o, NormSlab s) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -489,7 +490,9 @@ __global__ __launch_bounds__(256) void normApplyKernel(NormArgs a, NormOut o, No
 }
 
 // The same in 8 bits: a row's columns by `lanes` threads, K each, and R rows at a time.
-// 46208 x 384 bf16, SiLU: 27 us (2.0 TB/s); vector instructions bound it.
+// 46208 x 384 bf16, SiLU: 27 us (2.0 TB/s); vector instructions bound it. In 16 bits four
+// groups a thread (4097 to 8192 channels) take 256 registers, one wave a SIMD: 4096 x 8192
+// bf16 60 us (1.7 TB/s).
 template<typename T, int ACT, int K, int R>
 __global__ __launch_bounds__(256) void normQuantKernel(NormArgs a, NormOut o, int lanes, int chunks, int chunkRows) {
   constexpr int VEC = 16 / (int)sizeof(T);

@@ -37,7 +37,7 @@ __device__ __forceinline__ float slope(float v) {
   else if constexpr(sizeof(T) == 4) return fmaf(0.5f, erfcf(-0.70710678118654752f * v), v * expf(-0.5f * v * v) * 0.39894228040143268f);
   else {
     // erfc(|v| / sqrt(2)) / 2 = t poly(t) e^(-v^2 / 2), t = 1 / (1 + 0.4 |v| / sqrt(2)), right
-    // to 1.3e-7 of it: the gradients of weight and bias are fp32, so activateFast's 4.2e-6,
+    // to 1.6e-7 of it, and to 6e-7 (1.1e-7 rms) with its roundings: the gradients of weight and bias are fp32, so activateFast's 4.2e-6,
     // which has the same sign in many values, would be seen in their sums.
     const float t = __builtin_amdgcn_rcpf(fmaf(0.282842712f, fabsf(v), 1.0f));
     float poly = fmaf(t, 0.025129477f, -0.0914449404f);
@@ -234,7 +234,7 @@ constexpr int BACK_AHEAD = 2;  // rows of a thread under way
 // Items that no workgroup's registers hold: first the sums of chunks of positions, then,
 // behind their join, the results of the same chunks, u computed in both (kept, it would be
 // as many bytes again as x in fp32, twice as many in 16 bits). 8 x 4096 x 320 fp32, SiLU:
-// 26 us (3.2 TB/s) and 25 (5.0), the joins 8 and 4.
+// 26 us (3.2 TB/s) and 25 (5.0), the joins 9 and 5.
 template<typename T, int ACT, bool APPLY>
 __global__ __launch_bounds__(256) void normBackPartsKernel(NormArgs a, NormBackArgs k, BackParts s) {
   constexpr int VEC = 16 / (int)sizeof(T);
