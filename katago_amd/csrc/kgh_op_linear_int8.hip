@@ -196,9 +196,9 @@ __global__ __launch_bounds__(64 * WM * WN, PER_CU * WM * WN / 4) void linear8Dma
 // Any strides and alignment: tiles of 2 x 2 waves of 32 RB x 32 CB, steps of 128 bytes
 // of K, loaded into registers two steps ahead, put into one LDS buffer while the other
 // one's products run. 8192 x 4096 x 8192 bf16, rows 7 bytes apart, 612 us, 46208 x 1000 x
-// 384 bf16 66. In 16 bits 128 x 128 tiles take 257 to 272 registers a lane, so that a SIMD has one
-// wave, and nothing covers a step's wait; whether loads that straddle cache lines or that
-// bounds it is not measured.
+// 384 bf16 66. In 16 bits 128 x 128 tiles take 257 to 272 registers a lane, so that a SIMD
+// has one wave, and nothing covers a step's wait; whether that bounds it or loads that
+// straddle cache lines do is not measured.
 template<typename T, int RB, int CB, int ACT>
 __global__ __launch_bounds__(256) void linear8TileKernel(LinearArgs a, Scales s, int rowTiles, int colTiles) {
   constexpr int STEP = 128, BM = 64 * RB, BN = 64 * CB, LOADS = 2 * (RB + CB);

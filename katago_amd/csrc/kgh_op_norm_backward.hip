@@ -37,8 +37,9 @@ __device__ __forceinline__ float slope(float v) {
   else if constexpr(sizeof(T) == 4) return fmaf(0.5f, erfcf(-0.70710678118654752f * v), v * expf(-0.5f * v * v) * 0.39894228040143268f);
   else {
     // erfc(|v| / sqrt(2)) / 2 = t poly(t) e^(-v^2 / 2), t = 1 / (1 + 0.4 |v| / sqrt(2)), right
-    // to 1.6e-7 of it, and to 6e-7 (1.1e-7 rms) with its roundings: the gradients of weight and bias are fp32, so activateFast's 4.2e-6,
-    // which has the same sign in many values, would be seen in their sums.
+    // to 1.6e-7 of it, and to 6e-7 (1.1e-7 rms) with its roundings: the gradients of weight
+    // and bias are fp32, so activateFast's 4.2e-6, which has the same sign in many values,
+    // would be seen in their sums.
     const float t = __builtin_amdgcn_rcpf(fmaf(0.282842712f, fabsf(v), 1.0f));
     float poly = fmaf(t, 0.025129477f, -0.0914449404f);
     poly = fmaf(t, poly, 0.0845342149f);
